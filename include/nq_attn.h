@@ -52,6 +52,9 @@ extern "C" {
 
 #define NQ_DTYPE_BF16 0
 #define NQ_DTYPE_F32 1
+#define NQ_PREF_SIGMOID 0
+#define NQ_PREF_HINGE 1
+#define NQ_PREF_IPO 2
 #define NQ_QWEIGHT_BF16 0x200
 #define NQ_KWEIGHT_BF16 0x400
 
@@ -487,6 +490,91 @@ int nq_qk_norm_rope_bwd(const void* x, const int64_t* x_strides, const void* dy,
                         int B, int S, int H, int D, int dtype, float eps, const float* cos_tab,
                         const float* sin_tab, int max_pos, const int32_t* pos, const int32_t* pos_base,
                         int pos0, void* stream);
+
+/*
+ * Log-probabilities of labels: logprobs[n] = z[labels[n]] - log(sum_v exp(z[v])), z the
+ * n-th row of logits / temperature, V contiguous elements at any element's alignment.
+ * The B * S rows lie at b * batch_stride + s * row_stride (elements); labels, logprobs
+ * and stats follow b * S + s.  A label equal to ignore_index gives 0 and its row is not
+ * read; any other outside [0, V) gives NaN, as do a row of -inf, one with NaN and one
+ * with +inf.  stats: two floats per row for the backward.  workspace:
+ * nq_token_logprobs_workspace_bytes(B * S, V), 8-byte aligned (few rows are split over
+ * the device).
+ *
+ * The backward writes dlogits (B * S, V) contiguous, in the logits' dtype:
+ * dlogprobs[n] (1[v = label] - softmax) / temperature; zeros in ignored rows, NaN where
+ * the label is outside the vocabulary.
+ */
+int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int V);
+int nq_token_logprobs(const void* logits, int64_t batch_stride, int64_t row_stride,
+                      const int64_t* labels, float* logprobs, float* stats, void* workspace,
+                      int64_t workspace_bytes, int64_t B, int64_t S, int V, int dtype,
+                      float temperature, int64_t ignore_index, void* stream);
+int nq_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t row_stride,
+                          const int64_t* labels, const float* stats, const float* dlogprobs,
+                          void* dlogits, int64_t B, int64_t S, int V, int dtype, float temperature,
+                          int64_t ignore_index, void* stream);
+
+/*
+ * Preference loss over B pairs of sequences.  Each side: fp32 log-probabilities of its
+ * tokens (B rows of Sc or Sr, row strides in elements), those of the reference model
+ * (NULL: zeros) and a mask (a byte per token, nonzero = kept; NULL: all kept; what a
+ * masked token holds is not read).  d = sum of lp - ref over the kept tokens, or with
+ * `average` their mean (0 if none is kept); with h = beta (d_chosen - d_rejected) a pair's
+ * loss is
+ *   NQ_PREF_SIGMOID  -(1 - label_smoothing) log s(h) - label_smoothing log s(-h)
+ *   NQ_PREF_HINGE    max(0, 1 - h)
+ *   NQ_PREF_IPO      (d_chosen - d_rejected - 1 / (2 beta))^2
+ * loss: the mean over pairs; rewards (B): beta d; coef (2, B), for the backward: d loss /
+ * d lp of a pair's kept chosen and rejected tokens.  workspace:
+ * nq_preference_loss_workspace_bytes(B), 8-byte aligned.
+ *
+ * The backward writes dchosen (B, Sc) and drejected (B, Sr), contiguous (NULL: left out),
+ * for the scalar dloss: zeros in masked tokens.
+ */
+int64_t nq_preference_loss_workspace_bytes(int B);
+int nq_preference_loss(const float* chosen, int64_t chosen_stride, const float* rejected,
+                       int64_t rejected_stride, const float* ref_chosen, int64_t ref_chosen_stride,
+                       const float* ref_rejected, int64_t ref_rejected_stride,
+                       const uint8_t* chosen_mask, int64_t chosen_mask_stride,
+                       const uint8_t* rejected_mask, int64_t rejected_mask_stride, float* loss,
+                       float* chosen_reward, float* rejected_reward, float* coef, void* workspace,
+                       int64_t workspace_bytes, int B, int64_t Sc, int64_t Sr, int kind, double beta,
+                       double label_smoothing, int average, void* stream);
+int nq_preference_loss_bwd(const float* coef, const float* dloss, const uint8_t* chosen_mask,
+                           int64_t chosen_mask_stride, const uint8_t* rejected_mask,
+                           int64_t rejected_mask_stride, float* dchosen, float* drejected, int B,
+                           int64_t Sc, int64_t Sr, void* stream);
+
+/*
+ * Clipped policy loss with a KL term over B sequences of S tokens (fp32 rows with
+ * strides in elements, as above).  Per kept token, with r = exp(lp - old), A its
+ * sequence's advantage (advantages[b * stride]; with advantages_per_token
+ * advantages[b * stride + s]) and q = ref - lp:
+ *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1)
+ * loss: the mean over all kept tokens, or with mean_of_means the mean over the sequences
+ * of each one's mean (0 for one with no kept token).  kl and clipped: the kept tokens'
+ * mean of exp(q) - q - 1 (0 without ref_logprobs) and the share of them that the clip
+ * decides.  With nothing kept all three are 0.  weight (B), for the backward: a kept
+ * token's share of the loss.  workspace: nq_policy_loss_workspace_bytes(B, S), 8-byte
+ * aligned.
+ *
+ * The backward writes dlogprobs (B, S) contiguous for the scalar dloss: zeros in masked
+ * tokens.
+ */
+int64_t nq_policy_loss_workspace_bytes(int B, int64_t S);
+int nq_policy_loss(const float* logprobs, int64_t logprobs_stride, const float* old_logprobs,
+                   int64_t old_stride, const float* ref_logprobs, int64_t ref_stride,
+                   const float* advantages, int64_t advantages_stride, int advantages_per_token,
+                   const uint8_t* mask, int64_t mask_stride, float* loss, float* kl, float* clipped,
+                   float* weight, void* workspace, int64_t workspace_bytes, int B, int64_t S,
+                   double clip_low, double clip_high, double kl_coef, int mean_of_means, void* stream);
+int nq_policy_loss_bwd(const float* logprobs, int64_t logprobs_stride, const float* old_logprobs,
+                       int64_t old_stride, const float* ref_logprobs, int64_t ref_stride,
+                       const float* advantages, int64_t advantages_stride, int advantages_per_token,
+                       const uint8_t* mask, int64_t mask_stride, const float* weight,
+                       const float* dloss, float* dlogprobs, int B, int64_t S, double clip_low,
+                       double clip_high, double kl_coef, void* stream);
 
 #ifdef __cplusplus
 }

@@ -22,6 +22,7 @@ NQ_ERR_WORKSPACE = 3
 NQ_DTYPE_BF16 = 0
 NQ_DTYPE_F32 = 1
 NQ_DECODE_F32_SPLIT = 0x100
+NQ_PREF_SIGMOID, NQ_PREF_HINGE, NQ_PREF_IPO = 0, 1, 2
 NQ_QWEIGHT_BF16 = 0x200
 NQ_KWEIGHT_BF16 = 0x400
 
@@ -29,6 +30,7 @@ _p = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _i64p = ctypes.POINTER(ctypes.c_int64)
 
 # name -> (restype, argtypes); mirrors include/nq_attn.h
@@ -181,6 +183,44 @@ SIGNATURES = {
         _f32, _p, _p, _i32,                          # eps, cos, sin, max_pos
         _p, _p, _i32,                                # pos, pos_base, pos0
         _p,                                          # stream
+    ]),
+    "nq_token_logprobs_workspace_bytes": (_i64, [_i64, _i32]),  # rows, V
+    "nq_token_logprobs": (_i32, [
+        _p, _i64, _i64, _p,                          # logits, batch_stride, row_stride, labels
+        _p, _p, _p, _i64,                            # logprobs, stats, workspace, workspace_bytes
+        _i64, _i64, _i32, _i32,                      # B, S, V, dtype
+        _f32, _i64, _p,                              # temperature, ignore_index, stream
+    ]),
+    "nq_token_logprobs_bwd": (_i32, [
+        _p, _i64, _i64, _p,                          # logits, batch_stride, row_stride, labels
+        _p, _p, _p,                                  # stats, dlogprobs, dlogits
+        _i64, _i64, _i32, _i32,                      # B, S, V, dtype
+        _f32, _i64, _p,                              # temperature, ignore_index, stream
+    ]),
+    "nq_preference_loss_workspace_bytes": (_i64, [_i32]),  # B
+    "nq_preference_loss": (_i32, [
+        _p, _i64, _p, _i64, _p, _i64, _p, _i64,      # chosen, rejected, ref_chosen, ref_rejected (+ strides)
+        _p, _i64, _p, _i64,                          # chosen_mask, rejected_mask (+ strides)
+        _p, _p, _p, _p, _p, _i64,                    # loss, rewards, coef, workspace, workspace_bytes
+        _i32, _i64, _i64, _i32, _f64, _f64, _i32,    # B, Sc, Sr, kind, beta, label_smoothing, average
+        _p,                                          # stream
+    ]),
+    "nq_preference_loss_bwd": (_i32, [
+        _p, _p, _p, _i64, _p, _i64,                  # coef, dloss, masks (+ strides)
+        _p, _p, _i32, _i64, _i64, _p,                # dchosen, drejected, B, Sc, Sr, stream
+    ]),
+    "nq_policy_loss_workspace_bytes": (_i64, [_i32, _i64]),  # B, S
+    "nq_policy_loss": (_i32, [
+        _p, _i64, _p, _i64, _p, _i64,                # logprobs, old, ref (+ strides)
+        _p, _i64, _i32, _p, _i64,                    # advantages, stride, per_token, mask, stride
+        _p, _p, _p, _p, _p, _i64,                    # loss, kl, clipped, weight, workspace, workspace_bytes
+        _i32, _i64, _f64, _f64, _f64, _i32, _p,      # B, S, clip_low, clip_high, kl_coef, mean_of_means, stream
+    ]),
+    "nq_policy_loss_bwd": (_i32, [
+        _p, _i64, _p, _i64, _p, _i64,                # logprobs, old, ref (+ strides)
+        _p, _i64, _i32, _p, _i64,                    # advantages, stride, per_token, mask, stride
+        _p, _p, _p,                                  # weight, dloss, dlogprobs
+        _i32, _i64, _f64, _f64, _f64, _p,            # B, S, clip_low, clip_high, kl_coef, stream
     ]),
 }
 

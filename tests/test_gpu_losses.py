@@ -1,0 +1,524 @@
+"""Log-probabilities of labels, the preference loss and the policy loss on the kernels,
+against the same formulas in 64 bits.
+
+Tolerances are sums of roundings: u = 2^-24 for each fp32 operation on a value, half a
+step of the output's type for the result.
+"""
+
+import math
+
+import pytest
+import torch
+
+import nano_qwen_amd as nq
+from tests.helpers import randn, say
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+U = 2.0 ** -24
+
+
+def half_step(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def within(got, want, tol, what):
+    got = got.detach().double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN in other places"
+    assert torch.equal(torch.isinf(got), torch.isinf(want)), f"{what}: infinities in other places"
+    ok = torch.isfinite(want)
+    err = (got - want).abs()
+    tol = tol.expand_as(err) if isinstance(tol, torch.Tensor) else torch.full_like(err, tol)
+    bad = (err > tol) & ok
+    assert not bad.any(), (what, int(bad.sum()), float(err[ok].max()), float((err / tol)[bad].max()))
+
+
+# ---------------------------------------------------------------- token_logprobs
+
+def token_reference(x, labels, dy, T, ignore=-100):
+    """(logprobs, dlogits, their tolerances before the output's own rounding), in 64 bits."""
+    V = x.shape[-1]
+    z = x.double() / T
+    logp = torch.log_softmax(z, -1)  # subtracts the maximum first: exact also at the types' ends
+    p = torch.exp(logp)
+    at = labels.clamp(0, V - 1)[..., None].long()
+    keep = labels != ignore
+    bad = keep & ((labels < 0) | (labels >= V))
+    lp = logp.gather(-1, at)[..., 0]
+    lp = torch.where(bad, torch.nan, torch.where(keep, lp, 0.0))
+    g = torch.where(keep, dy.double(), 0.0) / T
+    g = torch.where(bad, torch.nan, g)[..., None]
+    dz = torch.where(keep[..., None], -p * g, 0.0)
+    dz = dz.scatter_add(-1, at, g)
+    # exponents (x - m) c carry |z - m| u each, a thread adds V / 256 terms one after the
+    # other, waves and workgroups join in some 16 steps of 4 operations
+    fin = torch.where(torch.isfinite(z), z, torch.nan)
+    span = torch.nan_to_num(torch.nan_to_num(fin, -math.inf).amax(-1) - torch.nan_to_num(fin, math.inf).amin(-1), 0, 0, 0)
+    steps = (span * 2 + V / 256 + 80) * U
+    tol_lp = steps + 4 * U * lp.abs().nan_to_num(0, 0, 0)
+    tol_dz = g.abs().nan_to_num(0) * (p.nan_to_num(0) * steps[..., None] + 4 * U) + 1e-37
+    return lp, dz, tol_lp, tol_dz
+
+
+def run_token(x, labels, dy, T=1.0, **kw):
+    xd = x.to(DEV).requires_grad_()
+    lp = nq.token_logprobs(xd, labels.to(DEV), temperature=T, **kw)
+    (dx,) = torch.autograd.grad(lp, xd, dy.to(DEV))
+    return lp, dx
+
+
+def check_token(x, labels, dy, T=1.0, what="", **kw):
+    lp, dx = run_token(x, labels, dy, T, **kw)
+    assert lp.dtype == F32 and lp.shape == labels.shape and dx.dtype == x.dtype and dx.shape == x.shape
+    want, dwant, tol, dtol = token_reference(x, labels, dy, T, kw.get("ignore_index", -100))
+    within(lp, want, tol, f"{what} logprobs")
+    within(dx, dwant, dtol + half_step(x.dtype) * dwant.abs().nan_to_num(0), f"{what} dlogits")
+    with torch.no_grad():
+        assert torch.equal(nq.token_logprobs(x.to(DEV), labels.to(DEV), temperature=T, **kw).nan_to_num(9), lp.nan_to_num(9))
+
+
+# rows of less than a vector, of whole vectors and not, of one and of many slices; one row to
+# more than the split is for
+@pytest.mark.parametrize("rows,V", [(1, 1), (1, 8), (3, 7), (2, 9), (5, 1000), (4, 8192), (3, 8200), (2, 50257), (1, 151936),
+                                    (2100, 133), (260, 16391)])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_token_logprobs(rows, V, dt):
+    say(f"token_logprobs {rows}x{V} {dt}")
+    x = randn(rows, V, seed=7, dtype=dt, scale=3)
+    labels = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(8))
+    labels[rows // 2] = V - 1
+    if rows > 3:
+        labels[::3] = -100
+    check_token(x, labels, randn(rows, seed=9), T=0.7 if V % 2 else 1.0, what=f"{rows}x{V}")
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("rows", [3, 3000])
+def test_token_logprobs_of_special_rows(rows, dt):
+    """Masked vocabularies, rows of -inf, infinities, NaN, labels outside, ignored rows of NaN."""
+    say(f"token_logprobs special rows {rows} {dt}")
+    V = 4099
+    x = randn(12, V, seed=17, dtype=dt)
+    inf = float("inf")
+    x[0, 5:] = -inf                      # five tokens left, the label among them
+    x[1, :4098] = -inf                   # only the last element, in the tail
+    x[2] = -inf
+    x[3, 77] = inf
+    x[4, 4098] = inf
+    x[5, 4098] = float("nan")
+    x[6, 0] = float("nan")
+    x[7, :4000] = -inf                   # the first threads and slices see nothing but -inf
+    x[8] = torch.finfo(dt).min           # the type's lowest value everywhere
+    x[9, ::2] = torch.finfo(dt).min      # and as a mask
+    x[9, 1] = torch.finfo(dt).max / 2
+    labels = torch.tensor([2, 4098, 3, 77, 0, 1, 0, 4050, 9, 1, 4099, -1])
+    x, labels = x.repeat(rows // 3 + 1, 1)[:max(rows, 12)], labels.repeat(rows // 3 + 1)[:max(rows, 12)]
+    check_token(x, labels, 1 + randn(len(x), seed=18).abs(), what="special")
+    # ignored rows are not read and get zeros, whatever they hold
+    lp, dx = run_token(x, torch.full_like(labels, -100), torch.full((len(x),), float("nan")))
+    assert not lp.any() and not dx.any()
+    # a label of -inf among finite ones: -inf, and a finite gradient
+    y = randn(rows, V, seed=19, dtype=dt)
+    y[:, 3] = -inf
+    check_token(y, torch.full((rows,), 3), torch.ones(rows), what="label of -inf")
+
+
+def test_token_logprobs_shapes_strides_types():
+    say("token_logprobs shapes and strides")
+    big = randn(3, 6, 5, 72, seed=27)
+    lab = torch.randint(0, 64, (3, 6, 5), generator=torch.Generator().manual_seed(28))
+    dy = randn(3, 6, 5, seed=29)
+    views = {
+        "sliced": (big[..., 3:67], lab, dy),
+        "short sequences": (big[0, :, :4, :64], lab[0, :, :4], dy[0, :, :4]),
+        "four axes that do not fold": (big[:, ::2, 1:, :64], lab[:, ::2, 1:], dy[:, ::2, 1:]),
+        "transposed": (big[0, 0].t()[:64, :][:, :5].t(), lab[0, 0], dy[0, 0]),
+        "one row": (big[0, 0, 0, :64], lab[0, 0, 0], dy[0, 0, 0]),
+        "expanded": (big[0, :1, 0, :64].expand(6, 64), lab[0, :, 0], dy[0, :, 0]),
+        "other ignore_index": (big[0, 0, :, :64], lab[0, 0], dy[0, 0]),
+    }
+    for name, (x, y, g) in views.items():
+        dev = torch.empty_strided(x.shape, x.stride(), device=DEV) if name != "expanded" else x[:1].to(DEV).expand(x.shape)
+        if name != "expanded":
+            dev.copy_(x)
+        dev = dev.detach().requires_grad_()
+        kw = dict(ignore_index=int(y.flatten()[0])) if name == "other ignore_index" else {}
+        for labels in (y, y.to(torch.int32)):
+            lp = nq.token_logprobs(dev, labels.to(DEV), **kw)
+            (dx,) = torch.autograd.grad(lp, dev, g.to(DEV))
+            want, dwant, tol, dtol = token_reference(x, y, g, 1.0, kw.get("ignore_index", -100))
+            within(lp, want, tol, name)
+            within(dx, dwant, dtol + half_step(F32) * dwant.abs(), name)
+    # a gradient broadcast by a sum, and rows at a misaligned base address
+    for dt in (BF, F32):
+        x = randn(4, 66, seed=30, dtype=dt)
+        y = torch.tensor([0, 64, 3, -100])
+        dev = x.to(DEV)
+        leaf = dev[:, 1:].detach().requires_grad_()
+        (dx,) = torch.autograd.grad(nq.token_logprobs(leaf, y.to(DEV)).sum(), leaf)
+        _, dwant, _, dtol = token_reference(x[:, 1:], y, torch.ones(4), 1.0)
+        within(dx, dwant, dtol + half_step(dt) * dwant.abs(), "misaligned")
+    for shape in ((0, 7), (2, 0, 7)):
+        x = torch.zeros(shape, device=DEV, requires_grad=True)
+        lp = nq.token_logprobs(x, torch.zeros(shape[:-1], dtype=torch.long, device=DEV))
+        assert lp.shape == shape[:-1] and torch.autograd.grad(lp.sum(), x)[0].shape == shape
+
+
+def test_token_logprobs_past_32_bits():
+    """Rows whose offsets pass 2^31 elements and 2^32 bytes."""
+    say("token_logprobs past 2^31 elements")
+    V, S = 150000, 15000
+    x = torch.zeros(S, V, dtype=BF, device=DEV)
+    assert x.numel() > 2 ** 31
+    rows = torch.tensor([0, 14316, 14317, 14999])
+    part = randn(4, V, seed=31, dtype=BF)
+    x[rows.to(DEV)] = part.to(DEV)
+    labels = torch.full((S,), -100)
+    labels[rows] = torch.tensor([0, 1, V - 1, 7])
+    dy = randn(S, seed=32)
+    x.requires_grad_()
+    lp = nq.token_logprobs(x, labels.to(DEV))
+    (dx,) = torch.autograd.grad(lp, x, dy.to(DEV))
+    want, dwant, tol, dtol = token_reference(part, labels[rows], dy[rows], 1.0)
+    within(lp[rows.to(DEV)], want, tol, "far rows")
+    within(dx[rows.to(DEV)], dwant, dtol + half_step(BF) * dwant.abs(), "far rows' gradient")
+    dx[rows.to(DEV)] = 0
+    assert not dx.any()
+
+
+def test_token_logprobs_differences():
+    """The gradient against central differences of the operator itself."""
+    say("token_logprobs differences")
+    x, v = randn(6, 37, seed=33).to(DEV), randn(6, 37, seed=34).to(DEV)
+    y, g = torch.arange(6, device=DEV) * 5, randn(6, seed=35).to(DEV)
+
+    def f(t):
+        return (nq.token_logprobs(x + t * v, y, temperature=1.3) * g).sum(dtype=torch.float64)
+    xg = x.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(nq.token_logprobs(xg, y, temperature=1.3), xg, g)
+    h = 2.0 ** -6
+    diff = float((f(h) - f(-h)) / (2 * h))
+    # third derivative along v under 6 |g| |v/T|^3 per row, each value off by some 100 u
+    bound = float(6 * g.abs().sum() * (v.abs().max() / 1.3) ** 3) * h * h / 6 + 2 * 100 * U * float(g.abs().sum()) / (2 * h)
+    assert abs(diff - float((dx * v).double().sum())) <= bound
+
+
+def test_token_logprobs_refusals():
+    x, y = torch.zeros(4, 9, device=DEV), torch.zeros(4, dtype=torch.long, device=DEV)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        nq.token_logprobs(x.cpu(), y)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        nq.token_logprobs(x, y.cpu())
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        nq.token_logprobs(x.half(), y)
+    with pytest.raises(TypeError, match="labels"):
+        nq.token_logprobs(x, y.float())
+    with pytest.raises(ValueError, match="one label per row"):
+        nq.token_logprobs(x, y[:3])
+    with pytest.raises(ValueError, match="last axis"):
+        nq.token_logprobs(x[:, :0], y)
+    for t in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            nq.token_logprobs(x, y, temperature=t)
+    with pytest.raises(RuntimeError):
+        xg = x.clone().requires_grad_()
+        (d,) = torch.autograd.grad(nq.token_logprobs(xg, y).sum(), xg, create_graph=True)
+        torch.autograd.grad(d.sum(), xg)
+
+
+# ---------------------------------------------------------------- preference_loss
+
+def preference_reference(c, r, rc, rr, mc, mr, kind, beta, e, average):
+    c, r = (t.double().requires_grad_() for t in (c, r))
+    d = []
+    for lp, ref, m in ((c, rc, mc), (r, rr, mr)):
+        t = lp - (0 if ref is None else ref.double())
+        m = torch.ones_like(t, dtype=torch.bool) if m is None else m
+        t = torch.where(m, t, 0.0).reshape(len(lp), -1).sum(1)
+        d.append(t / m.reshape(len(lp), -1).sum(1).clamp(min=1) if average else t)
+    h = beta * (d[0] - d[1])
+    if kind == "sigmoid":
+        ls = torch.nn.functional.logsigmoid
+        loss = -(1 - e) * ls(h) - e * ls(-h)
+    elif kind == "hinge":
+        loss = torch.relu(1 - h)
+    else:
+        loss = (d[0] - d[1] - 1 / (2 * beta)) ** 2
+    loss = loss.mean()
+    return [t.detach() for t in (loss, beta * d[0], beta * d[1], *torch.autograd.grad(loss, (c, r)))]
+
+
+def ragged(B, S, seed):
+    g = torch.Generator().manual_seed(seed)
+    m = torch.arange(S) < torch.randint(0, S + 1, (B, 1), generator=g)
+    m[B // 2] = False  # a sequence with nothing left
+    return m
+
+
+@pytest.mark.parametrize("B,Sc,Sr", [(1, 1, 1), (3, 40, 17), (16, 1024, 5), (17, 9, 33), (4, 1025, 300), (300, 70, 64),
+                                     (2, 0, 3)])
+@pytest.mark.parametrize("kind,e", [("sigmoid", 0.0), ("sigmoid", 0.2), ("hinge", 0.0), ("ipo", 0.0)])
+@pytest.mark.parametrize("average", [False, True])
+def test_preference_loss(B, Sc, Sr, kind, e, average):
+    say(f"preference_loss {B} {Sc} {Sr} {kind} {e} {average}")
+    c, r, rc, rr = (-randn(B, S, seed=40 + i).abs() for i, S in enumerate((Sc, Sr, Sc, Sr)))
+    mc, mr = ragged(B, Sc, 44), ragged(B, Sr, 45)
+    for masks, refs in (((mc, mr), (rc, rr)), ((None, mr), (None, rr)), ((mc, None), (rc, None))):
+        want = preference_reference(c, r, *refs, *masks, kind, 0.3, e, average)
+        # what a masked token holds has no effect
+        ins = [t.clone() for t in (c, r)] + [None if t is None else t.clone() for t in refs]
+        for t, m in zip(ins, masks * 2):
+            if t is not None and m is not None:
+                t[~m] = float("nan")
+        cd, rd, rcd, rrd = (None if t is None else t.to(DEV) for t in ins)
+        cd.requires_grad_(), rd.requires_grad_()
+        loss, wc, wr = nq.preference_loss(cd, rd, rcd, rrd, chosen_mask=None if masks[0] is None else masks[0].to(DEV),
+                                          rejected_mask=None if masks[1] is None else masks[1].to(DEV), beta=0.3,
+                                          label_smoothing=e, kind=kind, average=average)
+        grads = torch.autograd.grad(2.5 * loss, (cd, rd))
+        assert loss.shape == () and wc.shape == wr.shape == (B,) and not wc.requires_grad
+        # sums in 64 bits; results rounded once, gradients twice more by the factor
+        for name, got, ref, k in zip(("loss", "wc", "wr", "dc", "dr"), (loss, wc, wr, *grads), want, (1, 1, 1, 2.5, 2.5)):
+            within(got, k * ref, 4 * U * (k * ref).abs() + 1e-12, name)
+
+
+def test_preference_loss_far_margins_and_rows():
+    """Margins that overflow an exponential; sequences' sums given as such; strided rows; bf16; gradients of broadcasts."""
+    say("preference_loss margins, strides")
+    c = torch.tensor([1e5, -1e5, 0.0, 3000.0, -800.0])
+    r = torch.zeros(5)
+    for kind in ("sigmoid", "hinge", "ipo"):
+        want = preference_reference(c[:, None], r[:, None], None, None, None, None, kind, 1.0, 0.0, False)
+        cd, rd = c.to(DEV).requires_grad_(), r.to(DEV).requires_grad_()
+        loss, *_ = nq.preference_loss(cd, rd, beta=1.0, kind=kind)
+        grads = torch.autograd.grad(loss, (cd, rd))
+        within(loss, want[0], 4 * U * want[0].abs(), kind)
+        for g, w in zip(grads, want[3:]):
+            within(g, w[:, 0], 4 * U * w[:, 0].abs() + 1e-40, kind)
+    both = -randn(8, 30, seed=46).abs()      # one forward over both sides, the views of it as they are
+    mask = ragged(8, 30, 47)
+    leaf = both.to(DEV).requires_grad_()
+    m = mask.to(DEV)
+    ref = -randn(30, 8, seed=48).abs()
+    loss, *_ = nq.preference_loss(leaf[::2, 1:], leaf[1::2, 1:], ref.to(DEV).t()[:4, 1:], ref.to(DEV).t()[4:, 1:],
+                                  chosen_mask=m[::2, 1:], rejected_mask=m[1::2, 1:].int())
+    (g,) = torch.autograd.grad(loss, leaf)
+    want = preference_reference(both[::2, 1:], both[1::2, 1:], ref.t()[:4, 1:], ref.t()[4:, 1:], mask[::2, 1:],
+                                mask[1::2, 1:], "sigmoid", 0.1, 0.0, False)
+    within(loss, want[0], 4 * U * want[0].abs(), "strided")
+    full = torch.zeros(8, 30, dtype=torch.float64)
+    full[::2, 1:], full[1::2, 1:] = want[3], want[4]
+    within(g, full, 4 * U * full.abs(), "strided gradient")
+    # bf16 log-probabilities, one side without a gradient, an expanded side
+    one = both[:1].to(BF)
+    leaf = one.to(DEV).requires_grad_()
+    loss, *_ = nq.preference_loss(leaf.expand(4, 30), both[:4].to(DEV))
+    (g,) = torch.autograd.grad(loss, leaf)
+    want = preference_reference(one.float().expand(4, 30), both[:4], None, None, None, None, "sigmoid", 0.1, 0.0, False)
+    within(loss, want[0], 4 * U * want[0].abs(), "expanded")
+    # torch sums the four rows' gradients, each rounded to bf16
+    within(g, want[3].sum(0, keepdim=True), 4 * 2.0 ** -8 * want[3].abs().sum(0, keepdim=True), "expanded gradient")
+
+
+def test_preference_loss_refusals():
+    x = torch.zeros(3, 5, device=DEV)
+    bad = [(ValueError, dict(kind="other")), (ValueError, dict(beta=0.0)), (ValueError, dict(beta=float("inf"))),
+           (ValueError, dict(label_smoothing=0.5)), (ValueError, dict(label_smoothing=0.1, kind="ipo")),
+           (ValueError, dict(ref_chosen=x[:2])), (ValueError, dict(rejected_mask=x[:, :4] > 0)),
+           (TypeError, dict(ref_chosen=x.half())), (RuntimeError, dict(chosen_mask=x.cpu() > 0))]
+    for err, kw in bad:
+        with pytest.raises(err):
+            nq.preference_loss(x, x, **kw)
+    for a, b in ((x, x[:2]), (x[:0], x[:0]), (x[None], x[None]), (x.half(), x.half()), (x.cpu(), x.cpu())):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            nq.preference_loss(a, b)
+
+
+# ---------------------------------------------------------------- policy_loss
+
+def policy_reference(lp, old, adv, ref, mask, low, high, c, reduction):
+    lp = lp.double().requires_grad_()
+    mask = torch.ones(lp.shape, dtype=torch.bool) if mask is None else mask
+    a = adv.double() if adv.dim() == 2 else adv.double()[:, None].expand(lp.shape)
+    d = torch.where(mask, lp - old.double(), 0.0)
+    r = torch.exp(d)
+    clip = r.clamp(1 - low, 1 + high)
+    each = -torch.minimum(r * a, clip * a)
+    cut = (clip * a < r * a) & mask
+    kl = torch.zeros_like(d)
+    if ref is not None:
+        q = torch.where(mask, ref.double() - lp, 0.0)
+        kl = torch.expm1(q) - q
+        each = each + c * kl
+    n = mask.sum().clamp(min=1)
+    rows = mask.sum(1).clamp(min=1)
+    kept = torch.where(mask, each, 0.0)
+    loss = kept.sum() / n if reduction == "token" else (kept.sum(1) / rows).mean()
+    (grad,) = torch.autograd.grad(loss, lp)
+    # a term: the exponent's rounding |d| u, some 8 operations; its share likewise in the gradient
+    share = (1 / n if reduction == "token" else 1 / (rows[:, None] * len(lp))).double()
+    size = ((r * a).abs() + abs(c) * (kl.abs() + (lp - lp + 1) * (torch.expm1(-torch.log1p(kl))).abs() + kl.abs().sqrt() * 2)).detach()
+    tol = torch.where(mask, size * (d.abs().detach() + 16) * U * share, 0.0)
+    kl_mean = torch.where(mask, kl, 0.0).sum().detach() / n
+    return loss.detach(), kl_mean, cut.sum() / n.double(), grad, tol
+
+
+@pytest.mark.parametrize("B,S", [(1, 1), (3, 40), (16, 1024), (17, 33), (2, 1025), (2, 5000), (300, 70), (3, 0)])
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+@pytest.mark.parametrize("c,per_token", [(0.0, False), (0.05, False), (0.3, True)])
+def test_policy_loss(B, S, reduction, c, per_token):
+    say(f"policy_loss {B} {S} {reduction} {c} {per_token}")
+    lp = -randn(B, S, seed=50).abs()
+    old, ref = lp + 0.3 * randn(B, S, seed=51), lp + 0.4 * randn(B, S, seed=52)
+    adv = randn(B, S, seed=53) if per_token else randn(B, seed=53)
+    for mask in (ragged(B, S, 54), None, torch.zeros(B, S, dtype=torch.bool)):
+        want = policy_reference(lp, old, adv, ref if c else None, mask, 0.2, 0.28, c, reduction)
+        ins = [t.clone() for t in (lp, old, ref)]
+        if mask is not None:
+            for t in ins:
+                t[~mask] = float("nan")  # what a masked token holds has no effect
+        l, o, r = (t.to(DEV) for t in ins)
+        l.requires_grad_()
+        loss, kl, clipped = nq.policy_loss(l, o, adv.to(DEV), ref_logprobs=r if c else None,
+                                           mask=None if mask is None else mask.to(DEV), clip_low=0.2, clip_high=0.28,
+                                           kl_coef=c, reduction=reduction)
+        (g,) = torch.autograd.grad(3.0 * loss, l)
+        assert loss.shape == kl.shape == clipped.shape == () and not kl.requires_grad
+        within(loss, want[0], float(want[4].sum()) + U * want[0].abs() + 1e-14, "loss")
+        within(kl, want[1], 16 * U * want[1] + 1e-14, "kl")
+        within(clipped, want[2], U * want[2], "clipped")
+        within(g, 3 * want[3], 3 * want[4] + 4 * U * (3 * want[3]).abs(), "gradient")
+
+
+def test_policy_loss_borders_and_small_ratios():
+    """Tokens next to a clip border, KL terms of nearly equal policies, ratios that overflow."""
+    say("policy_loss borders")
+    hi = math.log1p(0.2)
+    base = torch.tensor(-3.0)
+    steps = torch.arange(-40, 41) * 2.0 ** -23
+    old = torch.full((2, 81), -3.0)
+    lp = (base.double() + hi + steps.double()).float().expand(2, 81).clone()
+    lp[1] = (base.double() + math.log1p(-0.2) + steps.double()).float()
+    adv = torch.tensor([1.0, -1.0])
+    want = policy_reference(lp, old, adv, None, None, 0.2, 0.2, 0.0, "token")
+    l = lp.to(DEV).requires_grad_()
+    loss, _, clipped = nq.policy_loss(l, old.to(DEV), adv.to(DEV))
+    (g,) = torch.autograd.grad(loss, l)
+    assert 0 < float(want[2]) < 1
+    within(clipped, want[2], U, "share at the border")
+    within(g, want[3], want[4] + 4 * U * want[3].abs(), "gradient at the border")
+    # e^q - q - 1 of q from 2^-20 to 8, both signs
+    q = torch.cat([2.0 ** torch.arange(-20, 3.1, 0.1), -2.0 ** torch.arange(-20, 3.1, 0.1)])
+    for i in range(0, len(q), 20):
+        lp = torch.zeros(1, len(q[i:i + 20]))
+        ref = q[i:i + 20].float()[None]
+        want = policy_reference(lp, lp, torch.zeros(1), ref, None, 0.2, 0.2, 1.0, "token")
+        l = lp.to(DEV).requires_grad_()
+        loss, kl, _ = nq.policy_loss(l, lp.to(DEV), torch.zeros(1, device=DEV), ref_logprobs=ref.to(DEV), kl_coef=1.0)
+        (g,) = torch.autograd.grad(loss, l)
+        within(kl, want[1], 16 * U * want[1], "kl")
+        within(g, want[3], 8 * U * want[3].abs(), "kl gradient")
+    # ratios that overflow: the clip decides where it applies, infinity where it does not
+    l = torch.zeros(2, 2, device=DEV, requires_grad=True)
+    o = torch.full((2, 2), -200.0, device=DEV)
+    loss, _, clipped = nq.policy_loss(l[:1].detach(), o[:1], torch.ones(1, device=DEV))
+    assert abs(float(loss) + 1.2) < 1e-6 and float(clipped) == 1
+    assert float(nq.policy_loss(l[:1].detach(), o[:1], -torch.ones(1, device=DEV))[0]) == float("inf")
+
+
+def test_policy_loss_strides_and_refusals():
+    say("policy_loss strides, refusals")
+    lp = -randn(4, 20, seed=56).abs()
+    old = lp + 0.2 * randn(4, 20, seed=57)
+    adv, m = randn(8, seed=58), ragged(4, 20, 59)
+    want = policy_reference(lp[:, 3:], old[:, 3:], adv[::2], None, m[:, 3:], 0.2, 0.2, 0.0, "sequence")
+    l = lp.to(DEV).requires_grad_()
+    loss, *_ = nq.policy_loss(l[:, 3:], old.t().contiguous().to(DEV).t()[:, 3:], adv.to(DEV)[::2], mask=m.to(DEV)[:, 3:].float(),
+                              reduction="sequence")
+    (g,) = torch.autograd.grad(loss, l)
+    within(loss, want[0], float(want[4].sum()) + U * want[0].abs(), "strided")
+    within(g[:, 3:], want[3], want[4] + 4 * U * want[3].abs(), "strided gradient")
+    assert not g[:, :3].any()
+    x, a = torch.zeros(3, 5, device=DEV), torch.zeros(3, device=DEV)
+    bad = [(ValueError, dict(clip_low=1.5)), (ValueError, dict(clip_low=-0.1)), (ValueError, dict(clip_high=float("nan"))),
+           (ValueError, dict(kl_coef=0.1)), (ValueError, dict(reduction="sum")), (ValueError, dict(mask=x[:2] > 0)),
+           (ValueError, dict(ref_logprobs=x[:, :2])), (TypeError, dict(ref_logprobs=x.half())),
+           (RuntimeError, dict(mask=x.cpu() > 0)), (ValueError, dict(kl_coef=float("inf"), ref_logprobs=x))]
+    for err, kw in bad:
+        with pytest.raises(err):
+            nq.policy_loss(x, x, a, **kw)
+    for args in ((x[0], x[0], a), (x[:0], x[:0], a[:0]), (x, x[:2], a), (x, x, a[:2]), (x, x, x[:, :2]), (x.half(), x, a),
+                 (x.cpu(), x.cpu(), a.cpu())):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            nq.policy_loss(*args)
+
+
+# ---------------------------------------------------------------- streams, graphs, bits
+
+def test_losses_on_another_stream_and_twice():
+    """On a stream of their own, beside the same calls on another, each call's bits are those of the call alone."""
+    say("losses on streams")
+    x = randn(64, 30011, seed=60, dtype=BF).to(DEV)
+    y = torch.randint(0, 30011, (64,), device=DEV)
+    m = ragged(32, 2, 61).to(DEV)
+
+    def step():
+        leaf = x.detach().requires_grad_()
+        lp = nq.token_logprobs(leaf, y)
+        loss, *_ = nq.preference_loss(lp[:32, None].expand(32, 2), lp[32:, None].expand(32, 2), chosen_mask=m)
+        pol, *_ = nq.policy_loss(lp.view(8, 8), lp.detach().view(8, 8) + 0.1, torch.ones(8, device=DEV))
+        return [loss.detach(), pol.detach(), lp.detach(), *torch.autograd.grad(loss + pol, leaf)]
+
+    want = step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(2):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step())
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_losses_in_a_graph():
+    """Forward and backward captured, replayed on new inputs with eager work between."""
+    say("losses in a HIP graph")
+    B, S, V = 6, 11, 5003
+    x = torch.empty(2 * B, S, V, device=DEV, dtype=BF, requires_grad=True)
+    y = torch.empty(2 * B, S, device=DEV, dtype=torch.long)
+    ref = torch.empty(2 * B, S, device=DEV)
+
+    def fill(i):
+        with torch.no_grad():
+            x.copy_(randn(2 * B, S, V, seed=70 + i, dtype=BF, scale=2))
+            y.copy_(torch.randint(-1, V, (2 * B, S), generator=torch.Generator().manual_seed(80 + i)))
+            y.masked_fill_(y == -1, -100)
+            ref.copy_(-randn(2 * B, S, seed=90 + i).abs() * 10)
+
+    def step():
+        lp = nq.token_logprobs(x, y)
+        keep = y != -100
+        loss, rc, rr = nq.preference_loss(lp[:B], lp[B:], ref[:B], ref[B:], chosen_mask=keep[:B], rejected_mask=keep[B:])
+        pol, kl, cut = nq.policy_loss(lp, ref, ref[:, 0], ref_logprobs=ref, mask=keep, kl_coef=1e-3)
+        grads = torch.autograd.grad(loss + pol, x)
+        return [t.detach() for t in (loss, rc, rr, pol, kl, cut, *grads)]
+
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(3):
+        fill(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
