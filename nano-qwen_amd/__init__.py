@@ -37,7 +37,7 @@ from .model import ModelConfig, Qwen3Model, TransformerBlock
 from .generate import TextGenerator, generate_greedy_batch
 from .ops import attention_backward, attention_merge_, qk_norm_rope_backward
 from .autograd import attention_core, flash_attention_train
-from .losses import policy_loss, preference_loss, token_logprobs
+from .losses import linear_logprobs, policy_loss, preference_loss, token_logprobs
 from .ring import RingAttention, ring_attention_all_ranks, ring_schedule, ring_step, split_sequence
 
 __all__ = [
@@ -48,5 +48,5 @@ __all__ = [
     "PagedKVCache", "attention_decode_paged", "kv_append_paged",
     "attention_merge_", "RingAttention", "ring_step", "ring_schedule", "split_sequence",
     "ring_attention_all_ranks", "attention_backward", "qk_norm_rope_backward", "attention_core",
-    "flash_attention_train", "token_logprobs", "preference_loss", "policy_loss",
+    "flash_attention_train", "token_logprobs", "linear_logprobs", "preference_loss", "policy_loss",
 ]

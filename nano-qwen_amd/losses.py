@@ -1,6 +1,7 @@
-"""What a model is trained with, on the kernels: from its logits to a scalar loss.
+"""What a model is trained with, on the kernels: from its hidden states to a scalar loss.
 
-``token_logprobs`` gives the log-probability of each label; ``preference_loss`` and
+``token_logprobs`` gives the log-probability of each label, ``linear_logprobs`` the same from
+the last hidden states and the LM head without the logits; ``preference_loss`` and
 ``policy_loss`` take such log-probabilities, those of a reference or an earlier policy
 and a mask, and give a scalar.  Each has its gradient as a kernel.  They serve the
 reference's preference and policy training (its training/ loops), which composes the
@@ -14,7 +15,6 @@ gradients of gradients raise, as they do for the attention kernels.
 from __future__ import annotations
 
 import math
-from contextlib import nullcontext
 from typing import Optional, Tuple
 
 import torch
@@ -22,16 +22,28 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 
-__all__ = ["token_logprobs", "preference_loss", "policy_loss"]
+__all__ = ["token_logprobs", "linear_logprobs", "preference_loss", "policy_loss"]
 
 IGNORE_INDEX = -100
 
 _KINDS = {"sigmoid": _lib.NQ_PREF_SIGMOID, "hinge": _lib.NQ_PREF_HINGE, "ipo": _lib.NQ_PREF_IPO}
 
 
-def _on(t: torch.Tensor):
-    """A launch goes to the current device: make it the operands'."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+# The device takes less than the host for most of these calls, and the backward's Python runs
+# on autograd's own thread, where it takes some three times as long as alone: operands that
+# need no gradient go through ``apply`` as one tuple, and little stands around a launch.
+
+def _launch(t: torch.Tensor, fn, name: str, *args) -> None:
+    """fn(*args, stream) on t's device (a launch goes to the current one)."""
+    index = t.get_device()
+    args += (torch._C._cuda_getCurrentRawStream(index),)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _first_order(backward):
@@ -44,15 +56,12 @@ def _first_order(backward):
     return call
 
 
-def _check_devices(*ts: Optional[torch.Tensor]) -> None:
-    ops._require_device(*ts)
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"the operands lie on different devices: {sorted(map(str, devices))}")
-
-
-def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _check_devices(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    ops._require_device(first, *others)
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"the operands lie on different devices: {first.device} and {t.device}")
 
 
 def _check_temperature(temperature: float) -> float:
@@ -95,33 +104,32 @@ def _rows_2d(x: torch.Tensor):
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, temperature: float, ignore_index: int):
+    def forward(ctx, logits, rest):
+        labels, temperature, ignore_index = rest
         x, B, S, bs, rs = _rows_2d(logits)
         V = x.shape[-1]
-        out = torch.empty(labels.shape, dtype=torch.float32, device=x.device)
-        stats = torch.empty(B * S, 2, dtype=torch.float32, device=x.device)
+        out = x.new_empty(labels.shape, dtype=torch.float32)
+        stats = x.new_empty((B * S, 2), dtype=torch.float32)
         lib = _lib.load()
-        ws = _workspace(lib.nq_token_logprobs_workspace_bytes(B * S, V), x.device)
-        with _on(x):
-            _lib.check(lib.nq_token_logprobs(ops._ptr(x), bs, rs, ops._ptr(labels), ops._ptr(out), ops._ptr(stats),
-                                             ops._ptr(ws), ws.numel() if ws is not None else 0, B, S, V, ops._code(x),
-                                             temperature, ignore_index, ops._stream(x)), "nq_token_logprobs")
+        nbytes = lib.nq_token_logprobs_workspace_bytes(B * S, V)
+        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        tail = (B, S, V, ops._code(x), temperature, ignore_index)
+        _launch(x, lib.nq_token_logprobs, "nq_token_logprobs", ops._ptr(x), bs, rs, ops._ptr(labels), ops._ptr(out),
+                ops._ptr(stats), ops._ptr(ws), nbytes, *tail)
         ctx.save_for_backward(logits, labels, stats)
-        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        ctx.tail = tail
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, dy):
         logits, labels, stats = ctx.saved_tensors
-        x, B, S, bs, rs = _rows_2d(logits)
+        x, _, _, bs, rs = _rows_2d(logits)
         dy = dy.contiguous()
-        dx = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
-        with _on(x):
-            _lib.check(_lib.load().nq_token_logprobs_bwd(
-                ops._ptr(x), bs, rs, ops._ptr(labels), ops._ptr(stats), ops._ptr(dy), ops._ptr(dx), B, S, x.shape[-1],
-                ops._code(x), ctx.temperature, ctx.ignore_index, ops._stream(x)), "nq_token_logprobs_bwd")
-        return dx, None, None, None
+        dx = x.new_empty(logits.shape)
+        _launch(x, _lib.load().nq_token_logprobs_bwd, "nq_token_logprobs_bwd", ops._ptr(x), bs, rs, ops._ptr(labels),
+                ops._ptr(stats), ops._ptr(dy), ops._ptr(dx), *ctx.tail)
+        return dx, None
 
 
 def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: float = 1.0,
@@ -146,7 +154,82 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
     temperature = _check_temperature(temperature)
     if labels.numel() == 0:
         return logits.sum(-1).float()  # empty, with logits' place in the graph
-    return _TokenLogprobs.apply(logits, labels, temperature, int(ignore_index))
+    return _TokenLogprobs.apply(logits, (labels, temperature, int(ignore_index)))
+
+
+class _LinearLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, rest):
+        labels, temperature, ignore_index = rest
+        x, w, B, S, bs, rs = _head_operands(hidden, weight)
+        V, H = w.shape
+        out = x.new_empty(labels.shape, dtype=torch.float32)
+        stats = x.new_empty((B * S, 2), dtype=torch.float32)
+        lib = _lib.load()
+        ws = x.new_empty(lib.nq_linear_logprobs_workspace_bytes(B * S, V, H), dtype=torch.uint8)
+        _launch(x, lib.nq_linear_logprobs, "nq_linear_logprobs", x.data_ptr(), bs, rs, w.data_ptr(), labels.data_ptr(),
+                out.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(), B, S, V, H, temperature, ignore_index)
+        ctx.save_for_backward(hidden, weight, labels, stats)
+        ctx.tail = temperature, ignore_index
+        return out
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, dy):
+        hidden, weight, labels, stats = ctx.saved_tensors
+        x, w, B, S, bs, rs = _head_operands(hidden, weight)
+        V, H = w.shape
+        dy = dy.contiguous()
+        dh = x.new_empty(hidden.shape) if ctx.needs_input_grad[0] else None
+        dw = w.new_empty((V, H)) if ctx.needs_input_grad[1] else None
+        lib = _lib.load()
+        ws = x.new_empty(lib.nq_linear_logprobs_bwd_workspace_bytes(B * S, V, H), dtype=torch.uint8)
+        _launch(x, lib.nq_linear_logprobs_bwd, "nq_linear_logprobs_bwd", x.data_ptr(), bs, rs, w.data_ptr(),
+                labels.data_ptr(), stats.data_ptr(), dy.data_ptr(), ops._ptr(dh), ops._ptr(dw), ws.data_ptr(),
+                ws.numel(), B, S, V, H, *ctx.tail)
+        return dh, dw, None
+
+
+def _head_operands(hidden: torch.Tensor, weight: torch.Tensor):
+    """(hidden, weight, B, S, batch stride, row stride), copied where rows are not 16-byte aligned."""
+    x, B, S, bs, rs = _rows_2d(hidden)
+    if bs % 8 or rs % 8 or x.data_ptr() % 16:
+        x, B, S, bs, rs = _rows_2d(hidden.contiguous().clone() if hidden.is_contiguous() else hidden.contiguous())
+    w = weight.contiguous()
+    return x, w if w.data_ptr() % 16 == 0 else w.clone(), B, S, bs, rs
+
+
+def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, temperature: float = 1.0,
+                    ignore_index: int = IGNORE_INDEX) -> torch.Tensor:
+    """``token_logprobs(hidden @ weight.T, labels)`` without the logits, fp32 and shaped like ``labels``.
+
+    hidden: (..., H) bf16 hidden states, rows at any strides; weight: (V, H) bf16, an LM
+    head's; H a multiple of 8.  Logits are held in fp32 and never stored; the backward forms
+    their gradient again from two numbers a row, in bf16, a range of the vocabulary at a time
+    (at most 1 GiB), and gives hidden and weight gradients summed in fp32.  Rows whose label
+    is ``ignore_index`` take no part in the products.  Labels outside [0, V) give NaN, and so
+    do their row's and the weight's gradients.  An fp32 head goes through its logits:
+    ``token_logprobs(F.linear(hidden, weight), labels)``.
+    """
+    _check_devices(hidden, weight, labels)
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError(f"hidden and weight must be bfloat16, got {hidden.dtype} and {weight.dtype}; "
+                        "token_logprobs takes the logits of other types")
+    if hidden.dim() == 0 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden {tuple(hidden.shape)} must be (..., H) and weight {tuple(weight.shape)} (V, H)")
+    V, H = weight.shape
+    if V == 0 or H == 0 or H % 8:
+        raise ValueError(f"the kernels take at least one entry and widths that are multiples of 8, got {V} and {H}")
+    labels = _check_labels(labels, hidden.shape[:-1])
+    temperature = _check_temperature(temperature)
+    if labels.numel() == 0:
+        return torch.nn.functional.linear(hidden, weight)[..., 0].float()  # empty, with its place in the graph
+    if labels.numel() > _HEAD_MOST or V > _HEAD_MOST:
+        raise ValueError(f"at most 2^24 rows and entries in one call, got {labels.numel()} and {V}")
+    return _LinearLogprobs.apply(hidden, weight, (labels, temperature, int(ignore_index)))
+
+
+_HEAD_MOST = 1 << 24
 
 
 # ---------------------------------------------------------------------------
@@ -177,30 +260,30 @@ def _mask_rows(mask: Optional[torch.Tensor], name: str, shape) -> Optional[torch
     return _rows(mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0)
 
 
-def _pitch(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.stride(0)
+def _with_pitch(*ts: Optional[torch.Tensor]):
+    """Pointer and row stride of each."""
+    args = ()
+    for t in ts:
+        args += (None, 0) if t is None else (t.data_ptr(), t.stride(0))
+    return args
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, kind: int, beta: float,
-                smoothing: float, average: bool):
-        (B, Sc), Sr, dev = chosen.shape, rejected.shape[1], chosen.device
-        new = torch.empty
-        loss = new((), dtype=torch.float32, device=dev)
-        reward_c, reward_r = (new(B, dtype=torch.float32, device=dev) for _ in range(2))
-        coef = new(2, B, dtype=torch.float32, device=dev)
+    def forward(ctx, chosen, rejected, rest):
+        ref_chosen, ref_rejected, chosen_mask, rejected_mask, kind, beta, smoothing, average = rest
+        (B, Sc), Sr = chosen.shape, rejected.shape[1]
+        loss, reward_c, reward_r = chosen.new_empty(()), chosen.new_empty(B), chosen.new_empty(B)
         lib = _lib.load()
-        ws = _workspace(lib.nq_preference_loss_workspace_bytes(B), dev)
-        p = ops._ptr
-        with _on(chosen):
-            _lib.check(lib.nq_preference_loss(
-                p(chosen), _pitch(chosen), p(rejected), _pitch(rejected), p(ref_chosen), _pitch(ref_chosen),
-                p(ref_rejected), _pitch(ref_rejected), p(chosen_mask), _pitch(chosen_mask), p(rejected_mask),
-                _pitch(rejected_mask), p(loss), p(reward_c), p(reward_r), p(coef), p(ws), ws.numel(), B, Sc, Sr, kind,
-                beta, smoothing, int(average), ops._stream(chosen)), "nq_preference_loss")
+        nbytes = lib.nq_preference_loss_workspace_bytes(B)
+        coef = chosen.new_empty((2, B))
+        ws = chosen.new_empty(nbytes, dtype=torch.uint8)
+        _launch(chosen, lib.nq_preference_loss, "nq_preference_loss",
+                *_with_pitch(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask), loss.data_ptr(),
+                reward_c.data_ptr(), reward_r.data_ptr(), coef.data_ptr(), ws.data_ptr(), nbytes, B, Sc, Sr, kind,
+                beta, smoothing, average)
         ctx.save_for_backward(coef, chosen_mask, rejected_mask)
-        ctx.lens = Sc, Sr
+        ctx.sizes = B, Sc, Sr
         ctx.mark_non_differentiable(reward_c, reward_r)
         ctx.set_materialize_grads(False)  # no zeros for the rewards' gradients
         return loss, reward_c, reward_r
@@ -209,17 +292,15 @@ class _PreferenceLoss(torch.autograd.Function):
     @_first_order
     def backward(ctx, dloss, *_):
         if dloss is None:
-            return (None,) * 10
+            return None, None, None
         coef, chosen_mask, rejected_mask = ctx.saved_tensors
-        (Sc, Sr), B = ctx.lens, coef.shape[1]
-        dc, dr = (torch.empty(B, S, dtype=torch.float32, device=coef.device) if need else None
-                  for S, need in zip((Sc, Sr), ctx.needs_input_grad))
-        p = ops._ptr
-        with _on(coef):
-            _lib.check(_lib.load().nq_preference_loss_bwd(
-                p(coef), p(dloss), p(chosen_mask), _pitch(chosen_mask), p(rejected_mask), _pitch(rejected_mask), p(dc),
-                p(dr), B, Sc, Sr, ops._stream(coef)), "nq_preference_loss_bwd")
-        return dc, dr, None, None, None, None, None, None, None, None
+        B, Sc, Sr = ctx.sizes
+        need = ctx.needs_input_grad
+        dc = coef.new_empty((B, Sc)) if need[0] else None
+        dr = coef.new_empty((B, Sr)) if need[1] else None
+        _launch(coef, _lib.load().nq_preference_loss_bwd, "nq_preference_loss_bwd", coef.data_ptr(), dloss.data_ptr(),
+                *_with_pitch(chosen_mask, rejected_mask), ops._ptr(dc), ops._ptr(dr), B, Sc, Sr)
+        return dc, dr, None
 
 
 def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: Optional[torch.Tensor] = None,
@@ -260,9 +341,9 @@ def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: Op
     sc, sr = chosen.shape, rejected.shape
     return _PreferenceLoss.apply(
         _token_rows(chosen, "chosen", sc), _token_rows(rejected, "rejected", sr),
-        _token_rows(_detached(ref_chosen), "ref_chosen", sc), _token_rows(_detached(ref_rejected), "ref_rejected", sr),
-        _mask_rows(chosen_mask, "chosen_mask", sc), _mask_rows(rejected_mask, "rejected_mask", sr),
-        _KINDS[kind], float(beta), float(label_smoothing), bool(average))
+        (_token_rows(_detached(ref_chosen), "ref_chosen", sc), _token_rows(_detached(ref_rejected), "ref_rejected", sr),
+         _mask_rows(chosen_mask, "chosen_mask", sc), _mask_rows(rejected_mask, "rejected_mask", sr),
+         _KINDS[kind], float(beta), float(label_smoothing), int(bool(average))))
 
 
 def _detached(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -271,19 +352,19 @@ def _detached(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, lp, old, ref, adv, mask, low: float, high: float, kl_coef: float, mean_of_means: bool):
-        (B, S), dev = lp.shape, lp.device
-        loss, kl, clipped = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
-        weight = torch.empty(B, dtype=torch.float32, device=dev)
+    def forward(ctx, lp, rest):
+        old, ref, adv, mask, low, high, kl_coef, mean_of_means = rest
+        B, S = lp.shape
+        loss, kl, clipped = lp.new_empty(()), lp.new_empty(()), lp.new_empty(())
+        weight = lp.new_empty(B)
         lib = _lib.load()
-        ws = _workspace(lib.nq_policy_loss_workspace_bytes(B, S), dev)
+        nbytes = lib.nq_policy_loss_workspace_bytes(B, S)
+        ws = lp.new_empty(nbytes, dtype=torch.uint8)
+        _launch(lp, lib.nq_policy_loss, "nq_policy_loss", *_with_pitch(lp, old, ref, adv), adv.dim() - 1,
+                *_with_pitch(mask), loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(), weight.data_ptr(),
+                ws.data_ptr(), nbytes, B, S, low, high, kl_coef, mean_of_means)
         ctx.save_for_backward(lp, old, ref, adv, mask, weight)
-        ctx.clip = low, high, kl_coef
-        p = ops._ptr
-        with _on(lp):
-            _lib.check(lib.nq_policy_loss(
-                *_policy_operands(lp, old, ref, adv, mask), p(loss), p(kl), p(clipped), p(weight), p(ws), ws.numel(),
-                B, S, low, high, kl_coef, int(mean_of_means), ops._stream(lp)), "nq_policy_loss")
+        ctx.tail = B, S, low, high, kl_coef
         ctx.mark_non_differentiable(kl, clipped)
         ctx.set_materialize_grads(False)
         return loss, kl, clipped
@@ -292,22 +373,12 @@ class _PolicyLoss(torch.autograd.Function):
     @_first_order
     def backward(ctx, dloss, *_):
         if dloss is None:
-            return (None,) * 9
+            return None, None
         lp, old, ref, adv, mask, weight = ctx.saved_tensors
-        B, S = lp.shape
-        grad = torch.empty(B, S, dtype=torch.float32, device=lp.device)
-        p = ops._ptr
-        with _on(lp):
-            _lib.check(_lib.load().nq_policy_loss_bwd(
-                *_policy_operands(lp, old, ref, adv, mask), p(weight), p(dloss), p(grad), B, S, *ctx.clip,
-                ops._stream(lp)), "nq_policy_loss_bwd")
-        return grad, None, None, None, None, None, None, None, None
-
-
-def _policy_operands(lp, old, ref, adv, mask):
-    p = ops._ptr
-    return (p(lp), _pitch(lp), p(old), _pitch(old), p(ref), _pitch(ref), p(adv), adv.stride(0), int(adv.dim() == 2),
-            p(mask), _pitch(mask))
+        grad = weight.new_empty(lp.shape)
+        _launch(weight, _lib.load().nq_policy_loss_bwd, "nq_policy_loss_bwd", *_with_pitch(lp, old, ref, adv),
+                adv.dim() - 1, *_with_pitch(mask), weight.data_ptr(), dloss.data_ptr(), grad.data_ptr(), *ctx.tail)
+        return grad, None
 
 
 def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *,
@@ -348,6 +419,7 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
     else:
         adv = _token_rows(adv, "advantages", shape)
     return _PolicyLoss.apply(
-        _token_rows(logprobs, "logprobs", shape), _token_rows(_detached(old_logprobs), "old_logprobs", shape),
-        _token_rows(_detached(ref_logprobs), "ref_logprobs", shape), adv, _mask_rows(mask, "mask", shape),
-        float(clip_low), float(clip_high), float(kl_coef), reduction == "sequence")
+        _token_rows(logprobs, "logprobs", shape),
+        (_token_rows(_detached(old_logprobs), "old_logprobs", shape),
+         _token_rows(_detached(ref_logprobs), "ref_logprobs", shape), adv, _mask_rows(mask, "mask", shape),
+         float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence")))

@@ -31,6 +31,7 @@ import torch.utils.checkpoint as checkpoint_utils
 from . import _lib, ops
 from .attention import Attention, KVCache
 from .config import AttentionConfig
+from .losses import linear_logprobs, token_logprobs
 from .norm import LayerRMSNormFn, layer_rms_norm, plain_rms_norm
 
 
@@ -216,10 +217,8 @@ class Qwen3Model(nn.Module):
             layer.attention.rope_positions = "cache" if fixed else "reference"
             layer.attention.cache_prefill_causal = bool(fixed)
 
-    def forward(self, input_ids: torch.Tensor, position_ids: Optional[torch.Tensor] = None,
-                attention_mask: Optional[torch.Tensor] = None,
-                kv_caches: Optional[List[KVCache]] = None,
-                labels: Optional[torch.Tensor] = None) -> dict:
+    def _trunk(self, input_ids: torch.Tensor, position_ids: Optional[torch.Tensor],
+               attention_mask: Optional[torch.Tensor], kv_caches: Optional[List[KVCache]]) -> torch.Tensor:
         hidden_states = self.embed(input_ids)
         for i, layer in enumerate(self.layers):
             kv_cache = kv_caches[i] if kv_caches is not None else None
@@ -231,13 +230,35 @@ class Qwen3Model(nn.Module):
                     layer, hidden_states, position_ids, attention_mask, kv_cache, use_reentrant=False)
             else:
                 hidden_states, _ = layer(hidden_states, position_ids, attention_mask, kv_cache)
-        hidden_states = self.norm(hidden_states)
+        return self.norm(hidden_states)
+
+    def forward(self, input_ids: torch.Tensor, position_ids: Optional[torch.Tensor] = None,
+                attention_mask: Optional[torch.Tensor] = None,
+                kv_caches: Optional[List[KVCache]] = None,
+                labels: Optional[torch.Tensor] = None) -> dict:
+        hidden_states = self._trunk(input_ids, position_ids, attention_mask, kv_caches)
         logits = self.lm_head(hidden_states)
         loss = None
         if labels is not None:
             loss = F.cross_entropy(logits[..., :-1, :].contiguous().view(-1, logits.shape[-1]),
                                    labels[..., 1:].contiguous().view(-1), ignore_index=-100)
         return {"logits": logits, "loss": loss, "aux_loss": None, "hidden_states": hidden_states}
+
+    def token_logprobs(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
+                       position_ids: Optional[torch.Tensor] = None,
+                       attention_mask: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
+        """The log-probability of each token given those before it, (B, S - 1) fp32.
+
+        labels (B, S), ``input_ids`` by default, are shifted as in ``forward``: entry [b, s]
+        is that of ``labels[b, s + 1]``, 0 where the label is -100.  What the preference and
+        policy losses take, without the logits: a bf16 LM head goes through
+        ``losses.linear_logprobs``, another through its logits."""
+        hidden = self._trunk(input_ids, position_ids, attention_mask, None)[:, :-1]
+        labels = (input_ids if labels is None else labels)[:, 1:]
+        weight = self.lm_head.weight
+        if hidden.dtype == weight.dtype == torch.bfloat16 and weight.shape[1] % 8 == 0:
+            return linear_logprobs(hidden, weight, labels, temperature=temperature)
+        return token_logprobs(self.lm_head(hidden), labels, temperature=temperature)
 
     @torch.no_grad()
     def count_parameters(self) -> dict:
