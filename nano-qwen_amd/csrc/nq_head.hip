@@ -21,20 +21,52 @@
 
 namespace nq {
 
-constexpr int HD_BM = 256;  // a tile's extent on the MFMA's row axis
-constexpr int HD_BK = 64;   // depth of a step
-constexpr int HD_WAVES = 8;
-constexpr int HD_PREP = 64;  // rows of a gathering workgroup
+constexpr int HD_BK = 64;    // depth of a step
+constexpr int HD_PREP = 16;  // rows of a gathering workgroup
+constexpr int HD_CUS = 256;
 
-// ---------------------------------------------------------------------------
-// The kept rows, in order: pos[row] = its place among them (-1: ignored), index the
-// reverse, hc their hidden states.  A workgroup counts the kept rows before its own 64 (the
-// labels are small and in L2) rather than wait for another launch.
-struct HeadRows {
+// A product's tile, BM (the MFMA's row axis) x BN, and how its waves share it: M x N of
+// them, each MT x NT blocks of 32 x 32.  OUT: rows that a wave puts out at a time.
+//   Wide  one workgroup a CU: 128 accumulator registers a lane, 128 KB of operands
+//   Few   at most 64 tokens, bound by reading the weights: three workgroups a CU, so that
+//         72 KB of them are in flight there
+struct Wide {
+  static constexpr int BM = 256, BN = 256, M = 2, N = 4, MT = 4, NT = 2, PER_CU = 1, OUT = 32;
+};
+struct Few {
+  static constexpr int BM = 128, BN = 64, M = 4, N = 1, MT = 1, NT = 2, PER_CU = 3, OUT = 16;
+};
+template <class C> constexpr int threads_of() { return C::M * C::N * 64; }
+
+// The rows as the caller holds them; for at most 64 a workgroup finds the kept ones by itself.
+struct HeadSource {
   const bf16* hidden;
   int64_t bs, rs, S;
   const int64_t* labels;
   int64_t rows, ignore;
+  __device__ __forceinline__ const bf16* row(int64_t r) const {
+    const int64_t b = r / S;
+    return hidden + b * bs + (r - b * S) * rs;
+  }
+  // by one wave: index[place] of each kept row; how many there are
+  __device__ __forceinline__ int few(int lane, int V, int* index, int* target) const {
+    const int64_t y = lane < rows ? labels[lane] : ignore;
+    const uint64_t kept = __builtin_amdgcn_ballot_w64(y != ignore);
+    if (y != ignore) {
+      const int place = __popcll(kept & ((1ull << lane) - 1));
+      index[place] = lane;
+      target[place] = y >= 0 && y < V ? (int)y : -1;
+    }
+    return __popcll(kept);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// The kept rows, in order: pos[row] = its place among them (-1: ignored), index the
+// reverse, hc their hidden states.  A workgroup counts the kept rows before its own 16 (the
+// labels are small and in L2) rather than wait for another launch.
+struct HeadRows {
+  HeadSource src;
   int H, V;
   int* count;
   int* pos;       // (rows)
@@ -44,7 +76,6 @@ struct HeadRows {
   // forward
   float* logprobs;
   floatx2* stats;
-  float* zlabel;  // (rows) by place
   // backward
   const float* dy;
   floatx4* coef;  // (rows) by place: m, -g / l, g = dy / T
@@ -56,7 +87,8 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r0 = (int64_t)blockIdx.x * HD_PREP;
   int n = 0;
-  for (int64_t r = tid; r < r0; r += 256) n += p.labels[r] != p.ignore;
+#pragma unroll 8
+  for (int64_t r = tid; r < r0; r += 256) n += p.src.labels[r] != p.src.ignore;
 #pragma unroll
   for (int k = 32; k >= 1; k >>= 1) n += __shfl_xor(n, k, 64);
   if (lane == 0) before[wave] = n;
@@ -64,18 +96,18 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows p) {
   const int base = before[0] + before[1] + before[2] + before[3];
   if (wave == 0) {
     const int64_t r = r0 + lane;
-    const int64_t y = r < p.rows ? p.labels[r] : p.ignore;
-    const bool kept = y != p.ignore;
+    const bool here = lane < HD_PREP && r < p.src.rows;
+    const int64_t y = here ? p.src.labels[r] : p.src.ignore;
+    const bool kept = y != p.src.ignore;
     const uint64_t ballot = __builtin_amdgcn_ballot_w64(kept);
     const int place = kept ? base + __popcll(ballot & ((1ull << lane) - 1)) : -1;
-    own[lane] = place;
-    if (r < p.rows) {
+    if (here) {
+      own[lane] = place;
       p.pos[r] = place;
       const bool inside = y >= 0 && y < p.V;
       if (kept) {
         p.index[place] = (int)r;
         p.target[place] = inside ? (int)y : -1;
-        if (p.zlabel) p.zlabel[place] = __builtin_nanf("");  // stays for a label outside the vocabulary
         if (p.dy) {
           const floatx2 st = p.stats[r];
           const float g = inside ? p.dy[r] * p.inv_t : __builtin_nanf("");
@@ -86,15 +118,14 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows p) {
         p.stats[r] = floatx2{0.f, 1.f};
       }
     }
-    if (r0 + HD_PREP >= p.rows && lane == 0) *p.count = base + __popcll(ballot);
+    if (r0 + HD_PREP >= p.src.rows && lane == 0) *p.count = base + __popcll(ballot);
   }
   __syncthreads();
   const int ch = p.H / 8;
-  for (int i = wave; i < HD_PREP && r0 + i < p.rows; i += 4) {
+  for (int i = wave; i < HD_PREP && r0 + i < p.src.rows; i += 4) {
     const int place = own[i];
     if (place < 0) continue;
-    const int64_t r = r0 + i, b = r / p.S;
-    const bf16x8* src = reinterpret_cast<const bf16x8*>(p.hidden + b * p.bs + (r - b * p.S) * p.rs);
+    const bf16x8* src = reinterpret_cast<const bf16x8*>(p.src.row(r0 + i));
     bf16x8* dst = reinterpret_cast<bf16x8*>(p.hc + (int64_t)place * p.H);
     for (int c = lane; c < ch; c += 64) dst[c] = src[c];
   }
@@ -110,55 +141,78 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows p) {
 //         banks.
 // HBM -> LDS without registers; what lies outside (rows past the extent, depths past the
 // end) is out of the descriptor's range and arrives as zeros.
-template <int EXT, bool ROW>
+template <int EXT, bool ROW, int WAVES>
 struct Stage {
   static constexpr int BYTES = EXT * HD_BK * 2;
-  static constexpr int NI = BYTES / 1024 / HD_WAVES;  // loads of a wave per step
-  static constexpr int LINE = ROW ? 128 : EXT * 2;    // bytes of an LDS row
+  static constexpr int NI = BYTES / 1024 / WAVES;   // loads of a wave per step
+  static constexpr int LINE = ROW ? 128 : EXT * 2;  // bytes of an LDS row
   static constexpr int ROWS_PER = 1024 / LINE;
-  const char* base;   // ROW: first row, else first depth
-  uint32_t line;      // bytes of a row in memory
-  uint32_t range;     // ROW: bytes from base to the end of the last row
-  int64_t extent;     // !ROW: columns from base that exist (bytes), so that none past a line's end is read
-  int depth;          // how many depths exist
+  static_assert(BYTES % (1024 * WAVES) == 0 && (WAVES * ROWS_PER) % 16 == 0, "a wave's loads keep their swizzle");
+  const char* base;  // ROW: first row, else first depth
+  uint32_t line;     // bytes of a row in memory
+  uint32_t range;    // ROW: bytes from base to the end of the last row; else of the columns that exist
+  int depth;         // how many depths exist
   uint32_t off, chunk;
 
-  // rows [e0, e0 + EXT) of `extent` rows of `ld` elements; depths [0, depth)
-  __device__ __forceinline__ void init(const bf16* p, int64_t ld, int64_t e0, int64_t n, int depth_, int wave,
-                                       int lane) {
+  __device__ __forceinline__ void lanes(int64_t ld, int wave, int lane) {
     line = (uint32_t)(ld * 2);
-    depth = depth_;
     const int r = wave * ROWS_PER + lane / (LINE / 16), pc = lane % (LINE / 16);
+    chunk = ROW ? (uint32_t)((pc ^ ((r >> 1) & 7)) * 16) : (uint32_t)((pc ^ ((r & 3) << 2)) * 16);
+    off = (uint32_t)r * line + chunk;
+  }
+  // extents [e0, e0 + EXT) of n, of depths [0, d)
+  __device__ __forceinline__ void at(const bf16* p, int64_t e0, int64_t n, int d) {
+    depth = d;
+    const int64_t left = n - e0;
     if (ROW) {
-      const int64_t left = n - e0;
-      base = reinterpret_cast<const char*>(p + e0 * ld);
+      base = reinterpret_cast<const char*>(p) + e0 * line;
       range = left <= 0 ? 0 : (uint32_t)((left < EXT ? left : EXT) * (int64_t)line);
-      chunk = (uint32_t)((pc ^ ((r >> 1) & 7)) * 8);  // first depth of the chunk
-      off = (uint32_t)r * line + chunk * 2;
     } else {
       base = reinterpret_cast<const char*>(p + e0);
-      extent = (n - e0) * 2;
-      chunk = (uint32_t)((pc ^ ((r & 3) << 2)) * 16);  // byte of the chunk in its line
-      off = (uint32_t)r * line + chunk;
+      range = left <= 0 ? 0 : (uint32_t)((left < EXT ? left : EXT) * 2);
     }
   }
   // the step at depth k0 into LDS at `tile`
   __device__ __forceinline__ void load(unsigned char* tile, int k0, int wave) const {
     constexpr uint32_t NONE = 0x80000000u;  // out of any range
+    const int left = depth - k0;
+    uint32_t o;
+    BufRsrc r;
     if (ROW) {
-      const BufRsrc r = make_rsrc(base, range);
-      const uint32_t o = k0 + (int)chunk < depth ? off + (uint32_t)k0 * 2 : NONE;
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-        buffer_load_lds16(r, tile + (wave + HD_WAVES * i) * 1024, o + (o == NONE ? 0u : i * (HD_WAVES * ROWS_PER) * line), 0u);
+      r = make_rsrc(base, range);
+      o = (int)chunk < 2 * left ? off + (uint32_t)k0 * 2 : NONE;
     } else {
-      const int left = depth - k0;
-      const BufRsrc r = make_rsrc(base + (int64_t)k0 * line, (uint32_t)(left < HD_BK ? left : HD_BK) * line);
-      const uint32_t o = (int64_t)chunk < extent ? off : NONE;
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-        buffer_load_lds16(r, tile + (wave + HD_WAVES * i) * 1024, o + (o == NONE ? 0u : i * (HD_WAVES * ROWS_PER) * line), 0u);
+      r = make_rsrc(base + (int64_t)k0 * line, (uint32_t)(left < HD_BK ? left : HD_BK) * line);
+      o = chunk < range ? off : NONE;
     }
+    const uint32_t step = o == NONE ? 0u : WAVES * ROWS_PER * line;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) buffer_load_lds16(r, tile + (wave + WAVES * i) * 1024, o + i * step, 0u);
+  }
+};
+
+// Stage<EXT, true> of rows that lie anywhere: their hidden states as the caller holds them.
+// Rows past the count repeat the first (nothing is kept of them), and depths past the end its
+// first chunk, against zeros of the other operand.
+template <int EXT, int WAVES>
+struct GatherStage {
+  static constexpr int BYTES = EXT * HD_BK * 2, NI = BYTES / 1024 / WAVES;
+  const char* row[NI];
+  int depth;
+  uint32_t chunk;
+  // row_of(r): where row r begins
+  template <typename F>
+  __device__ __forceinline__ void at(F row_of, int d, int wave, int lane) {
+    depth = d;
+    const int r = wave * 8 + lane / 8;
+    chunk = (uint32_t)(((lane % 8) ^ ((r >> 1) & 7)) * 16);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) row[i] = reinterpret_cast<const char*>(row_of(r + WAVES * 8 * i));
+  }
+  __device__ __forceinline__ void load(unsigned char* tile, int k0, int wave) const {
+    const int64_t o = (int)chunk < 2 * (depth - k0) ? (int64_t)k0 * 2 + chunk : 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) global_load_lds16(row[i] + o, tile + (wave + WAVES * i) * 1024);
   }
 };
 
@@ -182,16 +236,8 @@ struct Reads {
       }
     }
   }
-  template <int KK>
+  template <int KK, int T = 0>
   __device__ __forceinline__ void read(uint32_t buf, bf16x8 (&v)[NT]) const {
-    if constexpr (ROW) {
-      one<0, KK>(buf, v);
-    } else {
-      one<0, KK>(buf, v);
-    }
-  }
-  template <int T, int KK>
-  __device__ __forceinline__ void one(uint32_t buf, bf16x8 (&v)[NT]) const {
     if constexpr (T < NT) {
       if constexpr (ROW) {
         v[T] = lds_read_b128_nowait<T * 32 * 128>(a[KK] + buf);
@@ -203,360 +249,521 @@ struct Reads {
         const shortx8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         v[T] = __builtin_bit_cast(bf16x8, both);
       }
-      one<T + 1, KK>(buf, v);
+      read<KK, T + 1>(buf, v);
     }
   }
 };
 
-// How the eight waves share a tile of 256 x BN: each MT x NT blocks of 32 x 32.
-template <int BN> struct Waves;
-template <> struct Waves<256> { static constexpr int M = 2, N = 4, MT = 4, NT = 2; };
-template <> struct Waves<64> { static constexpr int M = 8, N = 1, MT = 1, NT = 2; };
+// A workgroup's stream of products.  Two LDS buffers: the next step's loads are in flight
+// while a step's 64 depths are multiplied, one barrier a step, and the step after a tile's
+// last is the next tile's first, so that its loads run under this tile's last products and
+// its epilogue.  The operands of the next 16 depths are read while these are multiplied.
+template <class C, bool AROW, bool BROW, bool GATHER = false>
+struct Product {
+  static constexpr int WAVES = C::M * C::N;
+  typedef Stage<C::BM, AROW, WAVES> A;
+  typedef std::conditional_t<GATHER, GatherStage<C::BN, WAVES>, Stage<C::BN, BROW, WAVES>> B;
+  static_assert(BROW || !GATHER, "rows are gathered");
+  static constexpr int BUF = A::BYTES + B::BYTES;
+  static constexpr int NB = C::MT < 2 ? C::MT : 2, CH = NB * 4;  // an output line: blocks, 16-byte chunks
+  static constexpr int OWN = C::OUT * CH * 16;  // bytes of a wave's own LDS,
+  static constexpr int PRIVATE = 2 * BUF;       // after the buffers
+  static constexpr int LDS = PRIVATE + WAVES * OWN;
+  static_assert(LDS * C::PER_CU <= 160 * 1024, "LDS of a CU");
+  typedef floatx16 Acc[C::MT][C::NT];
+  unsigned char* lds;
+  int wave, lane;
+  uint32_t cur;  // byte offset of the buffer whose step comes next
+  Reads<C::BM, AROW, C::MT> ra;
+  Reads<C::BN, BROW, C::NT> rb;
 
-// acc[mt][nt] += the wave's blocks of A B^T over `depth`.  Two LDS buffers: the next step's
-// loads are in flight while this step's 64 depths are multiplied, one barrier a step; the
-// operands of the next 16 depths are read while these are multiplied.
-template <int BN, bool AROW, bool BROW>
-__device__ __forceinline__ void head_product(unsigned char* lds, const Stage<HD_BM, AROW>& sa,
-                                             const Stage<BN, BROW>& sb, int depth, int wave, int lane,
-                                             floatx16 (&acc)[Waves<BN>::MT][Waves<BN>::NT]) {
-  using W = Waves<BN>;
-  constexpr int AB = Stage<HD_BM, AROW>::BYTES, BUF = AB + Stage<BN, BROW>::BYTES;
-  Reads<HD_BM, AROW, W::MT> ra;
-  Reads<BN, BROW, W::NT> rb;
-  ra.init(lds_addr(lds), (wave / W::N) * (W::MT * 32), lane);
-  rb.init(lds_addr(lds + AB), (wave % W::N) * (W::NT * 32), lane);
-  constexpr int PER = Reads<HD_BM, AROW, W::MT>::PER + Reads<BN, BROW, W::NT>::PER;
-  const int steps = (depth + HD_BK - 1) / HD_BK;
-  sa.load(lds, 0, wave);
-  sb.load(lds + AB, 0, wave);
-  for (int s = 0; s < steps; ++s) {
-    const uint32_t buf = (s & 1) * BUF;
-    wait_vmcnt0();
-    __syncthreads();  // the step has landed, and the other buffer's readers are done
-    __builtin_amdgcn_sched_barrier(0);
-    if (s + 1 < steps) {
-      sa.load(lds + (BUF - buf), (s + 1) * HD_BK, wave);
-      sb.load(lds + (BUF - buf) + AB, (s + 1) * HD_BK, wave);
-    }
-    bf16x8 a[2][W::MT], b[2][W::NT];
-    ra.template read<0>(buf, a[0]);
-    rb.template read<0>(buf, b[0]);
-    auto multiply = [&](int h) {
-#pragma unroll
-      for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-        for (int j = 0; j < W::NT; ++j) acc[i][j] = mfma32(a[h][i], b[h][j], acc[i][j]);
-    };
-    ra.template read<1>(buf, a[1]);
-    rb.template read<1>(buf, b[1]);
-    lgkm_wait<PER>();
-    multiply(0);
-    ra.template read<2>(buf, a[0]);
-    rb.template read<2>(buf, b[0]);
-    lgkm_wait<PER>();
-    multiply(1);
-    ra.template read<3>(buf, a[1]);
-    rb.template read<3>(buf, b[1]);
-    lgkm_wait<PER>();
-    multiply(0);
-    lgkm_wait<0>();
-    multiply(1);
+  __device__ __forceinline__ void init(unsigned char* l, int w, int ln) {
+    lds = l, wave = w, lane = ln, cur = 0;
+    ra.init(lds_addr(l), (w / C::N) * (C::MT * 32), ln);
+    rb.init(lds_addr(l + A::BYTES), (w % C::N) * (C::NT * 32), ln);
   }
-}
+  __device__ __forceinline__ void load(uint32_t buf, const A& a, const B& b, int k0) {
+    a.load(lds + buf, k0, wave);
+    b.load(lds + buf + A::BYTES, k0, wave);
+  }
+  // acc = the wave's blocks of A B^T; the first step is under way in the current buffer,
+  // and the one of (na, nb) is afterwards, if there is another tile.
+  __device__ __forceinline__ void run(const A& a, const B& b, bool more, const A& na, const B& nb, Acc& acc) {
+#pragma unroll
+    for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j) acc[i][j] = floatx16{};
+    constexpr int PER = Reads<C::BM, AROW, C::MT>::PER + Reads<C::BN, BROW, C::NT>::PER;
+    for (int k = 0; k < a.depth; k += HD_BK) {
+      wait_vmcnt0();
+      __syncthreads();  // the step has landed, and the other buffer's readers are done
+      __builtin_amdgcn_sched_barrier(0);
+      if (k + HD_BK < a.depth) load(BUF - cur, a, b, k + HD_BK);
+      else if (more) load(BUF - cur, na, nb, 0);
+      bf16x8 x[2][C::MT], y[2][C::NT];
+      auto multiply = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+          for (int j = 0; j < C::NT; ++j) acc[i][j] = mfma32(x[h][i], y[h][j], acc[i][j]);
+      };
+      ra.template read<0>(cur, x[0]);
+      rb.template read<0>(cur, y[0]);
+      ra.template read<1>(cur, x[1]);
+      rb.template read<1>(cur, y[1]);
+      lgkm_wait<PER>();
+      multiply(0);
+      ra.template read<2>(cur, x[0]);
+      rb.template read<2>(cur, y[0]);
+      lgkm_wait<PER>();
+      multiply(1);
+      ra.template read<3>(cur, x[1]);
+      rb.template read<3>(cur, y[1]);
+      lgkm_wait<PER>();
+      multiply(0);
+      lgkm_wait<0>();
+      multiply(1);
+      cur = BUF - cur;
+    }
+  }
+  // The wave's rows (one per lane of its column blocks j) of value(j, i, q), four values of
+  // row block i, to global rows of bf16 through the wave's own LDS: 16 bytes a lane in
+  // lines of 128 (or 64) bytes.  at(r): row r's first element, or NULL; cols: how many
+  // columns exist from there.
+  template <typename V, typename At>
+  __device__ __forceinline__ void store(V value, At at, int64_t cols) {
+    unsigned char* own = lds + PRIVATE + wave * OWN;
+    const int ch = lane % CH, mine = lane & 31;
+#pragma unroll
+    for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+      for (int i2 = 0; i2 < C::MT; i2 += NB)
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += C::OUT) {
+          if (C::OUT == 32 || mine / C::OUT == r0 / C::OUT) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                store4<bf16>(reinterpret_cast<bf16*>(own + (mine - r0) * (CH * 16) + (((i * 4 + q) ^ (mine % CH)) << 4) +
+                                                     (lane >> 5) * 8),
+                             value(j, i2 + i, q));
+          }
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int r = 0; r < C::OUT; r += 64 / CH) {
+            const int row = r + lane / CH;
+            const bf16x8 v = *reinterpret_cast<const bf16x8*>(own + row * (CH * 16) + ((ch ^ ((r0 + row) % CH)) << 4));
+            bf16* o = at(j * 32 + r0 + row);
+            const int col = i2 * 32 + ch * 8;
+            if (o && col < cols) *reinterpret_cast<bf16x8*>(o + col) = v;
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+  }
+};
 
-// Which tile a workgroup takes.  Workgroups go to the 8 XCDs in turn; each XCD gets a
-// contiguous run of tiles, in groups of 8 row tiles over all column tiles, so that the 32
-// that run at once on it share 8 + 4 operand tiles in its L2.
-__device__ __forceinline__ bool head_tile(int id, int nm, int nn, int& tm, int& tn) {
-  const int total = nm * nn, per = (total + 7) / 8;
-  const int w = (id & 7) * per + (id >> 3);
-  if ((id >> 3) >= per || w >= total) return false;
-  const int group = w / (8 * nn), left = nm - group * 8, g = left < 8 ? left : 8;
-  const int in = w - group * 8 * nn;
-  tn = in / g;
-  tm = group * 8 + in - tn * g;
-  return true;
+// The tiles of a workgroup.  Workgroups go to the 8 XCDs in turn; each XCD takes a contiguous
+// run of tiles, in groups of 8 row tiles over all column tiles, so that the 32 that it works
+// on at once share 8 + 4 operand tiles in its L2.
+struct Tiles {
+  int nm, nn, w, step, end;
+  __device__ __forceinline__ Tiles(int nm_, int nn_) : nm(nm_), nn(nn_) {
+    const int total = nm * nn, per = (total + 7) / 8, xcd = blockIdx.x & 7;
+    w = xcd * per + (blockIdx.x >> 3);
+    end = (xcd + 1) * per < total ? (xcd + 1) * per : total;
+    step = gridDim.x >> 3;
+  }
+  __device__ __forceinline__ bool has(int ahead) const { return w + ahead * step < end; }
+  __device__ __forceinline__ void get(int ahead, int& tm, int& tn) const {
+    const int v = w + ahead * step;
+    const int group = v / (8 * nn), left = nm - group * 8, g = left < 8 ? left : 8;
+    const int in = v - group * 8 * nn;
+    tn = in / g;
+    tm = group * 8 + in - tn * g;
+  }
+};
+template <class C>
+static int head_grid(int64_t tiles) {
+  const int64_t most = HD_CUS * C::PER_CU, n = (tiles + 7) / 8 * 8;
+  return (int)(n < most ? n : most);
 }
-static int head_grid(int64_t nm, int64_t nn) { return (int)((nm * nn + 7) / 8 * 8); }
 
 struct HeadParams {
+  HeadSource src;
   const bf16* hc;
   const bf16* w;
-  int64_t rows;      // tokens in all, kept or not
+  int64_t rows;  // tokens in all, kept or not
   int V, H;
   const int* count;
   const int* target;
-  float c;           // log2(e) / T
-  floatx2* part;     // forward: (vocabulary tiles, rows) partial (m, l)
+  float c;       // log2(e) / T
+  floatx2* part;  // forward: (vocabulary tiles, rows) partial (m, l)
   float* zlabel;
   const floatx4* coef;  // backward
-  bf16* dz;          // (rows, ldz): this range's v0 .. v0 + vc
+  bf16* dz;      // (rows, ldz): this range's v0 .. v0 + vc
   int64_t ldz;
-  int v0, vc;
+  int v0, vc, vmax;  // vmax: the largest range
   bf16* dw;
-  float* dh;         // (slabs, rows, H) fp32 partial sums
-  int slabs, add;
+  float* dh;     // fp32 partial sums, a slab after the other
+  int add;
 };
 
 // ---------------------------------------------------------------------------
 // z = hc w^T, vocabulary on the row axis: a lane holds one token's 64 (or 16) vocabulary
 // entries of each block, so their maximum and sum need no shuffles but one.  DZ: dz of a
 // range of the vocabulary instead of the statistics.
-template <int BN, bool DZ>
-__global__ __launch_bounds__(512) void head_logits_kernel(HeadParams p) {
-  using W = Waves<BN>;
+template <class C, bool DZ, bool GATHER = false>
+__global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams p) {
+  typedef Product<C, true, true, GATHER> P;
   extern __shared__ __align__(1024) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int count = *p.count;
-  int tm, tn;
-  const int vc = DZ ? p.vc : p.V;
-  if (!head_tile(blockIdx.x, (vc + HD_BM - 1) / HD_BM, (int)((p.rows + BN - 1) / BN), tm, tn)) return;
-  const int n0 = tn * BN, v0 = (DZ ? p.v0 : 0) + tm * HD_BM;
-  if (n0 >= count) return;
-  const int vend = DZ ? p.v0 + p.vc : p.V;
-  Stage<HD_BM, true> sa;
-  Stage<BN, true> sb;
-  sa.init(p.w, p.H, v0, vend, p.H, wave, lane);
-  sb.init(p.hc, p.H, n0, count, p.H, wave, lane);
-  floatx16 acc[W::MT][W::NT];
-#pragma unroll
-  for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-    for (int j = 0; j < W::NT; ++j) acc[i][j] = floatx16{};
-  head_product<BN, true, true>(lds, sa, sb, p.H, wave, lane, acc);
-
-  const int wm = wave / W::N, wn = wave % W::N;
-  const int vw = wm * (W::MT * 32) + (lane >> 5) * 4;  // the lane's first entry in the tile
-  __syncthreads();                                     // the buffers' readers are done
-#pragma unroll
-  for (int j = 0; j < W::NT; ++j) {
-    const int nl = wn * (W::NT * 32) + j * 32 + (lane & 31), n = n0 + nl;
-    const int y = n < count ? p.target[n] : -1;
-    const int at = y - v0 - vw;  // the label's entry relative to the lane's first
-    if (!DZ) {
-      if (wave_any(y >= 0 && at >= 0 && at < W::MT * 32 && !(at & 4))) {
-#pragma unroll
-        for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (y >= 0 && at == i * 32 + (e >> 2) * 8 + (e & 3)) p.zlabel[n] = acc[i][j][e];
-      }
-      if (v0 + HD_BM > p.V) {
-#pragma unroll
-        for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (v0 + vw + i * 32 + (e >> 2) * 8 + (e & 3) >= p.V) acc[i][j][e] = -INFINITY;
-      }
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
-      m = xor32_max(m);
-      const float base = finite_max(m);
-      float l = 0.f;
-#pragma unroll
-      for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) l += fast_exp2((acc[i][j][e] - base) * p.c);
-      l = xor32_sum(l);
-      if (lane < 32) reinterpret_cast<floatx2*>(lds)[wm * BN + nl] = floatx2{m, l};
-    } else {
-      const floatx4 k = n < count ? p.coef[n] : floatx4{};
-#pragma unroll
-      for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int vl = vw + i * 32 + q * 8;  // 4 consecutive entries
-          floatx4 d;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            d[e] = k[1] * fast_exp2((acc[i][j][q * 4 + e] - k[0]) * p.c);
-            if (at == i * 32 + q * 8 + e && y >= 0) d[e] += k[2];
-            if (v0 + vl + e >= vend) d[e] = 0.f;
-          }
-          store4<bf16>(reinterpret_cast<bf16*>(lds + nl * 512 + (((vl >> 3) ^ (nl & 31)) << 4) + (lane >> 5) * 8), d);
-        }
-    }
+  const int vend = DZ ? p.v0 + p.vc : p.V, vfirst = DZ ? p.v0 : 0;
+  // GATHER: the kept rows and their labels in the waves' own LDS, where nothing else lies before
+  // the first epilogue, and the labels in registers from there on
+  int* few_index = reinterpret_cast<int*>(lds + P::PRIVATE);
+  int count;
+  if (GATHER) {
+    count = p.src.few(lane, p.V, few_index + wave * 128, few_index + wave * 128 + 64);
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    count = __builtin_amdgcn_readfirstlane(*p.count);
   }
-  __syncthreads();
-  if (!DZ) {
-    for (int nl = threadIdx.x; nl < BN; nl += 512) {
-      if (n0 + nl < count) {
-        RowStat s{-INFINITY, 0.f};
+  Tiles t((vend - vfirst + C::BM - 1) / C::BM, (count + C::BN - 1) / C::BN);
+  if (!t.has(0)) return;
+  P prod;
+  prod.init(lds, wave, lane);
+  typename P::A a, na;
+  typename P::B b, nb;
+  a.lanes(p.H, wave, lane);
+  na = a;
+  int few_target[C::NT];
+  if constexpr (GATHER) {
+    const int* index = few_index + wave * 128;
+    b.at([&](int r) { return p.src.row(index[r < count ? r : 0]); }, p.H, wave, lane);
 #pragma unroll
-        for (int i = 0; i < W::M; ++i) {
-          const floatx2 v = reinterpret_cast<const floatx2*>(lds)[i * BN + nl];
-          s = join(s, RowStat{v[0], v[1]}, p.c);
-        }
-        p.part[(int64_t)tm * p.rows + n0 + nl] = floatx2{s.m, s.l};
-      }
+    for (int j = 0; j < C::NT; ++j) {
+      const int n = (wave % C::N) * (C::NT * 32) + j * 32 + (lane & 31);
+      few_target[j] = n < count ? index[64 + n] : -1;
     }
   } else {
-    const int ch = threadIdx.x & 31;
-    for (int nl = threadIdx.x >> 5; nl < BN; nl += 16) {
-      const int64_t col = (int64_t)(v0 - p.v0) + ch * 8;
-      if (n0 + nl < count && col < p.ldz)
-        *reinterpret_cast<bf16x8*>(p.dz + (int64_t)(n0 + nl) * p.ldz + col) =
-            *reinterpret_cast<const bf16x8*>(lds + nl * 512 + ((ch ^ (nl & 31)) << 4));
+    b.lanes(p.H, wave, lane);
+  }
+  nb = b;
+  int tm, tn, um = 0, un = 0;
+  t.get(0, tm, tn);
+  a.at(p.w, vfirst + tm * C::BM, vend, p.H);
+  if constexpr (!GATHER) b.at(p.hc, tn * C::BN, count, p.H);
+  prod.load(0, a, b, 0);
+  const int wm = wave / C::N, wn = wave % C::N;
+  const int vw = wm * (C::MT * 32) + (lane >> 5) * 4;  // the lane's first entry in the tile
+  for (;;) {
+    const bool more = t.has(1);
+    if (more) {
+      t.get(1, um, un);
+      na.at(p.w, vfirst + um * C::BM, vend, p.H);
+      if constexpr (!GATHER) nb.at(p.hc, un * C::BN, count, p.H);
     }
+    typename P::Acc acc;
+    prod.run(a, b, more, na, nb, acc);
+
+    const int n0 = tn * C::BN, v0 = vfirst + tm * C::BM;
+    if (!DZ) {
+      static_assert(C::M * C::BN * 8 <= P::LDS - P::PRIVATE, "room for the waves' statistics");
+      floatx2* red = reinterpret_cast<floatx2*>(lds + P::PRIVATE);
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j) {
+        const int nl = wn * (C::NT * 32) + j * 32 + (lane & 31), n = n0 + nl;
+        const int y = GATHER ? few_target[j] : n < count ? p.target[n] : -1;
+        const int at = y - v0 - vw;  // the label's entry relative to the lane's first
+        if (wave_any(y >= 0 && at >= 0 && at < C::MT * 32 && !(at & 4))) {
+#pragma unroll
+          for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (y >= 0 && at == i * 32 + (e >> 2) * 8 + (e & 3)) p.zlabel[n] = acc[i][j][e];
+        }
+        if (v0 + C::BM > p.V) {
+#pragma unroll
+          for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (v0 + vw + i * 32 + (e >> 2) * 8 + (e & 3) >= p.V) acc[i][j][e] = -INFINITY;
+        }
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+        m = xor32_max(m);
+        const float base = finite_max(m);
+        float l = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) l += fast_exp2((acc[i][j][e] - base) * p.c);
+        l = xor32_sum(l);
+        if (lane < 32) red[wm * C::BN + nl] = floatx2{m, l};
+      }
+      __syncthreads();  // the next write to `red` follows the next tile's barriers
+      for (int nl = threadIdx.x; nl < C::BN; nl += threads_of<C>()) {
+        if (n0 + nl < count) {
+          RowStat s{-INFINITY, 0.f};
+#pragma unroll
+          for (int i = 0; i < C::M; ++i) {
+            const floatx2 v = red[i * C::BN + nl];
+            s = join(s, RowStat{v[0], v[1]}, p.c);
+          }
+          p.part[(int64_t)tm * p.rows + n0 + nl] = floatx2{s.m, s.l};
+        }
+      }
+    } else {
+      floatx4 k[C::NT];
+      int at[C::NT];
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j) {
+        const int n = n0 + wn * (C::NT * 32) + j * 32 + (lane & 31);
+        k[j] = n < count ? p.coef[n] : floatx4{};
+        const int y = n < count ? p.target[n] : -1;
+        at[j] = y < 0 ? -1 : y - v0 - vw;
+      }
+      const int64_t col0 = (int64_t)tm * C::BM + wm * (C::MT * 32);
+      prod.store(
+          [&](int j, int i, int q) {
+            floatx4 d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              d[e] = k[j][1] * fast_exp2((acc[i][j][q * 4 + e] - k[j][0]) * p.c);
+              if (at[j] == i * 32 + q * 8 + e) d[e] += k[j][2];
+              if (v0 + vw + i * 32 + q * 8 + e >= vend) d[e] = 0.f;
+            }
+            return d;
+          },
+          [&](int r) {
+            const int n = n0 + wn * (C::NT * 32) + r;
+            return n < count ? p.dz + (int64_t)n * p.ldz + col0 : nullptr;
+          },
+          p.ldz - col0);
+    }
+    if (!more) break;
+    a = na, b = nb, tm = um, tn = un;
+    t.w += t.step;
   }
 }
 
-// The tiles' statistics of each kept row joined: 16 rows x 64 slots of tiles a workgroup.
+// The tiles' statistics of each kept row joined: R rows x 1024 / R slots of tiles a
+// workgroup.  GATHER: the kept rows found as the products did.
 struct HeadJoin {
+  HeadSource src;
   const floatx2* part;
-  const float* zlabel;
+  const float* zlabel;  // written for every kept row whose label is in the vocabulary
   const int* count;
   const int* index;
+  const int* target;
   float* logprobs;
   floatx2* stats;
-  int64_t rows;
-  int tiles;
+  int V, tiles;
   float c, inv_t;
 };
 
+template <int R, bool GATHER>
 __global__ __launch_bounds__(1024) void head_join_kernel(HeadJoin p) {
-  __shared__ RowStat red[64][17];
-  const int r = threadIdx.x & 15, slot = threadIdx.x >> 4;
-  const int count = *p.count;
-  const int n0 = blockIdx.x * 16, n = n0 + r;
+  constexpr int SLOTS = 1024 / R;
+  __shared__ RowStat red[SLOTS][R + 1];
+  __shared__ int few[128];
+  __shared__ int few_count;
+  const int r = threadIdx.x % R, slot = threadIdx.x / R;
+  int count;
+  if (GATHER) {
+    if (threadIdx.x < 64) {
+      const int lane = threadIdx.x, n = p.src.few(lane, p.V, few, few + 64);
+      if (lane == 0) few_count = n;
+      if (blockIdx.x == 0 && lane < p.src.rows && p.src.labels[lane] == p.src.ignore) {
+        p.logprobs[lane] = 0.f;
+        p.stats[lane] = floatx2{0.f, 1.f};
+      }
+    }
+    __syncthreads();
+    count = few_count;
+  } else {
+    count = *p.count;
+  }
+  const int n0 = blockIdx.x * R, n = n0 + r;
   if (n0 >= count) return;
   RowStat s{-INFINITY, 0.f};
   if (n < count) {
-#pragma unroll 4
-    for (int t = slot; t < p.tiles; t += 64) {
-      const floatx2 v = p.part[(int64_t)t * p.rows + n];
+#pragma unroll 8
+    for (int t = slot; t < p.tiles; t += SLOTS) {
+      const floatx2 v = p.part[(int64_t)t * p.src.rows + n];
       s = join(s, RowStat{v[0], v[1]}, p.c);
     }
   }
   red[slot][r] = s;
   __syncthreads();
-  for (int k = 32; k >= 1; k >>= 1) {
+  for (int k = SLOTS / 2; k >= 1; k >>= 1) {
     if (slot < k) red[slot][r] = join(red[slot][r], red[slot + k][r], p.c);
     __syncthreads();
   }
   if (slot == 0 && n < count) {
     s = red[0][r];
-    const int row = p.index[n];
-    p.logprobs[row] = (p.zlabel[n] - s.m) * p.inv_t - logf(s.l);
+    const int row = GATHER ? few[n] : p.index[n], y = GATHER ? few[64 + n] : p.target[n];
+    p.logprobs[row] = y < 0 ? __builtin_nanf("") : (p.zlabel[n] - s.m) * p.inv_t - logf(s.l);
     p.stats[row] = floatx2{s.m, s.l};
   }
 }
 
 // dw[v][h] = sum over kept tokens of dz[n][v] hc[n][h], v0 <= v < v0 + vc: both operands have
-// the depth (tokens) as their slow axis.  The tile goes out through LDS in whole lines.
-__global__ __launch_bounds__(512) void head_dw_kernel(HeadParams p) {
-  using W = Waves<256>;
+// the depth (tokens) as their slow axis.
+__global__ __launch_bounds__(threads_of<Wide>()) void head_dw_kernel(HeadParams p) {
+  typedef Wide C;
+  typedef Product<C, false, false> P;
   extern __shared__ __align__(1024) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int count = *p.count;
-  int th, tv;
-  if (!head_tile(blockIdx.x, (p.H + HD_BM - 1) / HD_BM, (p.vc + 255) / 256, th, tv)) return;
-  const int h0 = th * HD_BM, v0 = tv * 256;
-  Stage<HD_BM, false> sa;
-  Stage<256, false> sb;
-  sa.init(p.hc, p.H, h0, p.H, count, wave, lane);
-  sb.init(p.dz, p.ldz, v0, p.ldz, count, wave, lane);
-  floatx16 acc[W::MT][W::NT];
-#pragma unroll
-  for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-    for (int j = 0; j < W::NT; ++j) acc[i][j] = floatx16{};
-  if (count > 0) head_product<256, false, false>(lds, sa, sb, count, wave, lane, acc);
-  const int wm = wave / W::N, wn = wave % W::N;
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < W::NT; ++j) {
-    const int vl = wn * 64 + j * 32 + (lane & 31);
-#pragma unroll
-    for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int hl = wm * 128 + i * 32 + q * 8;
-        const floatx4 d{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
-        store4<bf16>(reinterpret_cast<bf16*>(lds + vl * 512 + (((hl >> 3) ^ (vl & 31)) << 4) + (lane >> 5) * 8), d);
-      }
-  }
-  __syncthreads();
-  const int ch = threadIdx.x & 31;
-  for (int vl = threadIdx.x >> 5; vl < 256; vl += 16) {
-    const int v = v0 + vl, h = h0 + ch * 8;
-    if (v < p.vc && h < p.H)
-      *reinterpret_cast<bf16x8*>(p.dw + (int64_t)(p.v0 + v) * p.H + h) =
-          *reinterpret_cast<const bf16x8*>(lds + vl * 512 + ((ch ^ (vl & 31)) << 4));
+  const int count = __builtin_amdgcn_readfirstlane(*p.count);
+  Tiles t((p.H + C::BM - 1) / C::BM, (p.vc + C::BN - 1) / C::BN);
+  if (!t.has(0)) return;
+  P prod;
+  prod.init(lds, wave, lane);
+  P::A a, na;
+  P::B b, nb;
+  a.lanes(p.H, wave, lane);
+  b.lanes(p.ldz, wave, lane);
+  na = a, nb = b;
+  int tm, tn, um = 0, un = 0;
+  t.get(0, tm, tn);
+  a.at(p.hc, tm * C::BM, p.H, count);
+  b.at(p.dz, tn * C::BN, p.vc, count);
+  if (count > 0) prod.load(0, a, b, 0);
+  const int wm = wave / C::N, wn = wave % C::N;
+  for (;;) {
+    const bool more = t.has(1);
+    if (more) {
+      t.get(1, um, un);
+      na.at(p.hc, um * C::BM, p.H, count);
+      nb.at(p.dz, un * C::BN, p.vc, count);
+    }
+    P::Acc acc;
+    prod.run(a, b, more, na, nb, acc);
+    const int h0 = tm * C::BM + wm * (C::MT * 32), v0 = tn * C::BN + wn * (C::NT * 32);
+    prod.store(
+        [&](int j, int i, int q) {
+          return floatx4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+        },
+        [&](int r) { return v0 + r < p.vc ? p.dw + (int64_t)(p.v0 + v0 + r) * p.H + h0 : nullptr; }, p.H - h0);
+    if (!more) break;
+    a = na, b = nb, tm = um, tn = un;
+    t.w += t.step;
   }
 }
 
-// dh[n][h] (+)= sum over this range's v of dz[n][v] w[v][h], fp32.  The depth (vocabulary) is
-// long and the tiles may be few: it is split over slabs, each with sums of its own, which
-// the last launch adds in order.
-template <int BN>
-__global__ __launch_bounds__(512) void head_dh_kernel(HeadParams p) {
-  using W = Waves<BN>;
+// The depth of dh's products (vocabulary) is long and its tiles may be few: it is split over
+// slabs, each with sums of its own, which the last launch adds in order.  As many as fill
+// the CUs' last round best, less a little for each one's sums.
+__host__ __device__ __forceinline__ int head_slabs(int64_t tiles, int vmax) {
+  const int64_t deep = (vmax + 8 * HD_BK - 1) / (8 * HD_BK);  // at least 8 steps each
+  int64_t best = 1, most = 0, rounds_of = 1;  // whole numbers: every kernel finds the same
+  for (int64_t s = 1; s <= 8; ++s) {
+    const int64_t n = tiles * s, rounds = (n + HD_CUS - 1) / HD_CUS, use = n * (100 - s);
+    if (s > 1 && n > 4 * HD_CUS) break;
+    if (use * rounds_of > most * rounds) most = use, rounds_of = rounds, best = s;
+  }
+  if (tiles * 8 <= HD_CUS) best = HD_CUS / tiles;
+  if (best > deep) best = deep;
+  return best < 1 ? 1 : (int)best;
+}
+
+// dh[n][h] (+)= sum over this range's v of dz[n][v] w[v][h], fp32.
+template <class C>
+__global__ __launch_bounds__(threads_of<C>()) void head_dh_kernel(HeadParams p) {
+  typedef Product<C, false, true> P;
   extern __shared__ __align__(1024) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int count = *p.count;
-  const int nh = (p.H + HD_BM - 1) / HD_BM, nn = (int)((p.rows + BN - 1) / BN);
-  int th, rest;
-  if (!head_tile(blockIdx.x, nh, nn * p.slabs, th, rest)) return;
-  const int slab = rest / nn, tn = rest - slab * nn;
-  const int h0 = th * HD_BM, n0 = tn * BN;
-  if (n0 >= count) return;
-  const int per = ((p.vc + p.slabs - 1) / p.slabs + HD_BK - 1) / HD_BK * HD_BK;
-  const int k0 = slab * per, depth = p.vc - k0 < per ? p.vc - k0 : per;
-  floatx16 acc[W::MT][W::NT];
-#pragma unroll
-  for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-    for (int j = 0; j < W::NT; ++j) acc[i][j] = floatx16{};
-  if (depth > 0) {
-    Stage<HD_BM, false> sa;
-    Stage<BN, true> sb;
-    sa.init(p.w + (int64_t)(p.v0 + k0) * p.H, p.H, h0, p.H, depth, wave, lane);
-    sb.init(p.dz + k0, p.ldz, n0, count, depth, wave, lane);
-    head_product<BN, false, true>(lds, sa, sb, depth, wave, lane, acc);
-  } else if (p.add) {
-    return;
-  }
-  const int wm = wave / W::N, wn = wave % W::N;
-#pragma unroll
-  for (int j = 0; j < W::NT; ++j) {
-    const int n = n0 + wn * (W::NT * 32) + j * 32 + (lane & 31);
-    if (n < count) {
-#pragma unroll
-      for (int i = 0; i < W::MT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int h = h0 + wm * (W::MT * 32) + i * 32 + q * 8 + (lane >> 5) * 4;
-          if (h < p.H) {
-            floatx4* o = reinterpret_cast<floatx4*>(p.dh + ((int64_t)slab * p.rows + n) * p.H + h);
-            floatx4 d{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
-            if (p.add) d += *o;
-            *o = d;
-          }
-        }
+  const int count = __builtin_amdgcn_readfirstlane(*p.count);
+  const int nh = (p.H + C::BM - 1) / C::BM, nn = (count + C::BN - 1) / C::BN;
+  if (nn == 0) return;
+  const int slabs = head_slabs((int64_t)nh * nn, p.vmax);
+  const int per = ((p.vc + slabs - 1) / slabs + HD_BK - 1) / HD_BK * HD_BK;
+  Tiles t(nh, nn * slabs);
+  if (!t.has(0)) return;
+  P prod;
+  prod.init(lds, wave, lane);
+  typename P::A a, na;
+  typename P::B b, nb;
+  a.lanes(p.H, wave, lane);
+  b.lanes(p.ldz, wave, lane);
+  na = a, nb = b;
+  auto place = [&](int th, int rest, typename P::A& x, typename P::B& y) {
+    const int slab = rest / nn, tn = rest - slab * nn, k0 = slab * per;
+    const int left = p.vc - k0, depth = left < 0 ? 0 : left < per ? left : per;
+    x.at(p.w + (int64_t)(p.v0 + (depth ? k0 : 0)) * p.H, th * C::BM, p.H, depth);
+    y.at(p.dz + (depth ? k0 : 0), tn * C::BN, count, depth);
+  };
+  int th, rest, uh = 0, us = 0;
+  t.get(0, th, rest);
+  place(th, rest, a, b);
+  if (a.depth) prod.load(0, a, b, 0);
+  const int wm = wave / C::N, wn = wave % C::N;
+  for (;;) {
+    const bool more = t.has(1);
+    if (more) {
+      t.get(1, uh, us);
+      place(uh, us, na, nb);
     }
+    typename P::Acc acc;
+    prod.run(a, b, more && na.depth, na, nb, acc);
+    if (!a.depth && more && na.depth) prod.load(prod.cur, na, nb, 0);  // nothing ran that would have begun it
+    const int slab = rest / nn, tn = rest - slab * nn;
+    if (a.depth || !p.add) {
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j) {
+        const int n = tn * C::BN + wn * (C::NT * 32) + j * 32 + (lane & 31);
+        if (n < count) {
+#pragma unroll
+          for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int h = th * C::BM + wm * (C::MT * 32) + i * 32 + q * 8 + (lane >> 5) * 4;
+              if (h < p.H) {
+                floatx4* o = reinterpret_cast<floatx4*>(p.dh + ((int64_t)slab * nn * C::BN + n) * p.H + h);
+                floatx4 d{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+                if (p.add) d += *o;
+                *o = d;
+              }
+            }
+        }
+      }
+    }
+    if (!more) break;
+    a = na, b = nb, th = uh, rest = us;
+    t.w += t.step;
   }
 }
 
 // dhidden: the slabs' sums, rounded, in the rows' own places; zeros in ignored rows.
-__global__ __launch_bounds__(256) void head_dh_out_kernel(const float* dh, int slabs, int64_t rows, int H,
-                                                          const int* pos, bf16* out) {
+struct HeadOut {
+  const float* dh;
+  const int* count;
+  const int* pos;
+  bf16* out;
+  int64_t rows;
+  int H, bm, bn, vmax;
+};
+__global__ __launch_bounds__(256) void head_dh_out_kernel(HeadOut p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int ch = H / 8;
-  if (i >= rows * ch) return;
+  const int ch = p.H / 8;
+  if (i >= p.rows * ch) return;
   const int64_t row = i / ch;
-  const int c = (int)(i - row * ch), place = pos[row];
+  const int c = (int)(i - row * ch), place = p.pos[row];
   floatx8 s{};
   if (place >= 0) {
-    const float* src = dh + (int64_t)place * H + c * 8;
+    const int nn = (*p.count + p.bn - 1) / p.bn;
+    const int slabs = head_slabs((int64_t)((p.H + p.bm - 1) / p.bm) * nn, p.vmax);
+    const int64_t stride = (int64_t)nn * p.bn * p.H;
+    const float* src = p.dh + (int64_t)place * p.H + c * 8;
     s = Vec8<float>::load_f32(src);
-    for (int k = 1; k < slabs; ++k) s += Vec8<float>::load_f32(src + k * rows * H);
+    for (int k = 1; k < slabs; ++k) s += Vec8<float>::load_f32(src + k * stride);
   }
-  store8<bf16>(out + row * H + c * 8, s);
+  store8<bf16>(p.out + row * p.H + c * 8, s);
 }
 
 }  // namespace nq
@@ -565,20 +772,21 @@ using namespace nq;
 
 static int64_t pad256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Tokens of a tile.
-static int head_bn(int64_t rows) { return rows <= 64 ? 64 : 256; }
+// Which tile: Few reads the weights once for up to 64 tokens.
+static bool head_few(int64_t rows) { return rows <= Few::BN; }
 
 // Where each piece of a workspace lies.
 struct HeadSpace {
   int64_t count, pos, index, target, zlabel, coef, hc, part, dz, dh, total;
   int64_t ldz;
-  int vc, slabs;
+  int vc;
 };
 
 constexpr int64_t HD_DZ_BYTES = (int64_t)1 << 30;  // the largest range's dz
 
 static HeadSpace head_space(int64_t rows, int V, int H, bool backward) {
   HeadSpace s{};
+  const int64_t bm = head_few(rows) ? Few::BM : Wide::BM, bn = head_few(rows) ? Few::BN : Wide::BN;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -592,24 +800,24 @@ static HeadSpace head_space(int64_t rows, int V, int H, bool backward) {
   s.hc = take(rows * H * 2);
   if (!backward) {
     s.zlabel = take(rows * 4);
-    s.part = take(rows * ((V + HD_BM - 1) / HD_BM) * 8);
+    s.part = take(rows * ((V + bm - 1) / bm) * 8);
   } else {
     s.coef = take(rows * 16);
-    // equal ranges of whole tiles
-    const int64_t most = HD_DZ_BYTES / (rows * 2) / HD_BM * HD_BM;
-    const int64_t vpad = pad256(V), step = most < HD_BM ? HD_BM : most;
-    const int64_t ranges = (vpad + step - 1) / step;
-    s.vc = (int)pad256((V + ranges - 1) / ranges);
-    if (s.vc > V) s.vc = V;
+    // ranges of whole tiles, as many as fill the CUs in whole rounds of dw's
+    const int64_t nh = (H + 255) / 256, unit = (nh < HD_CUS ? HD_CUS / nh : 1) * 256;
+    int64_t most = HD_DZ_BYTES / (rows * 2) / 256 * 256;
+    most = most < 256 ? 256 : most < unit ? most : most / unit * unit;
+    const int64_t ranges = (V + most - 1) / most, each = ((V + ranges - 1) / ranges + unit - 1) / unit * unit;
+    if (each < most) most = each;
+    s.vc = (int)(most < V ? most : V);
     s.ldz = (s.vc + 7) / 8 * 8;
-    const int bn = head_bn(rows);
-    const int64_t tiles = ((rows + bn - 1) / bn) * ((H + HD_BM - 1) / HD_BM);
-    int64_t slabs = 256 / tiles;
-    const int64_t deep = (s.vc + 8 * HD_BK - 1) / (8 * HD_BK);  // at least 8 steps each
-    if (slabs > deep) slabs = deep;
-    s.slabs = slabs < 1 ? 1 : (int)slabs;
     s.dz = take(rows * s.ldz * 2);
-    s.dh = take((int64_t)s.slabs * rows * H * 4);
+    // as many slabs as any number of kept rows takes
+    const int64_t tiles = ((rows + bn - 1) / bn) * ((H + bm - 1) / bm);
+    int64_t slots = 8 * tiles < HD_CUS ? HD_CUS : 8 * tiles;
+    if (slots > 4 * HD_CUS) slots = 4 * HD_CUS;
+    if (slots < tiles) slots = tiles;
+    s.dh = take(slots * bm * bn * 4);
   }
   s.total = at;
   return s;
@@ -650,20 +858,24 @@ static int head_check(const void* hidden, int64_t bs, int64_t rs, const void* we
   return NQ_OK;
 }
 
-// Dynamic LDS of a product: two buffers of both operands.
-static constexpr int head_lds(int bn) { return 2 * (HD_BM + bn) * HD_BK * 2; }
-
-// The attribute belongs to a kernel on a device; setting it is cheap and idempotent.
-static int head_allow(const void* kernel, int bytes) {
-  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == hipSuccess ? NQ_OK : nq_check_launch(e);
-}
-
-template <typename K>
-static int head_launch(K kernel, int grid, int bn, hipStream_t st, const HeadParams& p) {
-  if (int rc = head_allow(reinterpret_cast<const void*>(kernel), head_lds(bn))) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(512), head_lds(bn), st, p);
+// A launch with P's dynamic LDS (the attribute belongs to the kernel on the device; setting it
+// again is cheap).
+template <class P, typename K>
+static int head_launch(K kernel, int grid, int threads, hipStream_t st, const HeadParams& p) {
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+  if (e != hipSuccess) return nq_check_launch(e);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3((unsigned)threads), P::LDS, st, p);
   return nq_check_launch(hipGetLastError());
+}
+template <class C, bool DZ, bool GATHER = false>
+static int launch_logits(int64_t tiles, hipStream_t st, const HeadParams& p) {
+  return head_launch<Product<C, true, true, GATHER>>(head_logits_kernel<C, DZ, GATHER>, head_grid<C>(tiles),
+                                                     threads_of<C>(), st, p);
+}
+template <class C>
+static int launch_dh(int64_t tiles, hipStream_t st, const HeadParams& p) {
+  return head_launch<Product<C, false, true>>(head_dh_kernel<C>, head_grid<C>(tiles), threads_of<C>(), st, p);
 }
 
 extern "C" int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int64_t row_stride, const void* weight,
@@ -682,26 +894,30 @@ extern "C" int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int6
   const float inv = 1.f / temperature;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   HeadRows r{};
-  r.hidden = reinterpret_cast<const bf16*>(hidden), r.bs = batch_stride, r.rs = row_stride, r.S = S;
-  r.labels = labels, r.rows = rows, r.ignore = ignore_index, r.H = H, r.V = V;
+  r.src = HeadSource{reinterpret_cast<const bf16*>(hidden), batch_stride, row_stride, S, labels, rows, ignore_index};
+  r.H = H, r.V = V;
   r.count = reinterpret_cast<int*>(ws + s.count), r.pos = reinterpret_cast<int*>(ws + s.pos);
   r.index = reinterpret_cast<int*>(ws + s.index), r.target = reinterpret_cast<int*>(ws + s.target);
   r.hc = reinterpret_cast<bf16*>(ws + s.hc);
-  r.logprobs = logprobs, r.stats = reinterpret_cast<floatx2*>(stats), r.zlabel = reinterpret_cast<float*>(ws + s.zlabel);
-  hipLaunchKernelGGL(head_rows_kernel, dim3((unsigned)((rows + HD_PREP - 1) / HD_PREP)), dim3(256), 0, st, r);
+  r.logprobs = logprobs, r.stats = reinterpret_cast<floatx2*>(stats);
   HeadParams p{};
-  p.hc = r.hc, p.w = reinterpret_cast<const bf16*>(weight), p.rows = rows, p.V = V, p.H = H;
+  p.src = r.src, p.hc = r.hc, p.w = reinterpret_cast<const bf16*>(weight), p.rows = rows, p.V = V, p.H = H;
   p.count = r.count, p.target = r.target, p.c = inv * kLog2e;
-  p.part = reinterpret_cast<floatx2*>(ws + s.part), p.zlabel = r.zlabel;
-  const int bn = head_bn(rows), tiles = (V + HD_BM - 1) / HD_BM;
-  const int64_t nn = (rows + bn - 1) / bn;
-  if (tiles * nn > INT32_MAX / 2) return nq_fail(NQ_ERR_UNSUPPORTED, "too many tiles for one launch");
-  const int grid = head_grid(tiles, nn);
-  if (int rc = bn == 64 ? head_launch(head_logits_kernel<64, false>, grid, bn, st, p)
-                        : head_launch(head_logits_kernel<256, false>, grid, bn, st, p))
-    return rc;
-  HeadJoin j{p.part, p.zlabel, r.count, r.index, logprobs, r.stats, rows, tiles, p.c, inv};
-  hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(1024), 0, st, j);
+  p.part = reinterpret_cast<floatx2*>(ws + s.part), p.zlabel = reinterpret_cast<float*>(ws + s.zlabel);
+  const bool few = head_few(rows);
+  const int bm = few ? Few::BM : Wide::BM, bn = few ? Few::BN : Wide::BN, tiles = (V + bm - 1) / bm;
+  const int64_t all = tiles * ((rows + bn - 1) / bn);
+  if (all > INT32_MAX / 2) return nq_fail(NQ_ERR_UNSUPPORTED, "too many tiles for one launch");
+  const HeadJoin j{r.src, p.part, p.zlabel, r.count, r.index, r.target, logprobs, r.stats, V, tiles, p.c, inv};
+  if (few) {
+    // 33 rows of 1024 against 151936 entries: without the gathering launch 62 us for 69
+    if (int rc = launch_logits<Few, false, true>(all, st, p)) return rc;
+    hipLaunchKernelGGL((head_join_kernel<4, true>), dim3((unsigned)((rows + 3) / 4)), dim3(1024), 0, st, j);
+  } else {
+    hipLaunchKernelGGL(head_rows_kernel, dim3((unsigned)((rows + HD_PREP - 1) / HD_PREP)), dim3(256), 0, st, r);
+    if (int rc = launch_logits<Wide, false>(all, st, p)) return rc;
+    hipLaunchKernelGGL((head_join_kernel<16, false>), dim3((unsigned)((rows + 15) / 16)), dim3(1024), 0, st, j);
+  }
   return nq_check_launch(hipGetLastError());
 }
 
@@ -723,8 +939,8 @@ extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, 
   const float inv = 1.f / temperature;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   HeadRows r{};
-  r.hidden = reinterpret_cast<const bf16*>(hidden), r.bs = batch_stride, r.rs = row_stride, r.S = S;
-  r.labels = labels, r.rows = rows, r.ignore = ignore_index, r.H = H, r.V = V;
+  r.src = HeadSource{reinterpret_cast<const bf16*>(hidden), batch_stride, row_stride, S, labels, rows, ignore_index};
+  r.H = H, r.V = V;
   r.count = reinterpret_cast<int*>(ws + s.count), r.pos = reinterpret_cast<int*>(ws + s.pos);
   r.index = reinterpret_cast<int*>(ws + s.index), r.target = reinterpret_cast<int*>(ws + s.target);
   r.hc = reinterpret_cast<bf16*>(ws + s.hc);
@@ -735,26 +951,29 @@ extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, 
   p.hc = r.hc, p.w = reinterpret_cast<const bf16*>(weight), p.rows = rows, p.V = V, p.H = H;
   p.count = r.count, p.target = r.target, p.c = inv * kLog2e, p.coef = r.coef;
   p.dz = reinterpret_cast<bf16*>(ws + s.dz), p.ldz = s.ldz;
-  p.dw = reinterpret_cast<bf16*>(dweight), p.dh = reinterpret_cast<float*>(ws + s.dh), p.slabs = s.slabs;
-  const int bn = head_bn(rows), nh = (H + HD_BM - 1) / HD_BM;
-  const int64_t nn = (rows + bn - 1) / bn;
-  if (((int64_t)s.vc / 256 + 1) * (nn > nh ? nn : nh) > INT32_MAX / 2 || nn * s.slabs * nh > INT32_MAX / 2)
+  p.dw = reinterpret_cast<bf16*>(dweight), p.dh = reinterpret_cast<float*>(ws + s.dh), p.vmax = s.vc;
+  const bool few = head_few(rows);
+  const int bm = few ? Few::BM : Wide::BM, bn = few ? Few::BN : Wide::BN, nh = (H + bm - 1) / bm;
+  const int64_t nn = (rows + bn - 1) / bn, nw = (H + Wide::BM - 1) / Wide::BM;
+  if (((int64_t)s.vc / bm + 1) * nn > INT32_MAX / 2 || nn * nh * HD_CUS > INT32_MAX / 2 ||
+      ((int64_t)s.vc / Wide::BN + 1) * nw > INT32_MAX / 2)
     return nq_fail(NQ_ERR_UNSUPPORTED, "too many tiles for one launch");
   for (int v0 = 0; v0 < V; v0 += s.vc) {
     p.v0 = v0, p.vc = V - v0 < s.vc ? V - v0 : s.vc, p.add = v0 > 0;
-    const int nv = (p.vc + 255) / 256;
-    int rc = bn == 64 ? head_launch(head_logits_kernel<64, true>, head_grid(nv, nn), bn, st, p)
-                      : head_launch(head_logits_kernel<256, true>, head_grid(nv, nn), bn, st, p);
-    if (!rc && dhidden)
-      rc = bn == 64 ? head_launch(head_dh_kernel<64>, head_grid(nh, nn * s.slabs), bn, st, p)
-                    : head_launch(head_dh_kernel<256>, head_grid(nh, nn * s.slabs), bn, st, p);
-    if (!rc && dweight) rc = head_launch(head_dw_kernel, head_grid(nh, nv), 256, st, p);
+    const int64_t logits = (p.vc + bm - 1) / bm * nn;
+    int rc = few ? launch_logits<Few, true>(logits, st, p) : launch_logits<Wide, true>(logits, st, p);
+    // as many workgroups as the CUs hold: how many tiles there are goes by the kept rows
+    if (!rc && dhidden) rc = few ? launch_dh<Few>(INT32_MAX / 2, st, p) : launch_dh<Wide>(INT32_MAX / 2, st, p);
+    if (!rc && dweight) {
+      const int64_t tiles = nw * ((p.vc + Wide::BN - 1) / Wide::BN);
+      rc = head_launch<Product<Wide, false, false>>(head_dw_kernel, head_grid<Wide>(tiles), threads_of<Wide>(), st, p);
+    }
     if (rc) return rc;
   }
   if (dhidden) {
+    const HeadOut o{p.dh, r.count, r.pos, reinterpret_cast<bf16*>(dhidden), rows, H, bm, bn, s.vc};
     const int64_t n = rows * (H / 8);
-    hipLaunchKernelGGL(head_dh_out_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p.dh, s.slabs, rows, H,
-                       r.pos, reinterpret_cast<bf16*>(dhidden));
+    hipLaunchKernelGGL(head_dh_out_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, o);
   }
   return nq_check_launch(hipGetLastError());
 }

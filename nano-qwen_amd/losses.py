@@ -30,8 +30,8 @@ _KINDS = {"sigmoid": _lib.NQ_PREF_SIGMOID, "hinge": _lib.NQ_PREF_HINGE, "ipo": _
 
 
 # The device takes less than the host for most of these calls, and the backward's Python runs
-# on autograd's own thread, where it takes some three times as long as alone: operands that
-# need no gradient go through ``apply`` as one tuple, and little stands around a launch.
+# on autograd's own thread, where it takes some three times as long as alone: what needs no
+# gradient goes round autograd or through it as one tuple, and little stands around a launch.
 
 def _launch(t: torch.Tensor, fn, name: str, *args) -> None:
     """fn(*args, stream) on t's device (a launch goes to the current one)."""
@@ -56,12 +56,23 @@ def _first_order(backward):
     return call
 
 
+def _takes_gradient(*ts: torch.Tensor) -> bool:
+    """Whether autograd has a part in the call (forward mode: it refuses it)."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                return True
+    return ops._forward_ad._current_level >= 0
+
+
 def _check_devices(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    ops._require_device(first, *others)
-    index = first.get_device()
+    index = first.get_device()  # -1: on the host
     for t in others:
         if t is not None and t.get_device() != index:
+            ops._require_device(first, t)
             raise ValueError(f"the operands lie on different devices: {first.device} and {t.device}")
+    if index < 0 or not first.is_cuda:
+        ops._require_device(first)
 
 
 def _check_temperature(temperature: float) -> float:
@@ -74,9 +85,11 @@ def _check_temperature(temperature: float) -> float:
 def _check_labels(labels: torch.Tensor, rows_shape) -> torch.Tensor:
     if labels.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"labels must be int64 or int32, got {labels.dtype}")
-    if tuple(labels.shape) != tuple(rows_shape):
+    if labels.shape != rows_shape:
         raise ValueError(f"labels {tuple(labels.shape)} must hold one label per row {tuple(rows_shape)}")
-    return labels.to(torch.int64).contiguous()
+    if labels.dtype != torch.int64:
+        labels = labels.to(torch.int64)
+    return labels if labels.is_contiguous() else labels.contiguous()
 
 
 # ---------------------------------------------------------------------------
@@ -102,22 +115,25 @@ def _rows_2d(x: torch.Tensor):
     return x, x.shape[0], x.shape[1], x.stride(0), x.stride(1)
 
 
+def _token_forward(logits, labels, temperature: float, ignore_index: int):
+    x, B, S, bs, rs = _rows_2d(logits)
+    V = x.shape[-1]
+    out = x.new_empty(labels.shape, dtype=torch.float32)
+    stats = x.new_empty((B * S, 2), dtype=torch.float32)
+    lib = _lib.load()
+    nbytes = lib.nq_token_logprobs_workspace_bytes(B * S, V)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    tail = (B, S, V, ops._code(x), temperature, ignore_index)
+    _launch(x, lib.nq_token_logprobs, "nq_token_logprobs", x.data_ptr(), bs, rs, labels.data_ptr(), out.data_ptr(),
+            stats.data_ptr(), ops._ptr(ws), nbytes, *tail)
+    return out, stats, tail
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, rest):
-        labels, temperature, ignore_index = rest
-        x, B, S, bs, rs = _rows_2d(logits)
-        V = x.shape[-1]
-        out = x.new_empty(labels.shape, dtype=torch.float32)
-        stats = x.new_empty((B * S, 2), dtype=torch.float32)
-        lib = _lib.load()
-        nbytes = lib.nq_token_logprobs_workspace_bytes(B * S, V)
-        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        tail = (B, S, V, ops._code(x), temperature, ignore_index)
-        _launch(x, lib.nq_token_logprobs, "nq_token_logprobs", ops._ptr(x), bs, rs, ops._ptr(labels), ops._ptr(out),
-                ops._ptr(stats), ops._ptr(ws), nbytes, *tail)
-        ctx.save_for_backward(logits, labels, stats)
-        ctx.tail = tail
+        out, stats, ctx.tail = _token_forward(logits, *rest)
+        ctx.save_for_backward(logits, rest[0], stats)
         return out
 
     @staticmethod
@@ -147,30 +163,37 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
     than slice the logits: the gradient of a slice is a second pass over all of them.
     """
     _check_devices(logits, labels)
-    ops._code(logits)
+    if logits.dtype not in ops._DTYPES:
+        ops._code(logits)
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError(f"logits need a last axis of at least one element, got shape {tuple(logits.shape)}")
     labels = _check_labels(labels, logits.shape[:-1])
     temperature = _check_temperature(temperature)
     if labels.numel() == 0:
         return logits.sum(-1).float()  # empty, with logits' place in the graph
-    return _TokenLogprobs.apply(logits, (labels, temperature, int(ignore_index)))
+    rest = labels, temperature, int(ignore_index)
+    return _TokenLogprobs.apply(logits, rest) if _takes_gradient(logits) else _token_forward(logits, *rest)[0]
+
+
+def _linear_forward(hidden, weight, labels, temperature: float, ignore_index: int):
+    x, w, B, S, bs, rs = _head_operands(hidden, weight)
+    V, H = w.shape
+    out = x.new_empty(labels.shape, dtype=torch.float32)
+    stats = x.new_empty((B * S, 2), dtype=torch.float32)
+    lib = _lib.load()
+    nbytes = lib.nq_linear_logprobs_workspace_bytes(B * S, V, H)
+    ws = x.new_empty(nbytes, dtype=torch.uint8)
+    _launch(x, lib.nq_linear_logprobs, "nq_linear_logprobs", x.data_ptr(), bs, rs, w.data_ptr(), labels.data_ptr(),
+            out.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes, B, S, V, H, temperature, ignore_index)
+    return out, stats
 
 
 class _LinearLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, rest):
-        labels, temperature, ignore_index = rest
-        x, w, B, S, bs, rs = _head_operands(hidden, weight)
-        V, H = w.shape
-        out = x.new_empty(labels.shape, dtype=torch.float32)
-        stats = x.new_empty((B * S, 2), dtype=torch.float32)
-        lib = _lib.load()
-        ws = x.new_empty(lib.nq_linear_logprobs_workspace_bytes(B * S, V, H), dtype=torch.uint8)
-        _launch(x, lib.nq_linear_logprobs, "nq_linear_logprobs", x.data_ptr(), bs, rs, w.data_ptr(), labels.data_ptr(),
-                out.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(), B, S, V, H, temperature, ignore_index)
-        ctx.save_for_backward(hidden, weight, labels, stats)
-        ctx.tail = temperature, ignore_index
+        out, stats = _linear_forward(hidden, weight, *rest)
+        ctx.save_for_backward(hidden, weight, rest[0], stats)
+        ctx.tail = rest[1:]
         return out
 
     @staticmethod
@@ -183,10 +206,11 @@ class _LinearLogprobs(torch.autograd.Function):
         dh = x.new_empty(hidden.shape) if ctx.needs_input_grad[0] else None
         dw = w.new_empty((V, H)) if ctx.needs_input_grad[1] else None
         lib = _lib.load()
-        ws = x.new_empty(lib.nq_linear_logprobs_bwd_workspace_bytes(B * S, V, H), dtype=torch.uint8)
+        nbytes = lib.nq_linear_logprobs_bwd_workspace_bytes(B * S, V, H)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
         _launch(x, lib.nq_linear_logprobs_bwd, "nq_linear_logprobs_bwd", x.data_ptr(), bs, rs, w.data_ptr(),
                 labels.data_ptr(), stats.data_ptr(), dy.data_ptr(), ops._ptr(dh), ops._ptr(dw), ws.data_ptr(),
-                ws.numel(), B, S, V, H, *ctx.tail)
+                nbytes, B, S, V, H, *ctx.tail)
         return dh, dw, None
 
 
@@ -226,7 +250,10 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
         return torch.nn.functional.linear(hidden, weight)[..., 0].float()  # empty, with its place in the graph
     if labels.numel() > _HEAD_MOST or V > _HEAD_MOST:
         raise ValueError(f"at most 2^24 rows and entries in one call, got {labels.numel()} and {V}")
-    return _LinearLogprobs.apply(hidden, weight, (labels, temperature, int(ignore_index)))
+    rest = labels, temperature, int(ignore_index)
+    if _takes_gradient(hidden, weight):
+        return _LinearLogprobs.apply(hidden, weight, rest)
+    return _linear_forward(hidden, weight, *rest)[0]
 
 
 _HEAD_MOST = 1 << 24
@@ -240,22 +267,25 @@ def _token_rows(t: Optional[torch.Tensor], name: str, shape) -> Optional[torch.T
     """(B, S) fp32 rows with contiguous tokens, of (B, S) or (B,)."""
     if t is None:
         return None
-    if t.dtype not in ops._DTYPES:
-        raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.dtype != torch.float32:
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+        t = t.float()
+    if t.shape != shape:
         raise ValueError(f"{name} {tuple(t.shape)} must be shaped like its log-probabilities {tuple(shape)}")
-    return _rows(t.float() if t.dtype != torch.float32 else t)
+    return _rows(t)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    t = t if t.dim() == 2 else t[:, None]
+    if t.dim() == 1:
+        return t[:, None]
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
 def _mask_rows(mask: Optional[torch.Tensor], name: str, shape) -> Optional[torch.Tensor]:
     if mask is None:
         return None
-    if tuple(mask.shape) != tuple(shape):
+    if mask.shape != shape:
         raise ValueError(f"{name} {tuple(mask.shape)} must be shaped like its log-probabilities {tuple(shape)}")
     return _rows(mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0)
 
@@ -268,31 +298,32 @@ def _with_pitch(*ts: Optional[torch.Tensor]):
     return args
 
 
+def _preference_forward(chosen, rejected, rest):
+    """(loss, coef); rest: the rewards, which it writes, the references, the masks and the numbers."""
+    reward_c, reward_r, ref_chosen, ref_rejected, chosen_mask, rejected_mask, kind, beta, smoothing, average = rest
+    B, Sc = chosen.shape
+    loss, coef = chosen.new_empty(()), chosen.new_empty((2, B))
+    lib = _lib.load()
+    nbytes = lib.nq_preference_loss_workspace_bytes(B)
+    ws = chosen.new_empty(nbytes, dtype=torch.uint8)
+    _launch(chosen, lib.nq_preference_loss, "nq_preference_loss",
+            *_with_pitch(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask), loss.data_ptr(),
+            reward_c.data_ptr(), reward_r.data_ptr(), coef.data_ptr(), ws.data_ptr(), nbytes, B, Sc,
+            rejected.shape[1], kind, beta, smoothing, average)
+    return loss, coef
+
+
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, chosen, rejected, rest):
-        ref_chosen, ref_rejected, chosen_mask, rejected_mask, kind, beta, smoothing, average = rest
-        (B, Sc), Sr = chosen.shape, rejected.shape[1]
-        loss, reward_c, reward_r = chosen.new_empty(()), chosen.new_empty(B), chosen.new_empty(B)
-        lib = _lib.load()
-        nbytes = lib.nq_preference_loss_workspace_bytes(B)
-        coef = chosen.new_empty((2, B))
-        ws = chosen.new_empty(nbytes, dtype=torch.uint8)
-        _launch(chosen, lib.nq_preference_loss, "nq_preference_loss",
-                *_with_pitch(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask), loss.data_ptr(),
-                reward_c.data_ptr(), reward_r.data_ptr(), coef.data_ptr(), ws.data_ptr(), nbytes, B, Sc, Sr, kind,
-                beta, smoothing, average)
-        ctx.save_for_backward(coef, chosen_mask, rejected_mask)
-        ctx.sizes = B, Sc, Sr
-        ctx.mark_non_differentiable(reward_c, reward_r)
-        ctx.set_materialize_grads(False)  # no zeros for the rewards' gradients
-        return loss, reward_c, reward_r
+        loss, coef = _preference_forward(chosen, rejected, rest)
+        ctx.save_for_backward(coef, rest[4], rest[5])
+        ctx.sizes = *chosen.shape, rejected.shape[1]
+        return loss
 
     @staticmethod
     @_first_order
-    def backward(ctx, dloss, *_):
-        if dloss is None:
-            return None, None, None
+    def backward(ctx, dloss):
         coef, chosen_mask, rejected_mask = ctx.saved_tensors
         B, Sc, Sr = ctx.sizes
         need = ctx.needs_input_grad
@@ -339,41 +370,46 @@ def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: Op
         raise ValueError(f"chosen and rejected must hold the same number of sequences, at least one, "
                          f"got {chosen.shape[0]} and {rejected.shape[0]}")
     sc, sr = chosen.shape, rejected.shape
-    return _PreferenceLoss.apply(
-        _token_rows(chosen, "chosen", sc), _token_rows(rejected, "rejected", sr),
-        (_token_rows(_detached(ref_chosen), "ref_chosen", sc), _token_rows(_detached(ref_rejected), "ref_rejected", sr),
-         _mask_rows(chosen_mask, "chosen_mask", sc), _mask_rows(rejected_mask, "rejected_mask", sr),
-         _KINDS[kind], float(beta), float(label_smoothing), int(bool(average))))
+    chosen, rejected = _token_rows(chosen, "chosen", sc), _token_rows(rejected, "rejected", sr)
+    rewards = chosen.new_empty(sc[0]), chosen.new_empty(sc[0])
+    rest = (*rewards, _token_rows(_detached(ref_chosen), "ref_chosen", sc),
+            _token_rows(_detached(ref_rejected), "ref_rejected", sr), _mask_rows(chosen_mask, "chosen_mask", sc),
+            _mask_rows(rejected_mask, "rejected_mask", sr), _KINDS[kind], float(beta), float(label_smoothing),
+            int(bool(average)))
+    if _takes_gradient(chosen, rejected):
+        return (_PreferenceLoss.apply(chosen, rejected, rest), *rewards)
+    return (_preference_forward(chosen, rejected, rest)[0], *rewards)
 
 
 def _detached(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t.detach() if t is not None and t.requires_grad else t
 
 
+def _policy_forward(lp, rest):
+    """(loss, weight); rest: kl and clipped, which it writes, the other operands and the numbers."""
+    kl, clipped, old, ref, adv, mask, low, high, kl_coef, mean_of_means = rest
+    B, S = lp.shape
+    loss, weight = lp.new_empty(()), lp.new_empty(B)
+    lib = _lib.load()
+    nbytes = lib.nq_policy_loss_workspace_bytes(B, S)
+    ws = lp.new_empty(nbytes, dtype=torch.uint8)
+    _launch(lp, lib.nq_policy_loss, "nq_policy_loss", *_with_pitch(lp, old, ref, adv), adv.dim() - 1,
+            *_with_pitch(mask), loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(), weight.data_ptr(),
+            ws.data_ptr(), nbytes, B, S, low, high, kl_coef, mean_of_means)
+    return loss, weight
+
+
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, lp, rest):
-        old, ref, adv, mask, low, high, kl_coef, mean_of_means = rest
-        B, S = lp.shape
-        loss, kl, clipped = lp.new_empty(()), lp.new_empty(()), lp.new_empty(())
-        weight = lp.new_empty(B)
-        lib = _lib.load()
-        nbytes = lib.nq_policy_loss_workspace_bytes(B, S)
-        ws = lp.new_empty(nbytes, dtype=torch.uint8)
-        _launch(lp, lib.nq_policy_loss, "nq_policy_loss", *_with_pitch(lp, old, ref, adv), adv.dim() - 1,
-                *_with_pitch(mask), loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(), weight.data_ptr(),
-                ws.data_ptr(), nbytes, B, S, low, high, kl_coef, mean_of_means)
-        ctx.save_for_backward(lp, old, ref, adv, mask, weight)
-        ctx.tail = B, S, low, high, kl_coef
-        ctx.mark_non_differentiable(kl, clipped)
-        ctx.set_materialize_grads(False)
-        return loss, kl, clipped
+        loss, weight = _policy_forward(lp, rest)
+        ctx.save_for_backward(lp, *rest[2:6], weight)
+        ctx.tail = *lp.shape, *rest[6:9]
+        return loss
 
     @staticmethod
     @_first_order
-    def backward(ctx, dloss, *_):
-        if dloss is None:
-            return None, None
+    def backward(ctx, dloss):
         lp, old, ref, adv, mask, weight = ctx.saved_tensors
         grad = weight.new_empty(lp.shape)
         _launch(weight, _lib.load().nq_policy_loss_bwd, "nq_policy_loss_bwd", *_with_pitch(lp, old, ref, adv),
@@ -418,8 +454,11 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
         adv = _token_rows(adv, "advantages", shape[:1])[:, 0]
     else:
         adv = _token_rows(adv, "advantages", shape)
-    return _PolicyLoss.apply(
-        _token_rows(logprobs, "logprobs", shape),
-        (_token_rows(_detached(old_logprobs), "old_logprobs", shape),
-         _token_rows(_detached(ref_logprobs), "ref_logprobs", shape), adv, _mask_rows(mask, "mask", shape),
-         float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence")))
+    lp = _token_rows(logprobs, "logprobs", shape)
+    stats = lp.new_empty(()), lp.new_empty(())
+    rest = (*stats, _token_rows(_detached(old_logprobs), "old_logprobs", shape),
+            _token_rows(_detached(ref_logprobs), "ref_logprobs", shape), adv, _mask_rows(mask, "mask", shape),
+            float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence"))
+    if _takes_gradient(lp):
+        return (_PolicyLoss.apply(lp, rest), *stats)
+    return (_policy_forward(lp, rest)[0], *stats)
