@@ -516,28 +516,36 @@ int nq_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t row_
                           int64_t ignore_index, void* stream);
 
 /*
- * The same log-probabilities from hidden states and an LM head, without the logits: z =
+ * The same log-probabilities from hidden states and an LM head, without its logits: z =
  * hidden weight^T / temperature, hidden B * S rows of H bf16 elements at b * batch_stride +
  * s * row_stride (16-byte aligned, strides multiples of 8), weight (V, H) bf16 contiguous; H
  * a multiple of 8.  Ignored rows cost nothing beyond their zeros.  workspace:
  * nq_linear_logprobs_workspace_bytes(B * S, V, H), 256-byte aligned.
  *
- * The backward forms dz = dlogprobs[n] (1[v = label] - softmax) / temperature again, in
- * bf16, a range of the vocabulary at a time, and writes dhidden = dz weight (B * S, H) and
- * dweight = dz^T hidden (V, H), bf16, contiguous, both summed in fp32 (NULL: left out).
- * workspace: nq_linear_logprobs_bwd_workspace_bytes.
+ * kept: NULL, or nq_linear_logprobs_kept_bytes(B * S, V, H) bytes, 256-byte aligned, that the
+ * forward fills (2 bytes a logit) and the backward of the same operands takes: it saves a
+ * quarter of the products.  0 bytes: nothing is kept for these sizes (at most 64 rows, or
+ * more than 4 GiB).
+ *
+ * The backward forms dz = dlogprobs[n] (1[v = label] - softmax) / temperature in bf16, a
+ * range of the vocabulary at a time, from kept or from the products again, and writes
+ * dhidden = dz weight (B * S, H) and dweight = dz^T hidden (V, H), bf16, contiguous, both
+ * summed in fp32 (NULL: left out).  workspace: nq_linear_logprobs_bwd_workspace_bytes.
  */
 int64_t nq_linear_logprobs_workspace_bytes(int64_t rows, int V, int H);
+int64_t nq_linear_logprobs_kept_bytes(int64_t rows, int V, int H);
 int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int64_t row_stride,
                        const void* weight, const int64_t* labels, float* logprobs, float* stats,
-                       void* workspace, int64_t workspace_bytes, int64_t B, int64_t S, int V, int H,
-                       float temperature, int64_t ignore_index, void* stream);
+                       void* kept, int64_t kept_bytes, void* workspace, int64_t workspace_bytes,
+                       int64_t B, int64_t S, int V, int H, float temperature, int64_t ignore_index,
+                       void* stream);
 int64_t nq_linear_logprobs_bwd_workspace_bytes(int64_t rows, int V, int H);
 int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, int64_t row_stride,
                            const void* weight, const int64_t* labels, const float* stats,
-                           const float* dlogprobs, void* dhidden, void* dweight, void* workspace,
-                           int64_t workspace_bytes, int64_t B, int64_t S, int V, int H,
-                           float temperature, int64_t ignore_index, void* stream);
+                           const void* kept, int64_t kept_bytes, const float* dlogprobs,
+                           void* dhidden, void* dweight, void* workspace, int64_t workspace_bytes,
+                           int64_t B, int64_t S, int V, int H, float temperature,
+                           int64_t ignore_index, void* stream);
 
 /*
  * Preference loss over B pairs of sequences.  Each side: fp32 log-probabilities of its

@@ -198,16 +198,17 @@ SIGNATURES = {
         _f32, _i64, _p,                              # temperature, ignore_index, stream
     ]),
     "nq_linear_logprobs_workspace_bytes": (_i64, [_i64, _i32, _i32]),  # rows, V, H
+    "nq_linear_logprobs_kept_bytes": (_i64, [_i64, _i32, _i32]),  # rows, V, H
     "nq_linear_logprobs": (_i32, [
         _p, _i64, _i64, _p, _p,                      # hidden, batch_stride, row_stride, weight, labels
-        _p, _p, _p, _i64,                            # logprobs, stats, workspace, workspace_bytes
+        _p, _p, _p, _i64, _p, _i64,                  # logprobs, stats, kept, bytes, workspace, bytes
         _i64, _i64, _i32, _i32,                      # B, S, V, H
         _f32, _i64, _p,                              # temperature, ignore_index, stream
     ]),
     "nq_linear_logprobs_bwd_workspace_bytes": (_i64, [_i64, _i32, _i32]),  # rows, V, H
     "nq_linear_logprobs_bwd": (_i32, [
         _p, _i64, _i64, _p, _p,                      # hidden, batch_stride, row_stride, weight, labels
-        _p, _p, _p, _p, _p, _i64,                    # stats, dlogprobs, dhidden, dweight, workspace, bytes
+        _p, _p, _i64, _p, _p, _p, _p, _i64,          # stats, kept, bytes, dlogprobs, dhidden, dweight, workspace, bytes
         _i64, _i64, _i32, _i32,                      # B, S, V, H
         _f32, _i64, _p,                              # temperature, ignore_index, stream
     ]),

@@ -400,6 +400,9 @@ struct HeadParams {
   float c;       // log2(e) / T
   floatx2* part;  // forward: (vocabulary tiles, rows) partial (m, l)
   float* zlabel;
+  bf16* exps;    // kept for the backward: (rows, ldv) 2^((z - m) c) of the m of their 128 entries
+  float* exps_m;  // (groups of 128, rows)
+  int64_t ldv;
   const floatx4* coef;  // backward
   bf16* dz;      // (rows, ldz): this range's v0 .. v0 + vc
   int64_t ldz;
@@ -411,14 +414,15 @@ struct HeadParams {
 
 // ---------------------------------------------------------------------------
 // z = hc w^T, vocabulary on the row axis: a lane holds one token's 64 (or 16) vocabulary
-// entries of each block, so their maximum and sum need no shuffles but one.  DZ: dz of a
-// range of the vocabulary instead of the statistics.
-template <class C, bool DZ, bool GATHER = false>
+// entries of each block, so their maximum and sum need no shuffles but one.  KEEP: the
+// exponentials too, for the backward; DZ: dz of a range of the vocabulary instead.
+enum { STATS, KEEP, DZ };
+template <class C, int MODE, bool GATHER = false>
 __global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams p) {
   typedef Product<C, true, true, GATHER> P;
   extern __shared__ __align__(1024) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int vend = DZ ? p.v0 + p.vc : p.V, vfirst = DZ ? p.v0 : 0;
+  const int vend = MODE == DZ ? p.v0 + p.vc : p.V, vfirst = MODE == DZ ? p.v0 : 0;
   // GATHER: the kept rows and their labels in the waves' own LDS, where nothing else lies before
   // the first epilogue, and the labels in registers from there on
   int* few_index = reinterpret_cast<int*>(lds + P::PRIVATE);
@@ -468,12 +472,13 @@ __global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams
     prod.run(a, b, more, na, nb, acc);
 
     const int n0 = tn * C::BN, v0 = vfirst + tm * C::BM;
-    if (!DZ) {
-      static_assert(C::M * C::BN * 8 <= P::LDS - P::PRIVATE, "room for the waves' statistics");
-      floatx2* red = reinterpret_cast<floatx2*>(lds + P::PRIVATE);
+    if (MODE != DZ) {
+      // a wave's statistics in its own LDS
+      static_assert(C::NT * 32 * 8 <= P::OWN, "room for the waves' statistics");
+      floatx2 st[C::NT];
 #pragma unroll
       for (int j = 0; j < C::NT; ++j) {
-        const int nl = wn * (C::NT * 32) + j * 32 + (lane & 31), n = n0 + nl;
+        const int n = n0 + wn * (C::NT * 32) + j * 32 + (lane & 31);
         const int y = GATHER ? few_target[j] : n < count ? p.target[n] : -1;
         const int at = y - v0 - vw;  // the label's entry relative to the lane's first
         if (wave_any(y >= 0 && at >= 0 && at < C::MT * 32 && !(at & 4))) {
@@ -501,17 +506,39 @@ __global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams
 #pragma unroll
         for (int i = 0; i < C::MT; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) l += fast_exp2((acc[i][j][e] - base) * p.c);
+          for (int e = 0; e < 16; ++e) {
+            const float x = fast_exp2((acc[i][j][e] - base) * p.c);
+            l += x;
+            if (MODE == KEEP) acc[i][j][e] = x;
+          }
         l = xor32_sum(l);
-        if (lane < 32) red[wm * C::BN + nl] = floatx2{m, l};
+        st[j] = floatx2{m, l};
+        if (MODE == KEEP && lane < 32 && n < count) p.exps_m[(int64_t)(tm * C::M + wm) * p.rows + n] = m;
       }
-      __syncthreads();  // the next write to `red` follows the next tile's barriers
+      if (MODE == KEEP) {
+        static_assert(MODE != KEEP || C::MT * 32 == 128, "a maximum per 128 entries");
+        const int64_t col0 = (int64_t)tm * C::BM + wm * (C::MT * 32);
+        prod.store(
+            [&](int j, int i, int q) {
+              return floatx4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+            },
+            [&](int r) {
+              const int n = n0 + wn * (C::NT * 32) + r;
+              return n < count ? p.exps + (int64_t)n * p.ldv + col0 : nullptr;
+            },
+            p.ldv - col0);
+      }
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j)
+        if (lane < 32) reinterpret_cast<floatx2*>(lds + P::PRIVATE + wave * P::OWN)[j * 32 + lane] = st[j];
+      __syncthreads();  // the next writes there follow the next tile's barriers
       for (int nl = threadIdx.x; nl < C::BN; nl += threads_of<C>()) {
         if (n0 + nl < count) {
           RowStat s{-INFINITY, 0.f};
 #pragma unroll
           for (int i = 0; i < C::M; ++i) {
-            const floatx2 v = red[i * C::BN + nl];
+            const int w = i * C::N + nl / (C::NT * 32);
+            const floatx2 v = reinterpret_cast<const floatx2*>(lds + P::PRIVATE + w * P::OWN)[nl % (C::NT * 32)];
             s = join(s, RowStat{v[0], v[1]}, p.c);
           }
           p.part[(int64_t)tm * p.rows + n0 + nl] = floatx2{s.m, s.l};
@@ -548,6 +575,37 @@ __global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams
     if (!more) break;
     a = na, b = nb, tm = um, tn = un;
     t.w += t.step;
+  }
+}
+
+// dz of a range from the exponentials that the forward kept: a pass over both, bound by HBM,
+// in place of the range's product.  A kept exponential is half a step of bf16 off; the
+// label's own, which the label's gradient is one less than, comes from its fp32 logit.
+__global__ __launch_bounds__(256) void head_dz_kernel(HeadParams p) {
+  const int count = *p.count;
+  const unsigned across = (p.vc + 2047) / 2048, group = blockIdx.x / across;
+  const int col = (int)((blockIdx.x - group * across) * 256 + threadIdx.x) * 8;
+  if (col >= p.vc) return;
+  const int v = p.v0 + col;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t n = (int64_t)group * 4 + u;
+    if (n < count) {
+      const floatx4 k = p.coef[n];
+      const floatx8 x = Vec8<bf16>::load_f32(p.exps + n * p.ldv + v);
+      const float f = k[1] * fast_exp2((p.exps_m[(int64_t)(v >> 7) * p.rows + n] - k[0]) * p.c);
+      floatx8 d;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = f * x[e];
+      const int at = p.target[n] - v;
+      if (at >= 0 && at < 8) {
+        const float own = k[1] * fast_exp2((p.zlabel[n] - k[0]) * p.c) + k[2];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e == at) d[e] = own;
+      }
+      store8<bf16>(p.dz + n * p.ldz + col, d);
+    }
   }
 }
 
@@ -784,6 +842,24 @@ struct HeadSpace {
 
 constexpr int64_t HD_DZ_BYTES = (int64_t)1 << 30;  // the largest range's dz
 
+// What a forward keeps for its backward: the labels' logits, the maxima of each 128 entries
+// and the exponentials.  Up to 4 GiB (1.4% of the memory), and beyond 64 rows: a product of so
+// few is bound by the weights' bytes, of which this would save one pass in four.
+struct HeadKept {
+  int64_t zlabel, m, exps, total, ldv;
+};
+constexpr int64_t HD_KEPT_BYTES = (int64_t)4 << 30;
+
+static HeadKept head_kept(int64_t rows, int V) {
+  HeadKept k{};
+  k.ldv = (V + 7) / 8 * 8;
+  k.m = pad256(rows * 4);
+  k.exps = k.m + pad256(rows * ((V + 255) / 256 * 2) * 4);
+  k.total = k.exps + pad256(rows * k.ldv * 2);
+  if (head_few(rows) || k.total > HD_KEPT_BYTES) k.total = 0;
+  return k;
+}
+
 static HeadSpace head_space(int64_t rows, int V, int H, bool backward) {
   HeadSpace s{};
   const int64_t bm = head_few(rows) ? Few::BM : Wide::BM, bn = head_few(rows) ? Few::BN : Wide::BN;
@@ -830,13 +906,16 @@ static bool head_sizes_ok(int64_t rows, int V, int H) {
 extern "C" int64_t nq_linear_logprobs_workspace_bytes(int64_t rows, int V, int H) {
   return head_sizes_ok(rows, V, H) ? head_space(rows, V, H, false).total : 0;
 }
+extern "C" int64_t nq_linear_logprobs_kept_bytes(int64_t rows, int V, int H) {
+  return head_sizes_ok(rows, V, H) ? head_kept(rows, V).total : 0;
+}
 extern "C" int64_t nq_linear_logprobs_bwd_workspace_bytes(int64_t rows, int V, int H) {
   return head_sizes_ok(rows, V, H) ? head_space(rows, V, H, true).total : 0;
 }
 
 static int head_check(const void* hidden, int64_t bs, int64_t rs, const void* weight, const int64_t* labels,
-                      const void* stats, const void* workspace, int64_t workspace_bytes, int64_t B, int64_t S, int V,
-                      int H, float temperature, bool backward) {
+                      const void* stats, const void* kept, int64_t kept_bytes, const void* workspace,
+                      int64_t workspace_bytes, int64_t B, int64_t S, int V, int H, float temperature, bool backward) {
   if (B <= 0 || S <= 0 || V <= 0 || H <= 0)
     return nq_fail(NQ_ERR_INVALID, "sizes must be positive (B=%lld S=%lld V=%d H=%d)", (long long)B, (long long)S, V, H);
   if (H % 8) return nq_fail(NQ_ERR_UNSUPPORTED, "the width must be a multiple of 8, got %d", H);
@@ -851,11 +930,22 @@ static int head_check(const void* hidden, int64_t bs, int64_t rs, const void* we
   const float inv = 1.f / temperature;
   if (!(temperature > 0.f) || !isfinite(temperature) || !isfinite(inv * kLog2e))
     return nq_fail(NQ_ERR_INVALID, "the temperature must be positive and finite, and so must its reciprocal");
+  const int64_t keeps = head_kept(B * S, V).total;
+  if (kept && (!keeps || kept_bytes < keeps || (reinterpret_cast<uintptr_t>(kept) & 255u)))
+    return nq_fail(NQ_ERR_WORKSPACE, "kept too small or not 256-byte aligned: %lld bytes, need %lld (0: none is kept)",
+                   (long long)kept_bytes, (long long)keeps);
   const int64_t need = head_space(B * S, V, H, backward).total;
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return nq_fail(NQ_ERR_WORKSPACE, "workspace too small or not 256-byte aligned: %lld bytes, need %lld",
                    (long long)workspace_bytes, (long long)need);
   return NQ_OK;
+}
+
+static void head_kept_at(void* kept, int64_t rows, int V, HeadParams* p) {
+  const HeadKept k = head_kept(rows, V);
+  char* at = reinterpret_cast<char*>(kept);
+  p->zlabel = reinterpret_cast<float*>(at + k.zlabel), p->exps_m = reinterpret_cast<float*>(at + k.m);
+  p->exps = reinterpret_cast<bf16*>(at + k.exps), p->ldv = k.ldv;
 }
 
 // A launch with P's dynamic LDS (the attribute belongs to the kernel on the device; setting it
@@ -868,9 +958,9 @@ static int head_launch(K kernel, int grid, int threads, hipStream_t st, const He
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3((unsigned)threads), P::LDS, st, p);
   return nq_check_launch(hipGetLastError());
 }
-template <class C, bool DZ, bool GATHER = false>
+template <class C, int MODE, bool GATHER = false>
 static int launch_logits(int64_t tiles, hipStream_t st, const HeadParams& p) {
-  return head_launch<Product<C, true, true, GATHER>>(head_logits_kernel<C, DZ, GATHER>, head_grid<C>(tiles),
+  return head_launch<Product<C, true, true, GATHER>>(head_logits_kernel<C, MODE, GATHER>, head_grid<C>(tiles),
                                                      threads_of<C>(), st, p);
 }
 template <class C>
@@ -879,12 +969,12 @@ static int launch_dh(int64_t tiles, hipStream_t st, const HeadParams& p) {
 }
 
 extern "C" int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int64_t row_stride, const void* weight,
-                                  const int64_t* labels, float* logprobs, float* stats, void* workspace,
-                                  int64_t workspace_bytes, int64_t B, int64_t S, int V, int H, float temperature,
-                                  int64_t ignore_index, void* stream) {
+                                  const int64_t* labels, float* logprobs, float* stats, void* kept,
+                                  int64_t kept_bytes, void* workspace, int64_t workspace_bytes, int64_t B, int64_t S,
+                                  int V, int H, float temperature, int64_t ignore_index, void* stream) {
   nq_clear_error();
-  if (int rc = head_check(hidden, batch_stride, row_stride, weight, labels, stats, workspace, workspace_bytes, B, S, V,
-                          H, temperature, false))
+  if (int rc = head_check(hidden, batch_stride, row_stride, weight, labels, stats, kept, kept_bytes, workspace,
+                          workspace_bytes, B, S, V, H, temperature, false))
     return rc;
   if (!logprobs || (reinterpret_cast<uintptr_t>(logprobs) & 3u))
     return nq_fail(NQ_ERR_INVALID, "logprobs is required, aligned to fp32");
@@ -904,6 +994,7 @@ extern "C" int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int6
   p.src = r.src, p.hc = r.hc, p.w = reinterpret_cast<const bf16*>(weight), p.rows = rows, p.V = V, p.H = H;
   p.count = r.count, p.target = r.target, p.c = inv * kLog2e;
   p.part = reinterpret_cast<floatx2*>(ws + s.part), p.zlabel = reinterpret_cast<float*>(ws + s.zlabel);
+  if (kept) head_kept_at(kept, rows, V, &p);
   const bool few = head_few(rows);
   const int bm = few ? Few::BM : Wide::BM, bn = few ? Few::BN : Wide::BN, tiles = (V + bm - 1) / bm;
   const int64_t all = tiles * ((rows + bn - 1) / bn);
@@ -911,24 +1002,24 @@ extern "C" int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int6
   const HeadJoin j{r.src, p.part, p.zlabel, r.count, r.index, r.target, logprobs, r.stats, V, tiles, p.c, inv};
   if (few) {
     // 33 rows of 1024 against 151936 entries: without the gathering launch 62 us for 69
-    if (int rc = launch_logits<Few, false, true>(all, st, p)) return rc;
+    if (int rc = launch_logits<Few, STATS, true>(all, st, p)) return rc;
     hipLaunchKernelGGL((head_join_kernel<4, true>), dim3((unsigned)((rows + 3) / 4)), dim3(1024), 0, st, j);
   } else {
     hipLaunchKernelGGL(head_rows_kernel, dim3((unsigned)((rows + HD_PREP - 1) / HD_PREP)), dim3(256), 0, st, r);
-    if (int rc = launch_logits<Wide, false>(all, st, p)) return rc;
+    if (int rc = kept ? launch_logits<Wide, KEEP>(all, st, p) : launch_logits<Wide, STATS>(all, st, p)) return rc;
     hipLaunchKernelGGL((head_join_kernel<16, false>), dim3((unsigned)((rows + 15) / 16)), dim3(1024), 0, st, j);
   }
   return nq_check_launch(hipGetLastError());
 }
 
 extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, int64_t row_stride, const void* weight,
-                                      const int64_t* labels, const float* stats, const float* dlogprobs,
-                                      void* dhidden, void* dweight, void* workspace, int64_t workspace_bytes,
-                                      int64_t B, int64_t S, int V, int H, float temperature, int64_t ignore_index,
-                                      void* stream) {
+                                      const int64_t* labels, const float* stats, const void* kept,
+                                      int64_t kept_bytes, const float* dlogprobs, void* dhidden, void* dweight,
+                                      void* workspace, int64_t workspace_bytes, int64_t B, int64_t S, int V, int H,
+                                      float temperature, int64_t ignore_index, void* stream) {
   nq_clear_error();
-  if (int rc = head_check(hidden, batch_stride, row_stride, weight, labels, stats, workspace, workspace_bytes, B, S, V,
-                          H, temperature, true))
+  if (int rc = head_check(hidden, batch_stride, row_stride, weight, labels, stats, kept, kept_bytes, workspace,
+                          workspace_bytes, B, S, V, H, temperature, true))
     return rc;
   if (!dlogprobs || (reinterpret_cast<uintptr_t>(dlogprobs) & 3u) || !nq_aligned16(dhidden) || !nq_aligned16(dweight))
     return nq_fail(NQ_ERR_INVALID, "dlogprobs is required, and gradients must be 16-byte aligned");
@@ -951,6 +1042,7 @@ extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, 
   p.hc = r.hc, p.w = reinterpret_cast<const bf16*>(weight), p.rows = rows, p.V = V, p.H = H;
   p.count = r.count, p.target = r.target, p.c = inv * kLog2e, p.coef = r.coef;
   p.dz = reinterpret_cast<bf16*>(ws + s.dz), p.ldz = s.ldz;
+  if (kept) head_kept_at(const_cast<void*>(kept), rows, V, &p);
   p.dw = reinterpret_cast<bf16*>(dweight), p.dh = reinterpret_cast<float*>(ws + s.dh), p.vmax = s.vc;
   const bool few = head_few(rows);
   const int bm = few ? Few::BM : Wide::BM, bn = few ? Few::BN : Wide::BN, nh = (H + bm - 1) / bm;
@@ -961,7 +1053,13 @@ extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, 
   for (int v0 = 0; v0 < V; v0 += s.vc) {
     p.v0 = v0, p.vc = V - v0 < s.vc ? V - v0 : s.vc, p.add = v0 > 0;
     const int64_t logits = (p.vc + bm - 1) / bm * nn;
-    int rc = few ? launch_logits<Few, true>(logits, st, p) : launch_logits<Wide, true>(logits, st, p);
+    int rc = NQ_OK;
+    if (kept) {
+      // at most 2^31 kept values, 8192 a workgroup
+      hipLaunchKernelGGL(head_dz_kernel, dim3((unsigned)((p.vc + 2047) / 2048 * ((rows + 3) / 4))), dim3(256), 0, st, p);
+    } else {
+      rc = few ? launch_logits<Few, DZ>(logits, st, p) : launch_logits<Wide, DZ>(logits, st, p);
+    }
     // as many workgroups as the CUs hold: how many tiles there are goes by the kept rows
     if (!rc && dhidden) rc = few ? launch_dh<Few>(INT32_MAX / 2, st, p) : launch_dh<Wide>(INT32_MAX / 2, st, p);
     if (!rc && dweight) {

@@ -175,31 +175,34 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
     return _TokenLogprobs.apply(logits, rest) if _takes_gradient(logits) else _token_forward(logits, *rest)[0]
 
 
-def _linear_forward(hidden, weight, labels, temperature: float, ignore_index: int):
+def _linear_forward(hidden, weight, labels, temperature: float, ignore_index: int, keep: bool):
     x, w, B, S, bs, rs = _head_operands(hidden, weight)
     V, H = w.shape
     out = x.new_empty(labels.shape, dtype=torch.float32)
     stats = x.new_empty((B * S, 2), dtype=torch.float32)
     lib = _lib.load()
+    nkept = lib.nq_linear_logprobs_kept_bytes(B * S, V, H) if keep else 0
+    kept = x.new_empty(nkept, dtype=torch.uint8) if nkept else None
     nbytes = lib.nq_linear_logprobs_workspace_bytes(B * S, V, H)
     ws = x.new_empty(nbytes, dtype=torch.uint8)
     _launch(x, lib.nq_linear_logprobs, "nq_linear_logprobs", x.data_ptr(), bs, rs, w.data_ptr(), labels.data_ptr(),
-            out.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes, B, S, V, H, temperature, ignore_index)
-    return out, stats
+            out.data_ptr(), stats.data_ptr(), ops._ptr(kept), nkept, ws.data_ptr(), nbytes, B, S, V, H, temperature,
+            ignore_index)
+    return out, stats, kept
 
 
 class _LinearLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, rest):
-        out, stats = _linear_forward(hidden, weight, *rest)
-        ctx.save_for_backward(hidden, weight, rest[0], stats)
-        ctx.tail = rest[1:]
+        out, stats, kept = _linear_forward(hidden, weight, *rest)
+        ctx.save_for_backward(hidden, weight, rest[0], stats, kept)
+        ctx.tail = rest[1:3]
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, dy):
-        hidden, weight, labels, stats = ctx.saved_tensors
+        hidden, weight, labels, stats, kept = ctx.saved_tensors
         x, w, B, S, bs, rs = _head_operands(hidden, weight)
         V, H = w.shape
         dy = dy.contiguous()
@@ -209,8 +212,8 @@ class _LinearLogprobs(torch.autograd.Function):
         nbytes = lib.nq_linear_logprobs_bwd_workspace_bytes(B * S, V, H)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         _launch(x, lib.nq_linear_logprobs_bwd, "nq_linear_logprobs_bwd", x.data_ptr(), bs, rs, w.data_ptr(),
-                labels.data_ptr(), stats.data_ptr(), dy.data_ptr(), ops._ptr(dh), ops._ptr(dw), ws.data_ptr(),
-                nbytes, B, S, V, H, *ctx.tail)
+                labels.data_ptr(), stats.data_ptr(), ops._ptr(kept), 0 if kept is None else kept.numel(),
+                dy.data_ptr(), ops._ptr(dh), ops._ptr(dw), ws.data_ptr(), nbytes, B, S, V, H, *ctx.tail)
         return dh, dw, None
 
 
@@ -224,15 +227,21 @@ def _head_operands(hidden: torch.Tensor, weight: torch.Tensor):
 
 
 def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, temperature: float = 1.0,
-                    ignore_index: int = IGNORE_INDEX) -> torch.Tensor:
+                    ignore_index: int = IGNORE_INDEX, recompute: bool = False) -> torch.Tensor:
     """``token_logprobs(hidden @ weight.T, labels)`` without the logits, fp32 and shaped like ``labels``.
 
     hidden: (..., H) bf16 hidden states, rows at any strides; weight: (V, H) bf16, an LM
     head's; H a multiple of 8.  Logits are held in fp32 and never stored; the backward forms
-    their gradient again from two numbers a row, in bf16, a range of the vocabulary at a time
-    (at most 1 GiB), and gives hidden and weight gradients summed in fp32.  Rows whose label
-    is ``ignore_index`` take no part in the products.  Labels outside [0, V) give NaN, and so
-    do their row's and the weight's gradients.  An fp32 head goes through its logits:
+    their gradient in bf16, a range of the vocabulary at a time (at most 1 GiB), and gives
+    hidden and weight gradients summed in fp32.  Rows whose label is ``ignore_index`` take no
+    part in the products.  Labels outside [0, V) give NaN, and so do their row's and the
+    weight's gradients.
+
+    A call with a gradient keeps the softmax's numerators for it, in bf16, 2 bytes for each
+    entry of each row, where that is at most 4 GiB; with ``recompute``, and beyond, it keeps
+    two numbers a row and the backward repeats the first product (a fifth slower).
+
+    An fp32 head goes through its logits:
     ``token_logprobs(F.linear(hidden, weight), labels)``.
     """
     _check_devices(hidden, weight, labels)
@@ -252,8 +261,8 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
         raise ValueError(f"at most 2^24 rows and entries in one call, got {labels.numel()} and {V}")
     rest = labels, temperature, int(ignore_index)
     if _takes_gradient(hidden, weight):
-        return _LinearLogprobs.apply(hidden, weight, rest)
-    return _linear_forward(hidden, weight, *rest)[0]
+        return _LinearLogprobs.apply(hidden, weight, (*rest, not recompute))
+    return _linear_forward(hidden, weight, *rest, False)[0]
 
 
 _HEAD_MOST = 1 << 24

@@ -1,7 +1,8 @@
 """Log-probabilities straight from hidden states and an LM head, against 64 bits.
 
 Tolerances are sums of roundings: u = 2^-24 for each fp32 operation, half a step (2^-8) of
-bf16 for what is rounded to it: dz once, as the matrix cores' operand, and the gradients.
+bf16 for what is rounded to it: dz once, as the matrix cores' operand, the softmax's numerators
+that a forward keeps, and the gradients.
 """
 
 import pytest
@@ -40,8 +41,8 @@ def reference(h, w, labels, dy, T, ignore=-100):
     p = torch.exp(logp)
     dz = torch.where(keep[:, None], -p * g, 0.0).scatter_add(1, at, g)
     dh, dw = dz @ w, dz.t() @ h
-    # |dz| off by half a step and its softmax by err; fp32 sums over the terms
-    off = (dz.abs() * HALF + g.abs() * p * err[:, None] * 2 + 1e-37).nan_to_num(0)
+    # |dz| off by half a step and its softmax by another, where kept, and err; fp32 sums over the terms
+    off = (dz.abs() * HALF + (-p * g).abs() * HALF * 1.01 + g.abs() * p * err[:, None] * 2 + 1e-37).nan_to_num(0)
     tol_h = off @ w.abs() + V * U * (dz.abs().nan_to_num(0) @ w.abs()) + HALF * dh.abs().nan_to_num(0) + 1e-37
     tol_w = off.t() @ h.abs() + len(h) * U * (dz.abs().nan_to_num(0).t() @ h.abs()) + HALF * dw.abs().nan_to_num(0) + 1e-37
     return lp.view(shape), dh.view(*shape, H), dw, tol.view(shape), tol_h.view(*shape, H), tol_w
@@ -79,7 +80,8 @@ def test_linear_logprobs(rows, V, H):
     say(f"linear_logprobs {rows} x {V} x {H}")
     h, w, labels, dy = inputs((rows,), V, H, 100)
     labels[rows // 2] = V - 1
-    check(h, w, labels, dy, T=0.7 if V % 2 else 1.0, what=f"{rows}x{V}x{H}")
+    for recompute in (False, True):
+        check(h, w, labels, dy, T=0.7 if V % 2 else 1.0, what=f"{rows}x{V}x{H}", recompute=recompute)
 
 
 @pytest.mark.parametrize("rows,share", [(50, 0.5), (600, 0.3), (600, 0.97), (64, 1.0), (300, 1.0)])
@@ -92,29 +94,35 @@ def test_linear_logprobs_leaves_ignored_rows_out(rows, share):
     want = reference(h, w, labels, dy, 1.0, -7)
     h, dy = h.clone(), dy.clone()
     h[drop], dy[drop] = float("nan"), float("nan")
-    got = run(h, w, labels, dy, ignore_index=-7)
-    for name, a, ref, tol in zip(("logprobs", "dhidden", "dweight"), got, want, want[3:]):
-        within(a, ref, tol, name)
-    assert not got[0][drop.to(DEV)].any() and not got[1][drop.to(DEV)].any()
+    for recompute in (False, True):
+        got = run(h, w, labels, dy, ignore_index=-7, recompute=recompute)
+        for name, a, ref, tol in zip(("logprobs", "dhidden", "dweight"), got, want, want[3:]):
+            within(a, ref, tol, name)
+        assert not got[0][drop.to(DEV)].any() and not got[1][drop.to(DEV)].any()
 
 
-def test_linear_logprobs_special_values():
+@pytest.mark.parametrize("rows", [40, 140])
+@pytest.mark.parametrize("recompute", [False, True])
+def test_linear_logprobs_special_values(rows, recompute):
     """Labels outside the vocabulary, NaN and infinite hidden states, a masked-out vocabulary entry."""
-    say("linear_logprobs special values")
-    h, w, labels, dy = inputs((40,), 300, 64, 120)
+    say(f"linear_logprobs special values {rows} {recompute}")
+    h, w, labels, dy = inputs((rows,), 300, 64, 120)
     labels[3], labels[9] = 300, -1
-    lp, dh, dw = run(h, w, labels, dy)
+    lp, dh, dw = run(h, w, labels, dy, recompute=recompute)
     want = reference(h, w, labels, dy, 1.0)
     within(lp, want[0], want[3], "labels outside")
     within(dh, want[1], want[4], "labels outside, dhidden")
     assert torch.isnan(dw).all()
     labels[3], labels[9] = 0, 1
     h[5], h[6, 7] = float("nan"), float("inf")
-    lp, _, _ = run(h, w, labels, dy)
-    assert torch.isnan(lp[[5, 6]]).all() and torch.isfinite(lp).sum() == 38
-    # logits far apart: the others' probabilities vanish, and nothing overflows
-    h, w, labels, dy = inputs((40,), 300, 64, 121)
-    check(h * 64, w, labels, dy, what="far apart")
+    lp, dh, _ = run(h, w, labels, dy, recompute=recompute)
+    assert torch.isnan(lp[[5, 6]]).all() and torch.isfinite(lp).sum() == rows - 2
+    assert torch.isnan(dh[[5, 6]]).any(1).all() and torch.isfinite(dh).all(1).sum() == rows - 2
+    # logits far apart: the others' probabilities vanish, and nothing overflows; a label almost certain
+    h, w, labels, dy = inputs((rows,), 300, 64, 121)
+    check(h * 64, w, labels, dy, what="far apart", recompute=recompute)
+    h = (w[labels].float() * 3).to(BF)
+    check(h, w, labels, dy, what="certain labels", recompute=recompute)
 
 
 def test_linear_logprobs_strides_and_shapes():
@@ -146,9 +154,10 @@ def test_linear_logprobs_strides_and_shapes():
     assert lp.shape == (0, 41) and not torch.autograd.grad(lp.sum(), wl)[0].any()
 
 
-def test_linear_logprobs_several_ranges():
+@pytest.mark.parametrize("recompute", [False, True])
+def test_linear_logprobs_several_ranges(recompute):
     """So many rows that the backward takes the vocabulary in several ranges, the last a short one."""
-    say("linear_logprobs several ranges")
+    say(f"linear_logprobs several ranges {recompute}")
     rows, V, H = 70000, 9001, 64
     g = torch.Generator(device=DEV).manual_seed(140)
     h = torch.randn(rows, H, generator=g, device=DEV).to(BF).requires_grad_()
@@ -156,7 +165,7 @@ def test_linear_logprobs_several_ranges():
     labels = torch.randint(0, V, (rows,), generator=g, device=DEV)
     labels[::3] = -100
     dy = torch.randn(rows, generator=g, device=DEV)
-    lp = nq.linear_logprobs(h, w, labels)
+    lp = nq.linear_logprobs(h, w, labels, recompute=recompute)
     dh, dw = torch.autograd.grad(lp, (h, w), dy)
     # dw row by row over the kept rows of all; a sample of the rows of dh
     at = torch.arange(0, rows, 97, device=DEV)
