@@ -254,32 +254,10 @@ struct Reads {
   }
 };
 
-// The tiles of a workgroup.  Workgroups go to the 8 XCDs in turn; each XCD takes a contiguous
-// run of tiles, in groups of 8 row tiles over all column tiles, so that the 32 that it works
-// on at once share 8 + 4 operand tiles in its L2.
-struct Tiles {
-  int nm, nn, w, step, end;
-  __device__ __forceinline__ Tiles(int nm_, int nn_) : nm(nm_), nn(nn_) {
-    const int total = nm * nn, per = (total + 7) / 8, xcd = blockIdx.x & 7;
-    w = xcd * per + (blockIdx.x >> 3);
-    end = (xcd + 1) * per < total ? (xcd + 1) * per : total;
-    step = gridDim.x >> 3;
-  }
-  __device__ __forceinline__ bool has() const { return w < end; }
-  __device__ __forceinline__ void next() { w += step; }
-  __device__ __forceinline__ void get(int& tm, int& tn) const {
-    const int group = w / (8 * nn), left = nm - group * 8, g = left < 8 ? left : 8;
-    const int in = w - group * 8 * nn;
-    tn = in / g;
-    tm = group * 8 + in - tn * g;
-  }
-};
-
-// A workgroup's stream of products: the steps of all its tiles in turn, in two LDS buffers.
-// A step's last products are issued after the barrier that ends it: by then every wave has
-// read its operands, so that the loads of the step after next may overwrite them, and the
-// next step has landed, so that its first operands are read under those products.  The
-// loads run ahead of a tile's end into the next tile, under its epilogue.
+// A workgroup's stream of products.  Two LDS buffers: the next step's loads are in flight
+// while a step's 64 depths are multiplied, one barrier a step, and the step after a tile's
+// last is the next tile's first, so that its loads run under this tile's last products and
+// its epilogue.  The operands of the next 16 depths are read while these are multiplied.
 template <class C, bool AROW, bool BROW, bool GATHER = false>
 struct Product {
   static constexpr int WAVES = C::M * C::N;
@@ -304,71 +282,33 @@ struct Product {
     ra.init(lds_addr(l), (w / C::N) * (C::MT * 32), ln);
     rb.init(lds_addr(l + A::BYTES), (w % C::N) * (C::NT * 32), ln);
   }
-  // The steps still to load: a step of a tile's operands, which place(tile, a, b) sets, then
-  // the next; tiles of no depth have none.
-  template <class Place>
-  struct Cursor {
-    Tiles t;
-    A a;
-    B b;
-    int k;
-    bool valid;
-    Place place;
-    __device__ __forceinline__ Cursor(const Tiles& tiles, const A& a0, const B& b0, Place f)
-        : t(tiles), a(a0), b(b0), k(0), valid(tiles.has()), place(f) {
-      if (valid) {
-        place(t, a, b);
-        settle();
-      }
-    }
-    __device__ __forceinline__ void settle() {
-      while (k >= a.depth) {
-        t.next();
-        valid = t.has();
-        if (!valid) return;
-        place(t, a, b);
-        k = 0;
-      }
-    }
-  };
-  template <class Place>
-  __device__ __forceinline__ void load(uint32_t buf, Cursor<Place>& c) {
-    if (!c.valid) return;
-    c.a.load(lds + buf, c.k, wave);
-    c.b.load(lds + buf + A::BYTES, c.k, wave);
-    c.k += HD_BK;
-    c.settle();
+  __device__ __forceinline__ void load(uint32_t buf, const A& a, const B& b, int k0) {
+    a.load(lds + buf, k0, wave);
+    b.load(lds + buf + A::BYTES, k0, wave);
   }
-  // the first two steps
-  template <class Place>
-  __device__ __forceinline__ void begin(Cursor<Place>& c) {
-    load(0, c);
-    const bool second = c.valid;
-    load(BUF, c);
-    if (second) wait_vmcnt<A::NI + B::NI>();
-    else wait_vmcnt0();
-    __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  // acc = the wave's blocks of A B^T over `depth`
-  template <class Place>
-  __device__ __forceinline__ void run(int depth, Cursor<Place>& c, Acc& acc) {
+  // acc = the wave's blocks of A B^T; the first step is under way in the current buffer,
+  // and the one of (na, nb) is afterwards, if there is another tile.
+  __device__ __forceinline__ void run(const A& a, const B& b, bool more, const A& na, const B& nb, Acc& acc) {
 #pragma unroll
     for (int i = 0; i < C::MT; ++i)
 #pragma unroll
       for (int j = 0; j < C::NT; ++j) acc[i][j] = floatx16{};
-    if (depth <= 0) return;
     constexpr int PER = Reads<C::BM, AROW, C::MT>::PER + Reads<C::BN, BROW, C::NT>::PER;
-    bf16x8 x[2][C::MT], y[2][C::NT];
-    auto multiply = [&](int h) {
+    for (int k = 0; k < a.depth; k += HD_BK) {
+      wait_vmcnt0();
+      __builtin_amdgcn_s_barrier();  // the step has landed, and the other buffer's readers are done
+      __builtin_amdgcn_sched_barrier(0);
+      if (k + HD_BK < a.depth) load(BUF - cur, a, b, k + HD_BK);
+      else if (more) load(BUF - cur, na, nb, 0);
+      bf16x8 x[2][C::MT], y[2][C::NT];
+      auto multiply = [&](int h) {
 #pragma unroll
-      for (int i = 0; i < C::MT; ++i)
+        for (int i = 0; i < C::MT; ++i)
 #pragma unroll
-        for (int j = 0; j < C::NT; ++j) acc[i][j] = mfma32(x[h][i], y[h][j], acc[i][j]);
-    };
-    ra.template read<0>(cur, x[0]);
-    rb.template read<0>(cur, y[0]);
-    for (int k = 0; k < depth; k += HD_BK) {
+          for (int j = 0; j < C::NT; ++j) acc[i][j] = mfma32(x[h][i], y[h][j], acc[i][j]);
+      };
+      ra.template read<0>(cur, x[0]);
+      rb.template read<0>(cur, y[0]);
       ra.template read<1>(cur, x[1]);
       rb.template read<1>(cur, y[1]);
       lgkm_wait<PER>();
@@ -382,16 +322,8 @@ struct Product {
       lgkm_wait<PER>();
       multiply(0);
       lgkm_wait<0>();
-      wait_vmcnt0();
-      __syncthreads();
-      __builtin_amdgcn_sched_barrier(0);
-      load(cur, c);
-      cur = BUF - cur;
-      if (k + HD_BK < depth) {
-        ra.template read<0>(cur, x[0]);
-        rb.template read<0>(cur, y[0]);
-      }
       multiply(1);
+      cur = BUF - cur;
     }
   }
   // The wave's rows (one per lane of its column blocks j) of value(j, i, q), four values of
@@ -431,6 +363,26 @@ struct Product {
   }
 };
 
+// The tiles of a workgroup.  Workgroups go to the 8 XCDs in turn; each XCD takes a contiguous
+// run of tiles, in groups of 8 row tiles over all column tiles, so that the 32 that it works
+// on at once share 8 + 4 operand tiles in its L2.
+struct Tiles {
+  int nm, nn, w, step, end;
+  __device__ __forceinline__ Tiles(int nm_, int nn_) : nm(nm_), nn(nn_) {
+    const int total = nm * nn, per = (total + 7) / 8, xcd = blockIdx.x & 7;
+    w = xcd * per + (blockIdx.x >> 3);
+    end = (xcd + 1) * per < total ? (xcd + 1) * per : total;
+    step = gridDim.x >> 3;
+  }
+  __device__ __forceinline__ bool has(int ahead) const { return w + ahead * step < end; }
+  __device__ __forceinline__ void get(int ahead, int& tm, int& tn) const {
+    const int v = w + ahead * step;
+    const int group = v / (8 * nn), left = nm - group * 8, g = left < 8 ? left : 8;
+    const int in = v - group * 8 * nn;
+    tn = in / g;
+    tm = group * 8 + in - tn * g;
+  }
+};
 template <class C>
 static int head_grid(int64_t tiles) {
   const int64_t most = HD_CUS * C::PER_CU, n = (tiles + 7) / 8 * 8;
@@ -482,12 +434,13 @@ __global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams
     count = __builtin_amdgcn_readfirstlane(*p.count);
   }
   Tiles t((vend - vfirst + C::BM - 1) / C::BM, (count + C::BN - 1) / C::BN);
-  if (!t.has()) return;
+  if (!t.has(0)) return;
   P prod;
   prod.init(lds, wave, lane);
-  typename P::A a;
-  typename P::B b;
+  typename P::A a, na;
+  typename P::B b, nb;
   a.lanes(p.H, wave, lane);
+  na = a;
   int few_target[C::NT];
   if constexpr (GATHER) {
     const int* index = few_index + wave * 128;
@@ -500,21 +453,23 @@ __global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams
   } else {
     b.lanes(p.H, wave, lane);
   }
-  auto place = [&](const Tiles& u, typename P::A& x, typename P::B& y) {
-    int um, un;
-    u.get(um, un);
-    x.at(p.w, vfirst + um * C::BM, vend, p.H);
-    if constexpr (!GATHER) y.at(p.hc, un * C::BN, count, p.H);
-  };
-  typename P::template Cursor<decltype(place)> ahead(t, a, b, place);
-  prod.begin(ahead);
+  nb = b;
+  int tm, tn, um = 0, un = 0;
+  t.get(0, tm, tn);
+  a.at(p.w, vfirst + tm * C::BM, vend, p.H);
+  if constexpr (!GATHER) b.at(p.hc, tn * C::BN, count, p.H);
+  prod.load(0, a, b, 0);
   const int wm = wave / C::N, wn = wave % C::N;
   const int vw = wm * (C::MT * 32) + (lane >> 5) * 4;  // the lane's first entry in the tile
-  for (; t.has(); t.next()) {
-    int tm, tn;
-    t.get(tm, tn);
+  for (;;) {
+    const bool more = t.has(1);
+    if (more) {
+      t.get(1, um, un);
+      na.at(p.w, vfirst + um * C::BM, vend, p.H);
+      if constexpr (!GATHER) nb.at(p.hc, un * C::BN, count, p.H);
+    }
     typename P::Acc acc;
-    prod.run(p.H, ahead, acc);
+    prod.run(a, b, more, na, nb, acc);
 
     const int n0 = tn * C::BN, v0 = vfirst + tm * C::BM;
     if (MODE != DZ) {
@@ -617,6 +572,9 @@ __global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams
           },
           p.ldz - col0);
     }
+    if (!more) break;
+    a = na, b = nb, tm = um, tn = un;
+    t.w += t.step;
   }
 }
 
@@ -721,33 +679,38 @@ __global__ __launch_bounds__(threads_of<Wide>()) void head_dw_kernel(HeadParams 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int count = __builtin_amdgcn_readfirstlane(*p.count);
   Tiles t((p.H + C::BM - 1) / C::BM, (p.vc + C::BN - 1) / C::BN);
-  if (!t.has()) return;
+  if (!t.has(0)) return;
   P prod;
   prod.init(lds, wave, lane);
-  P::A a;
-  P::B b;
+  P::A a, na;
+  P::B b, nb;
   a.lanes(p.H, wave, lane);
   b.lanes(p.ldz, wave, lane);
-  auto place = [&](const Tiles& u, P::A& x, P::B& y) {
-    int um, un;
-    u.get(um, un);
-    x.at(p.hc, um * C::BM, p.H, count);
-    y.at(p.dz, un * C::BN, p.vc, count);
-  };
-  P::Cursor<decltype(place)> ahead(t, a, b, place);
-  prod.begin(ahead);
+  na = a, nb = b;
+  int tm, tn, um = 0, un = 0;
+  t.get(0, tm, tn);
+  a.at(p.hc, tm * C::BM, p.H, count);
+  b.at(p.dz, tn * C::BN, p.vc, count);
+  if (count > 0) prod.load(0, a, b, 0);
   const int wm = wave / C::N, wn = wave % C::N;
-  for (; t.has(); t.next()) {
-    int tm, tn;
-    t.get(tm, tn);
+  for (;;) {
+    const bool more = t.has(1);
+    if (more) {
+      t.get(1, um, un);
+      na.at(p.hc, um * C::BM, p.H, count);
+      nb.at(p.dz, un * C::BN, p.vc, count);
+    }
     P::Acc acc;
-    prod.run(count, ahead, acc);
+    prod.run(a, b, more, na, nb, acc);
     const int h0 = tm * C::BM + wm * (C::MT * 32), v0 = tn * C::BN + wn * (C::NT * 32);
     prod.store(
         [&](int j, int i, int q) {
           return floatx4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
         },
         [&](int r) { return v0 + r < p.vc ? p.dw + (int64_t)(p.v0 + v0 + r) * p.H + h0 : nullptr; }, p.H - h0);
+    if (!more) break;
+    a = na, b = nb, tm = um, tn = un;
+    t.w += t.step;
   }
 }
 
@@ -779,36 +742,36 @@ __global__ __launch_bounds__(threads_of<C>()) void head_dh_kernel(HeadParams p) 
   const int slabs = head_slabs((int64_t)nh * nn, p.vmax);
   const int per = ((p.vc + slabs - 1) / slabs + HD_BK - 1) / HD_BK * HD_BK;
   Tiles t(nh, nn * slabs);
-  if (!t.has()) return;
+  if (!t.has(0)) return;
   P prod;
   prod.init(lds, wave, lane);
-  typename P::A a;
-  typename P::B b;
+  typename P::A a, na;
+  typename P::B b, nb;
   a.lanes(p.H, wave, lane);
   b.lanes(p.ldz, wave, lane);
-  auto split = [&](const Tiles& u, int& th, int& tn, int& slab, int& k0) {
-    int rest;
-    u.get(th, rest);
-    slab = rest / nn, tn = rest - slab * nn, k0 = slab * per;
-    const int left = p.vc - k0;
-    return left < 0 ? 0 : left < per ? left : per;
+  na = a, nb = b;
+  auto place = [&](int th, int rest, typename P::A& x, typename P::B& y) {
+    const int slab = rest / nn, tn = rest - slab * nn, k0 = slab * per;
+    const int left = p.vc - k0, depth = left < 0 ? 0 : left < per ? left : per;
+    x.at(p.w + (int64_t)(p.v0 + (depth ? k0 : 0)) * p.H, th * C::BM, p.H, depth);
+    y.at(p.dz + (depth ? k0 : 0), tn * C::BN, count, depth);
   };
-  auto place = [&](const Tiles& u, typename P::A& x, typename P::B& y) {
-    int th, tn, slab, k0;
-    const int depth = split(u, th, tn, slab, k0);
-    if (!depth) k0 = 0;
-    x.at(p.w + (int64_t)(p.v0 + k0) * p.H, th * C::BM, p.H, depth);
-    y.at(p.dz + k0, tn * C::BN, count, depth);
-  };
-  typename P::template Cursor<decltype(place)> ahead(t, a, b, place);
-  prod.begin(ahead);
+  int th, rest, uh = 0, us = 0;
+  t.get(0, th, rest);
+  place(th, rest, a, b);
+  if (a.depth) prod.load(0, a, b, 0);
   const int wm = wave / C::N, wn = wave % C::N;
-  for (; t.has(); t.next()) {
-    int th, tn, slab, k0;
-    const int depth = split(t, th, tn, slab, k0);
+  for (;;) {
+    const bool more = t.has(1);
+    if (more) {
+      t.get(1, uh, us);
+      place(uh, us, na, nb);
+    }
     typename P::Acc acc;
-    prod.run(depth, ahead, acc);
-    if (depth || !p.add) {
+    prod.run(a, b, more && na.depth, na, nb, acc);
+    if (!a.depth && more && na.depth) prod.load(prod.cur, na, nb, 0);  // nothing ran that would have begun it
+    const int slab = rest / nn, tn = rest - slab * nn;
+    if (a.depth || !p.add) {
 #pragma unroll
       for (int j = 0; j < C::NT; ++j) {
         const int n = tn * C::BN + wn * (C::NT * 32) + j * 32 + (lane & 31);
@@ -828,6 +791,9 @@ __global__ __launch_bounds__(threads_of<C>()) void head_dh_kernel(HeadParams p) 
         }
       }
     }
+    if (!more) break;
+    a = na, b = nb, th = uh, rest = us;
+    t.w += t.step;
   }
 }
 
