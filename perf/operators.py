@@ -154,7 +154,8 @@ def _own(s):
     if c["kind"] == "preference":
         loss, rc, rr = nq.preference_loss(s["chosen"], s["rejected"], s["ref_chosen"], s["ref_rejected"],
                                           chosen_mask=s["chosen_mask"], rejected_mask=s["rejected_mask"],
-                                          beta=c["beta"], label_smoothing=c["smoothing"], kind=c["form"])
+                                          beta=c["beta"], kind=c["form"],
+                                          label_smoothing=c["smoothing"] if c["form"] == "sigmoid" else 0.0)
         return [loss, rc, rr, *torch.autograd.grad(loss, (s["chosen"], s["rejected"]))]
     loss, kl, clipped = nq.policy_loss(s["lp"], s["old"], s["adv"], ref_logprobs=s["ref"], mask=s["mask"],
                                        clip_low=c["low"], clip_high=c["high"], kl_coef=c["kl"], reduction=c["form"])
