@@ -22,7 +22,6 @@
 namespace nq {
 
 constexpr int HD_BK = 64;    // depth of a step
-constexpr int HD_PREP = 16;  // rows of a gathering workgroup
 constexpr int HD_CUS = 256;
 
 // A product's tile, BM (the MFMA's row axis) x BN, and how its waves share it: M x N of
@@ -63,10 +62,12 @@ struct HeadSource {
 
 // ---------------------------------------------------------------------------
 // The kept rows, in order: pos[row] = its place among them (-1: ignored), index the
-// reverse, hc their hidden states.  A workgroup counts the kept rows before its own 16 (the
-// labels are small and in L2) rather than wait for another launch.
+// reverse, hc their hidden states.  A workgroup counts the kept rows before its own (the
+// labels are small and in L2) rather than wait for another launch: 16 rows each, or more
+// where there would be over 2048 workgroups to read them.
 struct HeadRows {
   HeadSource src;
+  int64_t each;  // rows of a workgroup
   int H, V;
   int* count;
   int* pos;       // (rows)
@@ -83,55 +84,60 @@ struct HeadRows {
 };
 
 __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows p) {
-  __shared__ int before[4], own[HD_PREP];
+  __shared__ int before[4], own[64], kept_here;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r0 = (int64_t)blockIdx.x * HD_PREP;
+  const int64_t first = (int64_t)blockIdx.x * p.each;
+  const int64_t last = first + p.each < p.src.rows ? first + p.each : p.src.rows;
   int n = 0;
 #pragma unroll 8
-  for (int64_t r = tid; r < r0; r += 256) n += p.src.labels[r] != p.src.ignore;
+  for (int64_t r = tid; r < first; r += 256) n += p.src.labels[r] != p.src.ignore;
 #pragma unroll
   for (int k = 32; k >= 1; k >>= 1) n += __shfl_xor(n, k, 64);
   if (lane == 0) before[wave] = n;
   __syncthreads();
-  const int base = before[0] + before[1] + before[2] + before[3];
-  if (wave == 0) {
-    const int64_t r = r0 + lane;
-    const bool here = lane < HD_PREP && r < p.src.rows;
-    const int64_t y = here ? p.src.labels[r] : p.src.ignore;
-    const bool kept = y != p.src.ignore;
-    const uint64_t ballot = __builtin_amdgcn_ballot_w64(kept);
-    const int place = kept ? base + __popcll(ballot & ((1ull << lane) - 1)) : -1;
-    if (here) {
+  int base = before[0] + before[1] + before[2] + before[3];
+  const int ch = p.H / 8;
+  for (int64_t r0 = first; r0 < last; r0 += 64) {
+    const int here = (int)(last - r0 < 64 ? last - r0 : 64);
+    if (wave == 0) {
+      const int64_t r = r0 + lane;
+      const int64_t y = lane < here ? p.src.labels[r] : p.src.ignore;
+      const bool kept = y != p.src.ignore;
+      const uint64_t ballot = __builtin_amdgcn_ballot_w64(kept);
+      const int place = kept ? base + __popcll(ballot & ((1ull << lane) - 1)) : -1;
       own[lane] = place;
-      p.pos[r] = place;
-      const bool inside = y >= 0 && y < p.V;
-      if (kept) {
-        p.index[place] = (int)r;
-        p.target[place] = inside ? (int)y : -1;
-        if (p.dy) {
-          const floatx2 st = p.stats[r];
-          const float g = inside ? p.dy[r] * p.inv_t : __builtin_nanf("");
-          p.coef[place] = floatx4{st[0], -g / st[1], g, 0.f};
+      if (lane == 0) kept_here = __popcll(ballot);
+      if (lane < here) {
+        p.pos[r] = place;
+        const bool inside = y >= 0 && y < p.V;
+        if (kept) {
+          p.index[place] = (int)r;
+          p.target[place] = inside ? (int)y : -1;
+          if (p.dy) {
+            const floatx2 st = p.stats[r];
+            const float g = inside ? p.dy[r] * p.inv_t : __builtin_nanf("");
+            p.coef[place] = floatx4{st[0], -g / st[1], g, 0.f};
+          }
+        } else if (p.logprobs) {
+          p.logprobs[r] = 0.f;
+          p.stats[r] = floatx2{0.f, 1.f};
         }
-      } else if (p.logprobs) {
-        p.logprobs[r] = 0.f;
-        p.stats[r] = floatx2{0.f, 1.f};
       }
     }
-    if (r0 + HD_PREP >= p.src.rows && lane == 0) *p.count = base + __popcll(ballot);
+    __syncthreads();
+    base += kept_here;
+    for (int i = wave; i < here; i += 4) {
+      const int place = own[i];
+      if (place < 0) continue;
+      const bf16x8* src = reinterpret_cast<const bf16x8*>(p.src.row(r0 + i));
+      bf16x8* dst = reinterpret_cast<bf16x8*>(p.hc + (int64_t)place * p.H);
+      for (int c = lane; c < ch; c += 64) dst[c] = src[c];
+    }
+    __syncthreads();  // own's readers are done
   }
-  __syncthreads();
-  const int ch = p.H / 8;
-  for (int i = wave; i < HD_PREP && r0 + i < p.src.rows; i += 4) {
-    const int place = own[i];
-    if (place < 0) continue;
-    const bf16x8* src = reinterpret_cast<const bf16x8*>(p.src.row(r0 + i));
-    bf16x8* dst = reinterpret_cast<bf16x8*>(p.hc + (int64_t)place * p.H);
-    for (int c = lane; c < ch; c += 64) dst[c] = src[c];
-  }
+  if (last == p.src.rows && tid == 0) *p.count = base;
 }
 
-// ---------------------------------------------------------------------------
 // One operand of a product, (extent x depth), staged in LDS a step of 64 deep at a time.
 //   ROW   depth contiguous in memory: LDS rows of 128 bytes, an operand one 16-byte read.
 //         16-byte chunk c of row r lies at c ^ (r / 2 % 8): 16 consecutive rows' reads
@@ -958,6 +964,11 @@ static int head_launch(K kernel, int grid, int threads, hipStream_t st, const He
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3((unsigned)threads), P::LDS, st, p);
   return nq_check_launch(hipGetLastError());
 }
+static void launch_rows(HeadRows& r, hipStream_t st) {
+  const int64_t rows = r.src.rows;
+  r.each = rows <= 16 * 2048 ? 16 : ((rows + 2047) / 2048 + 63) / 64 * 64;
+  hipLaunchKernelGGL(head_rows_kernel, dim3((unsigned)((rows + r.each - 1) / r.each)), dim3(256), 0, st, r);
+}
 template <class C, int MODE, bool GATHER = false>
 static int launch_logits(int64_t tiles, hipStream_t st, const HeadParams& p) {
   return head_launch<Product<C, true, true, GATHER>>(head_logits_kernel<C, MODE, GATHER>, head_grid<C>(tiles),
@@ -1005,7 +1016,7 @@ extern "C" int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int6
     if (int rc = launch_logits<Few, STATS, true>(all, st, p)) return rc;
     hipLaunchKernelGGL((head_join_kernel<4, true>), dim3((unsigned)((rows + 3) / 4)), dim3(1024), 0, st, j);
   } else {
-    hipLaunchKernelGGL(head_rows_kernel, dim3((unsigned)((rows + HD_PREP - 1) / HD_PREP)), dim3(256), 0, st, r);
+    launch_rows(r, st);
     if (int rc = kept ? launch_logits<Wide, KEEP>(all, st, p) : launch_logits<Wide, STATS>(all, st, p)) return rc;
     hipLaunchKernelGGL((head_join_kernel<16, false>), dim3((unsigned)((rows + 15) / 16)), dim3(1024), 0, st, j);
   }
@@ -1037,7 +1048,7 @@ extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, 
   r.hc = reinterpret_cast<bf16*>(ws + s.hc);
   r.stats = reinterpret_cast<floatx2*>(const_cast<float*>(stats)), r.dy = dlogprobs;
   r.coef = reinterpret_cast<floatx4*>(ws + s.coef), r.inv_t = inv;
-  hipLaunchKernelGGL(head_rows_kernel, dim3((unsigned)((rows + HD_PREP - 1) / HD_PREP)), dim3(256), 0, st, r);
+  launch_rows(r, st);
   HeadParams p{};
   p.hc = r.hc, p.w = reinterpret_cast<const bf16*>(weight), p.rows = rows, p.V = V, p.H = H;
   p.count = r.count, p.target = r.target, p.c = inv * kLog2e, p.coef = r.coef;

@@ -165,8 +165,8 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
     _check_devices(logits, labels)
     if logits.dtype not in ops._DTYPES:
         ops._code(logits)
-    if logits.dim() == 0 or logits.shape[-1] == 0:
-        raise ValueError(f"logits need a last axis of at least one element, got shape {tuple(logits.shape)}")
+    if logits.dim() == 0 or not 0 < logits.shape[-1] < 2 ** 31:
+        raise ValueError(f"logits need a last axis of 1 to 2^31 - 1 elements, got shape {tuple(logits.shape)}")
     labels = _check_labels(labels, logits.shape[:-1])
     temperature = _check_temperature(temperature)
     if labels.numel() == 0:
@@ -460,7 +460,8 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
     shape = logprobs.shape
     adv = _detached(advantages)
     if adv.dim() == 1:
-        adv = _token_rows(adv, "advantages", shape[:1])[:, 0]
+        if adv.dtype != torch.float32 or adv.shape[0] != shape[0]:
+            adv = _token_rows(adv, "advantages", shape[:1])[:, 0]
     else:
         adv = _token_rows(adv, "advantages", shape)
     lp = _token_rows(logprobs, "logprobs", shape)

@@ -255,10 +255,14 @@ class Qwen3Model(nn.Module):
         ``losses.linear_logprobs``, another through its logits."""
         hidden = self._trunk(input_ids, position_ids, attention_mask, None)[:, :-1]
         labels = (input_ids if labels is None else labels)[:, 1:]
-        weight = self.lm_head.weight
-        if hidden.dtype == weight.dtype == torch.bfloat16 and weight.shape[1] % 8 == 0:
-            return linear_logprobs(hidden, weight, labels, temperature=temperature)
-        return token_logprobs(self.lm_head(hidden), labels, temperature=temperature)
+        head = self.lm_head
+        # only the product that it is: what a caller put in its place or hooked to it runs
+        plain = type(head) is nn.Linear and head.bias is None and not (
+            head._forward_hooks or head._forward_pre_hooks or head._backward_hooks or head._backward_pre_hooks)
+        if (plain and hidden.dtype == head.weight.dtype == torch.bfloat16 and head.weight.shape[1] % 8 == 0
+                and type(head.weight) is nn.Parameter):
+            return linear_logprobs(hidden, head.weight, labels, temperature=temperature)
+        return token_logprobs(head(hidden), labels, temperature=temperature)
 
     @torch.no_grad()
     def count_parameters(self) -> dict:

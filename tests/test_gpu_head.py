@@ -154,6 +154,23 @@ def test_linear_logprobs_strides_and_shapes():
     assert lp.shape == (0, 41) and not torch.autograd.grad(lp.sum(), wl)[0].any()
 
 
+def test_linear_logprobs_many_rows():
+    """More rows than 2048 gathering workgroups of 16 take: each counts those before its own."""
+    say("linear_logprobs many rows")
+    rows, V, H = 200003, 40, 8
+    g = torch.Generator(device=DEV).manual_seed(145)
+    h = torch.randn(rows, H, generator=g, device=DEV).to(BF).requires_grad_()
+    w = torch.randn(V, H, generator=g, device=DEV).to(BF)
+    labels = torch.randint(0, V, (rows,), generator=g, device=DEV)
+    labels[torch.rand(rows, generator=g, device=DEV) < 0.4] = -100
+    dy = torch.randn(rows, generator=g, device=DEV)
+    lp = nq.linear_logprobs(h, w, labels)
+    (dh,) = torch.autograd.grad(lp, h, dy)
+    want = reference(h.detach(), w, labels, dy, 1.0)
+    within(lp, want[0].cpu(), want[3].cpu(), "logprobs")
+    within(dh, want[1].cpu(), want[4].cpu(), "dhidden")
+
+
 @pytest.mark.parametrize("recompute", [False, True])
 def test_linear_logprobs_several_ranges(recompute):
     """So many rows that the backward takes the vocabulary in several ranges, the last a short one."""
@@ -291,6 +308,26 @@ def test_model_token_logprobs(dtype):
         # bf16: the loss's own path rounds logits, their gradient and each layer's to 2^-8 a piece
         lim = 0.05 if dtype == BF else 1e-4
         assert float((a.double() - b.double()).norm() / b.double().norm().clamp(min=1e-30)) < lim, name
+
+
+def test_model_token_logprobs_runs_what_stands_in_its_head():
+    """A hooked or replaced LM head runs as it is."""
+    say("model token_logprobs of a changed head")
+    model = small_model(BF)
+    ids = torch.randint(0, 997, (2, 9), generator=torch.Generator().manual_seed(8)).to(DEV)
+    with torch.no_grad():
+        plain = model.token_logprobs(ids)
+        handle = model.lm_head.register_forward_hook(lambda mod, args, out: out * 0.5)
+        halved = model.token_logprobs(ids)
+        handle.remove()
+        want = torch.log_softmax((model(ids)["logits"][:, :-1] * 0.5).double(), -1).gather(-1, ids[:, 1:, None])[..., 0]
+        within(halved, want.cpu(), 1e-4, "hooked head")
+        assert torch.equal(model.token_logprobs(ids), plain)
+        model.lm_head = torch.nn.Sequential(model.lm_head, torch.nn.Identity())
+        z = model(ids)["logits"][:, :-1].double()
+        want = torch.log_softmax(z, -1).gather(-1, ids[:, 1:, None])[..., 0]
+        within(model.token_logprobs(ids), want.cpu(), 1e-4, "replaced head")
+        assert model.token_logprobs(ids[:, :1]).shape == (2, 0)
 
 
 def test_preference_and_policy_steps_of_a_model():
