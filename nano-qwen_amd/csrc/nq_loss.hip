@@ -34,7 +34,7 @@ struct TokenParams {
   float c, inv_t;
 };
 
-constexpr int TOK_U = 4;  // vectors of 8 that a thread has in flight
+constexpr int TOK_U = 2;  // vectors of 8 that a thread has in flight (1163 us with 4 where 2 take 1094)
 
 template <typename T>
 __device__ __forceinline__ const T* token_row(const TokenParams& p, int64_t row) {
@@ -49,8 +49,11 @@ __device__ __forceinline__ float label_logprob(const TokenParams& p, const T* x,
   return ((float)x[y] - s.m) * p.inv_t - logf(s.l);
 }
 
-// A workgroup per row, or per slice of a row where the rows are few.
-template <typename T, bool SPLIT>
+// A workgroup per row, or per slice of a row where the rows are few.  Bound by HBM.
+// STREAM: logits of more bytes than the 256 MB cache holds are loaded past it: 1502 rows of
+// 151936 bf16 logits 90 us without, 80 with (5.7 TB/s).  Smaller ones stay in it for the
+// backward: 1026 rows of 50257 fp32, both, 112 us for 121.
+template <typename T, bool SPLIT, bool STREAM>
 __global__ __launch_bounds__(256) void token_logprobs_kernel(TokenParams p) {
   __shared__ RowStat red[4];
   const int tid = threadIdx.x;
@@ -81,7 +84,7 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(TokenParams p) {
     floatx8 v[TOK_U];
 #pragma unroll
     for (int u = 0; u < TOK_U; ++u) {
-      if (j + 256 * u < j1) v[u] = load8_any<T>(x + (int64_t)(j + 256 * u) * 8);
+      if (j + 256 * u < j1) v[u] = load8_any<T, STREAM>(x + (int64_t)(j + 256 * u) * 8);
       else v[u] = floatx8{} - INFINITY;
     }
     float m = s.m;
@@ -145,7 +148,10 @@ __global__ __launch_bounds__(256) void token_join_kernel(TokenParams p) {
 
 // d logits = dy (1[v = label] - p) / T, p = 2^((x - m) c) / l; zero in ignored rows
 // (which are not read), NaN where the label is outside the vocabulary.  Bound by HBM:
-// the logits in, their gradient out; a workgroup takes a slice of a row.
+// the logits in, their gradient out; a workgroup takes a slice of a row.  4 x 2048 rows of
+// 151936 bf16, a quarter ignored, with the forward: 1163 us with plain stores and 4 vectors a
+// thread, 1117 with streaming stores, 1050 with 2 vectors, 1019 with the forward's streaming
+// loads (6.23 GB: 6.1 TB/s).
 struct TokenBwdParams {
   TokenParams t;
   const float* dy;
@@ -153,7 +159,7 @@ struct TokenBwdParams {
   int slices;
 };
 
-constexpr int TOK_SLICE = 256 * TOK_U;  // vectors of a backward workgroup
+constexpr int TOK_SLICE = 256 * TOK_U;  // vectors of a workgroup
 
 template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(TokenBwdParams q) {
@@ -168,7 +174,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(TokenBwdParams 
   if (y == p.ignore) {
 #pragma unroll
     for (int u = 0; u < TOK_U; ++u)
-      if (j0 + 256 * u < nv) store8_any<T>(dx + (int64_t)(j0 + 256 * u) * 8, floatx8{});
+      if (j0 + 256 * u < nv) store8_stream<T>(dx + (int64_t)(j0 + 256 * u) * 8, floatx8{});
     if (tail) dx[nv * 8 + tid] = (T)0.f;
     return;
   }
@@ -189,7 +195,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(TokenBwdParams 
         const float d = k * fast_exp2((v[u][e] - st[0]) * p.c);
         v[u][e] = (int64_t)j * 8 + e == y ? g + d : d;
       }
-      store8_any<T>(dx + (int64_t)j * 8, v[u]);
+      store8_stream<T>(dx + (int64_t)j * 8, v[u]);
     }
   }
   if (tail) {
@@ -559,6 +565,19 @@ static int token_check(const void* logits, const int64_t* labels, const void* st
   return NQ_OK;
 }
 
+template <typename T>
+static void launch_tokens(const TokenParams& p, bool past, hipStream_t st) {
+  const dim3 grid((unsigned)(p.rows * p.splits)), block(256);
+  if (p.splits == 1) {
+    if (past) hipLaunchKernelGGL((token_logprobs_kernel<T, false, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((token_logprobs_kernel<T, false, false>), grid, block, 0, st, p);
+    return;
+  }
+  if (past) hipLaunchKernelGGL((token_logprobs_kernel<T, true, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((token_logprobs_kernel<T, true, false>), grid, block, 0, st, p);
+  hipLaunchKernelGGL((token_join_kernel<T>), dim3((unsigned)((p.rows + 3) / 4)), block, 0, st, p);
+}
+
 extern "C" int nq_token_logprobs(const void* logits, int64_t batch_stride, int64_t row_stride, const int64_t* labels,
                                  float* logprobs, float* stats, void* workspace, int64_t workspace_bytes, int64_t B,
                                  int64_t S, int V, int dtype, float temperature, int64_t ignore_index, void* stream) {
@@ -576,17 +595,9 @@ extern "C" int nq_token_logprobs(const void* logits, int64_t batch_stride, int64
                 reinterpret_cast<floatx2*>(workspace), rows, S, V, splits, ignore_index, inv * kLog2e, inv};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool b16 = dtype == NQ_DTYPE_BF16;
-  const dim3 grid((unsigned)(rows * splits)), join_grid((unsigned)((rows + 3) / 4));
-  if (splits == 1) {
-    if (b16) hipLaunchKernelGGL((token_logprobs_kernel<bf16, false>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((token_logprobs_kernel<float, false>), grid, dim3(256), 0, st, p);
-  } else if (b16) {
-    hipLaunchKernelGGL((token_logprobs_kernel<bf16, true>), grid, dim3(256), 0, st, p);
-    hipLaunchKernelGGL((token_join_kernel<bf16>), join_grid, dim3(256), 0, st, p);
-  } else {
-    hipLaunchKernelGGL((token_logprobs_kernel<float, true>), grid, dim3(256), 0, st, p);
-    hipLaunchKernelGGL((token_join_kernel<float>), join_grid, dim3(256), 0, st, p);
-  }
+  const bool past = rows * V * (b16 ? 2 : 4) > ((int64_t)256 << 20);
+  if (b16) launch_tokens<bf16>(p, past, st);
+  else launch_tokens<float>(p, past, st);
   return nq_check_launch(hipGetLastError());
 }
 

@@ -12,15 +12,17 @@ template <typename T> struct Any8;
 template <> struct Any8<bf16> { typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2))); };
 template <> struct Any8<float> { typedef float type __attribute__((ext_vector_type(8), aligned(4))); };
 
-template <typename T>
+template <typename T, bool STREAM = false>
 __device__ __forceinline__ floatx8 load8_any(const T* p) {
-  const typename Any8<T>::type v = *reinterpret_cast<const typename Any8<T>::type*>(p);
-  return __builtin_convertvector(v, floatx8);
+  const auto* q = reinterpret_cast<const typename Any8<T>::type*>(p);
+  return __builtin_convertvector(STREAM ? __builtin_nontemporal_load(q) : *q, floatx8);
 }
+// Written once and not read here again: past the caches.
 template <typename T>
-__device__ __forceinline__ void store8_any(T* p, floatx8 v) {
+__device__ __forceinline__ void store8_stream(T* p, floatx8 v) {
   typedef T V8 __attribute__((ext_vector_type(8)));
-  *reinterpret_cast<typename Any8<T>::type*>(p) = __builtin_convertvector(v, V8);
+  typedef typename Any8<T>::type A8;
+  __builtin_nontemporal_store((A8)__builtin_convertvector(v, V8), reinterpret_cast<A8*>(p));
 }
 
 // The maximum m of a set of values and l = sum of 2^((x - m) c) over it; (-inf, 0) for
