@@ -161,6 +161,10 @@ __device__ __forceinline__ BufRsrc make_rsrc(const void* base, uint32_t bytes) {
 __device__ __forceinline__ void buffer_load_lds16(BufRsrc r, void* lds, uint32_t voff, uint32_t soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 0);
 }
+// The same past the caches (nt), for data that is read once.
+__device__ __forceinline__ void buffer_load_lds16_nt(BufRsrc r, void* lds, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 2);
+}
 
 // s_waitcnt vmcnt(0): all of this wave's vector-memory loads (including
 // global_load_lds) have completed.

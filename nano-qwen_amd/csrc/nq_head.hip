@@ -4,14 +4,21 @@
 //   forward    z tile by tile; each tile leaves its rows' maximum and sum of exponentials
 //              (and the label's logit), which a second launch joins:
 //              logprob = (z[label] - m) / T - log l
-//   backward   dz = dy (1[v = label] - softmax) / T, formed again from the statistics a
-//              range of the vocabulary at a time, in bf16; dh += dz w and dw = dz^T h
+//   backward   dz = dy (1[v = label] - softmax) / T in bf16, a range of the vocabulary at a
+//              time, from the exponentials that the forward kept or from its product again;
+//              dh += dz w and dw = dz^T h
 //
-// Four products of 2 tokens vocabulary width operations each, all on one core: bf16 MFMA
-// with fp32 accumulation over tiles of 256 x 256 (or 64 tokens, where there are few).  dz
-// is rounded to bf16 once, as the matrix cores need it: half a step, 2^-8 of a value at
-// most, independent from term to term.  Ignored rows are left out first: the kept rows are
-// gathered to the front, and the products run over those.
+// Three or four products of 2 tokens vocabulary width operations each, all on one core:
+// bf16 MFMA with fp32 accumulation over tiles of 256 x 256 (or 64 tokens, where there are
+// few).  dz is rounded to bf16 once, as the matrix cores need it, and so is a kept
+// exponential: half a step, 2^-8 of a value at most, independent from term to term.  Ignored
+// rows are left out first: the kept rows are gathered to the front, and the products run over
+// those.
+//
+// Bound by the matrix cores at the clock that the power limit leaves them.  8192 x 2048 against
+// 151936 entries: forward 4.5 ms (1.14 PFLOP/s; a library product alone 3.9), with what it keeps
+// 4.9; dz 0.9 (5.5 TB/s), dh 4.2 and dw 4.3 (1.2 PFLOP/s; library products 3.8 and 4.7).
+// 3069 x 1024: forward 1.0 and 1.1 ms, dh and dw 0.97 each (library: 1.0, 1.2, 1.1).
 
 #include <math.h>
 
@@ -28,7 +35,8 @@ constexpr int HD_CUS = 256;
 // them, each MT x NT blocks of 32 x 32.  OUT: rows that a wave puts out at a time.
 //   Wide  one workgroup a CU: 128 accumulator registers a lane, 128 KB of operands
 //   Few   at most 64 tokens, bound by reading the weights: three workgroups a CU, so that
-//         72 KB of them are in flight there
+//         72 KB are in flight there (33 rows of 1024 against 151936 entries, 311 MB: 54 us,
+//         60 with two)
 struct Wide {
   static constexpr int BM = 256, BN = 256, M = 2, N = 4, MT = 4, NT = 2, PER_CU = 1, OUT = 32;
 };
@@ -147,7 +155,7 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows p) {
 //         banks.
 // HBM -> LDS without registers; what lies outside (rows past the extent, depths past the
 // end) is out of the descriptor's range and arrives as zeros.
-template <int EXT, bool ROW, int WAVES>
+template <int EXT, bool ROW, int WAVES, bool STREAM = false>
 struct Stage {
   static constexpr int BYTES = EXT * HD_BK * 2;
   static constexpr int NI = BYTES / 1024 / WAVES;   // loads of a wave per step
@@ -193,7 +201,10 @@ struct Stage {
     }
     const uint32_t step = o == NONE ? 0u : WAVES * ROWS_PER * line;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) buffer_load_lds16(r, tile + (wave + WAVES * i) * 1024, o + i * step, 0u);
+    for (int i = 0; i < NI; ++i) {
+      if (STREAM) buffer_load_lds16_nt(r, tile + (wave + WAVES * i) * 1024, o + i * step, 0u);
+      else buffer_load_lds16(r, tile + (wave + WAVES * i) * 1024, o + i * step, 0u);
+    }
   }
 };
 
@@ -264,10 +275,10 @@ struct Reads {
 // while a step's 64 depths are multiplied, one barrier a step, and the step after a tile's
 // last is the next tile's first, so that its loads run under this tile's last products and
 // its epilogue.  The operands of the next 16 depths are read while these are multiplied.
-template <class C, bool AROW, bool BROW, bool GATHER = false>
+template <class C, bool AROW, bool BROW, bool GATHER = false, bool STREAM = false>
 struct Product {
   static constexpr int WAVES = C::M * C::N;
-  typedef Stage<C::BM, AROW, WAVES> A;
+  typedef Stage<C::BM, AROW, WAVES, STREAM> A;
   typedef std::conditional_t<GATHER, GatherStage<C::BN, WAVES>, Stage<C::BN, BROW, WAVES>> B;
   static_assert(BROW || !GATHER, "rows are gathered");
   static constexpr int BUF = A::BYTES + B::BYTES;
@@ -423,9 +434,9 @@ struct HeadParams {
 // entries of each block, so their maximum and sum need no shuffles but one.  KEEP: the
 // exponentials too, for the backward; DZ: dz of a range of the vocabulary instead.
 enum { STATS, KEEP, DZ };
-template <class C, int MODE, bool GATHER = false>
+template <class C, int MODE, bool GATHER = false, bool STREAM = false>
 __global__ __launch_bounds__(threads_of<C>()) void head_logits_kernel(HeadParams p) {
-  typedef Product<C, true, true, GATHER> P;
+  typedef Product<C, true, true, GATHER, STREAM> P;
   extern __shared__ __align__(1024) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int vend = MODE == DZ ? p.v0 + p.vc : p.V, vfirst = MODE == DZ ? p.v0 : 0;
@@ -969,10 +980,10 @@ static void launch_rows(HeadRows& r, hipStream_t st) {
   r.each = rows <= 16 * 2048 ? 16 : ((rows + 2047) / 2048 + 63) / 64 * 64;
   hipLaunchKernelGGL(head_rows_kernel, dim3((unsigned)((rows + r.each - 1) / r.each)), dim3(256), 0, st, r);
 }
-template <class C, int MODE, bool GATHER = false>
+template <class C, int MODE, bool GATHER = false, bool STREAM = false>
 static int launch_logits(int64_t tiles, hipStream_t st, const HeadParams& p) {
-  return head_launch<Product<C, true, true, GATHER>>(head_logits_kernel<C, MODE, GATHER>, head_grid<C>(tiles),
-                                                     threads_of<C>(), st, p);
+  return head_launch<Product<C, true, true, GATHER, STREAM>>(head_logits_kernel<C, MODE, GATHER, STREAM>,
+                                                             head_grid<C>(tiles), threads_of<C>(), st, p);
 }
 template <class C>
 static int launch_dh(int64_t tiles, hipStream_t st, const HeadParams& p) {
@@ -1012,8 +1023,11 @@ extern "C" int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int6
   if (all > INT32_MAX / 2) return nq_fail(NQ_ERR_UNSUPPORTED, "too many tiles for one launch");
   const HeadJoin j{r.src, p.part, p.zlabel, r.count, r.index, r.target, logprobs, r.stats, V, tiles, p.c, inv};
   if (few) {
-    // 33 rows of 1024 against 151936 entries: without the gathering launch 62 us for 69
-    if (int rc = launch_logits<Few, STATS, true>(all, st, p)) return rc;
+    // 33 rows of 1024 against 151936 entries: 69 us with the gathering launch, 60 without it, 54
+    // with weights that the 256 MB cache cannot hold loaded past it
+    const bool past = (int64_t)V * H * 2 > ((int64_t)256 << 20);
+    if (int rc = past ? launch_logits<Few, STATS, true, true>(all, st, p) : launch_logits<Few, STATS, true>(all, st, p))
+      return rc;
     hipLaunchKernelGGL((head_join_kernel<4, true>), dim3((unsigned)((rows + 3) / 4)), dim3(1024), 0, st, j);
   } else {
     launch_rows(r, st);
