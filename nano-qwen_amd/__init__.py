@@ -20,6 +20,11 @@ require grad run the FlashAttention-2 backward kernels (``attention_backward``,
 ``qk_norm_rope_backward``; autograd Functions ``attention_core`` and
 ``flash_attention_train``) where the reference runs SDPA's autograd.
 
+Losses: ``token_logprobs`` and ``linear_logprobs`` (log-probabilities of labels from logits, or
+from hidden states and an LM head), ``preference_loss`` and ``policy_loss``, for what the
+reference's preference and policy loops compose from tensor operations;
+``Qwen3Model.token_logprobs`` gives what they take.
+
 Extensions with no reference counterpart: ``generate_greedy_batch`` (ragged
 batched greedy decoding against per-row cache lengths), ``PagedKVCache``
 (block-table page pool), ``attention_decode_paged`` (decode with the new

@@ -16,9 +16,9 @@
 // those.
 //
 // Bound by the matrix cores at the clock that the power limit leaves them.  8192 x 2048 against
-// 151936 entries: forward 4.5 ms (1.14 PFLOP/s; a library product alone 3.9), with what it keeps
-// 4.9; dz 0.9 (5.5 TB/s), dh 4.2 and dw 4.3 (1.2 PFLOP/s; library products 3.8 and 4.7).
-// 3069 x 1024: forward 1.0 and 1.1 ms, dh and dw 0.97 each (library: 1.0, 1.2, 1.1).
+// 151936 entries: the forward, with what it keeps, 4.5 ms (1.14 PFLOP/s; a library product of
+// its size alone 3.8), dz 0.9 (5.5 TB/s), dh 4.0 and dw 4.1 (library products 3.8 and 4.6).
+// 4 x 1023 rows of 1024, a quarter ignored: 0.93 ms, 0.34, 0.84 and 0.84 (library 1.0, 1.2 and 1.1).
 
 #include <math.h>
 
