@@ -98,21 +98,23 @@ def _check_labels(labels: torch.Tensor, rows_shape) -> torch.Tensor:
 
 def _rows_2d(x: torch.Tensor):
     """(x, B, S, batch stride, row stride): x as B sequences of S rows, copied only if its
-    leading axes do not fold into two or its last axis is not contiguous."""
+    leading axes do not fold into two or its last axis is not contiguous.  The stride of an
+    axis of one is anything, and 0 here."""
     V = x.shape[-1]
     if x.stride(-1) != 1 and V > 1:
         x = x.contiguous()
     if x.dim() == 1:
         return x, 1, 1, 0, 0
     if x.dim() == 2:
-        return x, 1, x.shape[0], 0, x.stride(0)
+        return x, 1, x.shape[0], 0, x.stride(0) if x.shape[0] > 1 else 0
     if x.dim() > 3:
         try:
             v = x.view(-1, *x.shape[-2:])
         except RuntimeError:
             v = x.contiguous().view(-1, *x.shape[-2:])
         x = v
-    return x, x.shape[0], x.shape[1], x.stride(0), x.stride(1)
+    B, S = x.shape[:2]
+    return x, B, S, x.stride(0) if B > 1 else 0, x.stride(1) if S > 1 else 0
 
 
 def _token_forward(logits, labels, temperature: float, ignore_index: int):

@@ -154,6 +154,24 @@ def test_linear_logprobs_strides_and_shapes():
     assert lp.shape == (0, 41) and not torch.autograd.grad(lp.sum(), wl)[0].any()
 
 
+@pytest.mark.parametrize("shape", [(1,), (1, 1), (3, 1), (1, 3)])
+def test_linear_logprobs_of_axes_of_one(shape):
+    """An axis of one has any stride, here no multiple of 16 bytes."""
+    say(f"linear_logprobs axes of one {shape}")
+    h, w, labels, dy = inputs(shape, 100, 64, 135)
+    big = torch.zeros(2 * 2 * 4 * 8 * 73, dtype=BF, device=DEV)
+    strides = [73 if n == 1 else 8 * 72 for n in shape] + [1]
+    view = big.as_strided((*shape, 64), strides)
+    with torch.no_grad():
+        view.copy_(h)
+    leaf, wl = view.detach().requires_grad_(), w.to(DEV).requires_grad_()
+    lp = nq.linear_logprobs(leaf, wl, labels.to(DEV))
+    got = (lp, *torch.autograd.grad(lp, (leaf, wl), dy.to(DEV)))
+    want = reference(h, w, labels, dy, 1.0)
+    for a, ref, tol in zip(got, want, want[3:]):
+        within(a, ref, tol, "axes of one")
+
+
 def test_linear_logprobs_many_rows():
     """More rows than 2048 gathering workgroups of 16 take: each counts those before its own."""
     say("linear_logprobs many rows")

@@ -522,3 +522,52 @@ def test_losses_in_a_graph():
         got = [t.clone() for t in outs]
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+def test_losses_under_autograd_modes():
+    """Saved tensors that travel to the host and back, a graph gone through twice, inputs written to before
+    the backward, inference mode, a mask or labels that change: the same bits or an error, never stale values."""
+    say("losses under autograd modes")
+    x = randn(2, 9, 301, seed=95, dtype=BF).to(DEV)
+    h = randn(2, 70, 64, seed=96).to(BF).to(DEV)
+    w = randn(90, 64, seed=97).to(BF).to(DEV)
+    y = torch.randint(0, 90, (2, 70), device=DEV)
+    m = ragged(2, 9, 98).to(DEV)
+    old = randn(2, 9, seed=99).to(DEV)
+
+    def losses(x, h, w, y=y, m=m):
+        lp = nq.token_logprobs(x, y[:, :9])
+        pref, *_ = nq.preference_loss(lp[:1], lp[1:], chosen_mask=m[:1], rejected_mask=m[1:])
+        pol, *_ = nq.policy_loss(lp, old, old[:, 0], mask=m)
+        return pref + pol + nq.linear_logprobs(h, w, y).sum()
+
+    def leaves():
+        return [t.clone().requires_grad_() for t in (x, h, w)]
+
+    ins = leaves()
+    loss = losses(*ins)
+    want = torch.autograd.grad(loss, ins, retain_graph=True)
+    for a, b in zip(torch.autograd.grad(loss, ins), want):
+        assert torch.equal(a, b)
+    ins = leaves()
+    with torch.autograd.graph.save_on_cpu():
+        loss = losses(*ins)
+    torch.empty(1 << 24, device=DEV).fill_(7)  # over what the forward held
+    for a, b in zip(torch.autograd.grad(loss, ins), want):
+        assert torch.equal(a, b)
+    for change in ("labels", "mask", "hidden"):
+        ins = leaves()
+        y2, m2, mid = y.clone(), m.clone(), ins[1] * 1
+        loss = losses(ins[0], mid, ins[2], y2, m2)
+        {"labels": y2, "mask": m2, "hidden": mid}[change].zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, ins)
+    with torch.inference_mode():
+        inside = losses(x, h, w)
+    with torch.no_grad():
+        assert torch.equal(inside, losses(x, h, w))
+    # transforms that the kernels have no part in are refused, not answered with other numbers
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: nq.token_logprobs(t, y[:, :9]), (x.float(),), (x.float(),))
+    with pytest.raises(Exception):
+        torch.vmap(lambda t: nq.token_logprobs(t, y[0, :9]))(x.float())
