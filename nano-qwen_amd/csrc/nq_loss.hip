@@ -49,15 +49,18 @@ __device__ __forceinline__ float label_logprob(const TokenParams& p, const T* x,
   return ((float)x[y] - s.m) * p.inv_t - logf(s.l);
 }
 
-// A workgroup per row, or per slice of a row where the rows are few.  Bound by HBM.
+// TEAM threads a row: a workgroup, or a wave where the row is no more than 4 vectors a lane
+// (65536 rows of 1000 in bf16: 33 us for 78); with SPLIT, where the rows are few, a workgroup a slice
+// of a row.  Bound by HBM.
 // STREAM: logits of more bytes than the 256 MB cache holds are loaded past it: 1502 rows of
 // 151936 bf16 logits 90 us without, 80 with (5.7 TB/s).  Smaller ones stay in it for the
 // backward: 1026 rows of 50257 fp32, both, 112 us for 121.
-template <typename T, bool SPLIT, bool STREAM>
+template <typename T, int TEAM, bool SPLIT, bool STREAM>
 __global__ __launch_bounds__(256) void token_logprobs_kernel(TokenParams p) {
   __shared__ RowStat red[4];
-  const int tid = threadIdx.x;
-  int64_t row = blockIdx.x;
+  const int tid = threadIdx.x % TEAM;
+  int64_t row = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
+  if (TEAM < 256 && row >= p.rows) return;
   int slice = 0;
   if (SPLIT) {
     slice = (int)(row % p.splits);
@@ -80,11 +83,11 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(TokenParams p) {
     j1 = j + per < nv ? j + per : nv;
   }
   RowStat s{-INFINITY, 0.f};
-  for (j += tid; j < j1; j += 256 * TOK_U) {
+  for (j += tid; j < j1; j += TEAM * TOK_U) {
     floatx8 v[TOK_U];
 #pragma unroll
     for (int u = 0; u < TOK_U; ++u) {
-      if (j + 256 * u < j1) v[u] = load8_any<T, STREAM>(x + (int64_t)(j + 256 * u) * 8);
+      if (j + TEAM * u < j1) v[u] = load8_any<T, STREAM>(x + (int64_t)(j + TEAM * u) * 8);
       else v[u] = floatx8{} - INFINITY;
     }
     float m = s.m;
@@ -106,10 +109,12 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(TokenParams p) {
   }
 #pragma unroll
   for (int k = 32; k >= 1; k >>= 1) s = join(s, RowStat{__shfl_xor(s.m, k, 64), __shfl_xor(s.l, k, 64)}, p.c);
-  if ((tid & 63) == 0) red[tid >> 6] = s;
-  __syncthreads();
+  if (TEAM == 256) {
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    __syncthreads();
+  }
   if (tid == 0) {
-    s = join(join(red[0], red[1], p.c), join(red[2], red[3], p.c), p.c);
+    if (TEAM == 256) s = join(join(red[0], red[1], p.c), join(red[2], red[3], p.c), p.c);
     if (SPLIT) {
       p.part[row * p.splits + slice] = floatx2{s.m, s.l};
     } else {
@@ -569,17 +574,17 @@ static int token_check(const void* logits, const int64_t* labels, const void* st
   return NQ_OK;
 }
 
-template <typename T>
-static void launch_tokens(const TokenParams& p, bool past, hipStream_t st) {
-  const dim3 grid((unsigned)(p.rows * p.splits)), block(256);
-  if (p.splits == 1) {
-    if (past) hipLaunchKernelGGL((token_logprobs_kernel<T, false, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((token_logprobs_kernel<T, false, false>), grid, block, 0, st, p);
-    return;
+template <typename T, bool STREAM>
+static void launch_tokens(const TokenParams& p, hipStream_t st) {
+  const dim3 block(256), waves((unsigned)((p.rows + 3) / 4)), grid((unsigned)(p.rows * p.splits));
+  if (p.splits > 1) {
+    hipLaunchKernelGGL((token_logprobs_kernel<T, 256, true, STREAM>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((token_join_kernel<T>), waves, block, 0, st, p);
+  } else if (p.V / 8 <= 256) {
+    hipLaunchKernelGGL((token_logprobs_kernel<T, 64, false, STREAM>), waves, block, 0, st, p);
+  } else {
+    hipLaunchKernelGGL((token_logprobs_kernel<T, 256, false, STREAM>), grid, block, 0, st, p);
   }
-  if (past) hipLaunchKernelGGL((token_logprobs_kernel<T, true, true>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((token_logprobs_kernel<T, true, false>), grid, block, 0, st, p);
-  hipLaunchKernelGGL((token_join_kernel<T>), dim3((unsigned)((p.rows + 3) / 4)), block, 0, st, p);
 }
 
 extern "C" int nq_token_logprobs(const void* logits, int64_t batch_stride, int64_t row_stride, const int64_t* labels,
@@ -600,8 +605,8 @@ extern "C" int nq_token_logprobs(const void* logits, int64_t batch_stride, int64
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool b16 = dtype == NQ_DTYPE_BF16;
   const bool past = rows * V * (b16 ? 2 : 4) > ((int64_t)256 << 20);
-  if (b16) launch_tokens<bf16>(p, past, st);
-  else launch_tokens<float>(p, past, st);
+  if (b16) past ? launch_tokens<bf16, true>(p, st) : launch_tokens<bf16, false>(p, st);
+  else past ? launch_tokens<float, true>(p, st) : launch_tokens<float, false>(p, st);
   return nq_check_launch(hipGetLastError());
 }
 

@@ -81,7 +81,7 @@ def check_token(x, labels, dy, T=1.0, what="", **kw):
 # rows of less than a vector, of whole vectors and not, of one and of many slices; one row to
 # more than the split is for
 @pytest.mark.parametrize("rows,V", [(1, 1), (1, 8), (3, 7), (2, 9), (5, 1000), (4, 8192), (3, 8200), (2, 50257), (1, 151936),
-                                    (2100, 133), (260, 16391)])
+                                    (2100, 133), (260, 16391), (6, 2055), (6, 2056)])
 @pytest.mark.parametrize("dt", [BF, F32])
 def test_token_logprobs(rows, V, dt):
     say(f"token_logprobs {rows}x{V} {dt}")
@@ -319,6 +319,53 @@ def test_preference_loss_far_margins_and_rows():
     within(loss, want[0], 4 * U * want[0].abs(), "expanded")
     # torch sums the four rows' gradients, each rounded to bf16
     within(g, want[3].sum(0, keepdim=True), 4 * 2.0 ** -8 * want[3].abs().sum(0, keepdim=True), "expanded gradient")
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "ipo"])
+def test_preference_loss_differences(kind):
+    """The gradients against central differences of the operator itself."""
+    say(f"preference_loss differences {kind}")
+    c, r, v, w = (0.3 * randn(5, 6, seed=49 + i).to(DEV) for i in range(4))
+
+    def f(t):
+        return nq.preference_loss(c + t * v, r + t * w, kind=kind, beta=0.5)[0]
+    cg, rg = c.clone().requires_grad_(), r.clone().requires_grad_()
+    dc, dr = torch.autograd.grad(nq.preference_loss(cg, rg, kind=kind, beta=0.5)[0], (cg, rg))
+    h = 2.0 ** -7
+    diff = float(f(h).double() - f(-h).double()) / (2 * h)
+    # along the step a pair's margin moves by s t: third derivatives under (beta s)^3 / 8 (sigmoid), none (the others,
+    # with no hinge within h of a corner); the ends off by u of the loss and of their rounded inputs
+    s = float((v.abs().sum(1) + w.abs().sum(1)).max())
+    size = float(f(0.0).abs()) + s + float((c.abs().sum(1) + r.abs().sum(1)).max()) * (1 + 2 * s)
+    bound = (0.5 * s) ** 3 * h * h / 6 + 4 * U * size / h
+    margin = 0.5 * (c.double().sum(1) - r.double().sum(1))
+    assert kind != "hinge" or float((margin - 1).abs().min()) > 0.5 * s * h
+    assert abs(diff - float((dc * v).double().sum() + (dr * w).double().sum())) <= bound
+
+
+def test_policy_loss_differences():
+    """The gradient against central differences of the operator itself, no token within a step of a border."""
+    say("policy_loss differences")
+    lp, v = -randn(4, 9, seed=61).abs(), randn(4, 9, seed=62)
+    d = 0.5 * randn(4, 9, seed=63)
+    h = 2.0 ** -8
+    for border in (math.log1p(0.2), math.log1p(-0.2)):
+        near = (d - border).abs() < 2 * h * v.abs().max()
+        d = torch.where(near, d + 4 * h * v.abs().max(), d)
+    for border in (math.log1p(0.2), math.log1p(-0.2)):
+        assert ((d - border).abs() > h * v.abs().max()).all()
+    old, ref, adv = lp - d, lp + 0.4 * randn(4, 9, seed=64), randn(4, seed=65)
+
+    def f(x):
+        return nq.policy_loss(x, old.to(DEV), adv.to(DEV), ref_logprobs=ref.to(DEV), kl_coef=0.3)[0]
+    x = lp.to(DEV).requires_grad_()
+    (g,) = torch.autograd.grad(f(x), x)
+    with torch.no_grad():
+        diff = float(f((lp + h * v).to(DEV)).double() - f((lp - h * v).to(DEV)).double()) / (2 * h)
+    # a term's third derivative is under (|r A| + 0.3 e^q) |v|^3, its value off by some 16 u and by u |lp| of its input
+    big = float((d.exp() * 2).max() * adv.abs().max() + 0.3 * 2 * (ref - lp).exp().max())
+    bound = big * float(v.abs().max()) ** 3 * h * h / 6 + big * (16 + float(lp.abs().max()) * 2) * U / h
+    assert abs(diff - float((g.cpu().double() * v).sum())) <= bound
 
 
 def test_preference_loss_refusals():
