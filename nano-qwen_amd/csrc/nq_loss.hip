@@ -49,9 +49,10 @@ __device__ __forceinline__ float label_logprob(const TokenParams& p, const T* x,
   return ((float)x[y] - s.m) * p.inv_t - logf(s.l);
 }
 
-// TEAM threads a row: a workgroup, or a wave where the row is no more than 4 vectors a lane
-// (65536 rows of 1000 in bf16: 33 us for 78); with SPLIT, where the rows are few, a workgroup a slice
-// of a row.  Bound by HBM.
+// TEAM threads a row: a workgroup; a wave where the row is no more than 4 vectors a lane (65536
+// rows of 1000 in bf16: 33 us for 78), or 16 where the rows fill the chip (16384 rows of 2500,
+// 5000, 8000: 20, 29, 44 us for 31, 39, 49; of 16000 alike); with SPLIT, where the rows are few, a
+// workgroup a slice of a row.  Bound by HBM.
 // STREAM: logits of more bytes than the 256 MB cache holds are loaded past it: 1502 rows of
 // 151936 bf16 logits 90 us without, 80 with (5.7 TB/s).  Smaller ones stay in it for the
 // backward: 1026 rows of 50257 fp32, both, 112 us for 121.
@@ -580,7 +581,7 @@ static void launch_tokens(const TokenParams& p, hipStream_t st) {
   if (p.splits > 1) {
     hipLaunchKernelGGL((token_logprobs_kernel<T, 256, true, STREAM>), grid, block, 0, st, p);
     hipLaunchKernelGGL((token_join_kernel<T>), waves, block, 0, st, p);
-  } else if (p.V / 8 <= 256) {
+  } else if (p.V / 8 <= (p.rows >= 2048 ? 1024 : 256)) {
     hipLaunchKernelGGL((token_logprobs_kernel<T, 64, false, STREAM>), waves, block, 0, st, p);
   } else {
     hipLaunchKernelGGL((token_logprobs_kernel<T, 256, false, STREAM>), grid, block, 0, st, p);

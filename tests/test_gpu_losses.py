@@ -81,7 +81,7 @@ def check_token(x, labels, dy, T=1.0, what="", **kw):
 # rows of less than a vector, of whole vectors and not, of one and of many slices; one row to
 # more than the split is for
 @pytest.mark.parametrize("rows,V", [(1, 1), (1, 8), (3, 7), (2, 9), (5, 1000), (4, 8192), (3, 8200), (2, 50257), (1, 151936),
-                                    (2100, 133), (260, 16391), (6, 2055), (6, 2056)])
+                                    (2100, 133), (260, 16391), (6, 2055), (6, 2056), (2049, 4100), (2048, 8199), (2048, 8200)])
 @pytest.mark.parametrize("dt", [BF, F32])
 def test_token_logprobs(rows, V, dt):
     say(f"token_logprobs {rows}x{V} {dt}")
