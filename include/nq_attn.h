@@ -524,8 +524,8 @@ int nq_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t row_
  *
  * kept: NULL, or nq_linear_logprobs_kept_bytes(B * S, V, H) bytes, 256-byte aligned, that the
  * forward fills (2 bytes a logit) and the backward of the same operands takes: it saves a
- * quarter of the products.  0 bytes: nothing is kept for these sizes (at most 64 rows, or
- * more than 4 GiB).
+ * quarter of the products.  0 bytes: nothing is kept for these sizes (at most 64 rows, H
+ * under 256, or more than 4 GiB).
  *
  * The backward forms dz = dlogprobs[n] (1[v = label] - softmax) / temperature in bf16, a
  * range of the vocabulary at a time, from kept or from the products again, and writes

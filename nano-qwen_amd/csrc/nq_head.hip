@@ -860,20 +860,23 @@ struct HeadSpace {
 constexpr int64_t HD_DZ_BYTES = (int64_t)1 << 30;  // the largest range's dz
 
 // What a forward keeps for its backward: the labels' logits, the maxima of each 128 entries
-// and the exponentials.  Up to 4 GiB (1.4% of the memory), and beyond 64 rows: a product of so
-// few is bound by the weights' bytes, of which this would save one pass in four.
+// and the exponentials.  Up to 4 GiB (1.4% of the memory); beyond 64 rows, as a product of so few
+// is bound by the weights' bytes, of which this would save one pass in four; and from a width of
+// 256, below which the product takes less than the exponentials' bytes (forward and backward
+// of 8192 rows against 151936 entries, kept and repeated: width 128 2978 and 2865 us, 256
+// 3437 and 3552, 1024 7771 and 9441; 2048 rows 809 and 755, 910 and 918, 2030 and 2428).
 struct HeadKept {
   int64_t zlabel, m, exps, total, ldv;
 };
 constexpr int64_t HD_KEPT_BYTES = (int64_t)4 << 30;
 
-static HeadKept head_kept(int64_t rows, int V) {
+static HeadKept head_kept(int64_t rows, int V, int H) {
   HeadKept k{};
   k.ldv = (V + 7) / 8 * 8;
   k.m = pad256(rows * 4);
   k.exps = k.m + pad256(rows * ((V + 255) / 256 * 2) * 4);
   k.total = k.exps + pad256(rows * k.ldv * 2);
-  if (head_few(rows) || k.total > HD_KEPT_BYTES) k.total = 0;
+  if (head_few(rows) || H < 256 || k.total > HD_KEPT_BYTES) k.total = 0;
   return k;
 }
 
@@ -924,7 +927,7 @@ extern "C" int64_t nq_linear_logprobs_workspace_bytes(int64_t rows, int V, int H
   return head_sizes_ok(rows, V, H) ? head_space(rows, V, H, false).total : 0;
 }
 extern "C" int64_t nq_linear_logprobs_kept_bytes(int64_t rows, int V, int H) {
-  return head_sizes_ok(rows, V, H) ? head_kept(rows, V).total : 0;
+  return head_sizes_ok(rows, V, H) ? head_kept(rows, V, H).total : 0;
 }
 extern "C" int64_t nq_linear_logprobs_bwd_workspace_bytes(int64_t rows, int V, int H) {
   return head_sizes_ok(rows, V, H) ? head_space(rows, V, H, true).total : 0;
@@ -947,7 +950,7 @@ static int head_check(const void* hidden, int64_t bs, int64_t rs, const void* we
   const float inv = 1.f / temperature;
   if (!(temperature > 0.f) || !isfinite(temperature) || !isfinite(inv * kLog2e))
     return nq_fail(NQ_ERR_INVALID, "the temperature must be positive and finite, and so must its reciprocal");
-  const int64_t keeps = head_kept(B * S, V).total;
+  const int64_t keeps = head_kept(B * S, V, H).total;
   if (kept && (!keeps || kept_bytes < keeps || (reinterpret_cast<uintptr_t>(kept) & 255u)))
     return nq_fail(NQ_ERR_WORKSPACE, "kept too small or not 256-byte aligned: %lld bytes, need %lld (0: none is kept)",
                    (long long)kept_bytes, (long long)keeps);
@@ -958,8 +961,8 @@ static int head_check(const void* hidden, int64_t bs, int64_t rs, const void* we
   return NQ_OK;
 }
 
-static void head_kept_at(void* kept, int64_t rows, int V, HeadParams* p) {
-  const HeadKept k = head_kept(rows, V);
+static void head_kept_at(void* kept, HeadParams* p) {
+  const HeadKept k = head_kept(p->rows, p->V, p->H);
   char* at = reinterpret_cast<char*>(kept);
   p->zlabel = reinterpret_cast<float*>(at + k.zlabel), p->exps_m = reinterpret_cast<float*>(at + k.m);
   p->exps = reinterpret_cast<bf16*>(at + k.exps), p->ldv = k.ldv;
@@ -1016,7 +1019,7 @@ extern "C" int nq_linear_logprobs(const void* hidden, int64_t batch_stride, int6
   p.src = r.src, p.hc = r.hc, p.w = reinterpret_cast<const bf16*>(weight), p.rows = rows, p.V = V, p.H = H;
   p.count = r.count, p.target = r.target, p.c = inv * kLog2e;
   p.part = reinterpret_cast<floatx2*>(ws + s.part), p.zlabel = reinterpret_cast<float*>(ws + s.zlabel);
-  if (kept) head_kept_at(kept, rows, V, &p);
+  if (kept) head_kept_at(kept, &p);
   const bool few = head_few(rows);
   const int bm = few ? Few::BM : Wide::BM, bn = few ? Few::BN : Wide::BN, tiles = (V + bm - 1) / bm;
   const int64_t all = tiles * ((rows + bn - 1) / bn);
@@ -1067,7 +1070,7 @@ extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, 
   p.hc = r.hc, p.w = reinterpret_cast<const bf16*>(weight), p.rows = rows, p.V = V, p.H = H;
   p.count = r.count, p.target = r.target, p.c = inv * kLog2e, p.coef = r.coef;
   p.dz = reinterpret_cast<bf16*>(ws + s.dz), p.ldz = s.ldz;
-  if (kept) head_kept_at(const_cast<void*>(kept), rows, V, &p);
+  if (kept) head_kept_at(const_cast<void*>(kept), &p);
   p.dw = reinterpret_cast<bf16*>(dweight), p.dh = reinterpret_cast<float*>(ws + s.dh), p.vmax = s.vc;
   const bool few = head_few(rows);
   const int bm = few ? Few::BM : Wide::BM, bn = few ? Few::BN : Wide::BN, nh = (H + bm - 1) / bm;

@@ -240,8 +240,9 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     weight's gradients.
 
     A call with a gradient keeps the softmax's numerators for it, in bf16, 2 bytes for each
-    entry of each row, where that is at most 4 GiB; with ``recompute``, and beyond, it keeps
-    two numbers a row and the backward repeats the first product (a fifth slower).
+    entry of each row, where that is faster (widths from 256, more than 64 rows) and at most
+    4 GiB; otherwise, and with ``recompute``, it keeps two numbers a row and the backward
+    repeats the first product (up to a fifth slower).
 
     An fp32 head goes through its logits:
     ``token_logprobs(F.linear(hidden, weight), labels)``.

@@ -86,9 +86,11 @@ def test_linear_logprobs_refuses(make, fn):
     for kw in (dict(ws=None), dict(n=100), dict(ws=ctypes.c_void_p((1 << 20) + 16))):
         refused(fn, WS, "workspace", *make(**kw))
     # kept: too small, misaligned, or for sizes that keep nothing
-    refused(fn, WS, "kept", *make(S=100, kept=P, nk=16))
-    refused(fn, WS, "kept", *make(S=100, kept=ctypes.c_void_p((1 << 20) + 16), nk=BIG))
-    refused(fn, WS, "kept", *make(S=64, kept=P, nk=BIG))
+    wide = dict(H=256, rs=256)
+    refused(fn, WS, "kept", *make(S=100, kept=P, nk=16, **wide))
+    refused(fn, WS, "kept", *make(S=100, kept=ctypes.c_void_p((1 << 20) + 16), nk=BIG, **wide))
+    refused(fn, WS, "kept", *make(S=64, kept=P, nk=BIG, **wide))
+    refused(fn, WS, "kept", *make(S=100, kept=P, nk=BIG))
     if fn.endswith("_bwd"):
         refused(fn, INV, "dlogprobs", *make(dy=None))
         refused(fn, INV, "aligned", *make(dw=ctypes.c_void_p((1 << 20) + 8)))
@@ -147,9 +149,10 @@ def test_workspaces():
     # kept: two bytes an entry, four a row and a maximum per 128 entries, each part from a multiple of 256
     def up(n):
         return -(-n // 256) * 256
-    assert lib.nq_linear_logprobs_kept_bytes(65, 1001, 64) == up(65 * 4) + up(65 * 8 * 4) + up(65 * 1008 * 2)
-    assert lib.nq_linear_logprobs_kept_bytes(64, 1001, 64) == 0
-    assert lib.nq_linear_logprobs_kept_bytes(16384, 151936, 64) == 0    # over 4 GiB
+    assert lib.nq_linear_logprobs_kept_bytes(65, 1001, 256) == up(65 * 4) + up(65 * 8 * 4) + up(65 * 1008 * 2)
+    assert lib.nq_linear_logprobs_kept_bytes(64, 1001, 256) == 0
+    assert lib.nq_linear_logprobs_kept_bytes(65, 1001, 248) == 0
+    assert lib.nq_linear_logprobs_kept_bytes(16384, 151936, 256) == 0    # over 4 GiB
     # the backward's gradient of the logits is held at most 1 GiB at a time, however many rows
     small, large = (lib.nq_linear_logprobs_bwd_workspace_bytes(r, 151936, 64) for r in (2048, 1 << 16))
     assert small < 2 ** 31 and large < 2 ** 31 + 2 ** 28
