@@ -26,6 +26,8 @@ __all__ = ["token_logprobs", "linear_logprobs", "preference_loss", "policy_loss"
 
 IGNORE_INDEX = -100
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
 _KINDS = {"sigmoid": _lib.NQ_PREF_SIGMOID, "hinge": _lib.NQ_PREF_HINGE, "ipo": _lib.NQ_PREF_IPO}
 
 
@@ -34,7 +36,14 @@ _KINDS = {"sigmoid": _lib.NQ_PREF_SIGMOID, "hinge": _lib.NQ_PREF_HINGE, "ipo": _
 # gradient goes round autograd or through it as one tuple, and little stands around a launch.
 
 def _launch(t: torch.Tensor, fn, name: str, *args) -> None:
-    """fn(*args, stream) on t's device (a launch goes to the current one)."""
+    """fn(*args, stream) on t's device (a launch goes to the current one).
+
+    A recording of tensor operations (``torch.jit.trace``, ``make_fx``) holds the outputs'
+    allocation and not the launch, and its replays would return what the memory holds: it is
+    refused.  ``torch.compile`` breaks its graph here and calls the kernel as it is."""
+    if (torch._C._is_tracing() or torch._C._get_dispatch_mode(_PROXY) is not None
+            or torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None):
+        raise RuntimeError(f"{name}: a trace of tensor operations cannot hold the kernels of the losses")
     index = t.get_device()
     args += (torch._C._cuda_getCurrentRawStream(index),)
     if index == torch._C._cuda_getDevice():
@@ -73,6 +82,11 @@ def _check_devices(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None
             raise ValueError(f"the operands lie on different devices: {first.device} and {t.device}")
     if index < 0 or not first.is_cuda:
         ops._require_device(first)
+    for t in (first, *others):
+        if t is not None and not t.data_ptr() and t.numel():
+            # distributed, functionalized and other wrapped tensors: a kernel would take the
+            # null pointer of an optional operand for one left out
+            raise TypeError(f"the kernels need tensors with memory of their own, got {type(t).__name__} without")
 
 
 def _check_temperature(temperature: float) -> float:

@@ -618,3 +618,38 @@ def test_losses_under_autograd_modes():
         torch.func.jvp(lambda t: nq.token_logprobs(t, y[:, :9]), (x.float(),), (x.float(),))
     with pytest.raises(Exception):
         torch.vmap(lambda t: nq.token_logprobs(t, y[0, :9]))(x.float())
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore:.*jit.*:DeprecationWarning")
+def test_losses_traced_and_compiled():
+    """A trace, which would hold uninitialised outputs, is refused; a compiled function breaks its graph at the
+    kernels and gives their bits; tensors without memory of their own are refused."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.testing._internal.two_tensor import TwoTensor
+    say("losses traced and compiled")
+    y = torch.randint(0, 77, (2, 6), generator=torch.Generator().manual_seed(1)).to(DEV)
+    h, w = randn(2, 6, 64, seed=2, dtype=BF).to(DEV), randn(77, 64, seed=3, dtype=BF).to(DEV)
+    x, lp = randn(2, 6, 77, seed=4).to(DEV), randn(2, 6, seed=5).to(DEV)
+    m = ragged(2, 6, 6).to(DEV)
+    calls = [(lambda x: nq.token_logprobs(x, y), x), (lambda h: nq.linear_logprobs(h, w, y), h),
+             (lambda t: nq.preference_loss(t[:1], t[1:], chosen_mask=m[:1], rejected_mask=m[1:])[0], lp),
+             (lambda t: nq.policy_loss(t, lp + 0.1, lp[:, 0], mask=m)[0], lp)]
+    for call, first in calls:
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, (first,), check_trace=False)
+        with pytest.raises(RuntimeError, match="trace"):
+            make_fx(call)(first)
+        with pytest.raises(TypeError, match="memory"):
+            call(TwoTensor(first, first))
+        torch._dynamo.reset()
+        compiled = torch.compile(lambda t: call(t * 2) * 3, backend="eager")
+        assert torch.equal(compiled(first), call(first * 2) * 3)
+        a, b = first.clone().requires_grad_(), first.clone().requires_grad_()
+        got, want = compiled(a), call(b * 2) * 3
+        assert torch.equal(got, want)
+        d = torch.ones_like(want)
+        assert torch.equal(torch.autograd.grad(got, a, d)[0], torch.autograd.grad(want, b, d)[0])
+    torch._dynamo.reset()
+    for kw in (dict(mask=TwoTensor(m, m)), dict(ref_logprobs=TwoTensor(lp, lp))):
+        with pytest.raises(TypeError, match="memory"):
+            nq.policy_loss(lp, lp, lp, **kw)

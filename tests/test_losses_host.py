@@ -164,3 +164,80 @@ def test_host_tensors_raise():
                  lambda: nq.preference_loss(x, x), lambda: nq.policy_loss(x, x, x[:, 0])):
         with pytest.raises(RuntimeError, match="HIP device"):
             call()
+
+
+# ---------------------------------------------------------------- calls with the kernels stubbed
+
+@pytest.fixture
+def stubbed(monkeypatch):
+    """The operators on host tensors, with a library that counts its launches and writes nothing."""
+    launches = []
+
+    class Library:
+        def __getattr__(self, name):
+            if name.endswith("_bytes"):
+                return lambda *args: 16
+            return lambda *args: launches.append(name) or 0
+
+    monkeypatch.setattr(_lib, "load", lambda: Library())
+    monkeypatch.setattr(nq.losses.ops, "_require_device", lambda *ts: None)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1)
+    return launches
+
+
+def loss_calls():
+    """Each operator as a function of its first operand, and one."""
+    y, lp = torch.tensor([1, 2, 0]), torch.zeros(3, 4)
+    w = torch.zeros(5, 8, dtype=torch.bfloat16)
+    return {
+        "token_logprobs": (lambda x: nq.token_logprobs(x, y), torch.zeros(3, 4)),
+        "linear_logprobs": (lambda h: nq.linear_logprobs(h, w, y), torch.zeros(3, 8, dtype=torch.bfloat16)),
+        "preference_loss": (lambda x: nq.preference_loss(x, lp, lp, lp)[0], torch.zeros(3, 4)),
+        "policy_loss": (lambda x: nq.policy_loss(x, lp, lp[:, 0])[0], torch.zeros(3, 4)),
+    }
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore:.*jit.*:DeprecationWarning")
+@pytest.mark.parametrize("name", ["token_logprobs", "linear_logprobs", "preference_loss", "policy_loss"])
+def test_traces_are_refused(stubbed, name):
+    """A trace would hold the allocation of the outputs without the kernel that writes them."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, x = loss_calls()[name]
+    call(x)
+    assert len(stubbed) == 1
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(call, (x,), check_trace=False)
+    for kw in ({}, dict(pre_dispatch=True)):
+        with pytest.raises(RuntimeError, match="trace"):
+            make_fx(call, **kw)(x)
+    # a traced backward of an eager forward
+    leaf = x.clone().requires_grad_()
+    out = call(leaf)
+    with pytest.raises(RuntimeError, match="trace"):
+        make_fx(lambda d: torch.autograd.grad(out, leaf, d, retain_graph=True))(torch.ones_like(out))
+    assert len(stubbed) == 2
+    torch.autograd.grad(out, leaf, torch.ones_like(out))
+    assert len(stubbed) == 3
+
+
+def test_tensors_without_memory_are_refused(stubbed):
+    """A wrapped tensor's null pointer stands for an operand left out: no mask, no reference."""
+    from torch.testing._internal.two_tensor import TwoTensor
+    for call, x in loss_calls().values():
+        with pytest.raises((TypeError, RuntimeError)):
+            torch.func.functionalize(call)(x)
+        with pytest.raises(TypeError, match="memory"):
+            call(TwoTensor(x, x))
+    x = torch.zeros(3, 4)
+    m = TwoTensor(x.bool(), x.bool())
+    r = TwoTensor(x, x)
+    for call in (lambda: nq.preference_loss(x, x, chosen_mask=m), lambda: nq.preference_loss(x, x, r, r),
+                 lambda: nq.policy_loss(x, x, x, mask=m), lambda: nq.policy_loss(x, x, x, ref_logprobs=r)):
+        with pytest.raises(TypeError, match="memory"):
+            call()
+    assert not stubbed
+    # no elements need no memory
+    nq.preference_loss(x[:, :0], x, chosen_mask=x[:, :0].bool())
+    nq.policy_loss(x[:, :0], x[:, :0], x[:, 0])
+    assert len(stubbed) == 2
