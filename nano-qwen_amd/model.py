@@ -181,6 +181,18 @@ class TransformerBlock(nn.Module):
         return hidden_states, None
 
 
+def _is_plain_product(head: nn.Module) -> bool:
+    """Whether calling ``head`` is x W^T and nothing else: no other class, no ``forward`` put on
+    the instance (as offloading and adapter code does), no compiled call, no hooks of its own
+    or of all modules."""
+    m = nn.modules.module
+    return (type(head) is nn.Linear and head.bias is None and "forward" not in head.__dict__
+            and getattr(head, "_compiled_call_impl", None) is None and not (
+                head._forward_hooks or head._forward_pre_hooks or head._backward_hooks or head._backward_pre_hooks
+                or m._global_forward_hooks or m._global_forward_pre_hooks or m._global_backward_hooks
+                or m._global_backward_pre_hooks))
+
+
 class Qwen3Model(nn.Module):
     """Embedding -> blocks -> RMSNorm -> LM head (transformer.py:78-156)."""
 
@@ -256,10 +268,7 @@ class Qwen3Model(nn.Module):
         hidden = self._trunk(input_ids, position_ids, attention_mask, None)[:, :-1]
         labels = (input_ids if labels is None else labels)[:, 1:]
         head = self.lm_head
-        # only the product that it is: what a caller put in its place or hooked to it runs
-        plain = type(head) is nn.Linear and head.bias is None and not (
-            head._forward_hooks or head._forward_pre_hooks or head._backward_hooks or head._backward_pre_hooks)
-        if (plain and hidden.dtype == head.weight.dtype == torch.bfloat16 and head.weight.shape[1] % 8 == 0
+        if (_is_plain_product(head) and hidden.dtype == head.weight.dtype == torch.bfloat16 and head.weight.shape[1] % 8 == 0
                 and type(head.weight) is nn.Parameter):
             return linear_logprobs(hidden, head.weight, labels, temperature=temperature)
         return token_logprobs(head(hidden), labels, temperature=temperature)

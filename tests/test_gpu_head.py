@@ -392,3 +392,25 @@ def test_preference_and_policy_steps_of_a_model():
     pol2, *_ = nq.policy_loss(lp2, lp.detach() + 0.05, adv, ref_logprobs=rlp, mask=mask, kl_coef=0.1, reduction="sequence")
     for a, b in zip(torch.autograd.grad(loss2 + pol2, params), got):
         assert torch.equal(a, b)
+
+
+def test_model_token_logprobs_runs_a_patched_head():
+    """What offloading and adapter code puts on the head's instance, and hooks of all modules, run."""
+    say("model token_logprobs of a patched head")
+    model = small_model(BF)
+    ids = torch.randint(0, 997, (2, 9), generator=torch.Generator().manual_seed(9)).to(DEV)
+    head = model.lm_head
+    inner = head.forward
+    with torch.no_grad():
+        plain = model.token_logprobs(ids)
+        head.forward = lambda x: inner(x) * 0.5
+        want = torch.log_softmax(model(ids)["logits"][:, :-1].double(), -1).gather(-1, ids[:, 1:, None])[..., 0]
+        within(model.token_logprobs(ids), want.cpu(), 1e-4, "patched forward")
+        del head.forward
+        handle = torch.nn.modules.module.register_module_forward_hook(
+            lambda mod, args, out: out * 0.5 if mod is head else None)
+        try:
+            within(model.token_logprobs(ids), want.cpu(), 1e-4, "global hook")
+        finally:
+            handle.remove()
+        assert torch.equal(model.token_logprobs(ids), plain)

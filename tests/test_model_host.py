@@ -86,3 +86,33 @@ def test_ragged_cache_rejects_bad_lengths(lens):
 def test_set_lengths_needs_storage():
     with pytest.raises(ValueError):
         KVCache().set_lengths(torch.tensor([1]))
+
+
+def test_token_logprobs_runs_what_its_head_is(monkeypatch):
+    """The LM head's weight is taken for the head only where calling the head is that product."""
+    import nano_qwen_amd.model as module
+    m = _model().to(torch.bfloat16)
+    cfg = ModelConfig(**MODEL)
+    monkeypatch.setattr(Qwen3Model, "_trunk",
+                        lambda self, ids, *args: torch.zeros(*ids.shape, cfg.hidden_size, dtype=torch.bfloat16))
+    monkeypatch.setattr(module, "linear_logprobs", lambda hidden, weight, labels, **kw: "weight")
+    monkeypatch.setattr(module, "token_logprobs", lambda logits, labels, **kw: logits)
+    ids = torch.tensor([[1, 2, 3]])
+    head = m.lm_head
+    assert m.token_logprobs(ids) == "weight"
+    head.forward = lambda x: "patched"
+    assert m.token_logprobs(ids) == "patched"
+    del head.forward
+    everywhere = torch.nn.modules.module
+    for register in (everywhere.register_module_forward_hook, everywhere.register_module_forward_pre_hook,
+                     everywhere.register_module_full_backward_hook, everywhere.register_module_full_backward_pre_hook,
+                     head.register_forward_hook, head.register_full_backward_hook):
+        handle = register(lambda *args: None)
+        try:
+            assert isinstance(m.token_logprobs(ids), torch.Tensor), register
+        finally:
+            handle.remove()
+    assert m.token_logprobs(ids) == "weight"
+    head.compile(backend="eager")
+    monkeypatch.setattr(head, "_compiled_call_impl", lambda x: "compiled")
+    assert m.token_logprobs(ids) == "compiled"
