@@ -584,6 +584,7 @@ int nq_preference_loss_bwd(const float* coef, const float* dloss, const uint8_t*
  * sequence's advantage (advantages[b * stride]; with advantages_per_token
  * advantages[b * stride + s]) and q = ref - lp:
  *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1)
+ * and where A is 0 the KL term alone, however large r.
  * loss: the mean over all kept tokens, or with mean_of_means the mean over the sequences
  * of each one's mean (0 for one with no kept token).  kl and clipped: the kept tokens'
  * mean of exp(q) - q - 1 (0 without ref_logprobs) and the share of them that the clip

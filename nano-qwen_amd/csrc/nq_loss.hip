@@ -404,8 +404,10 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, float
   const float r = expf((float)d);
   const bool hi = a > 0 && d > p.log_hi, lo = a < 0 && d < p.log_lo;
   o.cut = hi || lo;
-  o.term = hi ? -(p.bound_hi * a) : lo ? -(p.bound_lo * a) : -(r * a);
-  o.grad = o.cut ? 0.f : -(r * a);
+  // no advantage, no term, also where the ratio overflows (an infinity times zero); NaN stays
+  const float ra = a == 0.f && d == d ? 0.f : r * a;
+  o.term = hi ? -(p.bound_hi * a) : lo ? -(p.bound_lo * a) : -ra;
+  o.grad = o.cut ? 0.f : -ra;
   o.kl = 0.f;
   if (p.ref) {
     const float q = (float)((double)ref - (double)lp);

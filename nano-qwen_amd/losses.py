@@ -457,7 +457,7 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
 
       -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1)
 
-    ``clip_high`` defaults to ``clip_low``.  ``reduction``: "token", the mean over all kept
+    and where A is 0 the KL term alone, however large r.  ``clip_high`` defaults to ``clip_low``.  ``reduction``: "token", the mean over all kept
     tokens, or "sequence", the mean over the B sequences of each one's mean (0 for one
     without kept tokens).  Returns the loss, a scalar with a gradient for logprobs alone;
     and, without gradient, the kept tokens' mean of exp(q) - q - 1 (0 without a reference)

@@ -653,3 +653,34 @@ def test_losses_traced_and_compiled():
     for kw in (dict(mask=TwoTensor(m, m)), dict(ref_logprobs=TwoTensor(lp, lp))):
         with pytest.raises(TypeError, match="memory"):
             nq.policy_loss(lp, lp, lp, **kw)
+
+
+@pytest.mark.parametrize("B,S", [(2, 3), (20, 3)])
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_policy_loss_zero_advantage(B, S, reduction):
+    """A token without an advantage adds its KL term alone, also where its ratio overflows; NaN stays NaN."""
+    say(f"policy_loss zero advantage {B} {S} {reduction}")
+    lp = -randn(B, S, seed=62).abs()
+    old = lp + 0.1 * randn(B, S, seed=63)
+    old[1, 1], old[1, 2] = -300.0, -float("inf")
+    ref = lp + 0.3 * randn(B, S, seed=64)
+    adv = randn(B, seed=65)
+    adv[1] = 0
+    for c in (0.0, 0.2):
+        # the same tokens with ratios that do not overflow: the row's policy term is 0 either way
+        plain = old.clone()
+        plain[1] = lp[1]
+        want = policy_reference(lp, plain, adv, ref, None, 0.2, 0.28, c, reduction)
+        l = lp.to(DEV).requires_grad_()
+        loss, _, clipped = nq.policy_loss(l, old.to(DEV), adv.to(DEV), ref_logprobs=ref.to(DEV), clip_high=0.28, kl_coef=c,
+                                          reduction=reduction)
+        (g,) = torch.autograd.grad(loss, l)
+        within(loss, want[0], float(want[4].sum()) + U * want[0].abs() + 1e-14, "loss")
+        within(clipped, want[2], U * want[2], "clipped")
+        within(g, want[3], want[4] + 4 * U * want[3].abs(), "gradient")
+        assert c or not g[1].any()
+    old[1, 0] = float("nan")
+    l = lp.to(DEV).requires_grad_()
+    loss, *_ = nq.policy_loss(l, old.to(DEV), adv.to(DEV), reduction=reduction)
+    (g,) = torch.autograd.grad(loss, l)
+    assert torch.isnan(loss) and torch.isnan(g).sum() == 1 and torch.isnan(g[1, 0])
