@@ -290,7 +290,7 @@ __device__ __forceinline__ double pref_pair(const PrefParams& p, int b, int t, d
     slope = p.beta * (p.smoothing - 1 / (1 + exp(h)));
   } else if (p.kind == NQ_PREF_HINGE) {
     loss = h >= 1 ? 0 : 1 - h;  // NaN stays
-    slope = h >= 1 ? 0 : -p.beta;
+    slope = h >= 1 ? 0 : h < 1 ? -p.beta : h;
   } else {
     const double e = diff - 0.5 / p.beta;
     loss = e * e;

@@ -684,3 +684,17 @@ def test_policy_loss_zero_advantage(B, S, reduction):
     loss, *_ = nq.policy_loss(l, old.to(DEV), adv.to(DEV), reduction=reduction)
     (g,) = torch.autograd.grad(loss, l)
     assert torch.isnan(loss) and torch.isnan(g).sum() == 1 and torch.isnan(g[1, 0])
+
+
+@pytest.mark.parametrize("B", [3, 20])
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "ipo"])
+def test_preference_loss_of_nan(B, kind):
+    """A pair whose margin is NaN has NaN gradients, as its loss; the other pairs' are their own."""
+    say(f"preference_loss NaN {B} {kind}")
+    c, r = randn(B, 5, seed=66), randn(B, 5, seed=67)
+    c[1, 2] = float("nan")
+    leaves = [t.to(DEV).requires_grad_() for t in (c, r)]
+    loss, wc, wr = nq.preference_loss(*leaves, kind=kind)
+    assert torch.isnan(loss) and torch.isnan(wc).sum() == 1 and torch.isnan(wc[1]) and torch.isfinite(wr).all()
+    for g in torch.autograd.grad(loss, leaves):
+        assert torch.isnan(g[1]).all() and torch.isnan(g).sum() == 5
