@@ -284,9 +284,10 @@ __device__ __forceinline__ double pref_pair(const PrefParams& p, int b, int t, d
   const double diff = d[0] - d[1], h = p.beta * diff;
   double loss, slope;
   if (p.kind == NQ_PREF_SIGMOID) {
-    // -log s(h) without overflow
-    const double soft = log1p(exp(-fabs(h))) + (h < 0 ? -h : 0);
-    loss = p.smoothing != 0 ? soft + p.smoothing * h : soft;
+    // -log s(h) is log(1 + e^-|h|), which does not overflow, and -h where h < 0; -log s(-h) the
+    // same and h where h > 0: each side weighed by itself, as infinities of both would cancel
+    const double away = h < 0 ? -(1 - p.smoothing) * h : p.smoothing != 0 ? p.smoothing * h : 0;
+    loss = log1p(exp(-fabs(h))) + away;
     slope = p.beta * (p.smoothing - 1 / (1 + exp(h)));
   } else if (p.kind == NQ_PREF_HINGE) {
     loss = h >= 1 ? 0 : 1 - h;  // NaN stays

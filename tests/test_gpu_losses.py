@@ -698,3 +698,24 @@ def test_preference_loss_of_nan(B, kind):
     assert torch.isnan(loss) and torch.isnan(wc).sum() == 1 and torch.isnan(wc[1]) and torch.isfinite(wr).all()
     for g in torch.autograd.grad(loss, leaves):
         assert torch.isnan(g[1]).all() and torch.isnan(g).sum() == 5
+
+
+@pytest.mark.parametrize("B", [2, 20])
+@pytest.mark.parametrize("e", [0.0, 0.25])
+def test_preference_loss_of_infinite_margins(B, e):
+    """A label that the policy rules out: the margin is infinite, and so is the loss that weighs it."""
+    say(f"preference_loss infinite margins {B} {e}")
+    inf = float("inf")
+    for side, want in ((0, inf), (1, inf if e else 0.0)):
+        lps = [torch.zeros(B, 4), torch.zeros(B, 4)]
+        lps[side][1, 3] = -inf
+        leaves = [t.to(DEV).requires_grad_() for t in lps]
+        loss, *rewards = nq.preference_loss(*leaves, beta=0.5, label_smoothing=e)
+        # the other pairs' margins are 0: log 2 each
+        within(loss, torch.tensor(want + (B - 1) / B * math.log(2), dtype=torch.float64), 4 * U, f"side {side}")
+        assert float(rewards[side][1]) == -inf and torch.isfinite(rewards[1 - side]).all()
+        # beta (e - s(-h)): s(-h) is 1 at -inf, 0 at inf, 1/2 at 0
+        slope = torch.full((B,), 0.5 * (e - 0.5), dtype=torch.float64)
+        slope[1] = 0.5 * (e - (1 if side == 0 else 0))
+        for g, sign in zip(torch.autograd.grad(loss, leaves), (1, -1)):
+            within(g, (sign * slope / B)[:, None].expand(B, 4), 2 * U * slope.abs().max() / B, f"side {side} gradient")
