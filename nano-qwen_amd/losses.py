@@ -247,11 +247,11 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     """``token_logprobs(hidden @ weight.T, labels)`` without the logits, fp32 and shaped like ``labels``.
 
     hidden: (..., H) bf16 hidden states, rows at any strides; weight: (V, H) bf16, an LM
-    head's; H a multiple of 8.  Logits are held in fp32 and never stored; the backward forms
-    their gradient in bf16, a range of the vocabulary at a time (at most 1 GiB), and gives
-    hidden and weight gradients summed in fp32.  Rows whose label is ``ignore_index`` take no
-    part in the products.  Labels outside [0, V) give NaN, and so do their row's and the
-    weight's gradients.
+    head's; H a multiple of 8, at most 2^20; at most 2^24 rows and entries.  Logits are held
+    in fp32 and never stored; the backward forms their gradient in bf16, a range of the
+    vocabulary at a time (at most 1 GiB), and gives hidden and weight gradients summed in
+    fp32.  Rows whose label is ``ignore_index`` take no part in the products.  Labels outside
+    [0, V) give NaN, and so do their row's and the weight's gradients.
 
     A call with a gradient keeps the softmax's numerators for it, in bf16, 2 bytes for each
     entry of each row, where that is faster (widths from 256, more than 64 rows) and at most
@@ -268,8 +268,9 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     if hidden.dim() == 0 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"hidden {tuple(hidden.shape)} must be (..., H) and weight {tuple(weight.shape)} (V, H)")
     V, H = weight.shape
-    if V == 0 or H == 0 or H % 8:
-        raise ValueError(f"the kernels take at least one entry and widths that are multiples of 8, got {V} and {H}")
+    if V == 0 or H == 0 or H % 8 or H > _HEAD_WIDEST:
+        raise ValueError("the kernels take at least one entry and widths that are multiples of 8, up to 2^20, "
+                         f"got {V} and {H}")
     labels = _check_labels(labels, hidden.shape[:-1])
     temperature = _check_temperature(temperature)
     if labels.numel() == 0:
@@ -283,6 +284,8 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
 
 
 _HEAD_MOST = 1 << 24
+_HEAD_WIDEST = 1 << 20
+_MOST_SEQUENCES = 2 ** 31 - 1  # the C entries' int, to which ctypes cuts a larger number without a word
 
 
 # ---------------------------------------------------------------------------
@@ -395,6 +398,8 @@ def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: Op
     if chosen.shape[0] != rejected.shape[0] or chosen.shape[0] == 0:
         raise ValueError(f"chosen and rejected must hold the same number of sequences, at least one, "
                          f"got {chosen.shape[0]} and {rejected.shape[0]}")
+    if chosen.shape[0] > _MOST_SEQUENCES:
+        raise ValueError(f"at most 2^31 - 1 sequences in one call, got {chosen.shape[0]}")
     sc, sr = chosen.shape, rejected.shape
     chosen, rejected = _token_rows(chosen, "chosen", sc), _token_rows(rejected, "rejected", sr)
     rewards = chosen.new_empty(sc[0]), chosen.new_empty(sc[0])
@@ -466,6 +471,8 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
     _check_devices(logprobs, old_logprobs, advantages, ref_logprobs, mask)
     if logprobs.dim() != 2 or logprobs.shape[0] == 0:
         raise ValueError(f"logprobs must be (B, S) with at least one sequence, got shape {tuple(logprobs.shape)}")
+    if logprobs.shape[0] > _MOST_SEQUENCES:
+        raise ValueError(f"at most 2^31 - 1 sequences in one call, got {logprobs.shape[0]}")
     clip_high = clip_low if clip_high is None else clip_high
     if not 0 <= clip_low <= 1 or not (clip_high >= 0 and math.isfinite(clip_high)) or not math.isfinite(kl_coef):
         raise ValueError("clip_low must lie in [0, 1], clip_high be at least 0 and all finite, "

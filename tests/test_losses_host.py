@@ -241,3 +241,22 @@ def test_tensors_without_memory_are_refused(stubbed):
     nq.preference_loss(x[:, :0], x, chosen_mask=x[:, :0].bool())
     nq.policy_loss(x[:, :0], x[:, :0], x[:, 0])
     assert len(stubbed) == 2
+
+
+@pytest.mark.parametrize("over", [2 ** 31, 2 ** 32 + 4])
+def test_sizes_past_an_int_are_refused(stubbed, over):
+    """ctypes would cut them to 32 bits: 2^32 + 4 sequences to the first 4, a width of 2^32 + 8 to 8."""
+    many = torch.zeros(1).expand(over)
+    with pytest.raises(ValueError, match="sequences"):
+        nq.preference_loss(many, many)
+    with pytest.raises(ValueError, match="sequences"):
+        nq.policy_loss(many[:, None], many[:, None], many)
+    one = torch.zeros(1, dtype=torch.bfloat16)
+    for H in (over + 8 - over % 8, (1 << 20) + 8):
+        with pytest.raises(ValueError, match="2.20"):
+            nq.linear_logprobs(one.expand(3, H), one.expand(5, H), torch.zeros(3, dtype=torch.long))
+    with pytest.raises(ValueError, match="2.24"):
+        nq.linear_logprobs(one.expand(3, 8), one.expand(over, 8), torch.zeros(3, dtype=torch.long))
+    with pytest.raises(ValueError, match="2.31"):
+        nq.token_logprobs(torch.zeros(1).expand(3, over), torch.zeros(3, dtype=torch.long))
+    assert not stubbed
