@@ -29,6 +29,7 @@ struct TokenParams {
   floatx2* stats;  // per row (m, l)
   floatx2* part;   // (rows, splits) partial (m, l)
   int64_t rows, S;
+  int64_t row0;    // this launch's first row
   int V, splits;
   int64_t ignore;
   float c, inv_t;
@@ -61,12 +62,13 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(TokenParams p) {
   __shared__ RowStat red[4];
   const int tid = threadIdx.x % TEAM;
   int64_t row = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
-  if (TEAM < 256 && row >= p.rows) return;
   int slice = 0;
   if (SPLIT) {
     slice = (int)(row % p.splits);
     row /= p.splits;
   }
+  row += p.row0;
+  if (TEAM < 256 && row >= p.rows) return;
   const int64_t y = p.labels[row];
   if (y == p.ignore) {
     if (tid == 0 && slice == 0 && !SPLIT) {
@@ -171,8 +173,9 @@ template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(TokenBwdParams q) {
   const TokenParams& p = q.t;
   const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x / q.slices;
-  const int slice = (int)(blockIdx.x - row * q.slices);
+  const unsigned at = blockIdx.x / q.slices;
+  const int slice = (int)(blockIdx.x - at * q.slices);
+  const int64_t row = p.row0 + at;
   const int64_t y = p.labels[row];
   const int nv = p.V / 8, j0 = slice * TOK_SLICE + tid;
   T* dx = reinterpret_cast<T*>(q.dx) + row * p.V;
@@ -256,6 +259,7 @@ struct PrefParams {
   double* pair_loss;   // (B)
   const float* gout;   // backward: d / d loss
   int64_t blocks0;     // backward: workgroups of side 0
+  int64_t first;       // this launch's first pair, or workgroup of the backward
 };
 
 template <int TEAM>
@@ -310,8 +314,9 @@ __device__ __forceinline__ double pref_pair(const PrefParams& p, int b, int t, d
 template <int TEAM>
 __global__ __launch_bounds__(TEAM) void pref_pairs_kernel(PrefParams p) {
   __shared__ double lds[TEAM / 64];
-  const double loss = pref_pair<TEAM>(p, blockIdx.x, threadIdx.x, lds);
-  if (threadIdx.x == 0) p.pair_loss[blockIdx.x] = loss;
+  const int b = (int)(p.first + blockIdx.x);
+  const double loss = pref_pair<TEAM>(p, b, threadIdx.x, lds);
+  if (threadIdx.x == 0) p.pair_loss[b] = loss;
 }
 
 __global__ __launch_bounds__(256) void pref_mean_kernel(PrefParams p) {
@@ -339,10 +344,11 @@ __global__ __launch_bounds__(1024) void pref_one_kernel(PrefParams p) {
 
 // d loss / d lp: the pair's coefficient in kept tokens.  A thread per 4 tokens.
 __global__ __launch_bounds__(256) void pref_bwd_kernel(PrefParams p) {
-  const bool second = blockIdx.x >= p.blocks0;
+  const int64_t block = p.first + blockIdx.x;
+  const bool second = block >= p.blocks0;
   const PrefSide& s = p.side[second];
   const int64_t n = (int64_t)p.B * s.S;
-  const int64_t i0 = ((int64_t)blockIdx.x - (second ? p.blocks0 : 0)) * 1024 + threadIdx.x;
+  const int64_t i0 = (block - (second ? p.blocks0 : 0)) * 1024 + threadIdx.x;
   const float gout = *p.gout;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -369,6 +375,7 @@ struct PolicyParams {
   int64_t lp_rs, old_rs, ref_rs, adv_rs, mask_rs;
   int adv_per_token, B, mean_of_means, segs;
   int64_t S, seg_len;
+  int64_t first;      // this launch's first sequence, or workgroup of the backward
   float bound_hi, bound_lo, kl_coef;
   double log_hi, log_lo;
   float *loss, *kl, *clipped;
@@ -455,11 +462,11 @@ __device__ __forceinline__ PolicySums policy_sums(const PolicyParams& p, int b, 
 // Workgroup = a segment of a sequence.
 __global__ __launch_bounds__(256) void policy_sums_kernel(PolicyParams p) {
   __shared__ double lds[4];
-  const int b = blockIdx.x / p.segs, seg = blockIdx.x - b * p.segs;
+  const int at = blockIdx.x / p.segs, seg = blockIdx.x - at * p.segs, b = (int)(p.first + at);
   const int64_t k0 = seg * p.seg_len, k1 = k0 + p.seg_len < p.S ? k0 + p.seg_len : p.S;
   const PolicySums s = policy_sums<256>(p, b, k0, k1, threadIdx.x, lds);
   if (threadIdx.x == 0) {
-    double* o = p.part + (int64_t)blockIdx.x * 4;
+    double* o = p.part + ((int64_t)b * p.segs + seg) * 4;
     o[0] = s.term, o[1] = s.kl, o[2] = s.kept, o[3] = s.cut;
   }
 }
@@ -521,7 +528,7 @@ __global__ __launch_bounds__(1024) void policy_one_kernel(PolicyParams p) {
 
 __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyParams p) {
   const int64_t n = (int64_t)p.B * p.S;
-  const int64_t i0 = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+  const int64_t i0 = (p.first + blockIdx.x) * 1024 + threadIdx.x;
   const float gout = *p.gout;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -543,6 +550,15 @@ __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyParams p) {
 using namespace nq;
 
 static bool aligned_to(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// A launch has fewer than 2^32 threads: n groups of `each` workgroups of `threads`, in as many launches
+// as that takes, launch(first group, workgroups).
+template <typename F>
+static void in_launches(int64_t n, int64_t each, int threads, F launch) {
+  const int64_t most = (int64_t)UINT32_MAX / threads / each;
+  for (int64_t first = 0; first < n; first += most)
+    launch(first, dim3((unsigned)((n - first < most ? n - first : most) * each)));
+}
 
 // ------------------------------------------------------------------ token log-probabilities
 
@@ -579,15 +595,22 @@ static int token_check(const void* logits, const int64_t* labels, const void* st
 }
 
 template <typename T, bool STREAM>
-static void launch_tokens(const TokenParams& p, hipStream_t st) {
-  const dim3 block(256), waves((unsigned)((p.rows + 3) / 4)), grid((unsigned)(p.rows * p.splits));
+static void launch_tokens(TokenParams p, hipStream_t st) {
+  const dim3 block(256);
   if (p.splits > 1) {
+    const dim3 waves((unsigned)((p.rows + 3) / 4)), grid((unsigned)(p.rows * p.splits));
     hipLaunchKernelGGL((token_logprobs_kernel<T, 256, true, STREAM>), grid, block, 0, st, p);
     hipLaunchKernelGGL((token_join_kernel<T>), waves, block, 0, st, p);
   } else if (p.V / 8 <= (p.rows >= 2048 ? 1024 : 256)) {
-    hipLaunchKernelGGL((token_logprobs_kernel<T, 64, false, STREAM>), waves, block, 0, st, p);
+    in_launches((p.rows + 3) / 4, 1, 256, [&](int64_t first, dim3 grid) {
+      p.row0 = first * 4;
+      hipLaunchKernelGGL((token_logprobs_kernel<T, 64, false, STREAM>), grid, block, 0, st, p);
+    });
   } else {
-    hipLaunchKernelGGL((token_logprobs_kernel<T, 256, false, STREAM>), grid, block, 0, st, p);
+    in_launches(p.rows, 1, 256, [&](int64_t first, dim3 grid) {
+      p.row0 = first;
+      hipLaunchKernelGGL((token_logprobs_kernel<T, 256, false, STREAM>), grid, block, 0, st, p);
+    });
   }
 }
 
@@ -605,7 +628,7 @@ extern "C" int nq_token_logprobs(const void* logits, int64_t batch_stride, int64
   const int splits = token_splits(rows, V);
   if (rows * splits > INT32_MAX) return nq_fail(NQ_ERR_UNSUPPORTED, "too many rows for one launch");
   TokenParams p{logits, batch_stride, row_stride, labels, logprobs, reinterpret_cast<floatx2*>(stats),
-                reinterpret_cast<floatx2*>(workspace), rows, S, V, splits, ignore_index, inv * kLog2e, inv};
+                reinterpret_cast<floatx2*>(workspace), rows, S, 0, V, splits, ignore_index, inv * kLog2e, inv};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool b16 = dtype == NQ_DTYPE_BF16;
   const bool past = rows * V * (b16 ? 2 : 4) > ((int64_t)256 << 20);
@@ -627,13 +650,15 @@ extern "C" int nq_token_logprobs_bwd(const void* logits, int64_t batch_stride, i
   const int slices = (V / 8 + TOK_SLICE - 1) / TOK_SLICE > 0 ? (V / 8 + TOK_SLICE - 1) / TOK_SLICE : 1;
   if (rows * slices > INT32_MAX) return nq_fail(NQ_ERR_UNSUPPORTED, "too many rows for one launch");
   TokenBwdParams q{{logits, batch_stride, row_stride, labels, nullptr,
-                    reinterpret_cast<floatx2*>(const_cast<float*>(stats)), nullptr, rows, S, V, 1, ignore_index,
+                    reinterpret_cast<floatx2*>(const_cast<float*>(stats)), nullptr, rows, S, 0, V, 1, ignore_index,
                     inv * kLog2e, inv},
                    dlogprobs, dlogits, slices};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(rows * slices));
-  if (dtype == NQ_DTYPE_BF16) hipLaunchKernelGGL((token_logprobs_bwd_kernel<bf16>), grid, dim3(256), 0, st, q);
-  else hipLaunchKernelGGL((token_logprobs_bwd_kernel<float>), grid, dim3(256), 0, st, q);
+  in_launches(rows, slices, 256, [&](int64_t first, dim3 grid) {
+    q.t.row0 = first;
+    if (dtype == NQ_DTYPE_BF16) hipLaunchKernelGGL((token_logprobs_bwd_kernel<bf16>), grid, dim3(256), 0, st, q);
+    else hipLaunchKernelGGL((token_logprobs_bwd_kernel<float>), grid, dim3(256), 0, st, q);
+  });
   return nq_check_launch(hipGetLastError());
 }
 
@@ -678,14 +703,18 @@ extern "C" int nq_preference_loss(const float* chosen, int64_t chosen_stride, co
                  chosen_reward, coef, nullptr},
                 {rejected, ref_rejected, rejected_mask, rejected_stride, ref_rejected_stride, rejected_mask_stride, Sr,
                  rejected_reward, coef + B, nullptr}},
-               B, kind, average != 0, beta, label_smoothing, loss, reinterpret_cast<double*>(workspace), nullptr, 0};
+               B, kind, average != 0, beta, label_smoothing, loss, reinterpret_cast<double*>(workspace), nullptr, 0, 0};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (one) {
     hipLaunchKernelGGL(pref_one_kernel, dim3(1), dim3(1024), 0, st, p);
   } else {
     // 256 pairs of 4096 tokens: 10.5 us with 1024 threads a pair for 15.5 with 256
-    if (Sc > ONE_TOKENS || Sr > ONE_TOKENS) hipLaunchKernelGGL((pref_pairs_kernel<1024>), dim3((unsigned)B), dim3(1024), 0, st, p);
-    else hipLaunchKernelGGL((pref_pairs_kernel<256>), dim3((unsigned)B), dim3(256), 0, st, p);
+    const bool longer = Sc > ONE_TOKENS || Sr > ONE_TOKENS;
+    in_launches(B, 1, longer ? 1024 : 256, [&](int64_t first, dim3 grid) {
+      p.first = first;
+      if (longer) hipLaunchKernelGGL((pref_pairs_kernel<1024>), grid, dim3(1024), 0, st, p);
+      else hipLaunchKernelGGL((pref_pairs_kernel<256>), grid, dim3(256), 0, st, p);
+    });
     hipLaunchKernelGGL(pref_mean_kernel, dim3(1), dim3(256), 0, st, p);
   }
   return nq_check_launch(hipGetLastError());
@@ -716,8 +745,10 @@ extern "C" int nq_preference_loss_bwd(const float* coef, const float* dloss, con
   p.blocks0 = blocks[0];
   if (blocks[0] + blocks[1] == 0) return NQ_OK;
   if (blocks[0] + blocks[1] > INT32_MAX) return nq_fail(NQ_ERR_UNSUPPORTED, "too many tokens for one launch");
-  hipLaunchKernelGGL(pref_bwd_kernel, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0,
-                     reinterpret_cast<hipStream_t>(stream), p);
+  in_launches(blocks[0] + blocks[1], 1, 256, [&](int64_t first, dim3 grid) {
+    p.first = first;
+    hipLaunchKernelGGL(pref_bwd_kernel, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
+  });
   return nq_check_launch(hipGetLastError());
 }
 
@@ -781,7 +812,10 @@ extern "C" int nq_policy_loss(const float* logprobs, int64_t logprobs_stride, co
     return nq_fail(NQ_ERR_WORKSPACE, "workspace too small or not 8-byte aligned: %lld bytes, need %lld",
                    (long long)workspace_bytes, (long long)nq_policy_loss_workspace_bytes(B, S));
   if ((int64_t)B * p.segs > INT32_MAX) return nq_fail(NQ_ERR_UNSUPPORTED, "too many sequences for one launch");
-  hipLaunchKernelGGL(policy_sums_kernel, dim3((unsigned)(B * p.segs)), dim3(256), 0, st, p);
+  in_launches(B, p.segs, 256, [&](int64_t first, dim3 grid) {
+    p.first = first;
+    hipLaunchKernelGGL(policy_sums_kernel, grid, dim3(256), 0, st, p);
+  });
   hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(256), 0, st, p);
   return nq_check_launch(hipGetLastError());
 }
@@ -803,6 +837,9 @@ extern "C" int nq_policy_loss_bwd(const float* logprobs, int64_t logprobs_stride
   p.gout = dloss, p.grad = dlogprobs;
   const int64_t blocks = ((int64_t)B * S + 1023) / 1024;
   if (blocks > INT32_MAX) return nq_fail(NQ_ERR_UNSUPPORTED, "too many tokens for one launch");
-  hipLaunchKernelGGL(policy_bwd_kernel, dim3((unsigned)blocks), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
+  in_launches(blocks, 1, 256, [&](int64_t first, dim3 grid) {
+    p.first = first;
+    hipLaunchKernelGGL(policy_bwd_kernel, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
+  });
   return nq_check_launch(hipGetLastError());
 }

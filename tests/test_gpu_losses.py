@@ -719,3 +719,57 @@ def test_preference_loss_of_infinite_margins(B, e):
         slope[1] = 0.5 * (e - (1 if side == 0 else 0))
         for g, sign in zip(torch.autograd.grad(loss, leaves), (1, -1)):
             within(g, (sign * slope / B)[:, None].expand(B, 4), 2 * U * slope.abs().max() / B, f"side {side} gradient")
+
+
+def test_token_logprobs_more_rows_than_one_launch():
+    """A launch has fewer than 2^32 threads: 2^26 rows of a wave, 2^24 workgroups of the backward."""
+    rows, V = 2 ** 26 + 5, 3
+    say(f"token_logprobs {rows} rows")
+    g = torch.Generator(device=DEV).manual_seed(68)
+    x = torch.randn(rows, V, generator=g, device=DEV, dtype=BF).requires_grad_()
+    labels = torch.randint(0, V, (rows,), generator=g, device=DEV)
+    dy = torch.randn(rows, generator=g, device=DEV)
+    lp = nq.token_logprobs(x, labels)
+    (dx,) = torch.autograd.grad(lp, x, dy)
+    # the first and last rows, those around the launches' ends, and a sample of the rest
+    at = torch.cat([torch.arange(0, rows, 8191), torch.arange(2 ** 24 - 9, 2 ** 24 + 9), torch.arange(2 ** 26 - 99, rows)]).to(DEV)
+    xs = x.detach()[at].cpu()
+    want, dwant, tol, dtol = token_reference(xs, labels[at].cpu(), dy[at].cpu(), 1.0)
+    within(lp[at], want, tol, "logprobs")
+    within(dx[at], dwant, dtol + half_step(BF) * dwant.abs(), "dlogits")
+    # every row was written, once
+    assert bool((lp < 0).all()) and float(dx.sum(-1, dtype=torch.float32).abs().max()) < 0.1
+
+
+def test_losses_of_more_sequences_than_one_launch():
+    """2^24 workgroups of 256 threads, 2^22 of 1024."""
+    g = torch.Generator(device=DEV).manual_seed(69)
+    B = 2 ** 24 + 3
+    say(f"preference_loss and policy_loss {B} sequences")
+    c, r = (torch.randn(B, generator=g, device=DEV) for _ in range(2))
+    leaves = [t.clone().requires_grad_() for t in (c, r)]
+    loss, wc, wr = nq.preference_loss(*leaves, beta=0.5)
+    h = 0.5 * (c.double() - r.double())
+    # 1 / (1 + e^h) / B: a rounding of the slope, of the coefficient and of the mean
+    assert abs(float(loss.detach()) - float(torch.nn.functional.softplus(-h).mean())) < 4 * U
+    slope = -0.5 / (1 + torch.exp(h)) / B
+    for got, sign in zip(torch.autograd.grad(loss, leaves), (1, -1)):
+        assert float((got.double() / (sign * slope) - 1).abs().max()) < 4 * U
+    assert float((wc.double() - 0.5 * c).abs().max()) == 0 and float((wr.double() - 0.5 * r).abs().max()) == 0
+    l = (0.1 * c)[:, None].requires_grad_()
+    loss, _, clipped = nq.policy_loss(l, torch.zeros_like(l), r, reduction="sequence")
+    d, a = l.detach()[:, 0].double(), r.double()
+    hi, lo = (a > 0) & (d > math.log1p(0.2)), (a < 0) & (d < math.log1p(-0.2))
+    term = -torch.where(hi, 1.2 * a, torch.where(lo, 0.8 * a, d.exp() * a))
+    # each term in fp32: |d| < 1, the exponential and two products under 4 roundings of |term|
+    assert abs(float(loss.detach()) - float(term.mean())) < 8 * U * float(term.abs().mean())
+    assert abs(float(clipped) - float((hi | lo).double().mean())) < 2 * U
+    grad = torch.where(hi | lo, 0.0, -d.exp() * a) / B
+    (got,) = torch.autograd.grad(loss, l)
+    assert bool(((got[:, 0].double() - grad).abs() <= 8 * U * grad.abs()).all())
+    B = 2 ** 22 + 3
+    with torch.no_grad():
+        loss, wc, _ = nq.preference_loss(c[:B, None].expand(B, 1025), r[:B, None].expand(B, 1025), average=True, beta=0.5)
+    # averages of 1025 equal values in 64 bits
+    assert abs(float(loss) - float(torch.nn.functional.softplus(-h[:B]).mean())) < 4 * U
+    assert float((wc.double() - 0.5 * c[:B]).abs().max()) <= U * float(c[:B].abs().max())
