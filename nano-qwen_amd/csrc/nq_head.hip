@@ -1054,6 +1054,14 @@ extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, 
   if (!dhidden && !dweight) return NQ_OK;
   const int64_t rows = B * S;
   const HeadSpace s = head_space(rows, V, H, true);
+  const bool few = head_few(rows);
+  const int bm = few ? Few::BM : Wide::BM, bn = few ? Few::BN : Wide::BN, nh = (H + bm - 1) / bm;
+  const int64_t nn = (rows + bn - 1) / bn, nw = (H + Wide::BM - 1) / Wide::BM;
+  if (((int64_t)s.vc / bm + 1) * nn > INT32_MAX / 2 || nn * nh * HD_CUS > INT32_MAX / 2 ||
+      ((int64_t)s.vc / Wide::BN + 1) * nw > INT32_MAX / 2)
+    return nq_fail(NQ_ERR_UNSUPPORTED, "too many tiles for one launch");
+  if (dhidden && rows * (H / 8) > UINT32_MAX - 255)  // a launch has fewer than 2^32 threads
+    return nq_fail(NQ_ERR_UNSUPPORTED, "too many elements of hidden states for one launch");
   char* ws = reinterpret_cast<char*>(workspace);
   const float inv = 1.f / temperature;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -1072,12 +1080,6 @@ extern "C" int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, 
   p.dz = reinterpret_cast<bf16*>(ws + s.dz), p.ldz = s.ldz;
   if (kept) head_kept_at(const_cast<void*>(kept), &p);
   p.dw = reinterpret_cast<bf16*>(dweight), p.dh = reinterpret_cast<float*>(ws + s.dh), p.vmax = s.vc;
-  const bool few = head_few(rows);
-  const int bm = few ? Few::BM : Wide::BM, bn = few ? Few::BN : Wide::BN, nh = (H + bm - 1) / bm;
-  const int64_t nn = (rows + bn - 1) / bn, nw = (H + Wide::BM - 1) / Wide::BM;
-  if (((int64_t)s.vc / bm + 1) * nn > INT32_MAX / 2 || nn * nh * HD_CUS > INT32_MAX / 2 ||
-      ((int64_t)s.vc / Wide::BN + 1) * nw > INT32_MAX / 2)
-    return nq_fail(NQ_ERR_UNSUPPORTED, "too many tiles for one launch");
   for (int v0 = 0; v0 < V; v0 += s.vc) {
     p.v0 = v0, p.vc = V - v0 < s.vc ? V - v0 : s.vc, p.add = v0 > 0;
     const int64_t logits = (p.vc + bm - 1) / bm * nn;

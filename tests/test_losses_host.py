@@ -260,3 +260,11 @@ def test_sizes_past_an_int_are_refused(stubbed, over):
     with pytest.raises(ValueError, match="2.31"):
         nq.token_logprobs(torch.zeros(1).expand(3, over), torch.zeros(3, dtype=torch.long))
     assert not stubbed
+
+
+def test_linear_logprobs_backward_refuses_more_hidden_states_than_a_launch_writes():
+    """A thread writes 8 of the gradient's elements, and a launch of 2^32 threads would come out short."""
+    fn = "nq_linear_logprobs_bwd"
+    refused(fn, UNS, "hidden states", *head_bwd(S=1 << 24, H=2048, rs=2048))
+    refused(fn, UNS, "hidden states", *head_bwd(S=(1 << 23) + 1, H=4096, rs=4096))
+    refused(fn, UNS, "tiles", *head_bwd(S=1 << 24, H=1 << 20, rs=1 << 20))
