@@ -258,19 +258,22 @@ class Qwen3Model(nn.Module):
 
     def token_logprobs(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                        position_ids: Optional[torch.Tensor] = None,
-                       attention_mask: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
+                       attention_mask: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                       recompute: bool = False) -> torch.Tensor:
         """The log-probability of each token given those before it, (B, S - 1) fp32.
 
         labels (B, S), ``input_ids`` by default, are shifted as in ``forward``: entry [b, s]
         is that of ``labels[b, s + 1]``, 0 where the label is -100.  What the preference and
-        policy losses take, without the logits: a bf16 LM head goes through
-        ``losses.linear_logprobs``, another through its logits."""
+        policy losses take.  A bf16 LM head goes through ``losses.linear_logprobs``, which holds
+        no logits, but with a gradient keeps 2 bytes for each vocabulary entry of each token
+        until the backward, up to 4 GiB a call; with ``recompute`` it keeps none of them.
+        Another head goes through its logits."""
         hidden = self._trunk(input_ids, position_ids, attention_mask, None)[:, :-1]
         labels = (input_ids if labels is None else labels)[:, 1:]
         head = self.lm_head
         if (_is_plain_product(head) and hidden.dtype == head.weight.dtype == torch.bfloat16 and head.weight.shape[1] % 8 == 0
                 and type(head.weight) is nn.Parameter):
-            return linear_logprobs(hidden, head.weight, labels, temperature=temperature)
+            return linear_logprobs(hidden, head.weight, labels, temperature=temperature, recompute=recompute)
         return token_logprobs(head(hidden), labels, temperature=temperature)
 
     @torch.no_grad()

@@ -414,3 +414,29 @@ def test_model_token_logprobs_runs_a_patched_head():
         finally:
             handle.remove()
         assert torch.equal(model.token_logprobs(ids), plain)
+
+
+def test_model_token_logprobs_memory():
+    """What a call holds until its backward: two bytes a token and vocabulary entry, none with recompute."""
+    say("model token_logprobs memory")
+    cfg = ModelConfig(vocab_size=20000, hidden_size=256, intermediate_size=256, num_hidden_layers=1, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=64)
+    torch.manual_seed(3)
+    model = Qwen3Model(cfg).to(DEV, BF)
+    ids = torch.randint(0, 20000, (2, 501), generator=torch.Generator().manual_seed(10)).to(DEV)
+    held, grads, outs = [], [], []
+    for recompute in (False, True):
+        for _ in range(2):  # the second without the first call's lasting allocations
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            lp = model.token_logprobs(ids, recompute=recompute)
+            held.append(torch.cuda.memory_allocated() - before)
+            g = torch.autograd.grad(lp.sum(), model.lm_head.weight)[0]
+            outs.append(lp.detach())
+            del lp
+        grads.append(g)
+    logits = 2 * 1000 * 20000
+    assert held[1] - held[3] > 0.99 * logits and held[3] < 0.5 * logits
+    assert torch.equal(outs[1], outs[3])
+    # numerators rounded to bf16 once more: half a step of each
+    assert float((grads[0].double() - grads[1].double()).norm() / grads[1].double().norm()) < 2 * HALF

@@ -116,3 +116,14 @@ def test_token_logprobs_runs_what_its_head_is(monkeypatch):
     head.compile(backend="eager")
     monkeypatch.setattr(head, "_compiled_call_impl", lambda x: "compiled")
     assert m.token_logprobs(ids) == "compiled"
+
+
+def test_token_logprobs_passes_recompute_on(monkeypatch):
+    import nano_qwen_amd.model as module
+    m = _model().to(torch.bfloat16)
+    monkeypatch.setattr(Qwen3Model, "_trunk", lambda self, ids, *args: torch.zeros(
+        *ids.shape, ModelConfig(**MODEL).hidden_size, dtype=torch.bfloat16))
+    monkeypatch.setattr(module, "linear_logprobs", lambda hidden, weight, labels, **kw: kw)
+    ids = torch.tensor([[1, 2, 3]])
+    assert m.token_logprobs(ids) == dict(temperature=1.0, recompute=False)
+    assert m.token_logprobs(ids, temperature=0.5, recompute=True) == dict(temperature=0.5, recompute=True)
