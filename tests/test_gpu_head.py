@@ -440,3 +440,31 @@ def test_model_token_logprobs_memory():
     assert torch.equal(outs[1], outs[3])
     # numerators rounded to bf16 once more: half a step of each
     assert float((grads[0].double() - grads[1].double()).norm() / grads[1].double().norm()) < 2 * HALF
+
+
+# At most 64 rows: 768 workgroups of 128 entries each, which take a second tile from 98305 entries on;
+# weights of more than 256 MB are loaded past the cache.
+@pytest.mark.parametrize("rows,V,H", [(64, 100003, 64), (33, 151936, 8), (1, 131500, 1024), (33, 131500, 1024), (64, 151936, 1024)])
+def test_linear_logprobs_few_rows_of_many_tiles(rows, V, H):
+    say(f"linear_logprobs few rows {rows} x {V} x {H}")
+    g = torch.Generator(device=DEV).manual_seed(190)
+    h = torch.randn(rows, H, generator=g, device=DEV).to(BF).requires_grad_()
+    w = (torch.randn(V, H, generator=g, device=DEV) * 2 / H ** 0.5).to(BF).requires_grad_()
+    labels = torch.randint(0, V, (rows,), generator=g, device=DEV)
+    dy = torch.randn(rows, generator=g, device=DEV)
+    # tiles go to the 8 XCDs in runs, 96 of a run at first and the others second: a label in each run's last tiles
+    per = (-(-V // 128) + 7) // 8
+    assert per > 96
+    for i in range(min(rows, 16)):
+        labels[-1 - i] = min(((i % 8) * per + 96 + i // 8) * 128 + 5 * i, V - 1)
+    if rows > 1:
+        labels[0], labels[1:rows // 2:3] = V - 1, -100
+    lp = nq.linear_logprobs(h, w, labels)
+    dh, dw = torch.autograd.grad(lp, (h, w), dy)
+    want = reference(h.detach(), w.detach(), labels, dy, 1.0)
+    with torch.no_grad():
+        assert torch.equal(nq.linear_logprobs(h, w, labels), lp)
+    for name, got, ref, tol in zip(("logprobs", "dhidden"), (lp, dh), want, want[3:]):
+        within(got, ref.cpu(), tol.cpu(), name)
+    bad = (dw.double() - want[2]).abs() > want[5]
+    assert not bool(bad.any()) and bool(torch.isfinite(dw).all()), "dweight"

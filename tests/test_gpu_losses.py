@@ -773,3 +773,23 @@ def test_losses_of_more_sequences_than_one_launch():
     # averages of 1025 equal values in 64 bits
     assert abs(float(loss) - float(torch.nn.functional.softplus(-h[:B]).mean())) < 4 * U
     assert float((wc.double() - 0.5 * c[:B]).abs().max()) <= U * float(c[:B].abs().max())
+
+
+# Logits of more than 256 MB are loaded past the cache: rows cut into slices, a wave each and a workgroup each
+@pytest.mark.parametrize("rows,V,dt", [(1000, 151936, BF), (70000, 2055, BF), (16500, 8201, BF),
+                                       (600, 151936, F32), (70000, 1033, F32), (2100, 50257, F32)])
+def test_token_logprobs_past_the_cache(rows, V, dt):
+    say(f"token_logprobs past the cache {rows} x {V} {dt}")
+    assert rows * V * (2 if dt == BF else 4) > 2 ** 28
+    g = torch.Generator(device=DEV).manual_seed(33)
+    x = torch.randn(rows, V, generator=g, device=DEV, dtype=dt).mul_(3).requires_grad_()
+    labels = torch.randint(0, V, (rows,), generator=g, device=DEV)
+    labels[5::7], labels[3], labels[11] = -100, V - 1, 0
+    dy = torch.randn(rows, generator=g, device=DEV)
+    lp = nq.token_logprobs(x, labels, temperature=0.8)
+    (dx,) = torch.autograd.grad(lp, x, dy)
+    assert bool(torch.isfinite(lp).all())
+    for at in torch.arange(rows, device=DEV).split(max(1, 2 ** 25 // V)):
+        want, dwant, tol, dtol = token_reference(x.detach()[at], labels[at], dy[at], 0.8)
+        assert bool(((lp[at].double() - want).abs() <= tol).all()), int(at[0])
+        assert bool(((dx[at].double() - dwant).abs() <= dtol + half_step(dt) * dwant.abs()).all()), int(at[0])
