@@ -857,7 +857,8 @@ struct HeadSpace {
   int vc;
 };
 
-constexpr int64_t HD_DZ_BYTES = (int64_t)1 << 30;  // the largest range's dz
+// The largest range's dz; above 2^21 rows more, as a range has at least the 256 entries of a tile.
+constexpr int64_t HD_DZ_BYTES = (int64_t)1 << 30;
 
 // What a forward keeps for its backward: the labels' logits, the maxima of each 128 entries
 // and the exponentials.  Up to 4 GiB (1.4% of the memory); beyond 64 rows, as a product of so few

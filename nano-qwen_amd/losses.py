@@ -249,14 +249,14 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     hidden: (..., H) bf16 hidden states, rows at any strides; weight: (V, H) bf16, an LM
     head's; H a multiple of 8, at most 2^20; at most 2^24 rows and entries.  Logits are held
     in fp32 and never stored; the backward forms their gradient in bf16, a range of the
-    vocabulary at a time (at most 1 GiB), and gives hidden and weight gradients summed in
-    fp32.  Rows whose label is ``ignore_index`` take no part in the products.  Labels outside
+    vocabulary at a time (at most 1 GiB up to 2^21 rows, 512 bytes a row beyond), and gives
+    hidden and weight gradients summed in fp32.  Rows whose label is ``ignore_index`` take no part in the products.  Labels outside
     [0, V) give NaN, and so do their row's and the weight's gradients.
 
     A call with a gradient keeps the softmax's numerators for it, in bf16, 2 bytes for each
     entry of each row, where that is faster (widths from 256, more than 64 rows) and at most
     4 GiB; otherwise, and with ``recompute``, it keeps two numbers a row and the backward
-    repeats the first product (up to a fifth slower).
+    repeats the first product (about a fifth slower).
 
     An fp32 head goes through its logits:
     ``token_logprobs(F.linear(hidden, weight), labels)``.

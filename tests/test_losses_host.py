@@ -268,3 +268,14 @@ def test_linear_logprobs_backward_refuses_more_hidden_states_than_a_launch_write
     refused(fn, UNS, "hidden states", *head_bwd(S=1 << 24, H=2048, rs=2048))
     refused(fn, UNS, "hidden states", *head_bwd(S=(1 << 23) + 1, H=4096, rs=4096))
     refused(fn, UNS, "tiles", *head_bwd(S=1 << 24, H=1 << 20, rs=1 << 20))
+
+
+def test_linear_logprobs_backward_workspace_of_many_rows():
+    """The gradient of the logits: at most 1 GiB at a time up to 2^21 rows, 256 entries (512 bytes) a row beyond."""
+    def ws(rows, V):
+        return _lib.load().nq_linear_logprobs_bwd_workspace_bytes(rows, V, 64)
+    for rows in (1, 4096, 1 << 16, (1 << 20) + 1, 1 << 21):
+        assert ws(rows, 151936) - ws(rows, 8) <= 2 ** 30
+    for rows in ((1 << 21) + 1, 1 << 22, 1 << 24):
+        assert ws(rows, 151936) == ws(rows, 256)
+        assert ws(rows, 256) - ws(rows, 8) <= 512 * rows
