@@ -87,6 +87,8 @@ def _check_devices(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None
             # distributed, functionalized and other wrapped tensors: a kernel would take the
             # null pointer of an optional operand for one left out
             raise TypeError(f"the kernels need tensors with memory of their own, got {type(t).__name__} without")
+        if t is not None and t.is_neg():  # the imaginary part of a conjugate: its memory holds the opposite
+            raise TypeError("the kernels read a tensor's memory as it is: give resolve_neg() of a negative view")
 
 
 def _check_temperature(temperature: float) -> float:
@@ -157,7 +159,7 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, dy):
         logits, labels, stats = ctx.saved_tensors
         x, _, _, bs, rs = _rows_2d(logits)
-        dy = dy.contiguous()
+        dy = dy.resolve_neg().contiguous()
         dx = x.new_empty(logits.shape)
         _launch(x, _lib.load().nq_token_logprobs_bwd, "nq_token_logprobs_bwd", ops._ptr(x), bs, rs, ops._ptr(labels),
                 ops._ptr(stats), ops._ptr(dy), ops._ptr(dx), *ctx.tail)
@@ -221,7 +223,7 @@ class _LinearLogprobs(torch.autograd.Function):
         hidden, weight, labels, stats, kept = ctx.saved_tensors
         x, w, B, S, bs, rs = _head_operands(hidden, weight)
         V, H = w.shape
-        dy = dy.contiguous()
+        dy = dy.resolve_neg().contiguous()
         dh = x.new_empty(hidden.shape) if ctx.needs_input_grad[0] else None
         dw = w.new_empty((V, H)) if ctx.needs_input_grad[1] else None
         lib = _lib.load()
@@ -355,7 +357,7 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, dloss):
         coef, chosen_mask, rejected_mask = ctx.saved_tensors
         B, Sc, Sr = ctx.sizes
-        need = ctx.needs_input_grad
+        need, dloss = ctx.needs_input_grad, dloss.resolve_neg()
         dc = coef.new_empty((B, Sc)) if need[0] else None
         dr = coef.new_empty((B, Sr)) if need[1] else None
         _launch(coef, _lib.load().nq_preference_loss_bwd, "nq_preference_loss_bwd", coef.data_ptr(), dloss.data_ptr(),
@@ -442,7 +444,7 @@ class _PolicyLoss(torch.autograd.Function):
     @_first_order
     def backward(ctx, dloss):
         lp, old, ref, adv, mask, weight = ctx.saved_tensors
-        grad = weight.new_empty(lp.shape)
+        grad, dloss = weight.new_empty(lp.shape), dloss.resolve_neg()
         _launch(weight, _lib.load().nq_policy_loss_bwd, "nq_policy_loss_bwd", *_with_pitch(lp, old, ref, adv),
                 adv.dim() - 1, *_with_pitch(mask), weight.data_ptr(), dloss.data_ptr(), grad.data_ptr(), *ctx.tail)
         return grad, None

@@ -468,3 +468,23 @@ def test_linear_logprobs_few_rows_of_many_tiles(rows, V, H):
         within(got, ref.cpu(), tol.cpu(), name)
     bad = (dw.double() - want[2]).abs() > want[5]
     assert not bool(bad.any()) and bool(torch.isfinite(dw).all()), "dweight"
+
+
+def test_model_token_logprobs_under_autocast():
+    """fp32 weights under bf16 autocast: the head's logits are bf16, and the log-probabilities are theirs."""
+    say("model token_logprobs under autocast")
+    model = small_model(torch.float32)
+    ids = torch.randint(0, 997, (3, 21), generator=torch.Generator().manual_seed(11)).to(DEV)
+    with torch.autocast("cuda", torch.bfloat16):
+        lp = model.token_logprobs(ids)
+        z = model.lm_head(model(ids)["hidden_states"][:, :-1])
+    assert z.dtype == BF and lp.dtype == torch.float32
+    want = torch.log_softmax(z.double(), -1).gather(-1, ids[:, 1:, None])[..., 0]
+    within(lp, want.detach().cpu(), 1e-4, "logprobs")  # 997 exponentials of fp32, values under 10
+    grads = torch.autograd.grad(-lp.mean(), list(model.parameters()))
+    with torch.autocast("cuda", torch.bfloat16):
+        loss = model(ids, labels=ids)["loss"]
+    wants = torch.autograd.grad(loss.float(), list(model.parameters()))
+    for (name, _), a, b in zip(model.named_parameters(), grads, wants):
+        # logits, their gradient and each layer's rounded to 2^-8 a piece in both
+        assert a.dtype == torch.float32 and float((a.double() - b.double()).norm() / b.double().norm().clamp(min=1e-30)) < 0.05, name

@@ -793,3 +793,20 @@ def test_token_logprobs_past_the_cache(rows, V, dt):
         want, dwant, tol, dtol = token_reference(x.detach()[at], labels[at], dy[at], 0.8)
         assert bool(((lp[at].double() - want).abs() <= tol).all()), int(at[0])
         assert bool(((dx[at].double() - dwant).abs() <= dtol + half_step(dt) * dwant.abs()).all()), int(at[0])
+
+
+def test_losses_with_a_negative_view_as_gradient():
+    """A complex number's backward gives the imaginary part of a conjugate: its memory holds the opposite."""
+    say("losses with a negative view as gradient")
+    y = torch.tensor([1, 2, 0]).to(DEV)
+    h, w = randn(3, 64, seed=91, dtype=BF).to(DEV), randn(77, 64, seed=92, dtype=BF).to(DEV)
+    x, lp = randn(3, 77, seed=93).to(DEV), randn(3, 6, seed=94).to(DEV)
+    for call, first in ((lambda t: nq.token_logprobs(t, y), x), (lambda t: nq.linear_logprobs(t, w, y), h),
+                        (lambda t: nq.preference_loss(t, lp)[0], 0.5 * lp), (lambda t: nq.policy_loss(t, lp, lp[:, 0])[0], 0.9 * lp)):
+        leaf = first.clone().requires_grad_()
+        out = call(leaf)
+        d = randn(out.numel(), seed=95).view(out.shape).to(DEV)
+        view = torch._neg_view(-d)
+        assert view.is_neg()
+        want, got = (torch.autograd.grad(out, leaf, t, retain_graph=True)[0] for t in (d, view))
+        assert torch.equal(got, want) and bool(want.any())

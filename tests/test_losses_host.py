@@ -279,3 +279,18 @@ def test_linear_logprobs_backward_workspace_of_many_rows():
     for rows in ((1 << 21) + 1, 1 << 22, 1 << 24):
         assert ws(rows, 151936) == ws(rows, 256)
         assert ws(rows, 256) - ws(rows, 8) <= 512 * rows
+
+
+def test_negative_views_are_refused(stubbed):
+    """The imaginary part of a conjugate holds the opposite of what it stands for."""
+    lp = torch.complex(torch.zeros(3, 4), torch.ones(3, 4)).conj().imag
+    assert lp.is_neg() and float(lp[0, 0]) == -1
+    x, y, a = torch.zeros(3, 4), torch.tensor([1, 2, 0]), lp[:, 0]
+    for call in (lambda: nq.token_logprobs(lp, y), lambda: nq.preference_loss(lp, x), lambda: nq.preference_loss(a, a),
+                 lambda: nq.preference_loss(x, x, x, lp), lambda: nq.policy_loss(x, x, a),
+                 lambda: nq.policy_loss(x, x, lp), lambda: nq.policy_loss(x, torch._neg_view(x), x)):
+        with pytest.raises(TypeError, match="resolve_neg"):
+            call()
+    assert not stubbed
+    nq.policy_loss(x, lp.resolve_neg(), a.resolve_neg())
+    assert len(stubbed) == 1
