@@ -27,6 +27,8 @@ __all__ = ["token_logprobs", "linear_logprobs", "preference_loss", "policy_loss"
 IGNORE_INDEX = -100
 
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
+_is_tracing, _dispatch_mode = torch._C._is_tracing, torch._C._get_dispatch_mode
+_before_dispatch = torch._ops.mode_stack_state_for_pre_dispatch()  # get(0): the proxy mode there
 
 _KINDS = {"sigmoid": _lib.NQ_PREF_SIGMOID, "hinge": _lib.NQ_PREF_HINGE, "ipo": _lib.NQ_PREF_IPO}
 
@@ -41,8 +43,7 @@ def _launch(t: torch.Tensor, fn, name: str, *args) -> None:
     A recording of tensor operations (``torch.jit.trace``, ``make_fx``) holds the outputs'
     allocation and not the launch, and its replays would return what the memory holds: it is
     refused.  ``torch.compile`` breaks its graph here and calls the kernel as it is."""
-    if (torch._C._is_tracing() or torch._C._get_dispatch_mode(_PROXY) is not None
-            or torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None):
+    if _is_tracing() or _dispatch_mode(_PROXY) is not None or _before_dispatch.get(0) is not None:
         raise RuntimeError(f"{name}: a trace of tensor operations cannot hold the kernels of the losses")
     index = t.get_device()
     args += (torch._C._cuda_getCurrentRawStream(index),)
@@ -76,19 +77,24 @@ def _takes_gradient(*ts: torch.Tensor) -> bool:
 
 def _check_devices(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     index = first.get_device()  # -1: on the host
-    for t in others:
-        if t is not None and t.get_device() != index:
-            ops._require_device(first, t)
-            raise ValueError(f"the operands lie on different devices: {first.device} and {t.device}")
     if index < 0 or not first.is_cuda:
         ops._require_device(first)
-    for t in (first, *others):
-        if t is not None and not t.data_ptr() and t.numel():
-            # distributed, functionalized and other wrapped tensors: a kernel would take the
-            # null pointer of an optional operand for one left out
-            raise TypeError(f"the kernels need tensors with memory of their own, got {type(t).__name__} without")
-        if t is not None and t.is_neg():  # the imaginary part of a conjugate: its memory holds the opposite
-            raise TypeError("the kernels read a tensor's memory as it is: give resolve_neg() of a negative view")
+    _check_memory(first)
+    for t in others:
+        if t is not None:
+            if t.get_device() != index:
+                ops._require_device(first, t)
+                raise ValueError(f"the operands lie on different devices: {first.device} and {t.device}")
+            _check_memory(t)
+
+
+def _check_memory(t: torch.Tensor) -> None:
+    if t.data_ptr() == 0 and t.numel():
+        # distributed, functionalized and other wrapped tensors: a kernel would take the null
+        # pointer of an optional operand for one left out
+        raise TypeError(f"the kernels need tensors with memory of their own, got {type(t).__name__} without")
+    if t.is_neg():  # the imaginary part of a conjugate: its memory holds the opposite
+        raise TypeError("the kernels read a tensor's memory as it is: give resolve_neg() of a negative view")
 
 
 def _check_temperature(temperature: float) -> float:
