@@ -77,24 +77,24 @@ def _takes_gradient(*ts: torch.Tensor) -> bool:
 
 def _check_devices(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     index = first.get_device()  # -1: on the host
+    for t in others:
+        if t is not None and t.get_device() != index:
+            ops._require_device(first, t)
+            raise ValueError(f"the operands lie on different devices: {first.device} and {t.device}")
     if index < 0 or not first.is_cuda:
         ops._require_device(first)
-    _check_memory(first)
-    for t in others:
-        if t is not None:
-            if t.get_device() != index:
-                ops._require_device(first, t)
-                raise ValueError(f"the operands lie on different devices: {first.device} and {t.device}")
-            _check_memory(t)
 
 
-def _check_memory(t: torch.Tensor) -> None:
-    if t.data_ptr() == 0 and t.numel():
+def _memory(t: torch.Tensor) -> int:
+    """An operand's pointer, of a tensor that its memory says all of."""
+    pointer = t.data_ptr()
+    if pointer == 0 and t.numel():
         # distributed, functionalized and other wrapped tensors: a kernel would take the null
         # pointer of an optional operand for one left out
         raise TypeError(f"the kernels need tensors with memory of their own, got {type(t).__name__} without")
     if t.is_neg():  # the imaginary part of a conjugate: its memory holds the opposite
         raise TypeError("the kernels read a tensor's memory as it is: give resolve_neg() of a negative view")
+    return pointer
 
 
 def _check_temperature(temperature: float) -> float:
@@ -148,7 +148,7 @@ def _token_forward(logits, labels, temperature: float, ignore_index: int):
     nbytes = lib.nq_token_logprobs_workspace_bytes(B * S, V)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     tail = (B, S, V, ops._code(x), temperature, ignore_index)
-    _launch(x, lib.nq_token_logprobs, "nq_token_logprobs", x.data_ptr(), bs, rs, labels.data_ptr(), out.data_ptr(),
+    _launch(x, lib.nq_token_logprobs, "nq_token_logprobs", _memory(x), bs, rs, _memory(labels), out.data_ptr(),
             stats.data_ptr(), ops._ptr(ws), nbytes, *tail)
     return out, stats, tail
 
@@ -209,7 +209,7 @@ def _linear_forward(hidden, weight, labels, temperature: float, ignore_index: in
     kept = x.new_empty(nkept, dtype=torch.uint8) if nkept else None
     nbytes = lib.nq_linear_logprobs_workspace_bytes(B * S, V, H)
     ws = x.new_empty(nbytes, dtype=torch.uint8)
-    _launch(x, lib.nq_linear_logprobs, "nq_linear_logprobs", x.data_ptr(), bs, rs, w.data_ptr(), labels.data_ptr(),
+    _launch(x, lib.nq_linear_logprobs, "nq_linear_logprobs", _memory(x), bs, rs, _memory(w), _memory(labels),
             out.data_ptr(), stats.data_ptr(), ops._ptr(kept), nkept, ws.data_ptr(), nbytes, B, S, V, H, temperature,
             ignore_index)
     return out, stats, kept
@@ -331,6 +331,14 @@ def _with_pitch(*ts: Optional[torch.Tensor]):
     """Pointer and row stride of each."""
     args = ()
     for t in ts:
+        args += (None, 0) if t is None else (_memory(t), t.stride(0))
+    return args
+
+
+def _saved_pitch(*ts: Optional[torch.Tensor]):
+    """The same of what a forward took."""
+    args = ()
+    for t in ts:
         args += (None, 0) if t is None else (t.data_ptr(), t.stride(0))
     return args
 
@@ -367,7 +375,7 @@ class _PreferenceLoss(torch.autograd.Function):
         dc = coef.new_empty((B, Sc)) if need[0] else None
         dr = coef.new_empty((B, Sr)) if need[1] else None
         _launch(coef, _lib.load().nq_preference_loss_bwd, "nq_preference_loss_bwd", coef.data_ptr(), dloss.data_ptr(),
-                *_with_pitch(chosen_mask, rejected_mask), ops._ptr(dc), ops._ptr(dr), B, Sc, Sr)
+                *_saved_pitch(chosen_mask, rejected_mask), ops._ptr(dc), ops._ptr(dr), B, Sc, Sr)
         return dc, dr, None
 
 
@@ -451,8 +459,8 @@ class _PolicyLoss(torch.autograd.Function):
     def backward(ctx, dloss):
         lp, old, ref, adv, mask, weight = ctx.saved_tensors
         grad, dloss = weight.new_empty(lp.shape), dloss.resolve_neg()
-        _launch(weight, _lib.load().nq_policy_loss_bwd, "nq_policy_loss_bwd", *_with_pitch(lp, old, ref, adv),
-                adv.dim() - 1, *_with_pitch(mask), weight.data_ptr(), dloss.data_ptr(), grad.data_ptr(), *ctx.tail)
+        _launch(weight, _lib.load().nq_policy_loss_bwd, "nq_policy_loss_bwd", *_saved_pitch(lp, old, ref, adv),
+                adv.dim() - 1, *_saved_pitch(mask), weight.data_ptr(), dloss.data_ptr(), grad.data_ptr(), *ctx.tail)
         return grad, None
 
 

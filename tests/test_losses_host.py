@@ -286,11 +286,15 @@ def test_negative_views_are_refused(stubbed):
     lp = torch.complex(torch.zeros(3, 4), torch.ones(3, 4)).conj().imag
     assert lp.is_neg() and float(lp[0, 0]) == -1
     x, y, a = torch.zeros(3, 4), torch.tensor([1, 2, 0]), lp[:, 0]
-    for call in (lambda: nq.token_logprobs(lp, y), lambda: nq.preference_loss(lp, x), lambda: nq.preference_loss(a, a),
-                 lambda: nq.preference_loss(x, x, x, lp), lambda: nq.policy_loss(x, x, a),
-                 lambda: nq.policy_loss(x, x, lp), lambda: nq.policy_loss(x, torch._neg_view(x), x)):
+    whole = torch._neg_view(x)
+    for call in (lambda: nq.token_logprobs(whole, y), lambda: nq.preference_loss(whole, x), lambda: nq.preference_loss(a, a),
+                 lambda: nq.preference_loss(x, x, x, whole), lambda: nq.policy_loss(x, x, a),
+                 lambda: nq.policy_loss(x, x, whole), lambda: nq.policy_loss(x, whole, x),
+                 lambda: nq.linear_logprobs(torch.zeros(3, 8, dtype=torch.bfloat16),
+                                            torch._neg_view(torch.zeros(5, 8, dtype=torch.bfloat16)), y)):
         with pytest.raises(TypeError, match="resolve_neg"):
             call()
     assert not stubbed
     nq.policy_loss(x, lp.resolve_neg(), a.resolve_neg())
-    assert len(stubbed) == 1
+    nq.policy_loss(x, lp, x)  # whose rows are no vectors: copied, and resolved so
+    assert len(stubbed) == 2 and not lp.contiguous().is_neg() and float(lp.contiguous()[0, 0]) == -1
