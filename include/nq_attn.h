@@ -548,7 +548,7 @@ int nq_linear_logprobs_bwd(const void* hidden, int64_t batch_stride, int64_t row
                            int64_t ignore_index, void* stream);
 
 /*
- * Preference loss over B pairs of sequences.  Each side: fp32 log-probabilities of its
+ * Preference loss over B (at most 2^30) pairs of sequences.  Each side: fp32 log-probabilities of its
  * tokens (B rows of Sc or Sr, row strides in elements), those of the reference model
  * (NULL: zeros) and a mask (a byte per token, nonzero = kept; NULL: all kept; what a
  * masked token holds is not read).  d = sum of lp - ref over the kept tokens, or with
@@ -579,7 +579,7 @@ int nq_preference_loss_bwd(const float* coef, const float* dloss, const uint8_t*
                            int64_t Sc, int64_t Sr, void* stream);
 
 /*
- * Clipped policy loss with a KL term over B sequences of S tokens (fp32 rows with
+ * Clipped policy loss with a KL term over B (at most 2^30) sequences of S tokens (fp32 rows with
  * strides in elements, as above).  Per kept token, with r = exp(lp - old), A its
  * sequence's advantage (advantages[b * stride]; with advantages_per_token
  * advantages[b * stride + s]) and q = ref - lp:

@@ -229,6 +229,9 @@ __device__ __forceinline__ double team_sum(double v, double* lds) {
   return sum;
 }
 
+// Sequences of a call: the last launches' threads step over them by 256 in an int.
+constexpr int MOST_SEQUENCES = 1 << 30;
+
 // Where a launch of one workgroup does the whole forward: at most this many sequences,
 // a wave each, of at most this many tokens.
 constexpr int ONE_ROWS = 16, ONE_TOKENS = 1024;
@@ -672,6 +675,7 @@ static int pref_check(int B, int64_t Sc, int64_t Sr, const float* coef) {
   if (B <= 0 || Sc < 0 || Sr < 0)
     return nq_fail(NQ_ERR_INVALID, "B must be positive and the lengths not negative (B=%d Sc=%lld Sr=%lld)", B,
                    (long long)Sc, (long long)Sr);
+  if (B > MOST_SEQUENCES) return nq_fail(NQ_ERR_UNSUPPORTED, "at most 2^30 sequences in one call, got %d", B);
   if (Sc > ((int64_t)1 << 40) / B || Sr > ((int64_t)1 << 40) / B)
     return nq_fail(NQ_ERR_UNSUPPORTED, "too many tokens for one launch");
   if (!coef || !aligned_to(coef, 4)) return nq_fail(NQ_ERR_INVALID, "coef is required, aligned to fp32");
@@ -770,6 +774,7 @@ static int policy_params(PolicyParams* p, const float* logprobs, int64_t lp_rs, 
                          const uint8_t* mask, int64_t mask_rs, float* weight, int B, int64_t S, double clip_low,
                          double clip_high, double kl_coef) {
   if (B <= 0 || S < 0) return nq_fail(NQ_ERR_INVALID, "B must be positive and S not negative (B=%d S=%lld)", B, (long long)S);
+  if (B > MOST_SEQUENCES) return nq_fail(NQ_ERR_UNSUPPORTED, "at most 2^30 sequences in one call, got %d", B);
   if (S > ((int64_t)1 << 40) / B) return nq_fail(NQ_ERR_UNSUPPORTED, "too many tokens for one launch");
   if ((S && (!logprobs || !old)) || (!adv && (S || !adv_per_token)) || !weight)
     return nq_fail(NQ_ERR_INVALID, "logprobs, old logprobs, advantages and weight are required");

@@ -293,7 +293,7 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
 
 _HEAD_MOST = 1 << 24
 _HEAD_WIDEST = 1 << 20
-_MOST_SEQUENCES = 2 ** 31 - 1  # the C entries' int, to which ctypes cuts a larger number without a word
+_MOST_SEQUENCES = 1 << 30  # well within the C entries' int, to which ctypes cuts a larger number without a word
 
 
 # ---------------------------------------------------------------------------
@@ -397,7 +397,7 @@ def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: Op
       "hinge"    max(0, 1 - h)
       "ipo"      (d_chosen - d_rejected - 1 / (2 beta))^2
 
-    The loss is the mean over pairs, a scalar with gradients for chosen and rejected (the
+    The loss is the mean over pairs (at most 2^30), a scalar with gradients for chosen and rejected (the
     references get none); the rewards, beta d, are (B,) without gradient.
     """
     _check_devices(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask)
@@ -415,7 +415,7 @@ def preference_loss(chosen: torch.Tensor, rejected: torch.Tensor, ref_chosen: Op
         raise ValueError(f"chosen and rejected must hold the same number of sequences, at least one, "
                          f"got {chosen.shape[0]} and {rejected.shape[0]}")
     if chosen.shape[0] > _MOST_SEQUENCES:
-        raise ValueError(f"at most 2^31 - 1 sequences in one call, got {chosen.shape[0]}")
+        raise ValueError(f"at most 2^30 sequences in one call, got {chosen.shape[0]}")
     sc, sr = chosen.shape, rejected.shape
     chosen, rejected = _token_rows(chosen, "chosen", sc), _token_rows(rejected, "rejected", sr)
     rewards = chosen.new_empty(sc[0]), chosen.new_empty(sc[0])
@@ -468,7 +468,7 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
                 ref_logprobs: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                 clip_low: float = 0.2, clip_high: Optional[float] = None, kl_coef: float = 0.0,
                 reduction: str = "token") -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Clipped policy loss with a KL term over B sequences of tokens: (loss, kl, clipped).
+    """Clipped policy loss with a KL term over B sequences (at most 2^30) of tokens: (loss, kl, clipped).
 
     logprobs, old_logprobs, ref_logprobs: (B, S) log-probabilities of the sampled tokens
     under the policy, the policy that sampled them and a reference (needed with
@@ -488,7 +488,7 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
     if logprobs.dim() != 2 or logprobs.shape[0] == 0:
         raise ValueError(f"logprobs must be (B, S) with at least one sequence, got shape {tuple(logprobs.shape)}")
     if logprobs.shape[0] > _MOST_SEQUENCES:
-        raise ValueError(f"at most 2^31 - 1 sequences in one call, got {logprobs.shape[0]}")
+        raise ValueError(f"at most 2^30 sequences in one call, got {logprobs.shape[0]}")
     clip_high = clip_low if clip_high is None else clip_high
     if not 0 <= clip_low <= 1 or not (clip_high >= 0 and math.isfinite(clip_high)) or not math.isfinite(kl_coef):
         raise ValueError("clip_low must lie in [0, 1], clip_high be at least 0 and all finite, "

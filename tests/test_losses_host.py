@@ -298,3 +298,19 @@ def test_negative_views_are_refused(stubbed):
     nq.policy_loss(x, lp.resolve_neg(), a.resolve_neg())
     nq.policy_loss(x, lp, x)  # whose rows are no vectors: copied, and resolved so
     assert len(stubbed) == 2 and not lp.contiguous().is_neg() and float(lp.contiguous()[0, 0]) == -1
+
+
+def test_more_sequences_than_an_int_steps_over_are_refused(monkeypatch):
+    """The threads that finish a loss step over its sequences by 256 in an int, which would pass its end."""
+    for B in ((1 << 30) + 1, (1 << 31) - 1):
+        refused("nq_preference_loss", UNS, "sequences", *preference(B=B))
+        refused("nq_policy_loss", UNS, "sequences", *policy(B=B))
+        refused("nq_preference_loss_bwd", UNS, "sequences", P, P, None, 0, None, 0, P, P, B, 1, 1, None)
+        refused("nq_policy_loss_bwd", UNS, "sequences", P, 9, P, 9, None, 0, P, 1, 0, None, 0, P, P, P, B, 1, 0.2,
+                   0.2, 0.0, None)
+    monkeypatch.setattr(nq.losses.ops, "_require_device", lambda *ts: None)
+    many = torch.zeros(1).expand((1 << 30) + 1)
+    with pytest.raises(ValueError, match="sequences"):
+        nq.preference_loss(many, many)
+    with pytest.raises(ValueError, match="sequences"):
+        nq.policy_loss(many[:, None], many[:, None], many)
