@@ -238,10 +238,12 @@ def _own(s):
         nq.kv4_append(s["k"], s["v"], s["pool"], s["table"], row_offset=c["past"])
         return list(nq.kv4_gather(s["pool"], s["table"], S=c["past"] + c["S"], dtype=DTYPES[c["dtype"]]))
     if c["kind"] == "decode":
-        return [nq.attention_decode_kv4(s["q"], s["pool"], s["table"], s["lens"], max_len=c["T"])]
+        return [nq.attention_decode_kv4(s["q"], s["pool"], s["table"], s["lens"], max_len=max(s["host_lens"]))]
     if c["kind"] == "weights":
         pool = s["pool"] if c["cache"] == "kv4" else s["k_pool"]
-        return [nq.attention_key_weights(s["q"], pool, s["table"], s["lens"], s["lse"], max_len=c["T"])]
+        longest = max(s["host_lens"])
+        w = None if longest == c["T"] else torch.zeros(c["B"], c["Hkv"], c["T"], device=DEV)
+        return [nq.attention_key_weights(s["q"], pool, s["table"], s["lens"], s["lse"], max_len=longest, weights=w)]
     kept = nq.select_keys(s["weights"], s["lens"], keep=c["keep"], recent=c["recent"], first=c["first"])
     pools = s["pool"] if c["cache"] == "kv4" else (s["k_pool"], s["v_pool"])
     w = nq.kv_compact(pools, s["table"], s["new_table"], kept, weights=s["weights"])
