@@ -340,6 +340,24 @@ int nq_attn_decode_paged_fwd(const void* q, const int64_t* q_strides, const void
                              const int32_t* q_pos, int q_pos0, float sm_scale, void* stream);
 
 /*
+ * nq_attn_decode_paged_fwd that also writes lse (fp32 (B, Hq), NULL for none):
+ * the natural log-sum-exp of each head's scaled scores, -inf for a sequence
+ * without keys and NaN for one whose length is out of range.
+ */
+int nq_attn_decode_paged_lse_fwd(const void* q, const int64_t* q_strides, const void* k_new,
+                                 const int64_t* k_new_strides, const void* v_new,
+                                 const int64_t* v_new_strides, const float* k_weight, void* k_pool,
+                                 const int64_t* k_pool_strides, void* v_pool,
+                                 const int64_t* v_pool_strides, const int32_t* block_table,
+                                 int64_t bt_stride, int page_size, const int32_t* lens,
+                                 int32_t* lens_out, void* o, const int64_t* o_strides, void* workspace,
+                                 int64_t workspace_bytes, int B, int Hq, int Hkv, int D, int max_len,
+                                 int chunk, int dtype, const float* q_weight, float eps,
+                                 const float* cos_tab, const float* sin_tab, int max_pos,
+                                 const int32_t* q_pos, int q_pos0, float sm_scale, float* lse,
+                                 void* stream);
+
+/*
  * nq_attn_decode_paged_fwd without a workspace argument, allocating nothing.
  * It has no counterpart in the reference: it is for callers that cannot
  * allocate device memory (code under HIP graph capture, serving loops,
@@ -608,6 +626,115 @@ int nq_policy_loss_bwd(const float* logprobs, int64_t logprobs_stride, const flo
                        const uint8_t* mask, int64_t mask_stride, const float* weight,
                        const float* dloss, float* dlogprobs, int B, int64_t S, double clip_low,
                        double clip_high, double kl_coef, void* stream);
+
+/*
+ * 4-bit paged KV caches (no counterpart in the reference).  Rows of K (normed and
+ * rotated) and V are held in blocks of 32 elements: a code for each, {0, 1/2, 1, 3/2, 2,
+ * 3, 4, 6} with a sign bit above (E2M1), and a scale byte e per block, 2^(e - 127); e =
+ * 255 makes the block NaN.  The pool is num_pages pages of Hkv heads, strides {page,
+ * head} in bytes (multiples of 16, as its address); a page's head is contiguous and
+ * holds, for its page_size rows,
+ *   K codes (page_size, D/2) | V codes (page_size, D/2) | K scales (page_size, D/32) |
+ *   V scales (page_size, D/32)
+ * with two codes a byte, the even element low: page_size * 17 D / 16 bytes.  page_size is
+ * a multiple of 32 up to 2^20, head_dim 32, 64 or 128.  Tables as for the other paged
+ * caches, with bt_cols entries a sequence; an entry outside [0, num_pages) is never
+ * followed: rows there are not written, read as NaN, and make an attention NaN.
+ */
+
+/*
+ * Rows into 4-bit pages.  Token s of sequence b is row row_base[b] + s (row_base NULL:
+ * row0 + s).  K rows are normed with k_weight (NULL: not) and rotated at pos[b, s], else
+ * pos_base[b] + s, else pos0 + s, plus pos_shift[b] where given (cos_tab NULL: not
+ * rotated), in fp32, and rounded once.  q rows (NULL with Hq = 0: none) are normed with
+ * q_weight and rotated alike and written to q_out in dtype.  A block's scale is the
+ * smallest power of two, from 2^-126 to 2^125, of which its largest magnitude is at most
+ * 7 times; codes round to the nearest, halfway to the even code, beyond 6 to 6.  A block
+ * with an infinity or NaN becomes NaN.
+ * lens_out (may be NULL, must not alias row_base) receives row_base[b] + S.  A sequence
+ * whose rows do not all lie in [0, bt_cols * page_size) appends nothing and keeps its
+ * length there.
+ * dtype: of k, v, q and q_out, with NQ_QWEIGHT_BF16 / NQ_KWEIGHT_BF16.
+ */
+int nq_kv4_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                  const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+                  void* pool, const int64_t* pool_strides, int num_pages, const int32_t* block_table,
+                  int64_t bt_stride, int bt_cols, int page_size, int B, int S, int Hq, int Hkv, int D,
+                  int dtype, const void* q_weight, const void* k_weight, float eps, const float* cos_tab,
+                  const float* sin_tab, int max_pos, const int32_t* pos, const int32_t* pos_base,
+                  const int32_t* pos_shift, int pos0, const int32_t* row_base, int row0,
+                  int32_t* lens_out, void* stream);
+
+/*
+ * Rows row_base[b] + s (row_base NULL: row0 + s), s < S, of 4-bit pages as dtype: k, v
+ * (B, Hkv, S, D) with strides {batch, head, seq}.  Values are exact in either dtype (bf16
+ * below 2^-133 and above its largest number excepted).  Rows without a page are NaN.
+ */
+int nq_kv4_gather(const void* pool, const int64_t* pool_strides, int num_pages, const int32_t* block_table,
+                  int64_t bt_stride, int bt_cols, int page_size, void* k, const int64_t* k_strides,
+                  void* v, const int64_t* v_strides, int B, int S, int Hkv, int D, int dtype,
+                  const int32_t* row_base, int row0, void* stream);
+
+/*
+ * Single-token GQA attention over keys [0, lens[b]) of 4-bit pages.  q: (B, Hq, D),
+ * strides {batch, head}, normed and rotated (nq_kv4_append's q_out); o alike; lse: fp32
+ * (B, Hq) or NULL.  dtype: of q and o.  Lengths as in nq_attn_decode_fwd: zeros (and LSE
+ * -inf) without keys, NaN outside [0, max_len].  workspace: at least
+ * nq_attn_decode_kv4_workspace_bytes, 16-byte aligned; calls that overlap need one each.
+ */
+int64_t nq_attn_decode_kv4_workspace_bytes(int B, int Hq, int Hkv, int D);
+int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const void* pool,
+                       const int64_t* pool_strides, int num_pages, const int32_t* block_table,
+                       int64_t bt_stride, int bt_cols, int page_size, const int32_t* lens, void* o,
+                       const int64_t* o_strides, float* lse, void* workspace, int64_t workspace_bytes,
+                       int B, int Hq, int Hkv, int D, int max_len, int dtype, float sm_scale,
+                       void* stream);
+
+/*
+ * The attention weight each key of a paged cache got:
+ *   weights[b, h, t] (+)= sum over the query heads of kv head h and the S queries that see
+ *   key t of exp(sm_scale q . k_t - lse)
+ * for t < lens[b]; rows [lens[b], max_len) are set to 0, or left alone when accumulating.
+ * q: bf16 (B, Hq, S, D) as attended (normed and rotated), strides {batch, head, seq}; lse:
+ * fp32 (B, Hq, S) contiguous, -inf for a query without keys.  causal: query s sees keys up
+ * to lens[b] - S + s; else, and for S = 1, all.  k_pool: four_bit: 4-bit pages, strides
+ * {page, head} in bytes; else bf16 K pages, strides {page, head, row} in elements.
+ * weights: fp32, strides {batch, head}, max_len entries a head.  A length outside
+ * [0, max_len] gives NaN (accumulating: nothing), a page outside the pool NaN at its keys.
+ * Sums are taken in a fixed order.
+ */
+int nq_key_weights(const void* q, const int64_t* q_strides, const void* k_pool,
+                   const int64_t* pool_strides, int four_bit, int num_pages, const int32_t* block_table,
+                   int64_t bt_stride, int bt_cols, int page_size, const int32_t* lens, const float* lse,
+                   float* weights, const int64_t* weight_strides, int accumulate, int B, int Hq, int Hkv,
+                   int S, int D, int max_len, int causal, float sm_scale, void* stream);
+
+/*
+ * The rows of a cache worth keeping: kept (int32 (B, Hkv, keep), contiguous) receives, in
+ * ascending order, the first `first` rows, the last `recent` of lens[b], and of those in
+ * between the heaviest, equal weights by the lower index (NaN above every number); -1
+ * behind them where a sequence holds fewer than keep.  weights: fp32, strides {batch,
+ * head}, width entries a head.  first + recent <= keep.  A length outside [0, width]
+ * keeps nothing.
+ */
+int nq_select_keys(const float* weights, const int64_t* weight_strides, const int32_t* lens, int32_t* kept,
+                   int B, int Hkv, int width, int keep, int recent, int first, void* stream);
+
+/*
+ * Moves row kept[b, h, i] of each sequence's pages (block_table) to row i of its new pages
+ * (new_table, entries of which must not be pages of any block_table row), both in the same
+ * pool; -1 moves nothing.  v_pool NULL: k_pool is a 4-bit pool of head_dim, strides {page,
+ * head} in bytes.  Else K and V pools of rows of row_bytes, strides {page, head, row} in
+ * bytes.  weights_out (NULL: none; not weights) receives the kept rows' weights and 0
+ * behind them up to width; both fp32 with weight_strides {batch, head}.  Rows of the new
+ * pages behind the last one moved are left as they are.
+ */
+int nq_kv_compact(void* k_pool, const int64_t* k_strides, void* v_pool, const int64_t* v_strides,
+                  int row_bytes, int head_dim, int num_pages, const int32_t* block_table,
+                  int64_t bt_stride, int bt_cols, const int32_t* new_table, int64_t new_stride,
+                  int new_cols, int page_size, const int32_t* kept, const float* weights,
+                  float* weights_out, const int64_t* weight_strides, int width, int B, int Hkv, int keep,
+                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -43,6 +43,8 @@ from .generate import TextGenerator, generate_greedy_batch
 from .ops import attention_backward, attention_merge_, qk_norm_rope_backward
 from .autograd import attention_core, flash_attention_train
 from .losses import linear_logprobs, policy_loss, preference_loss, token_logprobs
+from .kv4 import (attention_decode_kv4, attention_key_weights, kv4_append, kv4_empty_pool, kv4_gather,
+                  kv_compact, select_keys)
 from .ring import RingAttention, ring_attention_all_ranks, ring_schedule, ring_step, split_sequence
 
 __all__ = [
@@ -54,4 +56,6 @@ __all__ = [
     "attention_merge_", "RingAttention", "ring_step", "ring_schedule", "split_sequence",
     "ring_attention_all_ranks", "attention_backward", "qk_norm_rope_backward", "attention_core",
     "flash_attention_train", "token_logprobs", "linear_logprobs", "preference_loss", "policy_loss",
+    "kv4_empty_pool", "kv4_append", "kv4_gather", "attention_decode_kv4", "attention_key_weights", "select_keys",
+    "kv_compact",
 ]

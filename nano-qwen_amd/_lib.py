@@ -126,6 +126,18 @@ SIGNATURES = {
         _p, _p, _i32,                                # cos, sin, max_pos
         _p, _i32, _f32, _p,                          # q_pos, q_pos0, sm_scale, stream
     ]),
+    "nq_attn_decode_paged_lse_fwd": (_i32, [
+        _p, _i64p,                                   # q, q_strides
+        _p, _i64p, _p, _i64p, _p,                    # k_new, v_new (+ strides), k_weight
+        _p, _i64p, _p, _i64p,                        # k_pool, v_pool (+ strides)
+        _p, _i64, _i32,                              # block_table, bt_stride, page_size
+        _p, _p,                                      # lens, lens_out
+        _p, _i64p, _p, _i64,                         # o, o_strides, workspace, workspace_bytes
+        _i32, _i32, _i32, _i32, _i32, _i32, _i32,    # B, Hq, Hkv, D, max_len, chunk, dtype
+        _p, _f32,                                    # q_weight, eps
+        _p, _p, _i32,                                # cos, sin, max_pos
+        _p, _i32, _f32, _p, _p,                      # q_pos, q_pos0, sm_scale, lse, stream
+    ]),
     "nq_attn_decode_paged_fwd_noalloc": (_i32, [
         _p, _i64p,                                   # q, q_strides
         _p, _i64p, _p, _i64p, _p,                    # k_new, v_new (+ strides), k_weight
@@ -236,6 +248,46 @@ SIGNATURES = {
         _p, _i64, _i32, _p, _i64,                    # advantages, stride, per_token, mask, stride
         _p, _p, _p,                                  # weight, dloss, dlogprobs
         _i32, _i64, _f64, _f64, _f64, _p,            # B, S, clip_low, clip_high, kl_coef, stream
+    ]),
+    "nq_kv4_append": (_i32, [
+        _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p,  # k, v, q, q_out (+ strides)
+        _p, _i64p, _i32, _p, _i64, _i32, _i32,       # pool, strides, num_pages, block_table, bt_stride, bt_cols, page_size
+        _i32, _i32, _i32, _i32, _i32, _i32,          # B, S, Hq, Hkv, D, dtype
+        _p, _p, _f32,                                # q_weight, k_weight, eps
+        _p, _p, _i32,                                # cos, sin, max_pos
+        _p, _p, _p, _i32,                            # pos, pos_base, pos_shift, pos0
+        _p, _i32, _p, _p,                            # row_base, row0, lens_out, stream
+    ]),
+    "nq_kv4_gather": (_i32, [
+        _p, _i64p, _i32, _p, _i64, _i32, _i32,       # pool, strides, num_pages, block_table, bt_stride, bt_cols, page_size
+        _p, _i64p, _p, _i64p,                        # k, v (+ strides)
+        _i32, _i32, _i32, _i32, _i32,                # B, S, Hkv, D, dtype
+        _p, _i32, _p,                                # row_base, row0, stream
+    ]),
+    "nq_attn_decode_kv4_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),  # B, Hq, Hkv, D
+    "nq_attn_decode_kv4": (_i32, [
+        _p, _i64p,                                   # q, q_strides
+        _p, _i64p, _i32, _p, _i64, _i32, _i32,       # pool, strides, num_pages, block_table, bt_stride, bt_cols, page_size
+        _p, _p, _i64p, _p, _p, _i64,                 # lens, o, o_strides, lse, workspace, workspace_bytes
+        _i32, _i32, _i32, _i32, _i32, _i32,          # B, Hq, Hkv, D, max_len, dtype
+        _f32, _p,                                    # sm_scale, stream
+    ]),
+    "nq_key_weights": (_i32, [
+        _p, _i64p,                                   # q, q_strides
+        _p, _i64p, _i32, _i32, _p, _i64, _i32, _i32,  # pool, strides, four_bit, num_pages, block_table, stride, cols, page_size
+        _p, _p, _p, _i64p, _i32,                     # lens, lse, weights, strides, accumulate
+        _i32, _i32, _i32, _i32, _i32, _i32,          # B, Hq, Hkv, S, D, max_len
+        _i32, _f32, _p,                              # causal, sm_scale, stream
+    ]),
+    "nq_select_keys": (_i32, [
+        _p, _i64p, _p, _p,                           # weights, strides, lens, kept
+        _i32, _i32, _i32, _i32, _i32, _i32, _p,      # B, Hkv, width, keep, recent, first, stream
+    ]),
+    "nq_kv_compact": (_i32, [
+        _p, _i64p, _p, _i64p, _i32, _i32, _i32,      # k_pool, v_pool (+ strides), row_bytes, head_dim, num_pages
+        _p, _i64, _i32, _p, _i64, _i32, _i32,        # block_table, stride, cols, new_table, stride, cols, page_size
+        _p, _p, _p, _i64p, _i32,                     # kept, weights, weights_out, strides, width
+        _i32, _i32, _i32, _p,                        # B, Hkv, keep, stream
     ]),
 }
 

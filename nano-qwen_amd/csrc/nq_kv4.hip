@@ -1,0 +1,658 @@
+// Rows into 4-bit pages, rows of 4-bit pages read back, and single-token attention
+// over them, for gfx950.  The page format is nq_kv4.hpp's.  No counterpart in the
+// reference, whose cache (model/attention.py:24-46) holds the model's type.
+
+#include <type_traits>
+
+#include "nq_common.hpp"
+#include "nq_decode.hpp"
+#include "nq_internal.hpp"
+#include "nq_kv4.hpp"
+
+namespace nq {
+
+// ---------------------------------------------------------------- rows into pages
+struct Kv4AppendParams {
+  const void *k, *v, *q;
+  int64_t ksb, ksh, kss, vsb, vsh, vss, qsb, qsh, qss;
+  void* q_out;
+  int64_t osb, osh, oss;
+  unsigned char* pool;
+  int64_t psb, psh;  // page and head strides (bytes)
+  int npages;
+  const int32_t* bt;
+  int64_t bts;
+  int64_t cap;  // rows that the block table maps
+  int page;
+  int B, S, Hq, Hkv;
+  const void *qw, *kw;
+  int q16, k16;
+  float eps;
+  const float *cos_tab, *sin_tab;
+  int max_pos;
+  const int32_t *pos, *pos_base, *pos_shift;
+  int pos0;
+  const int32_t* row_base;
+  int row0;
+  int32_t* lens_out;
+};
+
+// Largest magnitude's bits over groups of N = 2 or 4 lanes.
+template <int N>
+__device__ __forceinline__ uint32_t group_max_bits(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));  // quad xor 1
+  if (N == 4) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));  // quad xor 2
+  return v;
+}
+
+__device__ __forceinline__ uint32_t max_bits8(const floatx8& x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+  return m;
+}
+
+// Codes of 8 elements, rounded to the nearest (halfway: the even code) and to +-6
+// where beyond.
+__device__ __forceinline__ uint32_t kv4_codes8(const floatx8& x, float scale) {
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], scale, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], scale, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], scale, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
+  return c;
+}
+
+// One row of k, v or q to D/16 lanes: lane `sub` holds elements [8 sub, +8) and
+// [D/2 + 8 sub, +8), the layout of norm_row / rope_row, in which a block of 32 is
+// four lanes' first or second chunk (D = 32: both chunks of two lanes).  K rows are
+// normed and rotated in fp32 and rounded once, to their codes; q rows likewise, to
+// q_out.  HBM-bound: each row read once, 17 D / 32 bytes written.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendParams p) {
+  using L = Kv4<D>;
+  constexpr int LPR = D / 16;
+  const uint32_t HT = (uint32_t)(p.Hq + 2 * p.Hkv);
+  const int64_t gl = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row64 = gl / LPR;
+  const int sub = (int)(gl % LPR);
+  if (row64 >= (int64_t)p.B * p.S * HT) return;  // whole groups of LPR lanes leave together
+  const uint32_t row = (uint32_t)row64;
+  const uint32_t t = row / HT;
+  int h = (int)(row % HT);
+  const int s = (int)(t % (uint32_t)p.S), b = (int)(t / (uint32_t)p.S);
+  const int base = p.row_base ? p.row_base[b] : p.row0;
+  const bool fits = base >= 0 && (int64_t)base + p.S <= p.cap;
+  if (p.lens_out && h == 0 && s == 0 && sub == 0) p.lens_out[b] = fits ? base + p.S : base;
+  const bool is_q = h < p.Hq, is_k = !is_q && h < p.Hq + p.Hkv;
+  if (!is_q && !fits) return;
+  const T* src;
+  if (is_q) {
+    src = reinterpret_cast<const T*>(p.q) + b * p.qsb + h * p.qsh + s * p.qss;
+  } else if (is_k) {
+    h -= p.Hq;
+    src = reinterpret_cast<const T*>(p.k) + b * p.ksb + h * p.ksh + s * p.kss;
+  } else {
+    h -= p.Hq + p.Hkv;
+    src = reinterpret_cast<const T*>(p.v) + b * p.vsb + h * p.vsh + s * p.vss;
+  }
+  floatx8 x1 = Vec8<T>::load_f32(src + sub * 8), x2 = Vec8<T>::load_f32(src + D / 2 + sub * 8);
+  if (is_q || is_k) {
+    const void* w = is_q ? p.qw : p.kw;
+    if (w) {
+      const int w16 = is_q ? p.q16 : p.k16;
+      Weight8 a, c;
+      a.load(w, w16, sub * 8);
+      c.load(w, w16, D / 2 + sub * 8);
+      norm_row<D>(x1, x2, a.value(w16), c.value(w16), p.eps);
+    }
+    if (p.cos_tab) {
+      int at = row_position(p.pos, p.pos_base, p.pos0, b, s, p.S);
+      if (p.pos_shift) at += p.pos_shift[b];
+      at = table_row(at, p.max_pos);
+      rope_row(x1, x2, load_tab8(p.cos_tab, at, D / 2, sub * 8), load_tab8(p.sin_tab, at, D / 2, sub * 8));
+    }
+  }
+  if (is_q) {
+    T* dst = reinterpret_cast<T*>(p.q_out) + b * p.osb + h * p.osh + s * p.oss;
+    store8<T>(dst + sub * 8, x1);
+    store8<T>(dst + D / 2 + sub * 8, x2);
+    return;
+  }
+  uint32_t m1 = max_bits8(x1), m2 = max_bits8(x2);
+  if (D == 32) m1 = m2 = max(m1, m2);
+  constexpr int LPB = D == 32 ? 2 : 4;  // lanes of a block
+  const uint32_t e1 = kv4_scale_byte(group_max_bits<LPB>(m1)), e2 = kv4_scale_byte(group_max_bits<LPB>(m2));
+  const int r = base + s;
+  const int pid = p.bt[b * p.bts + r / p.page];
+  if ((uint32_t)pid >= (uint32_t)p.npages) return;  // not a page of the pool
+  const int in = r % p.page;
+  unsigned char* rec = p.pool + pid * p.psb + h * p.psh;
+  unsigned char* codes = rec + (is_k ? 0 : L::v_codes(p.page)) + in * L::CB;
+  unsigned char* scales = rec + (is_k ? L::k_scales(p.page) : L::v_scales(p.page)) + in * L::SB;
+  *reinterpret_cast<uint32_t*>(codes + sub * 4) = kv4_codes8(x1, kv4_scale(e1 == 255 ? 127 : e1));
+  *reinterpret_cast<uint32_t*>(codes + L::CB / 2 + sub * 4) = kv4_codes8(x2, kv4_scale(e2 == 255 ? 127 : e2));
+  if (sub % LPB == 0) {
+    scales[sub / LPB] = (unsigned char)e1;
+    if (D > 32) scales[L::SB / 2 + sub / LPB] = (unsigned char)e2;
+  }
+}
+
+// ---------------------------------------------------------------- rows read back
+struct Kv4GatherParams {
+  const unsigned char* pool;
+  int64_t psb, psh;
+  int npages;
+  const int32_t* bt;
+  int64_t bts;
+  int64_t cap;
+  int page;
+  void *k, *v;
+  int64_t ksb, ksh, kss, vsb, vsh, vss;
+  int B, S, Hkv;
+  const int32_t* row_base;
+  int row0;
+};
+
+// A row's 16 elements a lane (8 bytes of codes, a scale); the rows of a head
+// consecutive, so that reads and writes are both contiguous.  HBM-bound by its writes.
+// A row without a page reads as NaN.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4GatherParams p) {
+  using L = Kv4<D>;
+  constexpr int LPR = D / 16;
+  const int64_t gl = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row64 = gl / LPR;
+  const int sub = (int)(gl % LPR);
+  if (row64 >= (int64_t)p.B * p.S * p.Hkv) return;
+  const uint32_t row = (uint32_t)row64, t = row / (uint32_t)p.S;
+  const int s = (int)(row % (uint32_t)p.S), h = (int)(t % (uint32_t)p.Hkv), b = (int)(t / (uint32_t)p.Hkv);
+  const bool is_v = blockIdx.y;
+  const int64_t r = (int64_t)(p.row_base ? p.row_base[b] : p.row0) + s;
+  T* dst = is_v ? reinterpret_cast<T*>(p.v) + b * p.vsb + h * p.vsh + s * p.vss
+                : reinterpret_cast<T*>(p.k) + b * p.ksb + h * p.ksh + s * p.kss;
+  uint32_t c[2] = {0, 0}, e = 255;
+  if (r >= 0 && r < p.cap) {
+    const int pid = p.bt[b * p.bts + (int)r / p.page], in = (int)r % p.page;
+    if ((uint32_t)pid < (uint32_t)p.npages) {
+      const unsigned char* rec = p.pool + pid * p.psb + h * p.psh;
+      const uint2 w = *reinterpret_cast<const uint2*>(rec + (is_v ? L::v_codes(p.page) : 0) + in * L::CB + sub * 8);
+      c[0] = w.x;
+      c[1] = w.y;
+      e = rec[(is_v ? L::v_scales(p.page) : L::k_scales(p.page)) + in * L::SB + sub / 2];
+    }
+  }
+  const float scale = kv4_scale(e);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bf16x8 v = kv4_bf16x8(c[i], scale);
+    store8<T>(dst + sub * 16 + i * 8, __builtin_convertvector(v, floatx8));
+  }
+}
+
+// ---------------------------------------------------------------- decode
+// The schedule, the online softmax, the partials and their merge are those of the bf16
+// decode (nq_decode.hip); what differs is how a step's 32 keys reach the matrix cores.
+//   K: a 16-key tile is one load per lane of D/4 consecutive elements of a row, in the
+//     order in which the MFMA's k slots are taken (slot 8 g + j of MFMA i is element
+//     g D/4 + 8 i + j, for q as well), and one scale byte, since those elements lie in
+//     one block.  They become bf16 operands in registers, without LDS.
+//   V: whole rows as they lie in the page; a lane's codes become bf16 in registers, go
+//     to a wave-private LDS tile and come back transposed, as in the bf16 decode.
+// Codes times a power of two are exact in bf16, so the products are those of a bf16
+// cache that held the same values.  fp32 queries: q and the probabilities are split into
+// three bf16 terms each (8 + 8 + 8 significant bits), three MFMAs in place of one.
+constexpr int KV4_WG_PER_CU = 2;
+constexpr int KV4_MAX_WAVES = 256 * KV4_WG_PER_CU * DC_WAVES;
+constexpr int KV4_DEPTH = 2;  // steps whose loads are in flight
+
+// One step's codes and scales as loaded.
+template <int D> struct Kv4Step {
+  static constexpr int KW = D / 32;                    // K dwords a lane and 16-key tile
+  static constexpr int VB = D == 32 ? 8 : 16;          // V bytes a lane and load
+  static constexpr int VL = D / 4 / VB;                // V loads a step
+  uint32_t k[2][KW], ks[2];
+  uint32_t v[VL][VB / 4], vs[VL];
+};
+
+template <int N>
+__device__ __forceinline__ void kv4_load(uint32_t (&d)[N], BufRsrc r, int voff, int soff) {
+  if constexpr (N == 4) {
+    const auto w = __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = w[i];
+  } else if constexpr (N == 2) {
+    const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, 2);
+    d[0] = w[0];
+    d[1] = w[1];
+  } else {
+    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 2);
+  }
+}
+
+// x as the sum of NT bf16 vectors (NT = 1: x rounded).
+template <int NT>
+__device__ __forceinline__ void split_bf16(floatx8 x, bf16x8 (&out)[NT]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    out[t] = to_bf16x8(x);
+    if (t + 1 < NT) x -= __builtin_convertvector(out[t], floatx8);
+  }
+}
+
+struct Kv4DecodeParams {
+  DecodeParams d;  // kc: the pool; ksb, ksh: page and head strides in bytes
+  int npages;
+};
+
+template <int D, typename T>
+__global__ void __attribute__((amdgpu_flat_work_group_size(DC_THREADS, DC_THREADS), amdgpu_waves_per_eu(KV4_WG_PER_CU)))
+decode_kv4_kernel(Kv4DecodeParams pp) {
+  const DecodeParams& p = pp.d;
+  using F = Kv4<D>;
+  using L = DcTile<D>;
+  using Step = Kv4Step<D>;
+  constexpr int NT = std::is_same<T, float>::value ? 3 : 1;
+  constexpr int NDQ = D / 32, NDO = D / 16;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[DC_WAVES * L::BYTES];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t w = (int64_t)blockIdx.x * DC_WAVES + wave;
+  Walk at;
+  if (!at.start(p, lane, w)) return;
+  const int c16 = lane & 15, grp = lane >> 4;
+  unsigned char* vt = smem + wave * L::BYTES;
+
+  // byte offsets within a step's codes and scales
+  const int kvo = c16 * F::CB + grp * (D / 8), kso = c16 * F::SB + grp * (D / 4) / 32;
+  const int vvo = lane * Step::VB, vso = lane * Step::VB / 16;
+  // V pieces in the LDS tile: row and first 8-element chunk
+  constexpr int LPV = F::CB / Step::VB;  // lanes of a row
+  constexpr int CPP = Step::VB / 4;      // chunks of a piece
+  const int vprow = lane / LPV, vpc = (lane % LPV) * CPP;
+  const int jj = lane & 15;
+  const int vrow = 4 * grp + (jj >> 2);
+  const int voff = vrow * L::RB + ((L::vswz(vrow) >> 1) << 5) + (jj & 3) * 8;
+
+  while (true) {
+    const int b = at.b, ls = at.ls, nb = at.nb;
+    const int len = at.len_of(p, b);
+    const int kvh = at.j / p.NG, hg = at.j % p.NG;
+    const int nseg = (int)min((int64_t)(nb - ls), at.q1 - at.q);
+    const bool whole = ls == 0 && nseg == nb;
+    const int kbeg = ls * DC_STEP;
+    const int kend = min(len, (ls + nseg) * DC_STEP);
+
+    // block-table entries [wbase, wbase + 64) of this row, one per lane
+    int wbase = kbeg / p.page, win = 0;
+    bool lost = false;  // a page that is not in the pool: the row is NaN
+    auto load_window = [&](int first) {
+      const int npg = (kend + p.page - 1) / p.page;
+      wbase = first;
+      win = first + lane < npg ? p.bt[b * p.bts + first + lane] : 0;
+    };
+    load_window(wbase);
+    const unsigned char* heads = reinterpret_cast<const unsigned char*>(p.kc) + kvh * p.ksh;
+    auto load = [&](Step& st, int k0) {
+      const int pg = k0 / p.page;  // a step never crosses a page
+      if (pg - wbase >= 64) load_window(pg);
+      int pid = __builtin_amdgcn_readlane(win, pg - wbase);
+      if ((uint32_t)pid >= (uint32_t)pp.npages) {
+        pid = 0;
+        lost = true;
+      }
+      const int rel = k0 - pg * p.page;
+      const BufRsrc rs = make_rsrc(heads + pid * p.ksb, (uint32_t)(p.page * F::RB));
+      const int kc = rel * F::CB, ks = F::k_scales(p.page) + rel * F::SB;
+      const int vc = F::v_codes(p.page) + rel * F::CB, vs = F::v_scales(p.page) + rel * F::SB;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        kv4_load(st.k[t], rs, kvo, kc + t * 16 * F::CB);
+        st.ks[t] = __builtin_amdgcn_raw_buffer_load_b8(rs, kso, ks + t * 16 * F::SB, 2);
+      }
+#pragma unroll
+      for (int i = 0; i < Step::VL; ++i) {
+        kv4_load(st.v[i], rs, vvo, vc + i * 64 * Step::VB);
+        st.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, vso, vs + i * 4 * Step::VB, 2);
+      }
+    };
+
+    // ---- the query: lane (head c16, slot grp) holds elements grp D/4 + 8 i + j
+    const int gh = hg * 16 + c16;
+    const bool hvalid = gh < p.G;
+    const T* qrow = reinterpret_cast<const T*>(p.q) + b * p.qsb + (kvh * p.G + (hvalid ? gh : 0)) * p.qsh + grp * (D / 4);
+    floatx8 x[NDQ];
+#pragma unroll
+    for (int i = 0; i < NDQ; ++i) x[i] = Vec8<T>::load_f32(qrow + i * 8);
+
+    Step st[KV4_DEPTH];
+#pragma unroll
+    for (int u = 0; u < KV4_DEPTH; ++u)
+      if (u < nseg) load(st[u], kbeg + u * DC_STEP);
+
+    bf16x8 qop[NDQ][NT];
+#pragma unroll
+    for (int i = 0; i < NDQ; ++i) split_bf16<NT>(hvalid ? x[i] : floatx8{}, qop[i]);
+
+    float m_i = -INFINITY, l_i = 0.f;
+    floatx4 oacc[NDO];
+#pragma unroll
+    for (int dd = 0; dd < NDO; ++dd) oacc[dd] = floatx4{};
+
+    auto step = [&](Step& st, int s) {
+      const int k0 = kbeg + s * DC_STEP;
+      const bool part = k0 + DC_STEP > kend;
+      // V to the LDS tile (in-order within the wave: the previous step's reads of the
+      // tile have been served); rows past the last key as zeros, whatever they hold
+#pragma unroll
+      for (int i = 0; i < Step::VL; ++i) {
+        const int row = i * (64 / LPV) + vprow;
+        const bool gone = part && k0 + row >= kend;
+        const float scale = gone ? 1.0f : kv4_scale(st.vs[i]);
+#pragma unroll
+        for (int c = 0; c < CPP; ++c)
+          *reinterpret_cast<bf16x8*>(vt + row * L::RB + (((vpc + c) ^ L::vswz(row)) << 4)) =
+              kv4_bf16x8(gone ? 0u : st.v[i][c], scale);
+      }
+      floatx4 sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sc[t] = floatx4{};
+        const float scale = kv4_scale(st.ks[t]);
+#pragma unroll
+        for (int i = 0; i < NDQ; ++i) {
+          const bf16x8 a = kv4_bf16x8(st.k[t][i], scale);
+#pragma unroll
+          for (int n = NT - 1; n >= 0; --n) sc[t] = mfma16(a, qop[i][n], sc[t]);
+        }
+      }
+      if (s + KV4_DEPTH < nseg) load(st, k0 + KV4_DEPTH * DC_STEP);
+      if (part) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k0 + t * 16 + grp * 4 + i >= kend) sc[t][i] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[t][i]);
+      mx = fmaxf(mx, shfl_xor_f(mx, 16));
+      mx = fmaxf(mx, shfl_xor_f(mx, 32));
+      // without a finite score so far the row keeps m = -inf and exponentiates against 0
+      const float m_new = fmaxf(m_i, mx * p.scale_log2);
+      const float m_use = m_new > -INFINITY ? m_new : 0.f;
+      const float alpha = fast_exp2(m_i - m_use);
+      floatx8 pf;
+      float rs = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float pe = fast_exp2(__builtin_fmaf(sc[t][i], p.scale_log2, -m_use));
+          pf[t * 4 + i] = pe;
+          rs += pe;
+        }
+      bf16x8 pop[NT];
+      split_bf16<NT>(pf, pop);
+      l_i = __builtin_fmaf(l_i, alpha, rs);
+      m_i = m_new;
+#pragma unroll
+      for (int dd = 0; dd < NDO; ++dd) {
+        oacc[dd] *= alpha;
+        const unsigned char* src = vt + (voff ^ (dd << 5));
+        const bf16x8 a = lds_read_tr8(reinterpret_cast<const bf16*>(src),
+                                      reinterpret_cast<const bf16*>(src + 16 * L::RB));
+#pragma unroll
+        for (int n = NT - 1; n >= 0; --n) oacc[dd] = mfma16(a, pop[n], oacc[dd]);
+      }
+    };
+    for (int s = 0; s < nseg; s += KV4_DEPTH)
+#pragma unroll
+      for (int u = 0; u < KV4_DEPTH; ++u)
+        if (s + u < nseg) step(st[u], s + u);
+
+    // ---- flush the segment
+    l_i += shfl_xor_f(l_i, 16);
+    l_i += shfl_xor_f(l_i, 32);
+    if (lost) l_i = __builtin_nanf("");
+    const int64_t r = ((int64_t)b * p.Hkv + kvh) * p.NG + hg;
+    if (lane == 0) {
+      if (ls == 0) p.ws_rw[r * 2] = (int32_t)w;
+      if (ls + nseg == nb) p.ws_rw[r * 2 + 1] = (int32_t)w;
+    }
+    if (hvalid) {
+      if (whole) {
+        const int head = kvh * p.G + gh;
+        T* orow = reinterpret_cast<T*>(p.o) + b * p.osb + (int64_t)head * p.osh;
+        const float inv = 1.0f / l_i;
+#pragma unroll
+        for (int dd = 0; dd < NDO; ++dd) store4<T>(orow + dd * 16 + grp * 4, oacc[dd] * inv);
+        if (p.lse && grp == 0) p.lse[(int64_t)b * p.Hq + head] = row_lse(m_i, l_i);
+      } else {
+        const int64_t slot = w + r;
+        float* so = p.ws_o + (slot * 16 + c16) * D;
+#pragma unroll
+        for (int dd = 0; dd < NDO; ++dd) *reinterpret_cast<floatx4*>(so + dd * 16 + grp * 4) = oacc[dd];
+        if (grp == 0) *reinterpret_cast<floatx2*>(p.ws_ml + (slot * 16 + c16) * 2) = floatx2{m_i, l_i};
+      }
+    }
+    if (!at.next(p, nseg)) break;
+  }
+}
+
+static int64_t kv4_workspace(int B, int Hq, int Hkv, int D) {
+  const int64_t rows = (int64_t)B * Hkv * ((Hq / Hkv + 15) / 16);
+  return (KV4_MAX_WAVES + rows) * 16 * (D + 2) * (int64_t)sizeof(float) + rows * 2 * (int64_t)sizeof(int32_t);
+}
+
+template <int D, typename T>
+static hipError_t launch_decode_kv4(Kv4DecodeParams pp, hipStream_t st) {
+  DecodeParams& p = pp.d;
+  // a persistent grid, worked out once per device and variant
+  static int resident[64];
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  int waves = (dev >= 0 && dev < 64) ? __atomic_load_n(&resident[dev], __ATOMIC_RELAXED) : 0;
+  if (waves == 0) {
+    int cus = 0, per_cu = 0;
+    e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+    if (e == hipSuccess)
+      e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
+          &per_cu, reinterpret_cast<const void*>(decode_kv4_kernel<D, T>), DC_THREADS, 0);
+    if (e != hipSuccess) return e;
+    const int per = per_cu < 1 ? 1 : (per_cu > KV4_WG_PER_CU ? KV4_WG_PER_CU : per_cu);
+    waves = cus * per * DC_WAVES;
+    if (waves > KV4_MAX_WAVES) waves = KV4_MAX_WAVES;
+    if (dev >= 0 && dev < 64) __atomic_store_n(&resident[dev], waves, __ATOMIC_RELAXED);
+  }
+  p.nwaves = waves;
+  hipLaunchKernelGGL((decode_kv4_kernel<D, T>), dim3((unsigned)(waves / DC_WAVES)), dim3(DC_THREADS), 0, st, pp);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = (int64_t)p.B * p.rows_per_batch;
+  const int threads = rows * DC_MERGE_WIDE_PARTIALS <= waves ? DC_MERGE_MAX_THREADS : DC_THREADS;
+  hipLaunchKernelGGL((decode_merge_kernel<D, T>), dim3((unsigned)rows), dim3(threads),
+                     (threads / 16) * (D + 2) * sizeof(float), st, p);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- host checks
+// What every entry over 4-bit pages checks of them.
+static int kv4_check_pages(const void* pool, const int64_t* pool_strides, int num_pages, const int32_t* block_table,
+                           int64_t bt_stride, int bt_cols, int page_size, int Hkv, int D) {
+  if (!head_dim_ok(D)) return nq_fail(NQ_ERR_UNSUPPORTED, "head_dim must be 32, 64 or 128, got %d", D);
+  if (!pool || !pool_strides || !block_table) return nq_fail(NQ_ERR_INVALID, "a pool, its strides and a block table are required");
+  if (page_size <= 0 || page_size % DC_STEP || page_size > (1 << 20))
+    return nq_fail(NQ_ERR_UNSUPPORTED, "page_size must be a multiple of %d up to 2^20, got %d", DC_STEP, page_size);
+  if (num_pages <= 0 || bt_cols <= 0 || bt_stride < bt_cols)
+    return nq_fail(NQ_ERR_INVALID, "num_pages and bt_cols must be positive and rows of the table at least bt_cols apart");
+  const int64_t rec = (int64_t)page_size * 17 * D / 16;
+  if (!nq_aligned16(pool) || pool_strides[0] % 16 || pool_strides[1] % 16)
+    return nq_fail(NQ_ERR_INVALID, "the pool and its strides must be multiples of 16 bytes");
+  if (pool_strides[1] < rec && Hkv > 1) return nq_fail(NQ_ERR_INVALID, "the pool's heads must not overlap");
+  return NQ_OK;
+}
+
+static int kv4_check_strides(const char* name, const void* t, const int64_t* st, int esz) {
+  if (!st) return nq_fail(NQ_ERR_INVALID, "%s needs its strides", name);
+  if (!nq_aligned16(t)) return nq_fail(NQ_ERR_INVALID, "%s must be 16-byte aligned", name);
+  for (int i = 0; i < 3; ++i)
+    if ((st[i] * esz) % 16) return nq_fail(NQ_ERR_INVALID, "%s strides must be multiples of 16 bytes", name);
+  return NQ_OK;
+}
+
+}  // namespace nq
+
+using namespace nq;
+
+extern "C" int nq_kv4_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                             const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+                             void* pool, const int64_t* pool_strides, int num_pages, const int32_t* block_table,
+                             int64_t bt_stride, int bt_cols, int page_size, int B, int S, int Hq, int Hkv, int D,
+                             int dtype, const void* q_weight, const void* k_weight, float eps, const float* cos_tab,
+                             const float* sin_tab, int max_pos, const int32_t* pos, const int32_t* pos_base,
+                             const int32_t* pos_shift, int pos0, const int32_t* row_base, int row0,
+                             int32_t* lens_out, void* stream) {
+  nq_clear_error();
+  Kv4AppendParams p{};
+  const int dt = nq_take_weight_flags(dtype, &p.q16, &p.k16);
+  if (!nq_dtype_ok(dt) || ((p.q16 || p.k16) && dt != NQ_DTYPE_BF16))
+    return nq_fail(NQ_ERR_UNSUPPORTED, "unknown dtype code %d", dtype);
+  if (B <= 0 || S <= 0 || Hkv <= 0 || Hq < 0)
+    return nq_fail(NQ_ERR_INVALID, "sizes must be positive (B=%d S=%d Hkv=%d Hq=%d)", B, S, Hkv, Hq);
+  int rc = kv4_check_pages(pool, pool_strides, num_pages, block_table, bt_stride, bt_cols, page_size, Hkv, D);
+  if (rc != NQ_OK) return rc;
+  if (!k || !v) return nq_fail(NQ_ERR_INVALID, "k and v are required");
+  if ((Hq > 0) != (q != nullptr) || (q != nullptr) != (q_out != nullptr))
+    return nq_fail(NQ_ERR_INVALID, "q, q_out and Hq > 0 go together");
+  const int esz = nq_dtype_size(dt);
+  if ((rc = kv4_check_strides("k", k, k_strides, esz)) || (rc = kv4_check_strides("v", v, v_strides, esz))) return rc;
+  if (q && ((rc = kv4_check_strides("q", q, q_strides, esz)) || (rc = kv4_check_strides("q_out", q_out, q_out_strides, esz))))
+    return rc;
+  if ((cos_tab == nullptr) != (sin_tab == nullptr) || (cos_tab && max_pos <= 0))
+    return nq_fail(NQ_ERR_INVALID, "cos and sin tables go together, with max_pos > 0");
+  if (!nq_aligned16(q_weight) || !nq_aligned16(k_weight) || !nq_aligned16(cos_tab) || !nq_aligned16(sin_tab))
+    return nq_fail(NQ_ERR_INVALID, "norm weights and tables must be 16-byte aligned");
+  if (lens_out && lens_out == row_base) return nq_fail(NQ_ERR_INVALID, "lens_out must not alias row_base");
+  const int64_t rows = (int64_t)B * S * ((int64_t)Hq + 2 * (int64_t)Hkv);
+  if (rows > 0x7fffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more than 2^31 rows in one call");
+  p.k = k; p.ksb = k_strides[0]; p.ksh = k_strides[1]; p.kss = k_strides[2];
+  p.v = v; p.vsb = v_strides[0]; p.vsh = v_strides[1]; p.vss = v_strides[2];
+  if (q) {
+    p.q = q; p.qsb = q_strides[0]; p.qsh = q_strides[1]; p.qss = q_strides[2];
+    p.q_out = q_out; p.osb = q_out_strides[0]; p.osh = q_out_strides[1]; p.oss = q_out_strides[2];
+  }
+  p.pool = reinterpret_cast<unsigned char*>(pool); p.psb = pool_strides[0]; p.psh = pool_strides[1];
+  p.npages = num_pages; p.bt = block_table; p.bts = bt_stride; p.page = page_size;
+  p.cap = (int64_t)bt_cols * page_size;
+  if (p.cap > 0x7fffffff) p.cap = 0x7fffffff;
+  p.B = B; p.S = S; p.Hq = Hq; p.Hkv = Hkv; p.qw = q_weight; p.kw = k_weight; p.eps = eps;
+  p.cos_tab = cos_tab; p.sin_tab = sin_tab; p.max_pos = max_pos;
+  p.pos = pos; p.pos_base = pos_base; p.pos_shift = pos_shift; p.pos0 = pos0;
+  p.row_base = row_base; p.row0 = row0; p.lens_out = lens_out;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  return nq_check_launch(with_head_dim(D, [&](auto dc) {
+    constexpr int DD = decltype(dc)::value;
+    const int64_t blocks = (rows * (DD / 16) + 255) / 256;
+    if (dt == NQ_DTYPE_BF16)
+      hipLaunchKernelGGL((kv4_append_kernel<DD, bf16>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((kv4_append_kernel<DD, float>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    return hipGetLastError();
+  }));
+}
+
+extern "C" int nq_kv4_gather(const void* pool, const int64_t* pool_strides, int num_pages, const int32_t* block_table,
+                             int64_t bt_stride, int bt_cols, int page_size, void* k, const int64_t* k_strides,
+                             void* v, const int64_t* v_strides, int B, int S, int Hkv, int D, int dtype,
+                             const int32_t* row_base, int row0, void* stream) {
+  nq_clear_error();
+  if (!nq_dtype_ok(dtype)) return nq_fail(NQ_ERR_UNSUPPORTED, "unknown dtype code %d", dtype);
+  if (B <= 0 || S <= 0 || Hkv <= 0)
+    return nq_fail(NQ_ERR_INVALID, "sizes must be positive (B=%d S=%d Hkv=%d)", B, S, Hkv);
+  int rc = kv4_check_pages(pool, pool_strides, num_pages, block_table, bt_stride, bt_cols, page_size, Hkv, D);
+  if (rc != NQ_OK) return rc;
+  if (!k || !v) return nq_fail(NQ_ERR_INVALID, "k and v are required");
+  const int esz = nq_dtype_size(dtype);
+  if ((rc = kv4_check_strides("k", k, k_strides, esz)) || (rc = kv4_check_strides("v", v, v_strides, esz))) return rc;
+  const int64_t rows = (int64_t)B * S * Hkv;
+  if (rows > 0x7fffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more than 2^31 rows in one call");
+  Kv4GatherParams p{};
+  p.pool = reinterpret_cast<const unsigned char*>(pool); p.psb = pool_strides[0]; p.psh = pool_strides[1];
+  p.npages = num_pages; p.bt = block_table; p.bts = bt_stride; p.page = page_size;
+  p.cap = (int64_t)bt_cols * page_size;
+  if (p.cap > 0x7fffffff) p.cap = 0x7fffffff;
+  p.k = k; p.ksb = k_strides[0]; p.ksh = k_strides[1]; p.kss = k_strides[2];
+  p.v = v; p.vsb = v_strides[0]; p.vsh = v_strides[1]; p.vss = v_strides[2];
+  p.B = B; p.S = S; p.Hkv = Hkv; p.row_base = row_base; p.row0 = row0;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  return nq_check_launch(with_head_dim(D, [&](auto dc) {
+    constexpr int DD = decltype(dc)::value;
+    const dim3 grid((unsigned)((rows * (DD / 16) + 255) / 256), 2);
+    if (dtype == NQ_DTYPE_BF16)
+      hipLaunchKernelGGL((kv4_gather_kernel<DD, bf16>), grid, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((kv4_gather_kernel<DD, float>), grid, dim3(256), 0, st, p);
+    return hipGetLastError();
+  }));
+}
+
+extern "C" int64_t nq_attn_decode_kv4_workspace_bytes(int B, int Hq, int Hkv, int D) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv) return 0;
+  return kv4_workspace(B, Hq, Hkv, D);
+}
+
+extern "C" int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const void* pool,
+                                  const int64_t* pool_strides, int num_pages, const int32_t* block_table,
+                                  int64_t bt_stride, int bt_cols, int page_size, const int32_t* lens, void* o,
+                                  const int64_t* o_strides, float* lse, void* workspace, int64_t workspace_bytes,
+                                  int B, int Hq, int Hkv, int D, int max_len, int dtype, float sm_scale,
+                                  void* stream) {
+  nq_clear_error();
+  if (!nq_dtype_ok(dtype)) return nq_fail(NQ_ERR_UNSUPPORTED, "unknown dtype code %d", dtype);
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || max_len <= 0)
+    return nq_fail(NQ_ERR_INVALID, "sizes must be positive (B=%d Hq=%d Hkv=%d max_len=%d)", B, Hq, Hkv, max_len);
+  if (Hq % Hkv) return nq_fail(NQ_ERR_INVALID, "num_heads %d not divisible by num_kv_heads %d", Hq, Hkv);
+  int rc = kv4_check_pages(pool, pool_strides, num_pages, block_table, bt_stride, bt_cols, page_size, Hkv, D);
+  if (rc != NQ_OK) return rc;
+  if (!q || !o || !q_strides || !o_strides || !lens)
+    return nq_fail(NQ_ERR_INVALID, "q, o, their strides and lens are required");
+  if (!nq_aligned16(q) || !nq_aligned16(o)) return nq_fail(NQ_ERR_INVALID, "q and o must be 16-byte aligned");
+  const int esz = nq_dtype_size(dtype);
+  for (int i = 0; i < 2; ++i)
+    if ((q_strides[i] * esz) % 16 || (o_strides[i] * esz) % 16)
+      return nq_fail(NQ_ERR_INVALID, "q and o strides must be multiples of 16 bytes");
+  if ((max_len + page_size - 1) / page_size > bt_cols)
+    return nq_fail(NQ_ERR_INVALID, "the block table's %d columns hold fewer than max_len %d rows", bt_cols, max_len);
+  const int NG = (Hq / Hkv + 15) / 16;
+  if ((int64_t)B * Hkv * NG > 0x3fffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more than 2^30 (sequence, kv head) rows");
+  const int64_t need = kv4_workspace(B, Hq, Hkv, D);
+  if (!workspace || workspace_bytes < need || !nq_aligned16(workspace))
+    return nq_fail(NQ_ERR_WORKSPACE, "an aligned workspace of %lld bytes is required, %lld given", (long long)need,
+                   (long long)workspace_bytes);
+  Kv4DecodeParams pp{};
+  DecodeParams& p = pp.d;
+  p.q = q; p.qsb = q_strides[0]; p.qsh = q_strides[1];
+  p.kc = const_cast<void*>(pool); p.ksb = pool_strides[0]; p.ksh = pool_strides[1];
+  p.lens = lens; p.o = o; p.osb = o_strides[0]; p.osh = o_strides[1]; p.lse = lse;
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.NG = NG; p.max_len = max_len;
+  p.rows_per_batch = Hkv * NG;
+  while ((1 << p.hs) < (p.G < 16 ? p.G : 16)) ++p.hs;
+  const int64_t slots = KV4_MAX_WAVES + (int64_t)B * p.rows_per_batch;
+  p.ws_o = reinterpret_cast<float*>(workspace);
+  p.ws_ml = p.ws_o + slots * 16 * D;
+  p.ws_rw = reinterpret_cast<int32_t*>(p.ws_ml + slots * 16 * 2);
+  p.scale_log2 = (sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)D)) * kLog2e;
+  p.bt = block_table; p.bts = bt_stride; p.page = page_size;
+  pp.npages = num_pages;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  return nq_check_launch(with_head_dim(D, [&](auto dc) {
+    return dtype == NQ_DTYPE_BF16 ? launch_decode_kv4<decltype(dc)::value, bf16>(pp, st)
+                                  : launch_decode_kv4<decltype(dc)::value, float>(pp, st);
+  }));
+}

@@ -1,0 +1,418 @@
+"""Paged KV caches held in 4 bits, and eviction from paged caches by attention weight.
+
+``kv4_append`` stores rows in 4-bit pages, ``kv4_gather`` reads them back,
+``attention_decode_kv4`` attends them: 17/64 of a bf16 cache's bytes, which is what a
+decode step reads.  ``attention_key_weights`` gives the attention weight that each cached
+key got, ``select_keys`` the keys worth keeping, ``kv_compact`` moves them to other pages;
+these take 4-bit and plain pages.  ``PagedKVCache4`` and ``PagedKVCache.evict`` are made
+of them.
+
+A row is held in blocks of 32 elements: codes {0, 1/2, 1, 3/2, 2, 3, 4, 6} with a sign (E2M1)
+and a power of two per block (E8M0), 4.25 bits an element.  A pool is uint8 (num_pages, Hkv,
+page_size, 17 D / 16); its last two axes hold a page's K codes, V codes, K scales and V
+scales one after the other, not row by row.
+
+The calls take no part in autograd and refuse tensors that do.  They allocate through torch
+and record no memset, so they may be captured in graphs.  Host tensors raise: there is no
+CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _lib, ops
+
+__all__ = ["kv4_empty_pool", "kv4_append", "kv4_gather", "attention_decode_kv4",
+           "attention_key_weights", "select_keys", "kv_compact"]
+
+_HEAD_DIMS = {17 * d // 16: d for d in (32, 64, 128)}  # bytes of a row -> head_dim
+_MOST = 2 ** 31 - 1  # the C entries' int, to which ctypes cuts a larger number without a word
+
+
+class _DeviceCall(ops.KernelCall):
+    """A KernelCall that launches on its tensors' device, whichever is current."""
+
+    __slots__ = ("device",)
+
+    def __init__(self, t, fn, args, name, keep, result):
+        super().__init__(fn, (*args, ops._stream(t)), len(args), name, keep, result)
+        self.device = t.get_device()
+
+    def launch(self, stream: Optional[torch.cuda.Stream] = None):
+        if self.device == torch._C._cuda_getDevice():
+            return super().launch(stream)
+        with torch.cuda.device(self.device):
+            return super().launch(stream)
+
+
+def _check(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """Device tensors of one device that want no gradient."""
+    index = first.get_device()
+    for t in (first, *others):
+        if t is None:
+            continue
+        if t.get_device() != index or not t.is_cuda:
+            ops._require_device(first, t)
+            raise ValueError(f"{name}: the operands lie on different devices: {first.device} and {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or give it detached tensors")
+
+
+def _pool4(pool: torch.Tensor) -> Tuple[int, int, int, int]:
+    """(pages, Hkv, page_size, head_dim) of a 4-bit pool."""
+    if pool.dtype != torch.uint8 or pool.dim() != 4 or pool.shape[3] not in _HEAD_DIMS:
+        raise ValueError("a 4-bit pool is uint8 (pages, Hkv, page_size, 17 D / 16) with D 32, 64 or 128, "
+                         f"got {pool.dtype} {tuple(pool.shape)}")
+    n, H, P, row = pool.shape
+    if P <= 0 or P % 32:
+        raise ValueError(f"page_size must be a positive multiple of 32, got {P}")
+    if pool.stride(3) != 1 or pool.stride(2) != row or pool.stride(0) % 16 or pool.stride(1) % 16 or pool.data_ptr() % 16:
+        raise ValueError("a page's head must be contiguous and all of them 16-byte aligned")
+    return n, H, P, _HEAD_DIMS[row]
+
+
+def _strides2(t: torch.Tensor, scale: int = 1):
+    return (ctypes.c_int64 * 2)(t.stride(0) * scale, t.stride(1) * scale)
+
+
+def _lens(lens: torch.Tensor, B: int, dev, name: str = "lens") -> torch.Tensor:
+    lens = ops._i32(lens, dev)
+    if lens.numel() != B:
+        raise ValueError(f"{name} must hold one number per sequence ({B}), got shape {tuple(lens.shape)}")
+    return lens
+
+
+def _sizes(name: str, *sizes: int) -> None:
+    n = 1
+    for s in sizes:
+        n *= s
+    if n > _MOST:
+        raise ValueError(f"{name}: more than 2^31 - 1 rows in one call")
+
+
+def kv4_empty_pool(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """An uninitialised 4-bit pool (num_pages, num_kv_heads, page_size, 17 head_dim / 16)."""
+    if 17 * head_dim // 16 not in _HEAD_DIMS or head_dim % 32:
+        raise ValueError(f"head_dim must be 32, 64 or 128, got {head_dim}")
+    pool = torch.empty(num_pages, num_kv_heads, page_size, 17 * head_dim // 16, dtype=torch.uint8, device=device)
+    _pool4(pool)
+    return pool
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, *,
+               q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+               q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+               eps: float = 1e-6, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+               position_ids: Optional[torch.Tensor] = None, pos_offset: int = 0,
+               pos_base: Optional[torch.Tensor] = None, pos_shift: Optional[torch.Tensor] = None,
+               row_offset: int = 0, row_base: Optional[torch.Tensor] = None,
+               lens_out: Optional[torch.Tensor] = None, plan: bool = False):
+    """Store K (QK-Norm + RoPE of k) and V rows in 4-bit pages; q's rows in the same launch.
+
+    k/v: (B, Hkv, S, D) bf16 or fp32, any (b, h, s) strides.  Token s of sequence b is row
+    ``row_base[b] + s`` (else ``row_offset + s``).  k_weight None skips the norm, cos/sin
+    None the rotation.  Positions: ``position_ids``, else ``pos_base[b] + s``, else
+    ``pos_offset + s``, plus ``pos_shift[b]`` where given (rows evicted so far).  q: (B, Hq,
+    S, D), normed with q_weight and rotated alike into ``q_out`` (by default fresh), the
+    operand of ``attention_decode_kv4``.  ``lens_out`` (int32 (B,), not ``row_base``)
+    receives ``row_base[b] + S``.  Everything up to the codes is fp32: a row is rounded once.
+
+    A sequence whose rows lie outside its table's pages stores nothing and keeps its length
+    in ``lens_out``; rows whose page is not one of the pool's are not stored.
+    Returns q_out (None without q), or with ``plan=True`` a KernelCall.
+    """
+    _check("kv4_append", k, v, pool, block_table, q, q_out, pos_base, pos_shift, row_base, lens_out)
+    n, H, P, D = _pool4(pool)
+    if k.dim() != 4 or k.shape != v.shape or k.shape[1] != H or k.shape[3] != D:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be (B, {H}, S, {D}), as the pool")
+    if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+        raise TypeError("k, v and q must share one dtype")
+    dt = ops._code(k)
+    B, _, S, _ = k.shape
+    if q is None and (q_out is not None or q_weight is not None):
+        raise ValueError("q_out and q_weight go with q")
+    if q is not None:
+        if q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, S, D):
+            raise ValueError(f"q must be (B={B}, Hq, S={S}, D={D}), got {tuple(q.shape)}")
+        if q_out is None:
+            q_out = torch.empty(B, S, q.shape[1], D, dtype=q.dtype, device=q.device).transpose(1, 2)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise ValueError("q_out must match q in shape and dtype")
+        ops._rows_out(q_out, "q_out")
+        q = ops._rows_in(q)
+    dev = k.device
+    bt = ops._block_table(block_table, B, dev)
+    if row_base is None and not 0 <= row_offset <= bt.shape[1] * P - S:
+        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {bt.shape[1] * P}")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    if lens_out is not None:
+        if row_base is None:
+            raise ValueError("lens_out goes with row_base")
+        if lens_out.dtype != torch.int32 or not lens_out.is_contiguous() or lens_out.numel() != B:
+            raise ValueError("lens_out must be a contiguous int32 tensor of B elements")
+        if lens_out.data_ptr() == row_base.data_ptr() and B:
+            raise ValueError("lens_out must not alias row_base")
+    k, v = ops._rows_in(k), ops._rows_in(v)
+    cos_t, sin_t, max_pos = ops._tables(cos, sin, dev)
+    if cos_t is not None and cos_t.shape[1] != D // 2:
+        raise ValueError(f"the tables must be (max_pos, {D // 2}), got {tuple(cos_t.shape)}")
+    for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None and w.numel() != D:
+            raise ValueError(f"{what} must hold {D} elements, got {tuple(w.shape)}")
+    pos = None
+    if cos_t is not None:
+        if pos_shift is None:
+            pos = ops._positions(position_ids, pos_offset, pos_base, B, S, max_pos, dev)
+        elif position_ids is not None:
+            pos = ops._i32(position_ids, dev).expand(B, S).contiguous()
+    if B == 0 or S == 0:
+        return q_out
+    Hq = 0 if q is None else q.shape[1]
+    _sizes("kv4_append", B, S, Hq + 2 * H)
+    pb = None if pos_base is None else _lens(pos_base, B, dev, "pos_base")
+    ps = None if pos_shift is None else _lens(pos_shift, B, dev, "pos_shift")
+    rb = None if row_base is None else _lens(row_base, B, dev, "row_base")
+    qw, qf = ops._norm_weight(q_weight, dev, dt, _lib.NQ_QWEIGHT_BF16, plan)
+    kw, kf = ops._norm_weight(k_weight, dev, dt, _lib.NQ_KWEIGHT_BF16, plan)
+    st, ptr = _lib.strides3, ops._ptr
+    args = (ptr(k), st(k.stride()[:3]), ptr(v), st(v.stride()[:3]),
+            ptr(q), None if q is None else st(q.stride()[:3]),
+            ptr(q_out), None if q is None else st(q_out.stride()[:3]),
+            ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, B, S, Hq, H, D, dt | qf | kf,
+            ptr(qw), ptr(kw), float(eps), ptr(cos_t), ptr(sin_t), max_pos, ptr(pos), ptr(pb), ptr(ps),
+            int(pos_offset), ptr(rb), int(row_offset), ptr(lens_out))
+    call = _DeviceCall(k, _lib.load().nq_kv4_append, args, "nq_kv4_append",
+                       (k, v, q, pool, bt, qw, kw, cos_t, sin_t, pos, pb, ps, rb, lens_out), q_out)
+    return call if plan else call.launch()
+
+
+def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_offset: int = 0,
+               row_base: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
+               k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None, plan: bool = False):
+    """Rows ``row_base[b] + s`` (else ``row_offset + s``), s < S, of 4-bit pages as (k, v).
+
+    (B, Hkv, S, D) in ``dtype`` (bf16 or fp32, exact in both), by default fresh; ``k_out`` and
+    ``v_out`` may be views of larger buffers.  Rows without a page come back as NaN.
+    """
+    _check("kv4_gather", pool, block_table, row_base, k_out, v_out)
+    n, H, P, D = _pool4(pool)
+    B, dev = block_table.shape[0], pool.device
+    bt = ops._block_table(block_table, B, dev)
+    if S < 0 or (row_base is None and not 0 <= row_offset <= bt.shape[1] * P - S):
+        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {bt.shape[1] * P}")
+    shape = (B, H, S, D)
+    outs = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is None:
+            t = torch.empty(shape, dtype=dtype, device=dev)
+        elif tuple(t.shape) != shape or t.dtype != dtype:
+            raise ValueError(f"{name} must be {shape} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
+        outs.append(ops._rows_out(t, name))
+    k, v = outs
+    code = ops._code(k)
+    if 0 in shape:
+        return k, v
+    _sizes("kv4_gather", B, S, H)
+    rb = None if row_base is None else _lens(row_base, B, dev, "row_base")
+    st, ptr = _lib.strides3, ops._ptr
+    args = (ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, ptr(k), st(k.stride()[:3]),
+            ptr(v), st(v.stride()[:3]), B, S, H, D, code, ptr(rb), int(row_offset))
+    call = _DeviceCall(pool, _lib.load().nq_kv4_gather, args, "nq_kv4_gather", (pool, bt, rb), (k, v))
+    return call if plan else call.launch()
+
+
+def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
+                         max_len: int, sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                         return_lse: bool = False, workspace: Optional[torch.Tensor] = None, plan: bool = False):
+    """Single-token GQA attention over keys [0, lens[b]) of 4-bit pages.
+
+    q: (B, Hq, D) or (B, Hq, 1, D) bf16 or fp32, normed and rotated (``kv4_append``'s q_out).
+    ``max_len`` bounds the lengths; the block table must map every page up to it.  Returns
+    (B, Hq, D) in q's type, with ``return_lse`` also the fp32 (B, Hq) log-sum-exp of the
+    scaled scores.  A sequence without keys gives zeros and -inf, one whose length lies
+    outside [0, max_len], or whose pages are not the pool's, NaN.  Products are exact in the
+    stored values; bf16 q rounds the probabilities to bf16, fp32 q keeps 24 bits of both.
+    """
+    _check("attention_decode_kv4", q, pool, block_table, lens, out, workspace)
+    n, H, P, D = _pool4(pool)
+    if q.dim() == 4 and q.shape[2] == 1:
+        q = q[:, :, 0]
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % H:
+        raise ValueError(f"q must be (B, Hq, {D}) with Hq a multiple of the pool's {H} heads, got {tuple(q.shape)}")
+    B, Hq, _ = q.shape
+    dt, dev = ops._code(q), q.device
+    bt = ops._block_table(block_table, B, dev)
+    if not 0 < max_len <= bt.shape[1] * P:
+        raise ValueError(f"max_len must be in [1, {bt.shape[1] * P}] (block table columns x page_size), got {max_len}")
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=q.dtype, device=dev)
+    elif tuple(out.shape) != (B, Hq, D) or out.dtype != q.dtype:
+        raise ValueError(f"out must be {(B, Hq, D)} in {q.dtype}")
+    ops._rows_out(out, "out")
+    lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
+    if B == 0:
+        return (out, lse) if return_lse else out
+    _sizes("attention_decode_kv4", B, H, -(-Hq // H // 16) + 1)
+    lens_t = _lens(lens, B, dev)
+    q = ops._rows_in(q)
+    lib = _lib.load()
+    need = lib.nq_attn_decode_kv4_workspace_bytes(B, Hq, H, D)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    ptr = ops._ptr
+    args = (ptr(q), _strides2(q), ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, ptr(lens_t),
+            ptr(out), _strides2(out), ptr(lse), ptr(workspace), workspace.numel() * workspace.element_size(),
+            B, Hq, H, D, int(max_len), dt, 0.0 if sm_scale is None else float(sm_scale))
+    call = _DeviceCall(q, lib.nq_attn_decode_kv4, args, "nq_attn_decode_kv4", (q, pool, bt, lens_t, workspace),
+                       (out, lse) if return_lse else out)
+    return call if plan else call.launch()
+
+
+def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                          lse: torch.Tensor, *, max_len: int, weights: Optional[torch.Tensor] = None,
+                          causal: bool = True, sm_scale: Optional[float] = None, plan: bool = False):
+    """The attention weight that each cached key got, (B, Hkv, max_len) fp32.
+
+    Key t of sequence b and kv head h: the sum of ``exp(scale q . k_t - lse)`` over the query
+    heads of h and the queries that see t.  q: (B, Hq, S, D) bf16 as attended (normed and
+    rotated), the last S of the sequence's ``lens[b]`` tokens, ``causal`` or all seeing all;
+    lse: the (B, Hq, S) (or, S = 1, (B, Hq)) fp32 log-sum-exp their attention returned
+    (-inf: the query saw nothing).  k_pool: 4-bit pages or bf16 K pages (pages, Hkv,
+    page_size, D).  Keys from lens[b] on get 0.  With ``weights`` the sums are added to its
+    first max_len entries a head and it is returned.
+    """
+    _check("attention_key_weights", q, k_pool, block_table, lens, lse, weights)
+    four = k_pool.dtype == torch.uint8
+    if four:
+        n, H, P, D = _pool4(k_pool)
+    else:
+        ops._pool_check(k_pool, "k_pool")
+        n, H, P, D = k_pool.shape
+        if k_pool.dtype != torch.bfloat16:
+            raise TypeError(f"k_pool must be bfloat16 or a 4-bit pool, got {k_pool.dtype}")
+        if P <= 0 or P % 32:
+            raise ValueError(f"page_size must be a positive multiple of 32, got {P}")
+    if q.dtype != torch.bfloat16:
+        raise TypeError(f"q must be bfloat16, got {q.dtype}")
+    if q.dim() != 4 or q.shape[3] != D or q.shape[1] == 0 or q.shape[1] % H:
+        raise ValueError(f"q must be (B, Hq, S, {D}) with Hq a multiple of the pool's {H} heads, got {tuple(q.shape)}")
+    B, Hq, S, _ = q.shape
+    if lse.dtype != torch.float32 or lse.numel() != B * Hq * S or tuple(lse.shape) not in ((B, Hq, S), (B, Hq)):
+        raise ValueError(f"lse must be fp32 {(B, Hq, S)}, got {lse.dtype} {tuple(lse.shape)}")
+    dev = q.device
+    bt = ops._block_table(block_table, B, dev)
+    if not 0 < max_len <= bt.shape[1] * P:
+        raise ValueError(f"max_len must be in [1, {bt.shape[1] * P}] (block table columns x page_size), got {max_len}")
+    add = weights is not None
+    if not add:
+        weights = torch.empty(B, H, max_len, dtype=torch.float32, device=dev)
+    else:
+        _check_weights(weights, B, H, max_len)
+    if B == 0 or S == 0:
+        return weights if add else weights.zero_()
+    _sizes("attention_key_weights", B, Hq, S)
+    lens_t = _lens(lens, B, dev)
+    q, lse = ops._rows_in(q), lse.contiguous()
+    ptr = ops._ptr
+    args = (ptr(q), _lib.strides3(q.stride()[:3]), ptr(k_pool), _lib.strides3(k_pool.stride()[:3]), int(four), n,
+            ptr(bt), bt.stride(0), bt.shape[1], P, ptr(lens_t), ptr(lse), ptr(weights), _strides2(weights), int(add),
+            B, Hq, H, S, D, int(max_len), int(bool(causal)), 0.0 if sm_scale is None else float(sm_scale))
+    call = _DeviceCall(q, _lib.load().nq_key_weights, args, "nq_key_weights", (q, k_pool, bt, lens_t, lse), weights)
+    return call if plan else call.launch()
+
+
+def _check_weights(weights: torch.Tensor, B: int, H: int, least: int) -> None:
+    if (weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, H)
+            or weights.shape[2] < least or (weights.shape[2] > 1 and weights.stride(2) != 1)):
+        raise ValueError(f"weights must be fp32 ({B}, {H}, at least {least}) with contiguous keys, "
+                         f"got {weights.dtype} {tuple(weights.shape)}")
+
+
+def select_keys(weights: torch.Tensor, lens: torch.Tensor, *, keep: int, recent: int = 0, first: int = 0,
+                plan: bool = False):
+    """The cached rows that each kv head keeps, int32 (B, Hkv, keep) in ascending order.
+
+    weights: (B, Hkv, W) fp32; lens: the sequences' lengths, at most W.  Kept are the first
+    ``first`` rows, the last ``recent`` and, of those in between, the heaviest; equal weights
+    by the lower index, NaN above every number.  A sequence of no more than ``keep`` rows keeps
+    them all, with -1 behind them.
+    """
+    _check("select_keys", weights, lens)
+    if weights.dim() != 3:
+        raise ValueError(f"weights must be (B, Hkv, W), got {tuple(weights.shape)}")
+    B, H, W = weights.shape
+    _check_weights(weights, B, H, 1)
+    if keep <= 0 or recent < 0 or first < 0 or recent + first > keep or keep > _MOST:
+        raise ValueError(f"keep must be positive and hold first + recent, got {keep}, {first} and {recent}")
+    lens_t = _lens(lens, B, weights.device)
+    kept = torch.empty(B, H, keep, dtype=torch.int32, device=weights.device)
+    if B == 0 or H == 0:
+        return kept
+    _sizes("select_keys", B, H)
+    _sizes("select_keys", W)
+    args = (ops._ptr(weights), _strides2(weights), ops._ptr(lens_t), ops._ptr(kept), B, H, W, int(keep), int(recent),
+            int(first))
+    call = _DeviceCall(weights, _lib.load().nq_select_keys, args, "nq_select_keys", (weights, lens_t), kept)
+    return call if plan else call.launch()
+
+
+def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], block_table: torch.Tensor,
+               new_table: torch.Tensor, kept: torch.Tensor, *, weights: Optional[torch.Tensor] = None,
+               plan: bool = False):
+    """Move row ``kept[b, h, i]`` of each sequence to row i of its new pages, in the same pool.
+
+    pools: a 4-bit pool, or (k_pool, v_pool) of bf16 or fp32 pages.  ``new_table`` must name
+    pages that no row of ``block_table`` does (what they hold is overwritten while the old
+    pages are read).  ``kept`` as ``select_keys`` gives it; -1 moves nothing, and rows of the
+    new pages behind the last one moved are left as they are.  With ``weights`` (B, Hkv, W >=
+    keep) returns a fresh tensor of that shape with the kept rows' weights and 0 behind them,
+    else None.
+    """
+    four = isinstance(pools, torch.Tensor)
+    k_pool, v_pool = (pools, None) if four else pools
+    _check("kv_compact", k_pool, v_pool, block_table, new_table, kept, weights)
+    if four:
+        n, H, P, D = _pool4(k_pool)
+        ks, vs, row = _strides2(k_pool), None, 0
+    else:
+        for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
+            ops._pool_check(pool, name)
+            ops._code(pool)
+        if k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
+            raise ValueError(f"the pools differ: {tuple(k_pool.shape)} {k_pool.dtype} and {tuple(v_pool.shape)} {v_pool.dtype}")
+        n, H, P, D = k_pool.shape
+        if P <= 0 or P % 32:
+            raise ValueError(f"page_size must be a positive multiple of 32, got {P}")
+        e = k_pool.element_size()
+        ks, vs = (_lib.strides3([x * e for x in t.stride()[:3]]) for t in (k_pool, v_pool))
+        row = D * e
+    if kept.dtype != torch.int32 or kept.dim() != 3 or kept.shape[1] != H:
+        raise ValueError(f"kept must be int32 (B, {H}, keep), got {kept.dtype} {tuple(kept.shape)}")
+    B, _, keep = kept.shape
+    dev = k_pool.device
+    bt, new = ops._block_table(block_table, B, dev), ops._block_table(new_table, B, dev)
+    if new.shape[1] * P < keep:
+        raise ValueError(f"the new table maps {new.shape[1] * P} rows, {keep} are kept")
+    if B and new.data_ptr() == bt.data_ptr():
+        raise ValueError("new_table must name other pages than block_table")
+    out = None
+    if weights is not None:
+        _check_weights(weights, B, H, keep)
+        out = torch.empty_like(weights, memory_format=torch.contiguous_format)
+        if weights.stride() != out.stride():
+            weights = weights.contiguous()
+    if 0 in kept.shape:
+        return out if out is None or out.numel() == 0 else out.zero_()
+    _sizes("kv_compact", B, H, keep)
+    ptr, kept = ops._ptr, kept.contiguous()
+    args = (ptr(k_pool), ks, ptr(v_pool), vs, row, D, n, ptr(bt), bt.stride(0), bt.shape[1], ptr(new), new.stride(0),
+            new.shape[1], P, ptr(kept), ptr(weights), ptr(out), None if out is None else _strides2(out),
+            0 if out is None else out.shape[2], B, H, keep)
+    call = _DeviceCall(k_pool, _lib.load().nq_kv_compact, args, "nq_kv_compact",
+                       (k_pool, v_pool, bt, new, kept, weights), out)
+    return call if plan else call.launch()

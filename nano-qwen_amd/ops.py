@@ -715,7 +715,7 @@ def attention_decode_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
                            q_pos: Optional[torch.Tensor] = None, q_pos0: int = -1,
                            sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                            workspace: Optional[torch.Tensor] = None, chunk: int = 0,
-                           plan: bool = False):
+                           return_lse: bool = False, plan: bool = False):
     """Single-token GQA decode against a paged cache, with an optional fused append.
 
     q: (B, Hq, D) or (B, Hq, 1, D) pre-norm query; k_pool/v_pool:
@@ -731,7 +731,8 @@ def attention_decode_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     lens[b] and attended together with keys [0, lens[b]); ``lens_out`` (not
     aliasing lens) then receives lens + 1.  ``max_len`` bounds the keys
     attended per sequence (the appended one included); the block table must
-    map every page up to it.  Returns (B, Hq, D).
+    map every page up to it.  Returns (B, Hq, D), with ``return_lse`` also the
+    fp32 (B, Hq) log-sum-exp of the scaled scores.
     """
     _require_device(q, k_pool, v_pool, block_table, lens, k_new, v_new, lens_out, out)
     if q.dim() == 4:
@@ -789,11 +790,17 @@ def attention_decode_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         _ptr(out), o_str, _ptr(workspace), wbytes,
         B, Hq, Hkv, D, int(max_len), int(chunk), dt, _ptr(qw), float(eps),
         _ptr(cos_t), _ptr(sin_t), max_pos, _ptr(qp), int(q_pos0),
-        float(sm_scale) if sm_scale is not None else 0.0, _stream(q))
-    call = KernelCall(_lib.load().nq_attn_decode_paged_fwd, args, len(args) - 1,
-                      "nq_attn_decode_paged_fwd",
-                      (q, k_new, v_new, bt, lens_t, workspace, cos_t, sin_t, qp, qw, kw,
-                       q_str, o_str, kn_str, vn_str), out)
+        float(sm_scale) if sm_scale is not None else 0.0)
+    keep = (q, k_new, v_new, bt, lens_t, workspace, cos_t, sin_t, qp, qw, kw, q_str, o_str, kn_str, vn_str)
+    if return_lse:
+        lse = torch.empty(B, Hq, dtype=torch.float32, device=dev)
+        args += (_ptr(lse), _stream(q))
+        call = KernelCall(_lib.load().nq_attn_decode_paged_lse_fwd, args, len(args) - 1,
+                          "nq_attn_decode_paged_lse_fwd", keep, (out, lse))
+    else:
+        args += (_stream(q),)
+        call = KernelCall(_lib.load().nq_attn_decode_paged_fwd, args, len(args) - 1,
+                          "nq_attn_decode_paged_fwd", keep, out)
     return call if plan else call.launch()
 
 
