@@ -456,7 +456,7 @@ decode_stream_f32_kernel(DecodeParams p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t w = (int64_t)blockIdx.x * DC_WAVES + wave;
-  Walk at;
+  Walk<> at;
   if (!at.start(p, lane, w)) return;
   const int c16 = lane & 15, grp = lane >> 4, sub = lane % LPR;
   const int krow = (int)(c16 * p.kst * 4) + grp * 16, vrow = (int)(grp * 4 * p.vst * 4) + c16 * VW * 4;

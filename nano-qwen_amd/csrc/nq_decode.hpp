@@ -94,9 +94,12 @@ __device__ __forceinline__ int batch_len(const DecodeParams& p, int b) {
   const int l = p.lens[b];
   return (l < 0 || l > p.max_len - p.append) ? -1 : l + p.append;
 }
+// Steps of each of its rows.  COST: what the start of a row counts for in the split, in
+// steps; those come first, and hold no keys.
+template <int COST = 0>
 __device__ __forceinline__ int batch_steps(const DecodeParams& p, int b) {
   const int len = batch_len(p, b);
-  return len > 0 ? (len + DC_STEP - 1) / DC_STEP : 0;
+  return len > 0 ? (len + DC_STEP - 1) / DC_STEP + COST : 0;
 }
 __device__ __forceinline__ int64_t wave_sum_i64(int64_t v) {
 #pragma unroll
@@ -110,21 +113,23 @@ __device__ __forceinline__ int64_t lane_value_i64(int64_t v, int src) {
 }
 
 // Total number of steps N over all rows (same value in every lane).
+template <int COST = 0>
 __device__ inline int64_t total_steps(const DecodeParams& p, int lane) {
   int64_t acc = 0;
   for (int base = 0; base < p.B; base += 64) {
     const int b = base + lane;
-    if (b < p.B) acc += batch_steps(p, b);
+    if (b < p.B) acc += batch_steps<COST>(p, b);
   }
   return wave_sum_i64(acc) * p.rows_per_batch;
 }
 
 // The batch whose rows hold global step q (q < N), and the steps before it.
+template <int COST = 0>
 __device__ inline void find_batch(const DecodeParams& p, int lane, int64_t q, int& b_out, int64_t& before) {
   int64_t run = 0;
   for (int base = 0; base < p.B; base += 64) {
     const int b = base + lane;
-    const int64_t v = b < p.B ? (int64_t)batch_steps(p, b) * p.rows_per_batch : 0;
+    const int64_t v = b < p.B ? (int64_t)batch_steps<COST>(p, b) * p.rows_per_batch : 0;
     int64_t incl = v;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -175,9 +180,10 @@ __device__ __forceinline__ int64_t wave_begin(const DecodeParams& p, int64_t N, 
   return N * DC_ODD_W >= total ? split_weight(w) * N / total : w * N / We;
 }
 
-// A wave's walk over its range of steps, one row segment at a time, for the fp32
-// stream kernel.  (The bf16 one keeps the same walk in its own variables: through
+// A wave's walk over its range of steps, one row segment at a time, for the fp32 and
+// 4-bit stream kernels.  (The bf16 one keeps the same walk in its own variables: through
 // this struct it ran 1.2% slower at B64, 64/4 heads, up to 32768 keys.)
+template <int COST = 0>
 struct Walk {
   int64_t q, q1;      // the range's next step and its end
   int b, j, ls, nb;   // batch, row within it, first step within the row, steps of a row
@@ -189,21 +195,22 @@ struct Walk {
   }
   __device__ __forceinline__ int steps_of(const DecodeParams& p, int bb) const {
     const int l = len_of(p, bb);
-    return l > 0 ? (l + DC_STEP - 1) / DC_STEP : 0;
+    return l > 0 ? (l + DC_STEP - 1) / DC_STEP + COST : 0;
   }
-  // false: wave w has no steps
+  // false: wave w has no steps.  EVEN: ranges of one size, whichever XCD they run on
+  template <bool EVEN = false>
   __device__ __forceinline__ bool start(const DecodeParams& p, int lane, int64_t w) {
-    const int64_t N = lane_value_i64(total_steps(p, lane), 0);
+    const int64_t N = lane_value_i64(total_steps<COST>(p, lane), 0);
     if (N == 0) return false;
     const int64_t We = waves_used(p, N);
     if (w >= We) return false;
-    q = wave_begin(p, N, We, w);
-    q1 = wave_begin(p, N, We, w + 1);
+    q = EVEN ? w * N / We : wave_begin(p, N, We, w);
+    q1 = EVEN ? (w + 1) * N / We : wave_begin(p, N, We, w + 1);
     if (q >= q1) return false;
     lens_in_reg = p.B <= 64;
     lens_lane = lens_in_reg && lane < p.B ? batch_len(p, lane) : 0;
     int64_t before;
-    find_batch(p, lane, q, b, before);
+    find_batch<COST>(p, lane, q, b, before);
     nb = steps_of(p, b);
     j = (int)((q - before) / nb);
     ls = (int)((q - before) % nb);

@@ -191,8 +191,14 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4GatherParams p) {
 }
 
 // ---------------------------------------------------------------- decode
-// The schedule, the online softmax, the partials and their merge are those of the bf16
-// decode (nq_decode.hip); what differs is how a step's 32 keys reach the matrix cores.
+// o = softmax(scale q K^T) V over the keys [0, lens[b]) of each sequence.  Rows (sequence,
+// kv head, up to 16 query heads) are cut into steps of 32 keys as in the bf16 decode
+// (nq_decode.hip); a workgroup of eight waves takes a contiguous range of a row's steps,
+// its waves every eighth step each, and joins them in LDS.  Either a workgroup takes a
+// whole row and writes its output (few or short rows: one launch), or a persistent grid
+// shares the steps of all rows evenly, and partials meet in the bf16 decode's merge.
+//
+// How a step's 32 keys reach the matrix cores:
 //   K: a 16-key tile is one load per lane of D/4 consecutive elements of a row, in the
 //     order in which the MFMA's k slots are taken (slot 8 g + j of MFMA i is element
 //     g D/4 + 8 i + j, for q as well), and one scale byte, since those elements lie in
@@ -202,9 +208,26 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4GatherParams p) {
 // Codes times a power of two are exact in bf16, so the products are those of a bf16
 // cache that held the same values.  fp32 queries: q and the probabilities are split into
 // three bf16 terms each (8 + 8 + 8 significant bits), three MFMAs in place of one.
-constexpr int KV4_WG_PER_CU = 2;
-constexpr int KV4_MAX_WAVES = 256 * KV4_WG_PER_CU * DC_WAVES;
-constexpr int KV4_DEPTH = 2;  // steps whose loads are in flight
+//
+// The running maximum is raised only for a score more than 2^8 above it: most steps then
+// exchange nothing between lanes and rescale no output, and the sums, held in fp32, have
+// room for the larger terms.
+//
+// HBM-bound: 17/16 D bytes a cached row and kv head.  64 sequences of 1024 to 32768 keys, 64/4
+// heads, D = 128 (539 MB): 98.5 us with the merge, the workgroups on average at work for 77
+// us of it (7.0 TB/s).  Waves that each took a range of their own (2048 of them, and
+// partials) took 107; a whole row to a workgroup there 132, its rows differing in length.
+// Loads of two steps in flight a wave; three or four gained nothing.
+constexpr int KV4_ROW_WAVES = 8;          // of a workgroup that takes a row of its own
+constexpr int KV4_WAVES = 4;              // of one of the persistent grid's
+constexpr int KV4_PER_CU = 2;             // of which a CU holds this many
+constexpr int KV4_MAX_GROUPS = 256 * KV4_PER_CU;
+// What a row's start counts for in the split, in steps: its workgroup waits for block table,
+// first codes and the join, about 4.5 us, in which the CU's other one goes on.  At 0, 64
+// sequences of 1024 to 32768 keys (64/4 heads) took 105 us, at 24 101.
+constexpr int KV4_ROW_COST = 24;
+constexpr int KV4_DEPTH = 2;              // steps of a wave whose loads are in flight
+constexpr float KV4_SLACK = 8.f;          // log2 of how far a score may exceed the running maximum
 
 // One step's codes and scales as loaded.
 template <int D> struct Kv4Step {
@@ -240,13 +263,23 @@ __device__ __forceinline__ void split_bf16(floatx8 x, bf16x8 (&out)[NT]) {
   }
 }
 
+__device__ __forceinline__ float xor16_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor16_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 struct Kv4DecodeParams {
-  DecodeParams d;  // kc: the pool; ksb, ksh: page and head strides in bytes
+  DecodeParams d;  // kc: the pool; ksb, ksh: page and head strides in bytes; nwaves: workgroups
   int npages;
+  uint32_t pu, magic;  // steps of a page, floor(2^32 / pu)
 };
 
-template <int D, typename T>
-__global__ void __attribute__((amdgpu_flat_work_group_size(DC_THREADS, DC_THREADS), amdgpu_waves_per_eu(KV4_WG_PER_CU)))
+template <int D, typename T, bool ROWS, int W = ROWS ? KV4_ROW_WAVES : KV4_WAVES>
+__global__ void __attribute__((amdgpu_flat_work_group_size(W * 64, W * 64), amdgpu_waves_per_eu(2)))
 decode_kv4_kernel(Kv4DecodeParams pp) {
   const DecodeParams& p = pp.d;
   using F = Kv4<D>;
@@ -254,14 +287,39 @@ decode_kv4_kernel(Kv4DecodeParams pp) {
   using Step = Kv4Step<D>;
   constexpr int NT = std::is_same<T, float>::value ? 3 : 1;
   constexpr int NDQ = D / 32, NDO = D / 16;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[DC_WAVES * L::BYTES];
+  static_assert(L::BYTES == 16 * D * 4, "a wave's V tile holds its outputs");
+  __shared__ __attribute__((aligned(16))) unsigned char smem[W * L::BYTES];
+  __shared__ floatx2 part_ml[W][16];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t w = (int64_t)blockIdx.x * DC_WAVES + wave;
-  Walk at;
-  if (!at.start(p, lane, w)) return;
   const int c16 = lane & 15, grp = lane >> 4;
+  Walk<ROWS ? 0 : KV4_ROW_COST> at;
+  if constexpr (ROWS) {
+    const int r = blockIdx.x;
+    at.b = r / p.rows_per_batch;
+    at.j = r % p.rows_per_batch;
+    at.ls = 0;
+    at.lens_in_reg = false;
+    at.nb = batch_steps(p, at.b);
+    at.q = 0;
+    at.q1 = at.nb;
+    if (at.nb == 0) {  // no keys: zeros; a length out of range: NaN
+      const int kvh = at.j / p.NG, hg = at.j % p.NG, nh = min(16, p.G - hg * 16);
+      const int len = batch_len(p, at.b);
+      const float f = len < 0 ? __builtin_nanf("") : 0.f;
+      const int head0 = kvh * p.G + hg * 16;
+      T* out = reinterpret_cast<T*>(p.o) + at.b * p.osb + (int64_t)head0 * p.osh;
+      for (int t = threadIdx.x; t < nh * (D / 2); t += (W * 64))
+        store2<T>(out + (t / (D / 2)) * p.osh + (t % (D / 2)) * 2, f, f);
+      if (p.lse && threadIdx.x < (unsigned)nh) p.lse[(int64_t)at.b * p.Hq + head0 + threadIdx.x] = len < 0 ? f : -INFINITY;
+      return;
+    }
+  } else {
+    // Even ranges: weighted as the bf16 decode's are, 64 sequences of up to 32768 keys took
+    // 101 us, even 98.5.  (The wave of the walk is a workgroup here.)
+    if (!at.template start<true>(p, lane, blockIdx.x)) return;
+  }
   unsigned char* vt = smem + wave * L::BYTES;
 
   // byte offsets within a step's codes and scales
@@ -271,211 +329,273 @@ decode_kv4_kernel(Kv4DecodeParams pp) {
   constexpr int LPV = F::CB / Step::VB;  // lanes of a row
   constexpr int CPP = Step::VB / 4;      // chunks of a piece
   const int vprow = lane / LPV, vpc = (lane % LPV) * CPP;
+  int vwa[Step::VL][CPP];
+#pragma unroll
+  for (int i = 0; i < Step::VL; ++i)
+#pragma unroll
+    for (int c = 0; c < CPP; ++c) {
+      const int row = i * (64 / LPV) + vprow;
+      vwa[i][c] = row * L::RB + (((vpc + c) ^ L::vswz(row)) << 4);
+    }
   const int jj = lane & 15;
   const int vrow = 4 * grp + (jj >> 2);
   const int voff = vrow * L::RB + ((L::vswz(vrow) >> 1) << 5) + (jj & 3) * 8;
+  const int pbytes = p.page * F::RB, vbase = F::v_codes(p.page), ksbase = F::k_scales(p.page), vsbase = F::v_scales(p.page);
+  // floor(n / pu): the product with floor(2^32 / pu) falls at most one short
+  auto page_of = [&](uint32_t n) {
+    uint32_t g = __umulhi(n, pp.magic);
+    if (n - g * pp.pu >= pp.pu) ++g;
+    return (int)g;
+  };
 
   while (true) {
-    const int b = at.b, ls = at.ls, nb = at.nb;
+    // (said to be wave-uniform, which the buffer loads' scalar operands have to be)
+    constexpr int COST = ROWS ? 0 : KV4_ROW_COST;
+    const int span = uniform((int)min((int64_t)(at.nb - at.ls), at.q1 - at.q));
+    const int b = uniform(at.b), nb = uniform(at.nb) - COST, j = uniform(at.j), start = uniform(at.ls) - COST;
+    const int ls = max(start, 0), nseg = max(start + span, 0) - ls;
+    if (nseg == 0) {  // a part of the row's start, which holds no keys
+      if (!at.next(p, span)) break;
+      continue;
+    }
     const int len = at.len_of(p, b);
-    const int kvh = at.j / p.NG, hg = at.j % p.NG;
-    const int nseg = (int)min((int64_t)(nb - ls), at.q1 - at.q);
+    const int kvh = j / p.NG, hg = j % p.NG;
     const bool whole = ls == 0 && nseg == nb;
-    const int kbeg = ls * DC_STEP;
     const int kend = min(len, (ls + nseg) * DC_STEP);
+    const int mine = nseg > wave ? (nseg - wave + W - 1) / W : 0;  // steps ls + wave + 8 i
 
-    // block-table entries [wbase, wbase + 64) of this row, one per lane
-    int wbase = kbeg / p.page, win = 0;
+    // the pages of this wave's steps [wbase, wbase + 64), one per lane
+    int wbase = 0, win = 0;
     bool lost = false;  // a page that is not in the pool: the row is NaN
     auto load_window = [&](int first) {
-      const int npg = (kend + p.page - 1) / p.page;
       wbase = first;
-      win = first + lane < npg ? p.bt[b * p.bts + first + lane] : 0;
+      win = first + lane < mine ? p.bt[b * p.bts + page_of(ls + wave + (first + lane) * W)] : 0;
+      const bool bad = (uint32_t)win >= (uint32_t)pp.npages;
+      lost |= wave_any(bad);
+      if (bad) win = 0;
     };
-    load_window(wbase);
     const unsigned char* heads = reinterpret_cast<const unsigned char*>(p.kc) + kvh * p.ksh;
-    auto load = [&](Step& st, int k0) {
-      const int pg = k0 / p.page;  // a step never crosses a page
-      if (pg - wbase >= 64) load_window(pg);
-      int pid = __builtin_amdgcn_readlane(win, pg - wbase);
-      if ((uint32_t)pid >= (uint32_t)pp.npages) {
-        pid = 0;
-        lost = true;
-      }
-      const int rel = k0 - pg * p.page;
-      const BufRsrc rs = make_rsrc(heads + pid * p.ksb, (uint32_t)(p.page * F::RB));
-      const int kc = rel * F::CB, ks = F::k_scales(p.page) + rel * F::SB;
-      const int vc = F::v_codes(p.page) + rel * F::CB, vs = F::v_scales(p.page) + rel * F::SB;
+    // Past the wave's last step the loads go out all the same, over no bytes: behind a
+    // branch the compiler could not tell how many are in flight, and would wait for all
+    // of them at every step.
+    auto load = [&](Step& st, int i) {
+      if (i - wbase >= 64) load_window(i);
+      const int pid = __builtin_amdgcn_readlane(win, i - wbase);
+      const uint32_t n = ls + wave + i * W;
+      const int rel = (int)(n - uniform(page_of(n)) * pp.pu) * DC_STEP;
+      const BufRsrc rs = make_rsrc(heads + pid * p.ksb, i < mine ? (uint32_t)pbytes : 0u);
+      const int kc = rel * F::CB, ks = ksbase + rel * F::SB;
+      const int vc = vbase + rel * F::CB, vs = vsbase + rel * F::SB;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         kv4_load(st.k[t], rs, kvo, kc + t * 16 * F::CB);
         st.ks[t] = __builtin_amdgcn_raw_buffer_load_b8(rs, kso, ks + t * 16 * F::SB, 2);
       }
 #pragma unroll
-      for (int i = 0; i < Step::VL; ++i) {
-        kv4_load(st.v[i], rs, vvo, vc + i * 64 * Step::VB);
-        st.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, vso, vs + i * 4 * Step::VB, 2);
+      for (int l = 0; l < Step::VL; ++l) {
+        kv4_load(st.v[l], rs, vvo, vc + l * 64 * Step::VB);
+        st.vs[l] = __builtin_amdgcn_raw_buffer_load_b8(rs, vso, vs + l * 4 * Step::VB, 2);
       }
     };
-
-    // ---- the query: lane (head c16, slot grp) holds elements grp D/4 + 8 i + j
-    const int gh = hg * 16 + c16;
-    const bool hvalid = gh < p.G;
-    const T* qrow = reinterpret_cast<const T*>(p.q) + b * p.qsb + (kvh * p.G + (hvalid ? gh : 0)) * p.qsh + grp * (D / 4);
-    floatx8 x[NDQ];
-#pragma unroll
-    for (int i = 0; i < NDQ; ++i) x[i] = Vec8<T>::load_f32(qrow + i * 8);
-
-    Step st[KV4_DEPTH];
-#pragma unroll
-    for (int u = 0; u < KV4_DEPTH; ++u)
-      if (u < nseg) load(st[u], kbeg + u * DC_STEP);
-
-    bf16x8 qop[NDQ][NT];
-#pragma unroll
-    for (int i = 0; i < NDQ; ++i) split_bf16<NT>(hvalid ? x[i] : floatx8{}, qop[i]);
 
     float m_i = -INFINITY, l_i = 0.f;
     floatx4 oacc[NDO];
 #pragma unroll
     for (int dd = 0; dd < NDO; ++dd) oacc[dd] = floatx4{};
+    const int gh = hg * 16 + c16;
+    const bool hvalid = gh < p.G;
 
-    auto step = [&](Step& st, int s) {
-      const int k0 = kbeg + s * DC_STEP;
-      const bool part = k0 + DC_STEP > kend;
-      // V to the LDS tile (in-order within the wave: the previous step's reads of the
-      // tile have been served); rows past the last key as zeros, whatever they hold
+    if (mine > 0) {
+      load_window(0);
+      // ---- the query: lane (head c16, slot grp) holds elements grp D/4 + 8 i + j
+      const T* qrow =
+          reinterpret_cast<const T*>(p.q) + b * p.qsb + (kvh * p.G + (hvalid ? gh : 0)) * p.qsh + grp * (D / 4);
+      floatx8 x[NDQ];
 #pragma unroll
-      for (int i = 0; i < Step::VL; ++i) {
-        const int row = i * (64 / LPV) + vprow;
-        const bool gone = part && k0 + row >= kend;
-        const float scale = gone ? 1.0f : kv4_scale(st.vs[i]);
+      for (int i = 0; i < NDQ; ++i) x[i] = Vec8<T>::load_f32(qrow + i * 8);
+      Step st[KV4_DEPTH];
 #pragma unroll
-        for (int c = 0; c < CPP; ++c)
-          *reinterpret_cast<bf16x8*>(vt + row * L::RB + (((vpc + c) ^ L::vswz(row)) << 4)) =
-              kv4_bf16x8(gone ? 0u : st.v[i][c], scale);
-      }
-      floatx4 sc[2];
+      for (int u = 0; u < KV4_DEPTH; ++u) load(st[u], u);
+      bf16x8 qop[NDQ][NT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        sc[t] = floatx4{};
-        const float scale = kv4_scale(st.ks[t]);
+      for (int i = 0; i < NDQ; ++i) split_bf16<NT>(hvalid ? x[i] : floatx8{}, qop[i]);
+
+      auto step = [&](Step& st, int i) {
+        const int k0 = (ls + wave + i * W) * DC_STEP;
+        if (k0 + DC_STEP > kend) {  // value rows past the last key as zeros, whatever they hold
 #pragma unroll
-        for (int i = 0; i < NDQ; ++i) {
-          const bf16x8 a = kv4_bf16x8(st.k[t][i], scale);
+          for (int l = 0; l < Step::VL; ++l)
+            if (k0 + l * (64 / LPV) + vprow >= kend) {
+              st.vs[l] = 127;
 #pragma unroll
-          for (int n = NT - 1; n >= 0; --n) sc[t] = mfma16(a, qop[i][n], sc[t]);
+              for (int c = 0; c < CPP; ++c) st.v[l][c] = 0;
+            }
         }
-      }
-      if (s + KV4_DEPTH < nseg) load(st, k0 + KV4_DEPTH * DC_STEP);
-      if (part) {
+        floatx4 sc[2] = {floatx4{}, floatx4{}};
+#pragma unroll
+        for (int d = 0; d < NDQ; ++d)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const bf16x8 a = kv4_bf16x8(st.k[t][d], kv4_scale(st.ks[t]));
+#pragma unroll
+            for (int n = NT - 1; n >= 0; --n) sc[t] = mfma16(a, qop[d][n], sc[t]);
+          }
+        // V to the LDS tile (in-order within the wave: the previous step's reads of the
+        // tile have been served), and back transposed; the reads are issued together,
+        // and the softmax runs while they are served
+#pragma unroll
+        for (int l = 0; l < Step::VL; ++l) {
+          const float scale = kv4_scale(st.vs[l]);
+#pragma unroll
+          for (int c = 0; c < CPP; ++c)
+            *reinterpret_cast<bf16x8*>(vt + vwa[l][c]) = kv4_bf16x8(st.v[l][c], scale);
+        }
+        load(st, i + KV4_DEPTH);
+        bf16x8 vop[NDO];
+#pragma unroll
+        for (int dd = 0; dd < NDO; ++dd) {
+          const unsigned char* src = vt + (voff ^ (dd << 5));
+          vop[dd] = lds_read_tr8(reinterpret_cast<const bf16*>(src), reinterpret_cast<const bf16*>(src + 16 * L::RB));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (k0 + DC_STEP > kend) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k0 + t * 16 + grp * 4 + e >= kend) sc[t][e] = -INFINITY;
+        }
+        float mx = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (k0 + t * 16 + grp * 4 + i >= kend) sc[t][i] = -INFINITY;
-      }
-      float mx = -INFINITY;
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][e]);
+        mx *= p.scale_log2;
+        if (wave_any(mx > m_i + KV4_SLACK)) {
+          const float m_new = fmaxf(m_i, xor32_max(xor16_max(mx)));
+          const float alpha = m_new > -INFINITY ? fast_exp2(m_i - m_new) : 1.f;
+          l_i *= alpha;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[t][i]);
-      mx = fmaxf(mx, shfl_xor_f(mx, 16));
-      mx = fmaxf(mx, shfl_xor_f(mx, 32));
-      // without a finite score so far the row keeps m = -inf and exponentiates against 0
-      const float m_new = fmaxf(m_i, mx * p.scale_log2);
-      const float m_use = m_new > -INFINITY ? m_new : 0.f;
-      const float alpha = fast_exp2(m_i - m_use);
-      floatx8 pf;
-      float rs = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float pe = fast_exp2(__builtin_fmaf(sc[t][i], p.scale_log2, -m_use));
-          pf[t * 4 + i] = pe;
-          rs += pe;
+          for (int dd = 0; dd < NDO; ++dd) oacc[dd] *= alpha;
+          m_i = m_new;
         }
-      bf16x8 pop[NT];
-      split_bf16<NT>(pf, pop);
-      l_i = __builtin_fmaf(l_i, alpha, rs);
-      m_i = m_new;
+        // without a finite score so far the row keeps m = -inf and exponentiates against 0
+        const float m_use = m_i > -INFINITY ? m_i : 0.f;
+        floatx8 pf;
+        float rs = 0.f;
 #pragma unroll
-      for (int dd = 0; dd < NDO; ++dd) {
-        oacc[dd] *= alpha;
-        const unsigned char* src = vt + (voff ^ (dd << 5));
-        const bf16x8 a = lds_read_tr8(reinterpret_cast<const bf16*>(src),
-                                      reinterpret_cast<const bf16*>(src + 16 * L::RB));
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int n = NT - 1; n >= 0; --n) oacc[dd] = mfma16(a, pop[n], oacc[dd]);
-      }
-    };
-    for (int s = 0; s < nseg; s += KV4_DEPTH)
+          for (int e = 0; e < 4; ++e) {
+            const float pe = fast_exp2(__builtin_fmaf(sc[t][e], p.scale_log2, -m_use));
+            pf[t * 4 + e] = pe;
+            rs += pe;
+          }
+        bf16x8 pop[NT];
+        split_bf16<NT>(pf, pop);
+        l_i += rs;
 #pragma unroll
-      for (int u = 0; u < KV4_DEPTH; ++u)
-        if (s + u < nseg) step(st[u], s + u);
+        for (int dd = 0; dd < NDO; ++dd)
+#pragma unroll
+          for (int n = NT - 1; n >= 0; --n) oacc[dd] = mfma16(vop[dd], pop[n], oacc[dd]);
+      };
+      int i = 0;
+      for (; i + KV4_DEPTH <= mine; i += KV4_DEPTH)
+#pragma unroll
+        for (int u = 0; u < KV4_DEPTH; ++u) step(st[u], i + u);
+#pragma unroll
+      for (int u = 0; u < KV4_DEPTH - 1; ++u)
+        if (i + u < mine) step(st[u], i + u);
+    }
 
-    // ---- flush the segment
-    l_i += shfl_xor_f(l_i, 16);
-    l_i += shfl_xor_f(l_i, 32);
+    // ---- the waves' parts meet in LDS: maxima and sums first, then each wave's outputs,
+    // brought to the common maximum, in its own V tile
+    l_i = xor32_sum(xor16_sum(l_i));
     if (lost) l_i = __builtin_nanf("");
-    const int64_t r = ((int64_t)b * p.Hkv + kvh) * p.NG + hg;
-    if (lane == 0) {
-      if (ls == 0) p.ws_rw[r * 2] = (int32_t)w;
-      if (ls + nseg == nb) p.ws_rw[r * 2 + 1] = (int32_t)w;
+    if (grp == 0) part_ml[wave][c16] = floatx2{m_i, l_i};
+    __syncthreads();
+    const int used = min(nseg, W);  // waves that took steps
+    float M = -INFINITY;
+    for (int i = 0; i < used; ++i) M = fmaxf(M, part_ml[i][c16][0]);
+    const float f = M > -INFINITY ? fast_exp2(m_i - M) : 1.f;
+    if (wave < used) {
+#pragma unroll
+      for (int dd = 0; dd < NDO; ++dd)
+        *reinterpret_cast<floatx4*>(vt + c16 * (D * 4) + (((dd * 4 + grp) ^ (c16 & (D / 4 - 1))) << 4)) = oacc[dd] * f;
     }
-    if (hvalid) {
-      if (whole) {
-        const int head = kvh * p.G + gh;
-        T* orow = reinterpret_cast<T*>(p.o) + b * p.osb + (int64_t)head * p.osh;
-        const float inv = 1.0f / l_i;
-#pragma unroll
-        for (int dd = 0; dd < NDO; ++dd) store4<T>(orow + dd * 16 + grp * 4, oacc[dd] * inv);
-        if (p.lse && grp == 0) p.lse[(int64_t)b * p.Hq + head] = row_lse(m_i, l_i);
+    __syncthreads();
+    const int64_t r = ((int64_t)b * p.Hkv + kvh) * p.NG + hg;
+    const int64_t slot = blockIdx.x + r;
+    if (!ROWS && threadIdx.x == 0) {
+      if (ls == 0) p.ws_rw[r * 2] = (int32_t)blockIdx.x;
+      if (ls + nseg == nb) p.ws_rw[r * 2 + 1] = (int32_t)blockIdx.x;
+    }
+    for (int t = threadIdx.x; t < 16 * (D / 4); t += (W * 64)) {
+      const int h = t / (D / 4), c = t % (D / 4);
+      if (hg * 16 + h >= p.G) continue;
+      float top = -INFINITY, sum = 0.f;
+      for (int i = 0; i < used; ++i) top = fmaxf(top, part_ml[i][h][0]);
+      floatx4 acc = floatx4{};
+      for (int i = 0; i < used; ++i) {
+        const floatx2 ml = part_ml[i][h];
+        sum = __builtin_fmaf(ml[1], top > -INFINITY ? fast_exp2(ml[0] - top) : 1.f, sum);
+        acc += *reinterpret_cast<const floatx4*>(smem + i * L::BYTES + h * (D * 4) + ((c ^ (h & (D / 4 - 1))) << 4));
+      }
+      if (ROWS || whole) {
+        const int head = kvh * p.G + hg * 16 + h;
+        store4<T>(reinterpret_cast<T*>(p.o) + b * p.osb + (int64_t)head * p.osh + c * 4, acc * (1.0f / sum));
+        if (p.lse && c == 0) p.lse[(int64_t)b * p.Hq + head] = row_lse(top, sum);
       } else {
-        const int64_t slot = w + r;
-        float* so = p.ws_o + (slot * 16 + c16) * D;
-#pragma unroll
-        for (int dd = 0; dd < NDO; ++dd) *reinterpret_cast<floatx4*>(so + dd * 16 + grp * 4) = oacc[dd];
-        if (grp == 0) *reinterpret_cast<floatx2*>(p.ws_ml + (slot * 16 + c16) * 2) = floatx2{m_i, l_i};
+        *reinterpret_cast<floatx4*>(p.ws_o + (slot * 16 + h) * D + c * 4) = acc;
+        if (c == 0) *reinterpret_cast<floatx2*>(p.ws_ml + (slot * 16 + h) * 2) = floatx2{top, sum};
       }
     }
-    if (!at.next(p, nseg)) break;
+    if (ROWS || !at.next(p, span)) break;
+    __syncthreads();  // the tiles and sums are read; the next segment may write them
   }
 }
 
 static int64_t kv4_workspace(int B, int Hq, int Hkv, int D) {
   const int64_t rows = (int64_t)B * Hkv * ((Hq / Hkv + 15) / 16);
-  return (KV4_MAX_WAVES + rows) * 16 * (D + 2) * (int64_t)sizeof(float) + rows * 2 * (int64_t)sizeof(int32_t);
+  return (KV4_MAX_GROUPS + rows) * 16 * (D + 2) * (int64_t)sizeof(float) + rows * 2 * (int64_t)sizeof(int32_t);
+}
+
+// Whether each row goes to a workgroup of its own.  Its eight waves take about KV4_STEP_US
+// for a step each; the shared form takes KV4_SHARE_US more, for the schedule, the
+// partials' way to memory and the merge's launch.  Rows of one launch differ in length, and
+// the host knows no more than the longest: the shared work is taken as half of it.
+constexpr float KV4_STEP_US = 0.9f, KV4_SHARE_US = 7.f;
+static bool kv4_whole_rows(int64_t rows, int max_len, int cus) {
+  const int64_t turns = (max_len + DC_STEP * KV4_ROW_WAVES - 1) / (DC_STEP * KV4_ROW_WAVES);
+  const float own = (float)((rows + cus - 1) / cus) * turns * KV4_STEP_US;
+  const float shared = 0.5f * (float)rows * turns / cus * KV4_STEP_US + KV4_SHARE_US;
+  return own <= shared;
 }
 
 template <int D, typename T>
 static hipError_t launch_decode_kv4(Kv4DecodeParams pp, hipStream_t st) {
   DecodeParams& p = pp.d;
-  // a persistent grid, worked out once per device and variant
-  static int resident[64];
-  int dev = 0;
+  int dev = 0, cus = 0;
+  static int known[64];  // CUs of each device
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return e;
-  int waves = (dev >= 0 && dev < 64) ? __atomic_load_n(&resident[dev], __ATOMIC_RELAXED) : 0;
-  if (waves == 0) {
-    int cus = 0, per_cu = 0;
+  cus = (dev >= 0 && dev < 64) ? __atomic_load_n(&known[dev], __ATOMIC_RELAXED) : 0;
+  if (cus == 0) {
     e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
-    if (e == hipSuccess)
-      e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
-          &per_cu, reinterpret_cast<const void*>(decode_kv4_kernel<D, T>), DC_THREADS, 0);
     if (e != hipSuccess) return e;
-    const int per = per_cu < 1 ? 1 : (per_cu > KV4_WG_PER_CU ? KV4_WG_PER_CU : per_cu);
-    waves = cus * per * DC_WAVES;
-    if (waves > KV4_MAX_WAVES) waves = KV4_MAX_WAVES;
-    if (dev >= 0 && dev < 64) __atomic_store_n(&resident[dev], waves, __ATOMIC_RELAXED);
+    if (dev >= 0 && dev < 64) __atomic_store_n(&known[dev], cus, __ATOMIC_RELAXED);
   }
-  p.nwaves = waves;
-  hipLaunchKernelGGL((decode_kv4_kernel<D, T>), dim3((unsigned)(waves / DC_WAVES)), dim3(DC_THREADS), 0, st, pp);
+  const int64_t rows = (int64_t)p.B * p.rows_per_batch;
+  if (kv4_whole_rows(rows, p.max_len, cus)) {
+    hipLaunchKernelGGL((decode_kv4_kernel<D, T, true>), dim3((unsigned)rows), dim3(KV4_ROW_WAVES * 64), 0, st, pp);
+    return hipGetLastError();
+  }
+  const int groups = cus * KV4_PER_CU < KV4_MAX_GROUPS ? cus * KV4_PER_CU : KV4_MAX_GROUPS;
+  p.nwaves = groups;
+  hipLaunchKernelGGL((decode_kv4_kernel<D, T, false>), dim3((unsigned)groups), dim3(KV4_WAVES * 64), 0, st, pp);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t rows = (int64_t)p.B * p.rows_per_batch;
-  const int threads = rows * DC_MERGE_WIDE_PARTIALS <= waves ? DC_MERGE_MAX_THREADS : DC_THREADS;
+  const int threads = rows * DC_MERGE_WIDE_PARTIALS <= groups ? DC_MERGE_MAX_THREADS : DC_THREADS;
   hipLaunchKernelGGL((decode_merge_kernel<D, T>), dim3((unsigned)rows), dim3(threads),
                      (threads / 16) * (D + 2) * sizeof(float), st, p);
   return hipGetLastError();
@@ -643,13 +763,15 @@ extern "C" int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.NG = NG; p.max_len = max_len;
   p.rows_per_batch = Hkv * NG;
   while ((1 << p.hs) < (p.G < 16 ? p.G : 16)) ++p.hs;
-  const int64_t slots = KV4_MAX_WAVES + (int64_t)B * p.rows_per_batch;
+  const int64_t slots = KV4_MAX_GROUPS + (int64_t)B * p.rows_per_batch;
   p.ws_o = reinterpret_cast<float*>(workspace);
   p.ws_ml = p.ws_o + slots * 16 * D;
   p.ws_rw = reinterpret_cast<int32_t*>(p.ws_ml + slots * 16 * 2);
   p.scale_log2 = (sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)D)) * kLog2e;
   p.bt = block_table; p.bts = bt_stride; p.page = page_size;
   pp.npages = num_pages;
+  pp.pu = (uint32_t)(page_size / DC_STEP);
+  pp.magic = pp.pu == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / pp.pu);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return nq_check_launch(with_head_dim(D, [&](auto dc) {
     return dtype == NQ_DTYPE_BF16 ? launch_decode_kv4<decltype(dc)::value, bf16>(pp, st)
