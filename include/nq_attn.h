@@ -701,13 +701,15 @@ int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const void* pool
  * {page, head} in bytes; else bf16 K pages, strides {page, head, row} in elements.
  * weights: fp32, strides {batch, head}, max_len entries a head.  A length outside
  * [0, max_len] gives NaN (accumulating: nothing), a page outside the pool NaN at its keys.
- * Sums are taken in a fixed order.
+ * Sums are taken in a fixed order.  workspace: nq_key_weights_workspace_bytes (0: none,
+ * NULL allowed), 16-byte aligned.
  */
+int64_t nq_key_weights_workspace_bytes(int B, int Hq, int Hkv, int S, int max_len);
 int nq_key_weights(const void* q, const int64_t* q_strides, const void* k_pool,
                    const int64_t* pool_strides, int four_bit, int num_pages, const int32_t* block_table,
                    int64_t bt_stride, int bt_cols, int page_size, const int32_t* lens, const float* lse,
-                   float* weights, const int64_t* weight_strides, int accumulate, int B, int Hq, int Hkv,
-                   int S, int D, int max_len, int causal, float sm_scale, void* stream);
+                   float* weights, const int64_t* weight_strides, int accumulate, void* workspace,
+                   int64_t workspace_bytes, int B, int Hq, int Hkv, int S, int D, int max_len, int causal, float sm_scale, void* stream);
 
 /*
  * The rows of a cache worth keeping: kept (int32 (B, Hkv, keep), contiguous) receives, in

@@ -272,10 +272,11 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32, _i32, _i32,          # B, Hq, Hkv, D, max_len, dtype
         _f32, _p,                                    # sm_scale, stream
     ]),
+    "nq_key_weights_workspace_bytes": (_i64, [_i32] * 5),  # B, Hq, Hkv, S, max_len
     "nq_key_weights": (_i32, [
         _p, _i64p,                                   # q, q_strides
         _p, _i64p, _i32, _i32, _p, _i64, _i32, _i32,  # pool, strides, four_bit, num_pages, block_table, stride, cols, page_size
-        _p, _p, _p, _i64p, _i32,                     # lens, lse, weights, strides, accumulate
+        _p, _p, _p, _i64p, _i32, _p, _i64,           # lens, lse, weights, strides, accumulate, workspace, bytes
         _i32, _i32, _i32, _i32, _i32, _i32,          # B, Hq, Hkv, S, D, max_len
         _i32, _f32, _p,                              # causal, sm_scale, stream
     ]),

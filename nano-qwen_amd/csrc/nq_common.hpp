@@ -362,6 +362,23 @@ __device__ __forceinline__ int32_t ld_uniform(const int32_t* base, int64_t i) {
   return ((const __attribute__((address_space(4))) int32_t*)base)[i];
 }
 
+// n / d and n % d for n < 2^31 by a d known before the launch: the product with
+// floor(2^32 / d) falls at most one short.
+struct Divider {
+  uint32_t d, m;
+  Divider() = default;
+  explicit Divider(uint32_t by) : d(by), m(by == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / by)) {}
+  __host__ __device__ __forceinline__ int div(int n) const {
+    const uint32_t q = (uint32_t)(((uint64_t)(uint32_t)n * m) >> 32);
+    return (int)(q + ((uint32_t)n - q * d >= d));
+  }
+  __device__ __forceinline__ int div(int n, int& rem) const {
+    const int q = div(n);
+    rem = (int)((uint32_t)n - (uint32_t)q * d);
+    return q;
+  }
+};
+
 // Position of (b, s): explicit positions win, else base[b] + s, else pos0 + s.
 __device__ __forceinline__ int row_position(const int32_t* pos, const int32_t* pos_base, int pos0,
                                             int b, int s, int S) {

@@ -16,7 +16,7 @@ namespace nq {
 // the columns of the attention's probabilities, which a flash attention never forms: its
 // log-sum-exp gives them from q and K alone.  The product is taken as S = Q K^T, so a
 // lane holds one key and four (query, head) rows, and the sum over rows stays in it until
-// the end; K stays in registers while the rows pass.
+// the end; K stays in registers while the rows pass.  Rows run r = s G + g.
 struct KeyWeightParams {
   const bf16* q;
   int64_t qsb, qsh, qss;
@@ -25,123 +25,393 @@ struct KeyWeightParams {
   int npages;
   const int32_t* bt;
   int64_t bts;
-  int page;
+  Divider page;
   const int32_t* lens;
   const float* lse;  // (B, Hq, S)
   float* w;
   int64_t wsb, wsh;
   int add;           // add to w, else write it
-  int Hq, Hkv, G, S, max_len, causal;
+  int B, Hq, Hkv, S, max_len, causal;
+  Divider G;
   float scale_log2;
+  Divider range;           // keys of a workgroup
+  int same;                // workgroups of each chunk, 0: as many as it has ranges
+  int chunks, chunk_rows;  // rows of a workgroup: chunks > 1 write partial sums
+  float* part;             // (chunks, B, Hkv, max_len)
 };
 
-constexpr int KW_KEYS = 64;              // keys of a wave
-constexpr int KW_BLOCK = 4 * KW_KEYS;    // of a workgroup
-
+// The elements that lane slot grp holds of operand i, in eights: q's must be K's.  4-bit rows:
+// D/4 consecutive ones, as the decode's (one load, one scale); bf16 rows: as they lie, 64
+// consecutive bytes of a row to four lanes.
 template <int D, bool FOUR>
-__global__ void __launch_bounds__(256) key_weights_kernel(KeyWeightParams p) {
-  using F = Kv4<D>;
-  constexpr int NDQ = D / 32;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c16 = lane & 15, grp = lane >> 4;
-  const int b = blockIdx.z, kvh = blockIdx.y;
-  const int k0 = blockIdx.x * KW_BLOCK + wave * KW_KEYS;
-  const int len = ld_uniform(p.lens, b);
-  float* w = p.w + b * p.wsb + kvh * p.wsh;
-  if (k0 >= p.max_len) return;
-  const bool bad_len = len < 0 || len > p.max_len;
-  if (bad_len || k0 >= len) {  // no keys here
-    const int t = k0 + lane;
-    if (!p.add && t < p.max_len) w[t] = bad_len ? __builtin_nanf("") : 0.f;
-    return;
+__device__ __forceinline__ constexpr int eight_of(int grp, int i) {
+  return FOUR ? grp * (D / 32) + i : i * 4 + grp;
+}
+
+// 32 keys, as operands of the product (lane: key c16 of each 16, slot grp).  ONCE: read once,
+// past the caches.
+template <int D, bool FOUR, bool ONCE> struct Keys32 {
+  static constexpr int NDQ = D / 32;
+  typedef uint32_t codes_t __attribute__((ext_vector_type(NDQ)));
+  codes_t c[2];
+  uint32_t e[2];
+  bf16x8 k[2][FOUR ? 1 : NDQ];
+  template <typename V>
+  __device__ __forceinline__ static V fetch(const void* src) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(src));
+    else return *reinterpret_cast<const V*>(src);
   }
-  // K: lane (key c16, slot grp) holds elements grp D/4 + 8 i + j, as the decode
-  bf16x8 k[KW_KEYS / 16][NDQ];
-  bool lost[KW_KEYS / 32];
-#pragma unroll
-  for (int half = 0; half < KW_KEYS / 32; ++half) {
-    const int first = k0 + half * 32;  // 32 keys never cross a page
-    int pid = first < len ? ld_uniform(p.bt, b * p.bts + first / p.page) : 0;
-    lost[half] = (uint32_t)pid >= (uint32_t)p.npages;
-    if (lost[half]) pid = 0;
-    const int rel = first % p.page;
+  __device__ __forceinline__ void load(const KeyWeightParams& p, int pid, int kvh, int rel, int c16, int grp) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int row = rel + t * 16 + c16;
       if constexpr (FOUR) {
+        using F = Kv4<D>;
         const unsigned char* rec = reinterpret_cast<const unsigned char*>(p.pool) + pid * p.psb + kvh * p.psh;
-        const uint32_t* codes = reinterpret_cast<const uint32_t*>(rec + row * F::CB) + grp * NDQ;
-        const float scale = kv4_scale(rec[F::k_scales(p.page) + row * F::SB + grp * (D / 4) / 32]);
-#pragma unroll
-        for (int i = 0; i < NDQ; ++i) k[half * 2 + t][i] = kv4_bf16x8(codes[i], scale);
+        c[t] = fetch<codes_t>(rec + row * F::CB + grp * (D / 8));
+        e[t] = rec[F::k_scales(p.page.d) + row * F::SB + grp * (D / 4) / 32];
       } else {
-        const bf16* src = reinterpret_cast<const bf16*>(p.pool) + pid * p.psb + kvh * p.psh + row * p.pss + grp * (D / 4);
+        const bf16* src = reinterpret_cast<const bf16*>(p.pool) + pid * p.psb + kvh * p.psh + row * p.pss;
 #pragma unroll
-        for (int i = 0; i < NDQ; ++i) k[half * 2 + t][i] = Vec8<bf16>::load_bf16(src + i * 8);
+        for (int i = 0; i < NDQ; ++i) k[t][i] = fetch<bf16x8>(src + eight_of<D, FOUR>(grp, i) * 8);
       }
     }
   }
-  const int R = p.S * p.G;
-  const int hidden = p.causal ? len - p.S : 0x7fffffff;  // query s sees keys up to hidden + s
-  int r0 = 0;
-  if (p.causal && k0 > hidden) {
-    const int64_t first = (int64_t)(k0 - hidden) * p.G;  // rows before it see none of the wave's keys
-    r0 = (int)(first < R ? first : R) & ~15;
+  __device__ __forceinline__ bf16x8 operand(int t, int i) const {
+    if constexpr (FOUR) return kv4_bf16x8(c[t][i], kv4_scale(e[t]));
+    else return k[t][i];
   }
-  float acc[KW_KEYS / 16];
+};
+
+// Where a wave's keys lie: a lane holds the page of the 32 keys from `first` on, which never
+// cross one, and their first row there; past the last key its 32 again.  lost: the pages
+// that are none of the pool's, a bit a lane.
+struct KeyPages {
+  int pid, rel;
+  uint64_t lost;
+  __device__ __forceinline__ void load(const KeyWeightParams& p, int b, int first, int len) {
+    first = min(first, (len - 1) & ~31);
+    const int page = p.page.div(first, rel);
+    pid = p.bt[b * p.bts + page];
+    const bool bad = (uint32_t)pid >= (uint32_t)p.npages;
+    lost = __builtin_amdgcn_ballot_w64(bad);
+    if (bad) pid = 0;
+  }
+};
+
+// What a row's -lse adds to its scores, in log2 units: -inf (no weight) for a query that
+// sees no key and for rows past the last.
+__device__ __forceinline__ float row_offset(const KeyWeightParams& p, int b, int kvh, int r, int R) {
+  int g;
+  const int s = p.G.div(min(r, R - 1), g);
+  const float v = p.lse[((int64_t)b * p.Hq + kvh * p.G.d + g) * p.S + s];
+  return r >= R || v == -INFINITY ? -INFINITY : -v * kLog2e;
+}
+
+__device__ __forceinline__ float xor16_add(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- up to 16 rows (a decode step): every key's score in one MFMA tile.  HBM-bound: K read
+// once.  A wave has all its keys' loads in flight before the first product, 17 KB of 4-bit
+// keys: with 64 keys a wave, 64 sequences of up to 32768 keys (64/4 heads) took 108 us.
+template <int D, bool FOUR>
+__global__ void __launch_bounds__(256) key_weights_step_kernel(KeyWeightParams p) {
+  constexpr int NDQ = D / 32;
+  constexpr int RUN = FOUR ? 128 : 64;  // keys of a wave
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, grp = lane >> 4;
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const int k0 = (blockIdx.x * 4 + wave) * RUN;
+  if (k0 >= p.max_len) return;
+  const int len = ld_uniform(p.lens, b);
+  float* w = p.w + b * p.wsb + kvh * p.wsh;
+  const bool bad_len = len < 0 || len > p.max_len;
+  if (bad_len || k0 >= len) {  // no keys here
+    if (!p.add)
+      for (int t = k0 + lane; t < min(k0 + RUN, p.max_len); t += 64) w[t] = bad_len ? __builtin_nanf("") : 0.f;
+    return;
+  }
+  KeyPages at;
+  at.load(p, b, k0 + min(lane, RUN / 32 - 1) * 32, len);
+  const int R = p.S * p.G.d;
+  int g;
+  const int s = p.G.div(min(c16, R - 1), g);
+  const bf16* qrow = p.q + b * p.qsb + (int64_t)(kvh * p.G.d + g) * p.qsh + s * p.qss;
+  bf16x8 q[NDQ];
 #pragma unroll
-  for (int t = 0; t < KW_KEYS / 16; ++t) acc[t] = 0.f;
-  for (; r0 < R; r0 += 16) {
-    const int r = r0 + c16;
-    const bool valid = r < R;
-    const int s = (valid ? r : 0) / p.G, g = (valid ? r : 0) % p.G;
-    const bf16* qrow = p.q + b * p.qsb + (int64_t)(kvh * p.G + g) * p.qsh + s * p.qss + grp * (D / 4);
-    bf16x8 q[NDQ];
+  for (int i = 0; i < NDQ; ++i) q[i] = Vec8<bf16>::load_bf16(qrow + eight_of<D, FOUR>(grp, i) * 8);
+  float off[4];
+  int last[4];  // the last key that the row's query sees
 #pragma unroll
-    for (int i = 0; i < NDQ; ++i) q[i] = Vec8<bf16>::load_bf16(qrow + i * 8);
-    float off[4];
-    int last[4];
+  for (int e = 0; e < 4; ++e) {
+    const int re = grp * 4 + e;
+    off[e] = row_offset(p, b, kvh, re, R);
+    last[e] = p.causal ? len - p.S + p.G.div(re) : 0x7fffffff;
+  }
+  Keys32<D, FOUR, true> keys[RUN / 32];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int ri = r0 + grp * 4 + i, ok = ri < R;
-      const int si = (ok ? ri : 0) / p.G, gi = (ok ? ri : 0) % p.G;
-      const float v = p.lse[((int64_t)b * p.Hq + kvh * p.G + gi) * p.S + si];
-      off[i] = !ok || v == -INFINITY ? INFINITY : v * kLog2e;  // a row without keys, or past the last: no weight
-      last[i] = p.causal ? hidden + si : 0x7fffffff;
-    }
+  for (int i = 0; i < RUN / 32; ++i)
+    keys[i].load(p, __builtin_amdgcn_readlane(at.pid, i), kvh, __builtin_amdgcn_readlane(at.rel, i), c16, grp);
+  float old[RUN / 64];  // the weights so far
 #pragma unroll
-    for (int t = 0; t < KW_KEYS / 16; ++t) {
+  for (int i = 0; i < RUN / 64; ++i) {
+    const int t = min(k0 + i * 64 + lane, len - 1);
+    old[i] = p.add ? w[t] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < RUN / 64; ++i) {
+    float sum[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
       floatx4 sc = floatx4{};
 #pragma unroll
-      for (int i = 0; i < NDQ; ++i) sc = mfma16(q[i], k[t][i], sc);
-      const int key = k0 + t * 16 + c16;
+      for (int d = 0; d < NDQ; ++d) sc = mfma16(q[d], keys[2 * i + t / 2].operand(t & 1, d), sc);
+      const int key = k0 + i * 64 + t * 16 + c16;
+      float x = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = fast_exp2(__builtin_fmaf(sc[i], p.scale_log2, -off[i]));
-        acc[t] += key <= last[i] && off[i] != INFINITY ? e : 0.f;
+      for (int e = 0; e < 4; ++e) sc[e] = fast_exp2(__builtin_fmaf(sc[e], p.scale_log2, off[e]));
+      if (p.causal) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x += key <= last[e] ? sc[e] : 0.f;
+      } else {
+        x = (sc[0] + sc[1]) + (sc[2] + sc[3]);
       }
+      sum[t] = xor32_sum(xor16_add(x));
+      if (at.lost >> (2 * i + t / 2) & 1) sum[t] = __builtin_nanf("");
     }
+    const float mine = grp == 0 ? sum[0] : grp == 1 ? sum[1] : grp == 2 ? sum[2] : sum[3];
+    const int t = k0 + i * 64 + lane;
+    if (t < len) w[t] = old[i] + mine;
+    else if (!p.add && t < p.max_len) w[t] = 0.f;
   }
+}
+
+// ---- more rows (prompts): a workgroup holds a chunk of up to 256 rows in LDS, read once, and
+// its four waves pass their keys by it, 64 at a time, the next 64 on their way meanwhile.
+// No wave waits for another after the chunk is staged.  Bound by the exponentials' side: 16
+// rows and 64 keys take 16 x (4 + 8 + 4) cycles of scaling, exponential and sum, and the 16
+// products hold up the vector unit for some 11 cycles each of their 16.  Chunks > 1 write
+// partial sums that key_weights_sum_kernel adds, in order.
+constexpr int KW_ROWS = 256;   // rows of a chunk
+constexpr int KW_PASS = 256;   // keys that its waves take at a time
+
+// Ranges of keys that a chunk has: up to the last that its last query sees in a sequence of
+// max_len.  (In shorter ones it sees fewer; the workgroups past them find nothing to do.)
+__host__ __device__ __forceinline__ int chunk_ranges(const KeyWeightParams& p, int chunk) {
+  const int R = p.S * (int)p.G.d, end = R / KW_ROWS > chunk ? (chunk + 1) * KW_ROWS : R;
+  const int seen = p.causal ? p.max_len - p.S + p.G.div(end - 1) + 1 : p.max_len;
+  return seen > 0 ? p.range.div(seen + (int)p.range.d - 1) : 0;
+}
+
+template <int D, bool FOUR>
+__global__ void __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2)))
+key_weights_kernel(KeyWeightParams p) {
+  constexpr int NDQ = D / 32;
+  constexpr int RB = 2 * D, CPR = D / 8, RPB = 256 / RB;  // bytes and 16-byte chunks of a row, rows of 256 bytes
+  constexpr int PCS = KW_ROWS * CPR / 256;                // chunks a thread stages
+  __shared__ __attribute__((aligned(16))) unsigned char qt[KW_ROWS * RB];
+  __shared__ __attribute__((aligned(16))) float offs[KW_ROWS];
+  __shared__ __attribute__((aligned(16))) int lasts[KW_ROWS];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, grp = lane >> 4;
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  // the workgroups of chunk 0, then those of chunk 1, ...: as many as each has ranges, or
+  // (many chunks) as many as the last has
+  int chunk = 0, at_range = blockIdx.x;
+  if (p.same) {
+    chunk = blockIdx.x / p.same;
+    at_range = blockIdx.x % p.same;
+  } else {
+    for (int n; chunk + 1 < p.chunks && at_range >= (n = chunk_ranges(p, chunk)); ++chunk) at_range -= n;
+  }
+  const int range0 = at_range * (int)p.range.d;
+  const int len = ld_uniform(p.lens, b);
+  const bool bad_len = len < 0 || len > p.max_len;
+  const bool add = p.add && p.chunks == 1;
+  float* w = p.chunks > 1 ? p.part + (((int64_t)chunk * p.B + b) * p.Hkv + kvh) * p.max_len
+                          : p.w + b * p.wsb + kvh * p.wsh;
+  const int R = p.S * p.G.d, r0 = chunk * p.chunk_rows, rows = min(R - r0, p.chunk_rows);
+  const int hidden = p.causal ? len - p.S : 0x3fffffff;  // query s sees keys up to hidden + s
+  const int kend = rows > 0 ? min(len, p.causal ? hidden + p.G.div(r0 + rows - 1) + 1 : len) : 0;
+  if (bad_len || range0 >= kend) {  // no weight from this chunk
+    if (!add)
+      for (int t = range0 + threadIdx.x; t < min(range0 + (int)p.range.d, p.max_len); t += 256)
+        w[t] = bad_len ? __builtin_nanf("") : 0.f;
+    return;
+  }
+  // lane 2 i + u: half u of the wave's tile i, keys range0 + (4 i + wave) 64 + 32 u
+  const int tiles = p.range.d / KW_PASS;
+  KeyPages at;
+  {
+    const int l = min(lane, 2 * tiles - 1);
+    at.load(p, b, range0 + ((l >> 1) * 4 + wave) * 64 + (l & 1) * 32, len);
+  }
+  Keys32<D, FOUR, false> keys[2];
+  auto load_keys = [&](int i) {
 #pragma unroll
-  for (int t = 0; t < KW_KEYS / 16; ++t) {
-    acc[t] += shfl_xor_f(acc[t], 16);
-    acc[t] = xor32_sum(acc[t]);
-    if (lost[t / 2]) acc[t] = __builtin_nanf("");
+    for (int u = 0; u < 2; ++u)
+      keys[u].load(p, __builtin_amdgcn_readlane(at.pid, 2 * i + u), kvh, __builtin_amdgcn_readlane(at.rel, 2 * i + u), c16,
+                   grp);
+  };
+  load_keys(0);
+  {
+    // rows r0 + threadIdx.x / CPR + i STEP: the first by a division, each next by an addition
+    constexpr int STEP = 256 / CPR;
+    const int s0 = p.G.div(r0), qsh = (int)p.qsh, qss = (int)p.qss, G = (int)p.G.d;
+    const bf16* src = p.q + b * p.qsb + (int64_t)kvh * G * p.qsh + s0 * p.qss;  // 32-bit offsets from here
+    int g;
+    const int s = p.G.div(r0 + threadIdx.x / CPR, g);
+    int ds_g;
+    const int ds_s = p.G.div(STEP, ds_g);
+    const int step = ds_s * qss + ds_g * qsh, wrap = qss - G * qsh;
+    int row = threadIdx.x / CPR, at_row = (s - s0) * qss + g * qsh + (threadIdx.x % CPR) * 8;
+    unsigned char* dst = qt + row * RB + (((threadIdx.x % CPR) ^ ((row / RPB) % CPR)) << 4);
+    static_assert(STEP % (RPB * CPR) == 0, "the swizzle repeats every step");
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      bf16x8 piece[PCS / 2];
+#pragma unroll
+      for (int i = 0; i < PCS / 2; ++i) {
+        piece[i] = Vec8<bf16>::load_bf16(src + (row < rows ? at_row : 0));
+        row += STEP;
+        g += ds_g;
+        at_row += step + (g >= G ? wrap : 0);
+        g -= g >= G ? G : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < PCS / 2; ++i)
+        *reinterpret_cast<bf16x8*>(dst + (half * (PCS / 2) + i) * STEP * RB) = piece[i];
+    }
+    offs[threadIdx.x] = row_offset(p, b, kvh, r0 + threadIdx.x, r0 + rows);
+    lasts[threadIdx.x] = hidden + p.G.div(r0 + threadIdx.x);
   }
-  const float mine = grp == 0 ? acc[0] : grp == 1 ? acc[1] : grp == 2 ? acc[2] : acc[3];
-  const int t = k0 + lane;
-  if (t < len) w[t] = p.add ? w[t] + mine : mine;
-  else if (!p.add && t < p.max_len) w[t] = 0.f;
+  __syncthreads();
+  const int n = (rows + 15) / 16;
+  int qoff[NDQ];  // this lane's operands of 16 rows (the swizzle repeats every 16)
+#pragma unroll
+  for (int d = 0; d < NDQ; ++d) qoff[d] = c16 * RB + ((eight_of<D, FOUR>(grp, d) ^ ((c16 / RPB) % CPR)) << 4);
+
+#pragma unroll 1
+  for (int i = 0; i < tiles; ++i) {
+    const int k0 = range0 + (i * 4 + wave) * 64;
+    if (k0 >= p.max_len) break;
+    bf16x8 k[4][NDQ];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int d = 0; d < NDQ; ++d) k[t][d] = keys[t / 2].operand(t & 1, d);
+    if (i + 1 < tiles) load_keys(i + 1);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    auto pass = [&](int from, int to, auto masked) {
+      for (int rt = from; rt < to; ++rt) {
+        bf16x8 q[NDQ];
+#pragma unroll
+        for (int d = 0; d < NDQ; ++d) q[d] = *reinterpret_cast<const bf16x8*>(qt + rt * 16 * RB + qoff[d]);
+        floatx4 sc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sc[t] = floatx4{};
+#pragma unroll
+        for (int d = 0; d < NDQ; ++d)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) sc[t] = mfma16(q[d], k[t][d], sc[t]);
+        const floatx4 off = *reinterpret_cast<const floatx4*>(&offs[rt * 16 + grp * 4]);
+        int last[4];
+        if constexpr (decltype(masked)::value) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) last[e] = lasts[rt * 16 + grp * 4 + e];
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float pe = fast_exp2(__builtin_fmaf(sc[t][e], p.scale_log2, off[e]));
+            if constexpr (decltype(masked)::value) acc[t] += k0 + t * 16 + c16 <= last[e] ? pe : 0.f;
+            else acc[t] += pe;
+          }
+      }
+    };
+    // rows before `seen` see none of these keys, rows from `all` on see all of them
+    const int64_t G = p.G.d;
+    const int seen = p.causal ? (int)min(max((int64_t)(k0 - hidden) * G - r0, (int64_t)0), (int64_t)rows) / 16 : 0;
+    const int all =
+        p.causal ? ((int)min(max((int64_t)(k0 + 63 - hidden) * G - r0, (int64_t)0), (int64_t)(rows + 15)) + 15) / 16 : 0;
+    if (k0 < kend) {
+      pass(seen, min(all, n), std::true_type{});
+      pass(max(all, 0), n, std::false_type{});
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      acc[t] = xor32_sum(xor16_add(acc[t]));
+      if (at.lost >> (2 * i + t / 2) & 1) acc[t] = __builtin_nanf("");
+    }
+    const float mine = grp == 0 ? acc[0] : grp == 1 ? acc[1] : grp == 2 ? acc[2] : acc[3];
+    const int t = k0 + lane;
+    if (t < len) w[t] = add ? w[t] + mine : mine;
+    else if (!add && t < p.max_len) w[t] = 0.f;
+  }
+}
+
+// The chunks' partial sums, added in order: of the chunks whose ranges reach the key.
+__global__ void __launch_bounds__(256) key_weights_sum_kernel(KeyWeightParams p) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  if (t >= p.max_len) return;
+  const int range = p.range.div(t);
+  int c = 0;  // the first chunk that reaches the key (ranges grow with the chunk)
+  for (int hi = p.chunks; c < hi;) {
+    const int mid = (c + hi) / 2;
+    if (chunk_ranges(p, mid) <= range) c = mid + 1;
+    else hi = mid;
+  }
+  const float* src = p.part + ((int64_t)b * p.Hkv + kvh) * p.max_len + t;
+  const int64_t step = (int64_t)p.B * p.Hkv * p.max_len;
+  float sum = 0.f;
+#pragma unroll 4
+  for (; c < p.chunks; ++c) sum += src[c * step];
+  float* w = p.w + b * p.wsb + kvh * p.wsh + t;
+  const int len = ld_uniform(p.lens, b);
+  if (!p.add) *w = sum;
+  else if (len <= p.max_len && t < len) *w += sum;
+}
+
+// Chunks of the rows.
+static int key_weight_chunks(int64_t R) { return (int)((R + KW_ROWS - 1) / KW_ROWS); }
+
+// Workgroups of a (sequence, kv head).
+static int64_t key_weight_groups(const KeyWeightParams& p) {
+  int64_t n = 0;
+  for (int c = 0; c < p.chunks; ++c) n += chunk_ranges(p, c);
+  return n;
+}
+
+// Keys of a workgroup: the fewest with which all of them are resident at once, two a CU
+// (512 in all), so that none waits for another's end and each waits for its rows once; 1024
+// where more are needed anyway.  2 prompts of 2048, 16/8 heads, causal: 256 keys 48 us, 1024
+// 45, the 768 chosen 39 (480 workgroups); also launched for the ranges that a chunk does not
+// have, of which the XCDs get unequal shares, 56.
+constexpr int KW_FEW_CHUNKS = 64;
+static int key_weight_range(KeyWeightParams p) {
+  if (p.chunks <= KW_FEW_CHUNKS)
+    for (int range = KW_PASS; range <= 2048; range += KW_PASS) {
+      p.range = Divider(range);
+      if (key_weight_groups(p) * p.B * p.Hkv <= 512) return range;
+    }
+  return 1024;
 }
 
 // ---------------------------------------------------------------- selection
 // The rows that a (sequence, kv head) keeps: the first `first`, the last `recent`, and of
 // the rows between them the `keep - first - recent` heaviest, equal weights by the lower
-// index; in ascending order.  A workgroup of 16 waves per (sequence, head) finds the
-// smallest kept weight by a radix select over its bits (11 + 11 + 10, a histogram in LDS
-// for each), then writes the kept rows in order: each wave takes a contiguous share, and
-// its place in the output follows from the counts of the waves before it.
+// index; in ascending order.  A workgroup of 16 waves per (sequence, head), each with a
+// contiguous share of the weights, finds the smallest kept one by a radix select over its
+// bits (11 + 11 + 10, a histogram in LDS for each), then each wave writes its kept rows:
+// its place in the output follows from the counts of the waves before it.  The first 32
+// weights of a lane (32768 in all) stay in registers; of longer rows the rest is read five
+// times, from the cache.
 struct SelectParams {
   const float* w;
   int64_t wsb, wsh;
@@ -150,9 +420,9 @@ struct SelectParams {
   int Hkv, W, keep, recent, first;
 };
 
-constexpr int SEL_THREADS = 1024, SEL_WAVES = SEL_THREADS / 64, SEL_BINS = 2048;
+constexpr int SEL_THREADS = 1024, SEL_WAVES = SEL_THREADS / 64, SEL_BINS = 2048, SEL_HELD = 32;
 
-// Orders as the weights do: NaN above everything, -0 as +0.
+// Orders as the weights do: NaN above everything, -0 as +0.  0 is no weight's.
 __device__ __forceinline__ uint32_t weight_key(float f) {
   if (f != f) return 0xffffffffu;
   const uint32_t u = __float_as_uint(f + 0.0f);
@@ -164,10 +434,10 @@ __global__ void __launch_bounds__(SEL_THREADS) select_keys_kernel(SelectParams p
   __shared__ uint32_t wave_a[SEL_WAVES], wave_b[SEL_WAVES];
   __shared__ uint32_t found[2];
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float* w = p.w + b * p.wsb + h * p.wsh;
   int32_t* kept = p.kept + (int64_t)blockIdx.x * p.keep;
-  int n = p.lens[b];
+  int n = ld_uniform(p.lens, b);
   if (n < 0 || n > p.W) n = 0;  // not a length: nothing is kept
   if (n <= p.keep) {
     for (int i = tid; i < p.keep; i += SEL_THREADS) kept[i] = i < n ? i : -1;
@@ -179,17 +449,35 @@ __global__ void __launch_bounds__(SEL_THREADS) select_keys_kernel(SelectParams p
   for (int i = tid; i < p.recent; i += SEL_THREADS) kept[p.keep - p.recent + i] = hi + i;
   if (room == 0) return;
 
+  const int rounds = (hi - lo + SEL_THREADS - 1) / SEL_THREADS;  // 64 weights each
+  const int begin = min(lo + wave * rounds * 64, hi), end = min(begin + rounds * 64, hi);
+  uint32_t held[SEL_HELD];
+#pragma unroll
+  for (int r = 0; r < SEL_HELD; ++r)
+    if (r < rounds) held[r] = __float_as_uint(w[min(begin + r * 64 + lane, hi - 1)]);
+#pragma unroll
+  for (int r = 0; r < SEL_HELD; ++r) held[r] = begin + r * 64 + lane < end ? weight_key(__uint_as_float(held[r])) : 0u;
+  // f(key, index) for the wave's share, in order, all lanes each time; key 0: past the share
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int r = 0; r < SEL_HELD; ++r)
+      if (r < rounds) f(held[r], begin + r * 64 + lane);
+    for (int r = SEL_HELD; r < rounds; ++r) {
+      const int i = begin + r * 64 + lane;
+      f(i < end ? weight_key(w[i]) : 0u, i);
+    }
+  };
+
   uint32_t prefix = 0;  // the bits of the smallest kept key found so far
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     for (int i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = 0;
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += SEL_THREADS) {
-      const uint32_t key = weight_key(w[i]);
-      if (pass == 0 || key >> (shift + bits) == prefix >> (shift + bits))
+    each([&](uint32_t key, int) {
+      if (key && (pass == 0 || key >> (shift + bits) == prefix >> (shift + bits)))
         atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1u);
-    }
+    });
     __syncthreads();
     // counts from the top: thread t holds bins 2t and 2t + 1
     const uint32_t c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
@@ -216,14 +504,11 @@ __global__ void __launch_bounds__(SEL_THREADS) select_keys_kernel(SelectParams p
     __syncthreads();
   }
   // `room` of the keys equal to `prefix` are kept, the lowest indices
-  const int share = ((hi - lo + SEL_THREADS - 1) / SEL_THREADS) * 64;
-  const int begin = min(lo + wave * share, hi), end = min(begin + share, hi);
   uint32_t more = 0, same = 0;
-  for (int i = begin; i < end; i += 64) {
-    const uint32_t key = i + lane < end ? weight_key(w[i + lane]) : 0;
-    more += __popcll(__builtin_amdgcn_ballot_w64(i + lane < end && key > prefix));
-    same += __popcll(__builtin_amdgcn_ballot_w64(i + lane < end && key == prefix));
-  }
+  each([&](uint32_t key, int) {
+    more += __popcll(__builtin_amdgcn_ballot_w64(key > prefix));
+    same += __popcll(__builtin_amdgcn_ballot_w64(key == prefix));
+  });
   if (lane == 0) {
     wave_a[wave] = more;
     wave_b[wave] = same;
@@ -236,35 +521,36 @@ __global__ void __launch_bounds__(SEL_THREADS) select_keys_kernel(SelectParams p
   }
   at += min(ties, room);
   const uint64_t below = lane == 0 ? 0 : ~0ull >> (64 - lane);
-  for (int i = begin; i < end; i += 64) {
-    const bool in = i + lane < end;
-    const uint32_t key = in ? weight_key(w[i + lane]) : 0;
-    const uint64_t eq = __builtin_amdgcn_ballot_w64(in && key == prefix);
-    const bool take = in && (key > prefix || (key == prefix && ties + __popcll(eq & below) < room));
+  each([&](uint32_t key, int i) {
+    const uint64_t eq = __builtin_amdgcn_ballot_w64(key == prefix);
+    const bool take = key > prefix || (key == prefix && ties + __popcll(eq & below) < room);
     const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
     const uint32_t to = at + __popcll(taken & below);
-    if (take && to < (uint32_t)(p.keep - p.recent)) kept[to] = i + lane;  // (weights that change meanwhile)
+    if (take && to < (uint32_t)(p.keep - p.recent)) kept[to] = i;  // (weights that change meanwhile)
     at += __popcll(taken);
     ties += __popcll(eq);
-  }
+  });
 }
 
 // ---------------------------------------------------------------- moving rows
 // Row kept[b, h, i] of a sequence's pages to row i of its new pages, for every part of a
-// row (K and V rows; of 4-bit pages codes and scales), and its weight.  A thread per
-// piece of a row; HBM-bound, each kept row read and written once.
+// row (K and V rows; of 4-bit pages codes and scales), and its weight.  A workgroup moves
+// 64 rows: their places are worked out once, in LDS, then each thread has all its pieces
+// of a part in flight.  HBM-bound, each kept row read and written once, past the caches: 8
+// x 8 heads, 8192 of 32768 bf16 rows (D = 128, K and V, 537 MB) take 100 us, as a contiguous
+// copy of as much; through the caches 184.
 struct RowPart {
-  int64_t off;         // of the part within a page's head (bytes)
-  int stride, bytes;   // between rows, of a row
-  int pool;            // which pool
+  int64_t off;    // of the part within a page's head (bytes)
+  int stride;     // between rows (bytes)
+  int pool;        // which
+  Divider pieces;  // pieces of a row's part
 };
 struct CompactParams {
   unsigned char* pool[2];
   int64_t psb[2], psh[2];  // page and head strides (bytes)
   RowPart part[4];
-  int parts, unit[4], pieces[4];  // bytes of a piece, pieces of a row's part
-  int per_row;                    // pieces of a row, the weight's included
-  int npages, page, cols, new_cols;
+  int npages, cols, row_groups;
+  Divider page;
   const int32_t *bt, *new_bt;
   int64_t bts, nbts;
   const int32_t* kept;
@@ -274,38 +560,88 @@ struct CompactParams {
   int Hkv, keep, W;
 };
 
+constexpr int CP_ROWS = 64;  // rows of a workgroup
+
+// N pieces of a part that a thread has in flight.
+template <typename T, int N> struct Moves {
+  T v[N];
+  unsigned char* dst[N];
+  __device__ __forceinline__ void load(const CompactParams& p, const RowPart& q, int h, const int (*place)[4], int rows,
+                                       int first) {
+    unsigned char* pool = p.pool[q.pool] + h * p.psh[q.pool] + q.off;
+    const int64_t psb = p.psb[q.pool];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int id = first + u * 256;
+      dst[u] = nullptr;
+      if (id >= rows * (int)q.pieces.d) continue;
+      int piece;
+      const int* at = place[q.pieces.div(id, piece)];
+      if (at[0] < 0) continue;
+      const int o = piece * (int)sizeof(T);
+      v[u] = __builtin_nontemporal_load(reinterpret_cast<const T*>(pool + at[0] * psb + (int64_t)at[1] * q.stride + o));
+      dst[u] = pool + at[2] * psb + (int64_t)at[3] * q.stride + o;
+    }
+  }
+  __device__ __forceinline__ void store() {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (dst[u]) __builtin_nontemporal_store(v[u], reinterpret_cast<T*>(dst[u]));
+  }
+};
+
+// S: void for K and V pools, else a row's scales in 4-bit pages.
+template <typename S>
 __global__ void __launch_bounds__(256) compact_rows_kernel(CompactParams p) {
+  __shared__ int place[CP_ROWS][4];  // page and row: from, to; page -1: nothing to move
   const int b = blockIdx.z, h = blockIdx.y;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t moves = (int64_t)p.keep * p.per_row;
-  if (id >= moves) {  // weights of the rows that are no more
-    const int64_t t = id - moves + p.keep;
-    if (p.w_out && t < p.W) p.w_out[b * p.wsb + h * p.wsh + t] = 0.f;
+  if ((int)blockIdx.x >= p.row_groups) {  // weights of the rows that are no more
+    const int64_t t = (int64_t)((int)blockIdx.x - p.row_groups) * 256 + threadIdx.x + p.keep;
+    if (t < p.W) p.w_out[b * p.wsb + h * p.wsh + t] = 0.f;
     return;
   }
-  const int i = (int)(id / p.per_row);
-  int piece = (int)(id % p.per_row);
-  const int j = p.kept[((int64_t)b * p.Hkv + h) * p.keep + i];
-  const bool real = j >= 0 && j < p.cols * (int64_t)p.page;
-  int c = 0;
-  while (c < p.parts && piece >= p.pieces[c]) piece -= p.pieces[c++];
-  if (c == p.parts) {
-    if (p.w_out) p.w_out[b * p.wsb + h * p.wsh + i] = real && j < p.W ? p.w[b * p.wsb + h * p.wsh + j] : 0.f;
-    return;
+  const int i0 = blockIdx.x * CP_ROWS, rows = min(CP_ROWS, p.keep - i0);
+  if ((int)threadIdx.x < rows) {
+    const int i = i0 + threadIdx.x;
+    const int j = p.kept[((int64_t)b * p.Hkv + h) * p.keep + i];
+    int from = -1, to = -1, fr = 0, tr = 0;
+    if (j >= 0) {
+      const int col = p.page.div(j, fr);
+      if (col < p.cols) {
+        from = p.bt[b * p.bts + col];
+        to = p.new_bt[b * p.nbts + p.page.div(i, tr)];
+      }
+      if (p.w_out) p.w_out[b * p.wsb + h * p.wsh + i] = col < p.cols && j < p.W ? p.w[b * p.wsb + h * p.wsh + j] : 0.f;
+    } else if (p.w_out) {
+      p.w_out[b * p.wsb + h * p.wsh + i] = 0.f;
+    }
+    const bool real = (uint32_t)from < (uint32_t)p.npages && (uint32_t)to < (uint32_t)p.npages;
+    place[threadIdx.x][0] = real ? from : -1;
+    place[threadIdx.x][1] = fr;
+    place[threadIdx.x][2] = to;
+    place[threadIdx.x][3] = tr;
   }
-  if (!real) return;
-  const int from = p.bt[b * p.bts + j / p.page], to = p.new_bt[b * p.nbts + i / p.page];
-  if ((uint32_t)from >= (uint32_t)p.npages || (uint32_t)to >= (uint32_t)p.npages) return;  // not pages of the pool
-  const RowPart& q = p.part[c];
-  unsigned char* base = p.pool[q.pool] + h * p.psh[q.pool] + q.off;
-  const int64_t at = (int64_t)piece * p.unit[c];
-  const unsigned char* src = base + from * p.psb[q.pool] + (int64_t)(j % p.page) * q.stride + at;
-  unsigned char* dst = base + to * p.psb[q.pool] + (int64_t)(i % p.page) * q.stride + at;
-  switch (p.unit[c]) {
-    case 16: *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src); break;
-    case 4: *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src); break;
-    case 2: *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src); break;
-    default: *dst = *src;
+  __syncthreads();
+  // all loads before the stores: a store holds up what follows it for as long as a load
+  if constexpr (std::is_void<S>::value) {
+    for (int first = threadIdx.x; first < rows * (int)p.part[0].pieces.d; first += 256 * 4) {
+      Moves<bf16x8, 4> k, v;
+      k.load(p, p.part[0], h, place, rows, first);
+      v.load(p, p.part[1], h, place, rows, first);
+      k.store();
+      v.store();
+    }
+  } else {  // 64 rows of at most 64 code bytes: a piece a thread
+    Moves<bf16x8, 1> k, v;
+    Moves<S, 1> ks, vs;
+    k.load(p, p.part[0], h, place, rows, threadIdx.x);
+    v.load(p, p.part[1], h, place, rows, threadIdx.x);
+    ks.load(p, p.part[2], h, place, rows, threadIdx.x);
+    vs.load(p, p.part[3], h, place, rows, threadIdx.x);
+    k.store();
+    v.store();
+    ks.store();
+    vs.store();
   }
 }
 
@@ -321,10 +657,18 @@ static int evict_check_table(const int32_t* bt, int64_t stride, int cols, int pa
   return NQ_OK;
 }
 
+extern "C" int64_t nq_key_weights_workspace_bytes(int B, int Hq, int Hkv, int S, int max_len) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || S <= 0 || max_len <= 0 || Hq % Hkv) return 0;
+  const int64_t R = (int64_t)S * (Hq / Hkv);
+  const int64_t n = R <= 16 ? 1 : key_weight_chunks(R);
+  return n > 1 ? n * B * Hkv * max_len * (int64_t)sizeof(float) : 0;
+}
+
 extern "C" int nq_key_weights(const void* q, const int64_t* q_strides, const void* k_pool,
                               const int64_t* pool_strides, int four_bit, int num_pages, const int32_t* block_table,
                               int64_t bt_stride, int bt_cols, int page_size, const int32_t* lens, const float* lse,
-                              float* weights, const int64_t* weight_strides, int accumulate, int B, int Hq, int Hkv,
+                              float* weights, const int64_t* weight_strides, int accumulate, void* workspace,
+                              int64_t workspace_bytes, int B, int Hq, int Hkv,
                               int S, int D, int max_len, int causal, float sm_scale, void* stream) {
   nq_clear_error();
   if (!head_dim_ok(D)) return nq_fail(NQ_ERR_UNSUPPORTED, "head_dim must be 32, 64 or 128, got %d", D);
@@ -340,26 +684,59 @@ extern "C" int nq_key_weights(const void* q, const int64_t* q_strides, const voi
   if (!nq_aligned16(q) || !nq_aligned16(k_pool)) return nq_fail(NQ_ERR_INVALID, "q and the pool must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8) return nq_fail(NQ_ERR_INVALID, "q strides must be multiples of 16 bytes");
+  // a chunk of 256 rows is addressed with 32-bit offsets
+  if (q_strides[1] < 0 || q_strides[2] < 0 || q_strides[1] > (1 << 30) / (Hq / Hkv) || q_strides[2] > (1 << 30) / 257)
+    return nq_fail(NQ_ERR_UNSUPPORTED, "q strides of 256 rows exceed 2^30 elements, or are negative");
   for (int i = 0; i < (four_bit ? 2 : 3); ++i)
     if (pool_strides[i] % (four_bit ? 16 : 8)) return nq_fail(NQ_ERR_INVALID, "pool strides must be multiples of 16 bytes");
-  if (B > 65535 || Hkv > 65535 || (int64_t)S * (Hq / Hkv) > 0x3fffffff)
-    return nq_fail(NQ_ERR_UNSUPPORTED, "at most 65535 sequences and kv heads and 2^30 query rows a kv head");
+  if (B > 65535 || Hkv > 65535 || (int64_t)S * (Hq / Hkv) > (1 << 24) || max_len > (1 << 30))
+    return nq_fail(NQ_ERR_UNSUPPORTED, "at most 65535 sequences and kv heads, 2^24 query rows a kv head and 2^30 keys");
   KeyWeightParams p{};
   p.q = reinterpret_cast<const bf16*>(q); p.qsb = q_strides[0]; p.qsh = q_strides[1]; p.qss = q_strides[2];
   p.pool = k_pool; p.psb = pool_strides[0]; p.psh = pool_strides[1]; p.pss = four_bit ? 0 : pool_strides[2];
-  p.npages = num_pages; p.bt = block_table; p.bts = bt_stride; p.page = page_size;
+  p.npages = num_pages; p.bt = block_table; p.bts = bt_stride; p.page = Divider(page_size);
   p.lens = lens; p.lse = lse; p.w = weights; p.wsb = weight_strides[0]; p.wsh = weight_strides[1];
-  p.add = accumulate != 0; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.S = S; p.max_len = max_len;
+  p.add = accumulate != 0; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Divider(Hq / Hkv); p.S = S; p.max_len = max_len;
   p.causal = causal != 0 && S > 1;
   p.scale_log2 = (sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)D)) * kLog2e;
-  const dim3 grid((unsigned)((max_len + KW_BLOCK - 1) / KW_BLOCK), (unsigned)Hkv, (unsigned)B);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return nq_check_launch(with_head_dim(D, [&](auto dc) {
+  const int64_t R = (int64_t)S * p.G.d;
+  if (R <= 16) {
+    const int run = four_bit ? 512 : 256;  // keys of a workgroup
+    const dim3 grid((unsigned)((max_len + run - 1) / run), (unsigned)Hkv, (unsigned)B);
+    return nq_check_launch(with_head_dim(D, [&](auto dc) {
+      constexpr int DD = decltype(dc)::value;
+      if (four_bit) hipLaunchKernelGGL((key_weights_step_kernel<DD, true>), grid, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((key_weights_step_kernel<DD, false>), grid, dim3(256), 0, st, p);
+      return hipGetLastError();
+    }));
+  }
+  p.chunks = key_weight_chunks(R);
+  p.chunk_rows = KW_ROWS;
+  if (p.chunks > 1) {
+    const int64_t need = nq_key_weights_workspace_bytes(B, Hq, Hkv, S, max_len);
+    if (!workspace || workspace_bytes < need || !nq_aligned16(workspace))
+      return nq_fail(NQ_ERR_WORKSPACE, "an aligned workspace of %lld bytes is required, %lld given", (long long)need,
+                     (long long)workspace_bytes);
+    p.part = reinterpret_cast<float*>(workspace);
+  }
+  p.range = Divider(key_weight_range(p));
+  if (p.chunks > KW_FEW_CHUNKS) p.same = p.range.div(max_len + (int)p.range.d - 1);
+  const int64_t groups = p.same ? (int64_t)p.chunks * p.same : key_weight_groups(p);
+  if (groups > 0x7fffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more query rows and keys than one launch takes");
+  const dim3 grid((unsigned)groups, (unsigned)Hkv, (unsigned)B);
+  hipError_t e = with_head_dim(D, [&](auto dc) {
     constexpr int DD = decltype(dc)::value;
     if (four_bit) hipLaunchKernelGGL((key_weights_kernel<DD, true>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((key_weights_kernel<DD, false>), grid, dim3(256), 0, st, p);
     return hipGetLastError();
-  }));
+  });
+  if (e == hipSuccess && p.chunks > 1) {
+    hipLaunchKernelGGL(key_weights_sum_kernel, dim3((unsigned)((max_len + 255) / 256), (unsigned)Hkv, (unsigned)B), dim3(256),
+                       0, st, p);
+    e = hipGetLastError();
+  }
+  return nq_check_launch(e);
 }
 
 extern "C" int nq_select_keys(const float* weights, const int64_t* weight_strides, const int32_t* lens, int32_t* kept,
@@ -402,18 +779,16 @@ extern "C" int nq_kv_compact(void* k_pool, const int64_t* k_strides, void* v_poo
   if (four) {
     if (!head_dim_ok(head_dim)) return nq_fail(NQ_ERR_UNSUPPORTED, "head_dim must be 32, 64 or 128, got %d", head_dim);
     const int cb = head_dim / 2, sb = head_dim / 32;
-    p.parts = 4;
-    p.part[0] = RowPart{0, cb, cb, 0};
-    p.part[1] = RowPart{(int64_t)page_size * cb, cb, cb, 0};
-    p.part[2] = RowPart{(int64_t)page_size * 2 * cb, sb, sb, 0};
-    p.part[3] = RowPart{(int64_t)page_size * (2 * cb + sb), sb, sb, 0};
+    p.part[0] = RowPart{0, cb, 0, Divider(cb / 16)};
+    p.part[1] = RowPart{(int64_t)page_size * cb, cb, 0, Divider(cb / 16)};
+    p.part[2] = RowPart{(int64_t)page_size * 2 * cb, sb, 0, Divider(1)};
+    p.part[3] = RowPart{(int64_t)page_size * (2 * cb + sb), sb, 0, Divider(1)};
   } else {
     if (row_bytes <= 0 || row_bytes % 16 || row_bytes > (1 << 20) || k_strides[2] < row_bytes || v_strides[2] < row_bytes ||
         k_strides[2] > (1 << 30) || v_strides[2] > (1 << 30))
       return nq_fail(NQ_ERR_INVALID, "rows must be multiples of 16 bytes that do not overlap, got %d", row_bytes);
-    p.parts = 2;
-    p.part[0] = RowPart{0, (int)k_strides[2], row_bytes, 0};
-    p.part[1] = RowPart{0, (int)v_strides[2], row_bytes, 1};
+    p.part[0] = RowPart{0, (int)k_strides[2], 0, Divider(row_bytes / 16)};
+    p.part[1] = RowPart{0, (int)v_strides[2], 1, Divider(row_bytes / 16)};
     p.pool[1] = reinterpret_cast<unsigned char*>(v_pool); p.psb[1] = v_strides[0]; p.psh[1] = v_strides[1];
   }
   p.pool[0] = reinterpret_cast<unsigned char*>(k_pool); p.psb[0] = k_strides[0]; p.psh[0] = k_strides[1];
@@ -421,21 +796,18 @@ extern "C" int nq_kv_compact(void* k_pool, const int64_t* k_strides, void* v_poo
     if (!nq_aligned16(p.pool[i]) || p.psb[i] % 16 || p.psh[i] % 16 || (!four && (i ? v_strides : k_strides)[2] % 16))
       return nq_fail(NQ_ERR_INVALID, "the pools and their strides must be multiples of 16 bytes");
   }
-  p.per_row = 1;
-  for (int i = 0; i < p.parts; ++i) {
-    const int n = p.part[i].bytes;
-    p.unit[i] = n % 16 == 0 ? 16 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1;
-    p.pieces[i] = n / p.unit[i];
-    p.per_row += p.pieces[i];
-  }
-  p.npages = num_pages; p.page = page_size; p.cols = bt_cols; p.new_cols = new_cols;
+  p.npages = num_pages; p.page = Divider(page_size); p.cols = bt_cols;
   p.bt = block_table; p.bts = bt_stride; p.new_bt = new_table; p.nbts = new_stride;
   p.kept = kept; p.w = weights; p.w_out = weights_out;
   if (weights) { p.wsb = weight_strides[0]; p.wsh = weight_strides[1]; }
   p.Hkv = Hkv; p.keep = keep; p.W = weights ? width : keep;
-  const int64_t threads = (int64_t)keep * p.per_row + (p.W - keep);
-  if (threads > 0xffffffffll) return nq_fail(NQ_ERR_UNSUPPORTED, "more kept rows than one launch moves");
-  hipLaunchKernelGGL(compact_rows_kernel, dim3((unsigned)((threads + 255) / 256), (unsigned)Hkv, (unsigned)B), dim3(256),
-                     0, reinterpret_cast<hipStream_t>(stream), p);
+  p.row_groups = (keep + CP_ROWS - 1) / CP_ROWS;
+  const int64_t groups = p.row_groups + ((int64_t)p.W - keep + 255) / 256;
+  const dim3 grid((unsigned)groups, (unsigned)Hkv, (unsigned)B);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (!four) hipLaunchKernelGGL((compact_rows_kernel<void>), grid, dim3(256), 0, st, p);
+  else if (head_dim == 128) hipLaunchKernelGGL((compact_rows_kernel<uint32_t>), grid, dim3(256), 0, st, p);
+  else if (head_dim == 64) hipLaunchKernelGGL((compact_rows_kernel<uint16_t>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((compact_rows_kernel<unsigned char>), grid, dim3(256), 0, st, p);
   return nq_check_launch(hipGetLastError());
 }

@@ -318,11 +318,14 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
     _sizes("attention_key_weights", B, Hq, S)
     lens_t = _lens(lens, B, dev)
     q, lse = ops._rows_in(q), lse.contiguous()
+    lib = _lib.load()
+    need = lib.nq_key_weights_workspace_bytes(B, Hq, H, S, int(max_len))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     ptr = ops._ptr
     args = (ptr(q), _lib.strides3(q.stride()[:3]), ptr(k_pool), _lib.strides3(k_pool.stride()[:3]), int(four), n,
             ptr(bt), bt.stride(0), bt.shape[1], P, ptr(lens_t), ptr(lse), ptr(weights), _strides2(weights), int(add),
-            B, Hq, H, S, D, int(max_len), int(bool(causal)), 0.0 if sm_scale is None else float(sm_scale))
-    call = _DeviceCall(q, _lib.load().nq_key_weights, args, "nq_key_weights", (q, k_pool, bt, lens_t, lse), weights)
+            ptr(ws), need, B, Hq, H, S, D, int(max_len), int(bool(causal)), 0.0 if sm_scale is None else float(sm_scale))
+    call = _DeviceCall(q, lib.nq_key_weights, args, "nq_key_weights", (q, k_pool, bt, lens_t, lse, ws), weights)
     return call if plan else call.launch()
 
 

@@ -341,6 +341,8 @@ def check_weights(w, q, kv, table, lens, lse, scale, causal=True, base=None):
     (1, 4, 1, 128, 64, 100, [612]),
     (2, 4, 4, 64, 32, 257, [257, 300]),
     (1, 5, 1, 128, 32, 33, [2000]),
+    (2, 16, 2, 64, 64, 300, [1700, 301]),
+    (1, 64, 2, 32, 32, 600, [900]),
 ])
 def test_key_weights(B, Hq, Hkv, D, P, S, lens, four):
     say(f"key weights B{B} {Hq}/{Hkv} D{D} P{P} S{S} four={four}")
