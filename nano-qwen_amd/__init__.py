@@ -28,7 +28,11 @@ reference's preference and policy loops compose from tensor operations;
 Extensions with no reference counterpart: ``generate_greedy_batch`` (ragged
 batched greedy decoding against per-row cache lengths), ``PagedKVCache``
 (block-table page pool), ``attention_decode_paged`` (decode with the new
-token's K/V append fused in) and ``kv_append_paged``.
+token's K/V append fused in) and ``kv_append_paged``; ``PagedKVCache4``, a page
+pool that holds its rows in 4 bits (``kv4_append``, ``kv4_gather``,
+``attention_decode_kv4``), and ``PagedKVCache.evict``, which keeps the keys that
+got the most attention weight (``attention_key_weights``, ``select_keys``,
+``kv_compact``).
 """
 
 from .config import AttentionConfig
@@ -37,7 +41,7 @@ from .ops import (apply_rope, attention_decode, attention_decode_paged, attentio
                   decode_workspace_bytes, flash_attention, kv_append_paged, qk_norm_rope)
 from .norm import RMSNorm
 from .rope import RotaryEmbedding, apply_rotary_pos_emb, build_tables
-from .attention import Attention, KVCache, PagedKVCache, stats
+from .attention import Attention, KVCache, PagedKVCache, PagedKVCache4, stats
 from .model import ModelConfig, Qwen3Model, TransformerBlock
 from .generate import TextGenerator, generate_greedy_batch
 from .ops import attention_backward, attention_merge_, qk_norm_rope_backward
@@ -52,7 +56,7 @@ __all__ = [
     "apply_rotary_pos_emb", "build_tables", "flash_attention", "apply_rope",
     "qk_norm_rope", "attention_prefill", "attention_prefill_paged", "attention_decode", "decode_workspace_bytes", "stats",
     "ModelConfig", "Qwen3Model", "TransformerBlock", "TextGenerator", "generate_greedy_batch",
-    "PagedKVCache", "attention_decode_paged", "kv_append_paged",
+    "PagedKVCache", "PagedKVCache4", "attention_decode_paged", "kv_append_paged",
     "attention_merge_", "RingAttention", "ring_step", "ring_schedule", "split_sequence",
     "ring_attention_all_ranks", "attention_backward", "qk_norm_rope_backward", "attention_core",
     "flash_attention_train", "token_logprobs", "linear_logprobs", "preference_loss", "policy_loss",

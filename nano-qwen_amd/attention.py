@@ -44,7 +44,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 
-from . import autograd, ops
+from . import autograd, kv4, ops
 from .config import num_kv_groups
 from .norm import RMSNorm
 from .rope import RotaryEmbedding
@@ -260,14 +260,25 @@ class PagedKVCache:
     per-sequence lengths on the device; ``host_lens`` mirrors them (every
     step adds a known number of rows), so page allocation never reads the
     device.  ``set_lengths`` trims right-padded prompts after a batched
-    prefill, as ``KVCache.set_lengths`` does.
+    prefill, as ``KVCache.set_lengths`` does; ``expect_lengths`` says before it
+    how long they are, and it trims them itself.
+
+    With ``track_weights`` (bf16 models) ``weights`` (B, Hkv, rows) sums the
+    attention weight that each cached key gets, over query heads and over the
+    queries of each one-token step and the last ``track_weights`` of each longer
+    forward; ``evict`` then keeps the keys that got most.  A sequence's rows
+    close up, its positions go on: row r of sequence b stands at position
+    r + evicted[b] or before, and the next token at host_lens[b] + evicted[b].
     """
 
-    def __init__(self, num_pages: int, page_size: int = 64, max_pages_per_seq: Optional[int] = None):
+    def __init__(self, num_pages: int, page_size: int = 64, max_pages_per_seq: Optional[int] = None, *,
+                 track_weights: int = 0):
         if page_size <= 0 or page_size % 32:
             raise ValueError(f"page_size must be a positive multiple of 32, got {page_size}")
         if num_pages <= 0:
             raise ValueError("num_pages must be positive")
+        if track_weights < 0:
+            raise ValueError(f"track_weights is a number of queries, got {track_weights}")
         self.num_pages = num_pages
         self.page_size = page_size
         self.max_pages_per_seq = max_pages_per_seq or num_pages
@@ -279,6 +290,11 @@ class PagedKVCache:
         self.host_lens: list = []
         self._pages: list = []
         self._free = list(range(num_pages - 1, -1, -1))
+        self.track_weights = int(track_weights)
+        self.weights: Optional[torch.Tensor] = None
+        self.evicted: list = []                      # rows evicted of each sequence
+        self._shift: Optional[torch.Tensor] = None   # the same on the device, None while all are 0
+        self._expected: Optional[list] = None
 
     # -- sizes
     @property
@@ -290,7 +306,7 @@ class PagedKVCache:
     def free_pages(self) -> int:
         return len(self._free)
 
-    def _setup(self, B: int, H: int, D: int, dtype, device) -> None:
+    def _make_pools(self, H: int, D: int, dtype, device) -> None:
         if self.k_pool is None:
             shape = (self.num_pages, H, self.page_size, D)
             self.k_pool = torch.empty(shape, dtype=dtype, device=device)
@@ -298,11 +314,19 @@ class PagedKVCache:
         elif (self.k_pool.shape[1], self.k_pool.shape[3]) != (H, D) or self.k_pool.dtype != dtype:
             raise ValueError(f"pool holds {tuple(self.k_pool.shape)} {self.k_pool.dtype}, "
                              f"rows have Hkv={H} D={D} {dtype}")
+
+    def _setup(self, B: int, H: int, D: int, dtype, device) -> None:
+        if self.track_weights and dtype != torch.bfloat16:
+            raise TypeError(f"attention weights are tracked for bfloat16 models, got {dtype}")
+        self._make_pools(H, D, dtype, device)
         if self.block_table is None:
             self.block_table = torch.zeros(B, self.max_pages_per_seq, dtype=torch.int32, device=device)
             self.lens = torch.zeros(B, dtype=torch.int32, device=device)
             self.host_lens = [0] * B
             self._pages = [[] for _ in range(B)]
+            self.evicted = [0] * B
+            if self.track_weights:
+                self.weights = torch.zeros(B, H, self.max_pages_per_seq * self.page_size, device=device)
         elif self.block_table.shape[0] != B:
             raise ValueError(f"cache holds {self.block_table.shape[0]} sequences, the batch has {B}")
 
@@ -319,11 +343,14 @@ class PagedKVCache:
                 self._pages[b].append(self._free.pop())
                 changed = True
         if changed:
-            host = torch.zeros(self.block_table.shape, dtype=torch.int32)
-            for b, pages in enumerate(self._pages):
-                if pages:
-                    host[b, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
-            self.block_table.copy_(host, non_blocking=False)
+            self._write_table()
+
+    def _write_table(self) -> None:
+        host = torch.zeros(self.block_table.shape, dtype=torch.int32)
+        for b, pages in enumerate(self._pages):
+            if pages:
+                host[b, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        self.block_table.copy_(host, non_blocking=False)
 
     def _spare_lens(self) -> torch.Tensor:
         if self._lens_spare is None:
@@ -344,8 +371,97 @@ class PagedKVCache:
             keep = -(-n // self.page_size)
             while len(self._pages[b]) > keep:
                 self._free.append(self._pages[b].pop())
+        if self.weights is not None:
+            for b, n in enumerate(vals):
+                if n < self.host_lens[b]:
+                    self.weights[b, :, n:self.host_lens[b]] = 0
+        if any(n == 0 and e for n, e in zip(vals, self.evicted)):  # a sequence that begins anew
+            self.evicted = [e if n else 0 for n, e in zip(vals, self.evicted)]
+            self._write_shift()
         self.host_lens = vals
         self.lens.copy_(torch.tensor(vals, dtype=torch.int32))
+
+    def expect_lengths(self, lens) -> None:
+        """The next multi-token forward is right-padded: sequence b's chunk holds lens[b] tokens."""
+        vals = [int(x) for x in (lens.tolist() if torch.is_tensor(lens) else lens)]
+        if any(n < 1 for n in vals):
+            raise ValueError("every sequence needs at least one token")
+        self._expected = vals
+
+    # -- positions and weights
+    def _write_shift(self) -> None:
+        if not any(self.evicted):
+            self._shift = None
+            return
+        host = torch.tensor(self.evicted, dtype=torch.int32)
+        if self._shift is None:
+            self._shift = host.to(self.lens.device)
+        else:
+            self._shift.copy_(host)
+
+    def _next_positions(self) -> Optional[torch.Tensor]:
+        """Each sequence's next position (device), None while it is its length."""
+        return None if self._shift is None else self.lens + self._shift
+
+    def _take_expected(self, B: int, S: int) -> Optional[list]:
+        """What ``expect_lengths`` said of a chunk of S tokens."""
+        want, self._expected = self._expected, None
+        if want is not None and (len(want) != B or max(want) > S):
+            raise ValueError(f"expected lengths {want} do not fit a chunk of {S} tokens of {B} sequences")
+        return want
+
+    def _key_pool(self) -> torch.Tensor:
+        return self.k_pool
+
+    def _pools(self):
+        return self.k_pool, self.v_pool
+
+    def _add_weights(self, q_hat: torch.Tensor, lse: torch.Tensor) -> None:
+        """Add the weights of queries q_hat (B, Hq, S, D), the last S tokens of each sequence."""
+        kv4.attention_key_weights(q_hat, self._key_pool(), self.block_table, self.lens, lse,
+                                  max_len=max(max(self.host_lens), 1), weights=self.weights)
+
+    def evict(self, keep: int, *, recent: int = 0, first: int = 0) -> None:
+        """Cut every sequence of more than ``keep`` rows to that many: its first ``first``, its
+        last ``recent`` and, for each kv head, those of the rest with the most attention weight.
+
+        The kept rows move to other pages (as many as they need have to be free, for one
+        sequence at a time at least) and the old ones return to the pool.  Attention treats
+        them as before: their keys hold the positions they were rotated at.
+        """
+        if self.weights is None:
+            raise ValueError("evict needs a filled cache that tracks weights (track_weights)")
+        if keep <= 0 or recent < 0 or first < 0 or recent + first > keep:
+            raise ValueError(f"keep must be positive and hold first + recent, got {keep}, {first} and {recent}")
+        todo = [b for b, n in enumerate(self.host_lens) if n > keep]
+        each = -(-keep // self.page_size)
+        while todo:
+            n = min(len(todo), len(self._free) // each)
+            if n == 0:
+                raise RuntimeError(f"PagedKVCache is out of pages: evicting needs {each} free ones")
+            self._evict_some(todo[:n], keep, recent, first, each)
+            todo = todo[n:]
+
+    def _evict_some(self, rows: list, keep: int, recent: int, first: int, each: int) -> None:
+        dev = self.lens.device
+        new = [[self._free.pop() for _ in range(each)] for _ in rows]
+        whole = len(rows) == len(self.host_lens)
+        at = None if whole else torch.tensor(rows, device=dev)
+        table, lens, weights = ((t if whole else t.index_select(0, at)) for t in (self.block_table, self.lens, self.weights))
+        kept = kv4.select_keys(weights, lens, keep=keep, recent=recent, first=first)
+        w = kv4.kv_compact(self._pools(), table, torch.tensor(new, dtype=torch.int32).to(dev), kept, weights=weights)
+        if whole:
+            self.weights.copy_(w)
+        else:
+            self.weights.index_copy_(0, at, w)
+        for b, pages in zip(rows, new):
+            self._free.extend(reversed(self._pages[b]))
+            self._pages[b] = pages
+            self.evicted[b] += self.host_lens[b] - keep
+            self.host_lens[b] = keep
+        self._write_table()
+        self._write_shift()
+        self.lens.copy_(torch.tensor(self.host_lens, dtype=torch.int32))
 
     def free(self, b: int) -> None:
         """Drop sequence b (its pages return to the pool; its length becomes 0)."""
@@ -358,6 +474,10 @@ class PagedKVCache:
         self._lens_spare = None
         self.host_lens = []
         self._pages = []
+        self.weights = None
+        self.evicted = []
+        self._shift = None
+        self._expected = None
 
     def gather(self, b: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """Sequence b's K-hat and V as dense (Hkv, lens[b], D) tensors (a device copy)."""
@@ -366,6 +486,41 @@ class PagedKVCache:
         k = self.k_pool.index_select(0, pages).transpose(0, 1).reshape(self.k_pool.shape[1], -1, self.k_pool.shape[3])
         v = self.v_pool.index_select(0, pages).transpose(0, 1).reshape(self.v_pool.shape[1], -1, self.v_pool.shape[3])
         return k[:, :n], v[:, :n]
+
+
+class PagedKVCache4(PagedKVCache):
+    """A ``PagedKVCache`` whose rows are held in 4 bits: 17/64 of a bf16 cache's bytes.
+
+    Each block of 32 elements of a row is E2M1 codes and a power of two (4.25 bits an
+    element; ``kv4``), for bf16 and fp32 models.  A one-token forward stores its row and
+    attends what is stored, itself included.  A longer forward attends its own rows as they
+    are and the history as stored, and stores its rows.  ``pool`` is the uint8 page pool,
+    ``gather`` returns a sequence's rows as stored, in the model's type.
+    """
+
+    def __init__(self, num_pages: int, page_size: int = 64, max_pages_per_seq: Optional[int] = None, *,
+                 track_weights: int = 0):
+        super().__init__(num_pages, page_size, max_pages_per_seq, track_weights=track_weights)
+        self.pool: Optional[torch.Tensor] = None
+        self.dtype: Optional[torch.dtype] = None
+
+    def _make_pools(self, H: int, D: int, dtype, device) -> None:
+        if self.pool is None:
+            self.pool = kv4.kv4_empty_pool(self.num_pages, H, self.page_size, D, device)
+            self.dtype = dtype
+        elif (self.pool.shape[1], self.pool.shape[3]) != (H, 17 * D // 16) or self.dtype != dtype:
+            raise ValueError(f"pool holds {tuple(self.pool.shape)} of {self.dtype} rows, rows have Hkv={H} D={D} {dtype}")
+
+    def _key_pool(self) -> torch.Tensor:
+        return self.pool
+
+    def _pools(self):
+        return self.pool
+
+    def gather(self, b: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Sequence b's K-hat and V as stored, dense (Hkv, lens[b], D) tensors."""
+        k, v = kv4.kv4_gather(self.pool, self.block_table[b:b + 1], S=self.host_lens[b], dtype=self.dtype)
+        return k[0], v[0]
 
 
 class Attention(nn.Module):
@@ -537,30 +692,106 @@ class Attention(nn.Module):
         past = list(cache.host_lens)
         new = [n + S for n in past]
         if position_ids is None:  # positions continue from each sequence's length
-            ops.check_position_span(0, max(new), self.rotary_emb.max_position_embeddings)
-        cache._grow(new)
+            ops.check_position_span(0, max(n + e for n, e in zip(new, cache.evicted)),
+                                    self.rotary_emb.max_position_embeddings)
+        rot = {"eps": eps, "cos": cos, "sin": sin}
+        expected = cache._take_expected(B, S)
         if S == 1:
-            lens, lens_next = cache.lens, cache._spare_lens()
-            qp = position_ids
-            o = ops.attention_decode_paged(q4, cache.k_pool, cache.v_pool, cache.block_table, lens,
-                                           max_len=max(new), k_new=k4, v_new=v4, k_weight=kw,
-                                           lens_out=lens_next, q_weight=qw, eps=eps, cos=cos, sin=sin,
-                                           q_pos=qp, q_pos0=-1)
-            cache.lens, cache._lens_spare = lens_next, lens
-            cache.host_lens = new
+            cache._grow(new)
+            step = self._paged4_step if isinstance(cache, PagedKVCache4) else self._paged_step
+            o = step(q4, k4, v4, position_ids, cache, max(new), rot, qw, kw)
             return self.o_proj(o.reshape(B, 1, H * D))
         if len(set(past)) != 1:
             raise NotImplementedError("a multi-token forward into a PagedKVCache needs every sequence "
                                       "at the same length")
+        cache._grow(new)
         p0 = past[0]
-        pos = {"position_ids": position_ids} if position_ids is not None else {"pos_offset": p0}
-        # the chunk's K-hat (QK-Norm + RoPE fused) and V rows go into their
-        # pages, then its queries attend all p0 + S keys through the block
-        # table: no dense copy of the cache
-        ops.kv_append_paged(k4, v4, cache.k_pool, cache.v_pool, cache.block_table, k_weight=kw,
-                            eps=eps, cos=cos, sin=sin, row_offset=p0, **pos)
-        o = ops.attention_prefill_paged(q4, cache.k_pool, cache.v_pool, cache.block_table, T=p0 + S,
-                                        q_weight=qw, eps=eps, cos=cos, sin=sin, causal=True, **pos)
+        at = cache._next_positions()
+        if position_ids is not None:
+            pos = {"position_ids": position_ids}
+        else:
+            pos = {"pos_offset": p0} if at is None else {"pos_base": at}
+        track = cache.track_weights
+        if isinstance(cache, PagedKVCache4):
+            o, lse = self._paged4_chunk(q4, k4, v4, cache, p0, pos, rot, qw, kw)
+        else:
+            # the chunk's K-hat (QK-Norm + RoPE fused) and V rows go into their
+            # pages, then its queries attend all p0 + S keys through the block
+            # table: no dense copy of the cache
+            ops.kv_append_paged(k4, v4, cache.k_pool, cache.v_pool, cache.block_table, k_weight=kw,
+                                row_offset=p0, **rot, **pos)
+            o = ops.attention_prefill_paged(q4, cache.k_pool, cache.v_pool, cache.block_table, T=p0 + S,
+                                            q_weight=qw, causal=True, return_lse=bool(track), **rot, **pos)
+            o, lse = o if track else (o, None)
         cache.lens.add_(S)
         cache.host_lens = new
+        if expected is not None:
+            cache.set_lengths([p0 + n for n in expected])
+        if track:
+            q_hat, _, _ = ops.qk_norm_rope(q=q4, q_weight=qw, **rot, **pos)
+            self._observe(cache, q_hat, lse, expected, min(track, S))
         return self.o_proj(o.transpose(1, 2).reshape(B, S, H * D))
+
+    @staticmethod
+    def _observe(cache, q_hat, lse, expected, W):
+        """Add the weights of the last W queries of each sequence's chunk."""
+        B, H, S, D = q_hat.shape
+        if expected is None or min(expected) == S:
+            cache._add_weights(q_hat[:, :, S - W:], lse[:, :, S - W:])
+            return
+        # right-padded: the last W real ones; of a chunk with fewer the rest count for nothing
+        ends = torch.tensor(expected, device=q_hat.device)[:, None] - W + torch.arange(W, device=q_hat.device)
+        rows = ends.clamp(min=0)[:, None, :].expand(B, H, W)
+        q_win = q_hat.gather(2, rows[..., None].expand(B, H, W, D))
+        lse_win = lse.gather(2, rows).masked_fill(ends[:, None] < 0, float("-inf"))
+        cache._add_weights(q_win, lse_win)
+
+    def _paged_step(self, q4, k4, v4, position_ids, cache, longest, rot, qw, kw):
+        lens, lens_next = cache.lens, cache._spare_lens()
+        qp = position_ids if position_ids is not None else cache._next_positions()
+        o = ops.attention_decode_paged(q4, cache.k_pool, cache.v_pool, cache.block_table, lens,
+                                       max_len=longest, k_new=k4, v_new=v4, k_weight=kw,
+                                       lens_out=lens_next, q_weight=qw, q_pos=qp, q_pos0=-1,
+                                       return_lse=bool(cache.track_weights), **rot)
+        cache.lens, cache._lens_spare = lens_next, lens
+        cache.host_lens = [n + 1 for n in cache.host_lens]
+        if cache.track_weights:
+            o, lse = o
+            pos = {"pos_base": lens} if qp is None else {"position_ids": qp.reshape(-1, 1)}
+            q_hat, _, _ = ops.qk_norm_rope(q=q4, q_weight=qw, **rot, **pos)
+            cache._add_weights(q_hat, lse)
+        return o
+
+    def _paged4_step(self, q4, k4, v4, position_ids, cache, longest, rot, qw, kw):
+        """One launch normalises, rotates and stores, the next ones attend the stored row too."""
+        lens, lens_next = cache.lens, cache._spare_lens()
+        pos = {"position_ids": position_ids} if position_ids is not None else {"pos_base": lens, "pos_shift": cache._shift}
+        q_hat = kv4.kv4_append(k4, v4, cache.pool, cache.block_table, q=q4, q_weight=qw, k_weight=kw, row_base=lens,
+                               lens_out=lens_next, **rot, **pos)
+        track = bool(cache.track_weights)
+        o = kv4.attention_decode_kv4(q_hat, cache.pool, cache.block_table, lens_next, max_len=longest, return_lse=track)
+        cache.lens, cache._lens_spare = lens_next, lens
+        cache.host_lens = [n + 1 for n in cache.host_lens]
+        if track:
+            o, lse = o
+            cache._add_weights(q_hat, lse)
+        return o
+
+    def _paged4_chunk(self, q4, k4, v4, cache, p0, pos, rot, qw, kw):
+        """(o, lse or None) of a chunk over the stored history and its own rows, which it stores."""
+        B, H, S, D = q4.shape
+        T = p0 + S
+        # the attention's operands, as the prefill takes them: (B, T, Hkv, D) storage
+        k_hat, v_all = (torch.empty(B, T, k4.shape[1], D, dtype=k4.dtype, device=k4.device).transpose(1, 2)
+                        for _ in range(2))
+        if p0:
+            kv4.kv4_gather(cache.pool, cache.block_table, S=p0, dtype=k4.dtype, k_out=k_hat[:, :, :p0],
+                           v_out=v_all[:, :, :p0])
+            ops.qk_norm_rope(k=k4, v=v4, k_out=k_hat, v_out=v_all, k_weight=kw, kv_row_offset=p0, **rot, **pos)
+        else:
+            v_all = v4
+            ops.qk_norm_rope(k=k4, k_out=k_hat, k_weight=kw, **rot, **pos)
+        kv4.kv4_append(k_hat[:, :, p0:], v4, cache.pool, cache.block_table, row_offset=p0)
+        track = bool(cache.track_weights)
+        o = ops.attention_prefill(q4, k_hat, v_all, q_weight=qw, causal=True, return_lse=track, **rot, **pos)
+        return o if track else (o, None)

@@ -24,7 +24,7 @@ from typing import Callable, List, Optional, Sequence, Tuple
 import torch
 import torch.nn.functional as F
 
-from .attention import KVCache, PagedKVCache
+from .attention import KVCache, PagedKVCache, PagedKVCache4
 
 
 def _device_of(model) -> torch.device:
@@ -139,10 +139,14 @@ def _fixed_semantics(model):
             l.attention.rope_positions, l.attention.cache_prefill_causal = rp, cc
 
 
+_OBSERVED = 64  # queries of a prompt whose attention decides which of its keys are kept
+
+
 @torch.no_grad()
 def generate_greedy_batch(model, prompts: Sequence[Sequence[int]], max_new_tokens: int,
                           stop_tokens: Optional[Sequence[int]] = None,
-                          return_logits: bool = False, page_size: Optional[int] = None
+                          return_logits: bool = False, page_size: Optional[int] = None, kv_bits: int = 16,
+                          keep: Optional[int] = None, recent: Optional[int] = None, first: int = 4
                           ) -> Tuple[List[List[int]], Optional[List[torch.Tensor]]]:
     """Greedy decoding of several prompts at once against a ragged KV cache.
 
@@ -152,13 +156,26 @@ def generate_greedy_batch(model, prompts: Sequence[Sequence[int]], max_new_token
     decode step appends row b's key at slot ``len_b + t``, rotates it at that
     position and attends exactly its own keys.  With ``page_size`` the caches
     are ``PagedKVCache`` page pools (the padding's pages are returned after
-    the prefill) instead of dense per-row buffers.  A row stops at its first
+    the prefill) instead of dense per-row buffers.  ``kv_bits=4`` (with
+    ``page_size``) holds the cache in 4 bits (``PagedKVCache4``).  ``keep`` (with
+    ``page_size``, bf16 models) bounds the cache: a sequence that has grown a page
+    beyond ``keep`` rows is cut to them, its first ``first``, its last ``recent``
+    (by default a half of ``keep``) and those of the rest that got the most
+    attention weight.  A row stops at its first
     stop token (not included) or after ``max_new_tokens``.  Returns the
     generated tokens per row and, with ``return_logits``, the fp32 logits each
     token was chosen from (one (n_b, vocab) tensor per row).
     """
     if not prompts or any(len(p) == 0 for p in prompts):
         raise ValueError("every prompt needs at least one token")
+    if kv_bits not in (4, 16):
+        raise ValueError(f"kv_bits must be 4 or 16, got {kv_bits}")
+    if page_size is None and (kv_bits == 4 or keep is not None):
+        raise ValueError("kv_bits=4 and keep need page_size")
+    if keep is not None:
+        recent = keep // 2 if recent is None else recent
+        if keep <= 0 or recent < 0 or first < 0 or recent + first > keep:
+            raise ValueError(f"keep must be positive and hold first + recent, got {keep}, {first} and {recent}")
     dev = _device_of(model)
     B = len(prompts)
     lens = [len(p) for p in prompts]
@@ -172,8 +189,16 @@ def generate_greedy_batch(model, prompts: Sequence[Sequence[int]], max_new_token
         caches = [KVCache(max_seq_len=L + max_new_tokens) for _ in range(len(model.layers))]
     else:
         per_seq = -(-(L + max_new_tokens) // page_size)
-        caches = [PagedKVCache(B * per_seq, page_size=page_size, max_pages_per_seq=per_seq)
+        pages = B * per_seq
+        if keep is not None:  # the prompts, then what is kept, a page more, and a second copy while rows move
+            per_seq = max(-(-L // page_size), min(per_seq, -(-keep // page_size) + 2))
+            pages = B * per_seq + -(-keep // page_size)
+        cls = PagedKVCache4 if kv_bits == 4 else PagedKVCache
+        caches = [cls(pages, page_size=page_size, max_pages_per_seq=per_seq, track_weights=0 if keep is None else _OBSERVED)
                   for _ in range(len(model.layers))]
+        if keep is not None:
+            for c in caches:
+                c.expect_lengths(lens)
     out: List[List[int]] = [[] for _ in range(B)]
     steps: List[List[torch.Tensor]] = [[] for _ in range(B)]
     done = [False] * B
@@ -184,7 +209,10 @@ def generate_greedy_batch(model, prompts: Sequence[Sequence[int]], max_new_token
         logits = logits[torch.arange(B, device=dev), last]
         lens_t = torch.as_tensor(lens, dtype=torch.int32, device=dev)
         for c in caches:
-            c.set_lengths(lens_t.clone() if page_size is None else lens)
+            if keep is None:
+                c.set_lengths(lens_t.clone() if page_size is None else lens)
+            elif c.seq_len > keep:
+                c.evict(keep, recent=recent, first=first)
         for _ in range(max_new_tokens):
             nxt = logits.argmax(dim=-1)
             toks = nxt.tolist()
@@ -203,6 +231,9 @@ def generate_greedy_batch(model, prompts: Sequence[Sequence[int]], max_new_token
             if all(done):
                 break
             logits = model(input_ids=nxt[:, None], kv_caches=caches)["logits"][:, -1, :]
+            if keep is not None and caches[0].seq_len >= keep + page_size:
+                for c in caches:
+                    c.evict(keep, recent=recent, first=first)
     if not return_logits:
         return out, None
     vocab = logits.shape[-1]

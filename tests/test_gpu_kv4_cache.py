@@ -1,0 +1,278 @@
+"""The 4-bit cache and eviction through the module, the model and the generator."""
+
+import math
+
+import pytest
+import torch
+
+import nano_qwen_amd as nq
+from nano_qwen_amd import ModelConfig, Qwen3Model
+from nano_qwen_amd.config import AttentionConfig
+from tests import kv4_reference as ref
+from tests.golden.make_golden_model import MODEL, make_model_weights
+from tests.helpers import randn, say
+from tests.test_gpu_kv4 import decode_bound
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def module(seed=1, Hq=4, Hkv=2, D=64, dtype=torch.bfloat16):
+    cfg = AttentionConfig(hidden_size=Hq * D, num_attention_heads=Hq, num_key_value_heads=Hkv, head_dim=D,
+                          max_position_embeddings=1024)
+    torch.manual_seed(seed)
+    attn = nq.Attention(cfg)
+    with torch.no_grad():
+        attn.q_norm.weight.add_(0.05 * torch.randn(D))
+        attn.k_norm.weight.add_(0.05 * torch.randn(D))
+    attn = attn.to(DEV, dtype).eval()
+    attn.o_proj = torch.nn.Identity()  # the heads' outputs themselves
+    return attn
+
+
+def rows_of(attn, h, first):
+    """(q_hat, k_hat in fp32, v) of tokens h (B, S, hidden) at positions first[b] + s."""
+    B, S, _ = h.shape
+    H, Hkv, D = attn.num_heads, attn.num_kv_heads, attn.head_dim
+    q = attn.q_proj(h).view(B, S, H, D).transpose(1, 2)
+    k = attn.k_proj(h).view(B, S, Hkv, D).transpose(1, 2)
+    v = attn.v_proj(h).view(B, S, Hkv, D).transpose(1, 2)
+    cos, sin = attn.rotary_emb.tables_f32()
+    kw = dict(eps=attn.config.rms_norm_eps, cos=cos, sin=sin, pos_base=torch.tensor(first, dtype=torch.int32, device=DEV))
+    q_hat, _, _ = nq.qk_norm_rope(q=q, q_weight=attn.q_norm.weight, **kw)
+    k32 = torch.empty(B, Hkv, S, D, device=DEV)
+    nq.qk_norm_rope(k=k, k_out=k32, k_weight=attn.k_norm.weight, **kw)
+    return q_hat, k32, v
+
+
+def check_step(o, attn, q_hat, cache, what):
+    """A one-token output (B, 1, Hq D) against the attention over what the cache holds."""
+    B, H, _, D = q_hat.shape
+    for b in range(B):
+        k, v = cache.gather(b)
+        want, _, mass, spread = ref.attention(q_hat[b, :, 0], k.double(), v.double(), 1 / math.sqrt(D))
+        tol = decode_bound(o.dtype, want, mass, spread, k.shape[1], D)
+        if type(cache) is nq.PagedKVCache:  # its decode forms q_hat itself: a bf16 step of q at a border
+            tol = tol + mass * spread[:, None] * 2.0 ** -7
+        err = (o[b, 0].view(H, D).double() - want).abs()
+        assert (err <= tol).all(), f"{what} b={b}: {float((err / tol).max())}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@torch.no_grad()
+def test_module_steps_attend_what_is_stored(dtype):
+    """A prompt, a second chunk and single tokens over a page border, two sequences of one batch
+    trimmed to lengths of their own."""
+    say(f"PagedKVCache4 module {dtype}")
+    attn = module(dtype=dtype)
+    B, D = 2, 64
+    h = (0.5 * randn(B, 90, 256, seed=3)).to(DEV, dtype)
+    cache = nq.PagedKVCache4(num_pages=16, page_size=32)
+    out = attn(h[:, :40], kv_cache=cache)
+    plain = attn(h[:, :40])
+    assert torch.equal(out, plain)  # the first chunk attends its own rows, as without a cache
+    _, k32, v = rows_of(attn, h[:, :40], [0, 0])
+    for b in range(B):
+        k_got, v_got = cache.gather(b)
+        # the chunk's K-hat is rounded to the model's type on its way (the prefill's operand)
+        assert torch.equal(k_got.double(), ref.stored(k32.to(dtype)[b])) and torch.equal(v_got.double(), ref.stored(v[b]))
+    held = [cache.gather(b) for b in range(B)]
+    out = attn(h[:, 40:57], kv_cache=cache)
+    q_hat, k32, v = rows_of(attn, h[:, 40:57], [40, 40])
+    for b in range(B):
+        k = torch.cat([held[b][0].double(), k32.to(dtype)[b].double()], 1)
+        vv = torch.cat([held[b][1].double(), v[b].double()], 1)
+        for s in (0, 8, 16):
+            n = 41 + s
+            want, _, mass, spread = ref.attention(q_hat[b, :, s], k[:, :n], vv[:, :n], 1 / 8)
+            tol = decode_bound(dtype, want, mass, spread, n, D)
+            if dtype == torch.bfloat16:  # the prefill folds its scale into q before q's own rounding
+                tol = tol + mass * spread[:, None] * 2.0 ** -7
+            else:  # and forms q_hat in an order of its own
+                tol = tol + mass * spread[:, None] * 2.0 ** -18
+            err = (out[b, s].view(-1, D).double() - want).abs()
+            assert (err <= tol).all(), (b, s, float((err / tol).max()))
+    cache.set_lengths([57, 31])
+    for t in range(57, 64):
+        at = list(cache.host_lens)
+        o = attn(h[:, t:t + 1], kv_cache=cache)
+        q_hat, k32, v = rows_of(attn, h[:, t:t + 1], at)
+        check_step(o, attn, q_hat, cache, f"step {t}")
+        for b in range(B):
+            k_got, v_got = cache.gather(b)
+            assert torch.equal(k_got[:, -1].double(), ref.stored(k32)[b, :, 0])  # quantised from fp32
+            assert torch.equal(v_got[:, -1].double(), ref.stored(v)[b, :, 0])
+    assert cache.host_lens == [64, 38] and cache.lens.tolist() == [64, 38]
+    cache.free(0)
+    assert cache.host_lens == [0, 38]
+
+
+@pytest.mark.parametrize("kind", [nq.PagedKVCache, nq.PagedKVCache4])
+@torch.no_grad()
+def test_weights_and_eviction(kind):
+    say(f"tracked weights and eviction {kind.__name__}")
+    attn = module(seed=5)
+    B, H, Hkv, D, W = 3, 4, 2, 64, 16
+    h = (0.5 * randn(B, 200, 256, seed=6)).to(DEV, torch.bfloat16)
+    lens = [150, 60, 9]
+    cache = kind(num_pages=40, page_size=32, track_weights=W)
+    cache.expect_lengths(lens)
+    attn(h[:, :150], kv_cache=cache)
+    assert cache.host_lens == lens and cache.lens.tolist() == lens
+    q_all, k32, _ = rows_of(attn, h[:, :150], [0] * B)
+    total = []
+    for b, n in enumerate(lens):
+        k = cache.gather(b)[0].double()
+        w0 = min(W, n)
+        # the softmax is over the rows as the prefill saw them
+        exact = k32[b, :, :n].bfloat16().double()
+        s = (q_all[b, :, n - w0:n].double().reshape(Hkv, -1, D) @ exact.transpose(1, 2).contiguous() / 8).view(H, w0, n)
+        s = s.masked_fill(~torch.ones(w0, n, dtype=torch.bool, device=DEV).tril(n - w0), -math.inf)
+        want = ref.key_weights(q_all[b, :, n - w0:n], k, torch.logsumexp(s, -1), 1 / 8)
+        got = cache.weights[b, :, :n].double()
+        # the prefill's own rounding of q moves its scores, and so its lse, by up to 2^-8 of |q k|
+        spread = float((q_all[b].double().abs().reshape(Hkv, -1, D) @ exact.abs().transpose(1, 2).contiguous()).max()) / 8
+        assert ((got - want).abs() <= want * spread * 2.0 ** -7 + 1e-6).all()
+        assert (cache.weights[b, :, n:] == 0).all()
+        total.append(want)
+    # one more token: its weights are added
+    before = cache.weights.clone()
+    o = attn(h[:, 150:151], kv_cache=cache)
+    q_hat, _, _ = rows_of(attn, h[:, 150:151], lens)
+    check_step(o, attn, q_hat, cache, "tracked step")
+    added = (cache.weights - before).double().sum(-1)
+    assert torch.allclose(added, torch.full_like(added, H / Hkv), rtol=2e-2)
+    # eviction: sequences 0 and 1 shrink, 2 stays
+    held = [cache.gather(b) for b in range(B)]
+    w_before, free = cache.weights.clone(), cache.free_pages
+    cache.evict(40, recent=10, first=2)
+    assert cache.host_lens == [40, 40, 10] and cache.lens.tolist() == [40, 40, 10] and cache.evicted == [111, 21, 0]
+    assert cache.free_pages == free + 5 - 2  # 5 and 2 pages became 2 and 2
+    for b, n in enumerate((151, 61, 10)):
+        k, v = cache.gather(b)
+        for hh in range(Hkv):
+            keep = ref.select(w_before[b, hh].cpu(), n, 40, 10, 2) if n > 40 else list(range(n))
+            assert torch.equal(k[hh], held[b][0][hh, keep]) and torch.equal(v[hh], held[b][1][hh, keep])
+            assert torch.equal(cache.weights[b, hh, :len(keep)], w_before[b, hh, keep])
+            assert (cache.weights[b, hh, len(keep):] == 0).all()
+    # the next tokens stand where they would have
+    for t in range(151, 154):
+        at = [n + e for n, e in zip(cache.host_lens, cache.evicted)]
+        assert at == [151 + t - 151, 61 + t - 151, 10 + t - 151]
+        o = attn(h[:, t:t + 1], kv_cache=cache)
+        q_hat, k32, v = rows_of(attn, h[:, t:t + 1], at)
+        check_step(o, attn, q_hat, cache, f"step after eviction {t}")
+        for b in range(B):
+            k_last = cache.gather(b)[0][:, -1].double()
+            want = ref.stored(k32) if kind is nq.PagedKVCache4 else k32.bfloat16().double()
+            assert torch.equal(k_last, want[b, :, 0])
+    # a sequence that begins anew begins at position 0
+    cache.free(0)
+    assert cache.evicted == [0, 21, 0] and (cache.weights[0] == 0).all()
+    cache.reset()
+    assert cache.free_pages == 40 and cache.weights is None
+    attn(h[:, :5], kv_cache=cache)
+    assert cache.host_lens == [5, 5, 5]
+
+
+@torch.no_grad()
+def test_a_chunk_after_eviction_stands_after_all_its_tokens():
+    say("chunk after eviction")
+    attn = module(seed=7)
+    h = (0.5 * randn(2, 120, 256, seed=8)).to(DEV, torch.bfloat16)
+    for kind in (nq.PagedKVCache, nq.PagedKVCache4):
+        cache = kind(num_pages=20, page_size=32, track_weights=8)
+        attn(h[:, :100], kv_cache=cache)
+        cache.evict(64, recent=8)
+        held = [cache.gather(b) for b in range(2)]
+        out = attn(h[:, 100:110], kv_cache=cache)
+        q_hat, k32, v = rows_of(attn, h[:, 100:110], [100, 100])
+        for b in range(2):
+            k = torch.cat([held[b][0].double(), k32.bfloat16()[b].double()], 1)
+            vv = torch.cat([held[b][1].double(), v[b].double()], 1)
+            for s in (0, 9):
+                n = 65 + s
+                want, _, mass, spread = ref.attention(q_hat[b, :, s], k[:, :n], vv[:, :n], 1 / 8)
+                tol = decode_bound(torch.bfloat16, want, mass, spread, n, 64) + mass * spread[:, None] * 2.0 ** -7
+                assert ((out[b, s].view(-1, 64).double() - want).abs() <= tol).all()
+        assert cache.host_lens == [74, 74]
+
+
+def model(dtype=torch.bfloat16):
+    torch.manual_seed(0)
+    m = Qwen3Model(ModelConfig(**MODEL)).eval()
+    m.load_state_dict(make_model_weights(), strict=True)
+    return m.to(DEV, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_generation_with_a_4_bit_cache(dtype):
+    """The batch's first token comes from the prompts as they are; the rest runs on the cache."""
+    say(f"generate_greedy_batch kv_bits=4 {dtype}")
+    m = model(dtype)
+    g = torch.Generator().manual_seed(9)
+    prompts = [torch.randint(0, MODEL["vocab_size"], (n,), generator=g).tolist() for n in (70, 3, 33, 1)]
+    plain, _ = nq.generate_greedy_batch(m, prompts, 40, page_size=32)
+    four, logits = nq.generate_greedy_batch(m, prompts, 40, page_size=32, kv_bits=4, return_logits=True)
+    assert [len(x) for x in four] == [40] * 4
+    assert [x[0] for x in four] == [x[0] for x in plain]
+    assert all(torch.isfinite(x).all() for x in logits)
+    again, _ = nq.generate_greedy_batch(m, prompts, 40, page_size=32, kv_bits=4)
+    assert again == four
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_generation_with_a_bounded_cache(bits, monkeypatch):
+    say(f"generate_greedy_batch keep, {bits} bits")
+    m = model()
+    g = torch.Generator().manual_seed(10)
+    prompts = [torch.randint(0, MODEL["vocab_size"], (n,), generator=g).tolist() for n in (90, 40, 7)]
+    seen = []
+    real = nq.PagedKVCache.evict
+    monkeypatch.setattr(nq.PagedKVCache, "evict", lambda c, *a, **k: (seen.append(c), real(c, *a, **k))[1])
+    out, logits = nq.generate_greedy_batch(m, prompts, 80, page_size=32, kv_bits=bits, keep=48, return_logits=True)
+    assert [len(x) for x in out] == [80] * 3 and all(torch.isfinite(x).all() for x in logits)
+    assert seen and all(c.seq_len < 48 + 32 for c in seen) and max(seen[0].evicted) > 80
+    # nothing is evicted where nothing exceeds the bound: the same tokens as without one
+    plain, _ = nq.generate_greedy_batch(m, prompts, 20, page_size=32, kv_bits=bits)
+    bounded, _ = nq.generate_greedy_batch(m, prompts, 20, page_size=32, kv_bits=bits, keep=512)
+    assert bounded == plain
+
+
+@torch.no_grad()
+def test_a_captured_step_of_the_module_replays():
+    """A one-token step into a 4-bit cache, recorded once and replayed over new tokens, with eager
+    work in between."""
+    say("captured 4-bit step")
+    attn = module(seed=11)
+    h = (0.5 * randn(2, 60, 256, seed=12)).to(DEV, torch.bfloat16)
+
+    def fresh():
+        c = nq.PagedKVCache4(num_pages=8, page_size=32, max_pages_per_seq=4, track_weights=4)
+        attn(h[:, :50], kv_cache=c)
+        c._grow([64, 64])
+        return c
+    eager, graphed = fresh(), fresh()
+    x = h[:, 50:51].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    start = graphed.lens.clone()
+    with torch.cuda.stream(side):
+        attn(x, kv_cache=graphed)  # warm up; the next line takes it back
+        graphed.set_lengths([50, 50])
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(graphed.lens, start)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attn(x, kv_cache=graphed)
+        graphed._lens_spare.copy_(graphed.lens)  # the recorded step reads it
+    for t in range(50, 56):
+        x.copy_(h[:, t:t + 1])
+        graph.replay()
+        want = attn(h[:, t:t + 1], kv_cache=eager)
+        torch.cuda.synchronize()
+        # the recorded launches bound the lengths by 51 keys, as they stood
+        if t == 50:
+            assert torch.equal(out, want)
+        else:
+            assert torch.isnan(out).all()
