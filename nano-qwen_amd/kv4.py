@@ -20,6 +20,7 @@ CPU path.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
@@ -49,16 +50,30 @@ class _DeviceCall(ops.KernelCall):
             return super().launch(stream)
 
 
+def _launch(plan: bool, t, fn, args, name, keep, result):
+    """The planned call, or the result of launching it now on t's device and its current stream."""
+    if plan:
+        return _DeviceCall(t, fn, args, name, keep, result)
+    device = t.get_device()
+    if device == torch._C._cuda_getDevice():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+    return result
+
+
 def _check(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     """Device tensors of one device that want no gradient."""
-    index = first.get_device()
+    ops._require_device(first)
+    index, grad = first.get_device(), torch.is_grad_enabled()
     for t in (first, *others):
         if t is None:
             continue
-        if t.get_device() != index or not t.is_cuda:
-            ops._require_device(first, t)
+        if t.get_device() != index:
+            ops._require_device(t)
             raise ValueError(f"{name}: the operands lie on different devices: {first.device} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
+        if grad and t.requires_grad:
             raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or give it detached tensors")
 
 
@@ -70,17 +85,37 @@ def _pool4(pool: torch.Tensor) -> Tuple[int, int, int, int]:
     n, H, P, row = pool.shape
     if P <= 0 or P % 32:
         raise ValueError(f"page_size must be a positive multiple of 32, got {P}")
-    if pool.stride(3) != 1 or pool.stride(2) != row or pool.stride(0) % 16 or pool.stride(1) % 16 or pool.data_ptr() % 16:
+    page, head, step, one = pool.stride()
+    if one != 1 or step != row or page % 16 or head % 16 or pool.data_ptr() % 16:
         raise ValueError("a page's head must be contiguous and all of them 16-byte aligned")
     return n, H, P, _HEAD_DIMS[row]
 
 
-def _strides2(t: torch.Tensor, scale: int = 1):
-    return (ctypes.c_int64 * 2)(t.stride(0) * scale, t.stride(1) * scale)
+@lru_cache(maxsize=1024)  # of a program's few layouts: making one takes as long as a launch's other arguments
+def _int64s(*values: int) -> ctypes.Array:
+    return (ctypes.c_int64 * len(values))(*values)
 
 
-def _lens(lens: torch.Tensor, B: int, dev, name: str = "lens") -> torch.Tensor:
-    lens = ops._i32(lens, dev)
+def _strides2(t: torch.Tensor):
+    return _int64s(*t.stride()[:2])
+
+
+def _strides3(t: torch.Tensor):
+    return _int64s(*t.stride()[:3])
+
+
+def _i32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _table(table: torch.Tensor, B: int) -> torch.Tensor:
+    if table.dim() != 2 or table.shape[0] != B:
+        raise ValueError(f"a block table must be (B={B}, pages per sequence), got {tuple(table.shape)}")
+    return _i32(table)
+
+
+def _lens(lens: torch.Tensor, B: int, name: str = "lens") -> torch.Tensor:
+    lens = _i32(lens)
     if lens.numel() != B:
         raise ValueError(f"{name} must hold one number per sequence ({B}), got shape {tuple(lens.shape)}")
     return lens
@@ -142,10 +177,11 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
             q_out = torch.empty(B, S, q.shape[1], D, dtype=q.dtype, device=q.device).transpose(1, 2)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype:
             raise ValueError("q_out must match q in shape and dtype")
-        ops._rows_out(q_out, "q_out")
+        else:
+            ops._rows_out(q_out, "q_out")
         q = ops._rows_in(q)
     dev = k.device
-    bt = ops._block_table(block_table, B, dev)
+    bt = _table(block_table, B)
     if row_base is None and not 0 <= row_offset <= bt.shape[1] * P - S:
         raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {bt.shape[1] * P}")
     if (cos is None) != (sin is None):
@@ -169,26 +205,25 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
         if pos_shift is None:
             pos = ops._positions(position_ids, pos_offset, pos_base, B, S, max_pos, dev)
         elif position_ids is not None:
-            pos = ops._i32(position_ids, dev).expand(B, S).contiguous()
+            pos = _i32(position_ids.expand(B, S))
     if B == 0 or S == 0:
         return q_out
     Hq = 0 if q is None else q.shape[1]
     _sizes("kv4_append", B, S, Hq + 2 * H)
-    pb = None if pos_base is None else _lens(pos_base, B, dev, "pos_base")
-    ps = None if pos_shift is None else _lens(pos_shift, B, dev, "pos_shift")
-    rb = None if row_base is None else _lens(row_base, B, dev, "row_base")
+    pb = None if pos_base is None else _lens(pos_base, B, "pos_base")
+    ps = None if pos_shift is None else _lens(pos_shift, B, "pos_shift")
+    rb = None if row_base is None else _lens(row_base, B, "row_base")
     qw, qf = ops._norm_weight(q_weight, dev, dt, _lib.NQ_QWEIGHT_BF16, plan)
     kw, kf = ops._norm_weight(k_weight, dev, dt, _lib.NQ_KWEIGHT_BF16, plan)
-    st, ptr = _lib.strides3, ops._ptr
-    args = (ptr(k), st(k.stride()[:3]), ptr(v), st(v.stride()[:3]),
-            ptr(q), None if q is None else st(q.stride()[:3]),
-            ptr(q_out), None if q is None else st(q_out.stride()[:3]),
+    st, ptr = _strides3, ops._ptr
+    args = (ptr(k), st(k), ptr(v), st(v),
+            ptr(q), None if q is None else st(q),
+            ptr(q_out), None if q is None else st(q_out),
             ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, B, S, Hq, H, D, dt | qf | kf,
             ptr(qw), ptr(kw), float(eps), ptr(cos_t), ptr(sin_t), max_pos, ptr(pos), ptr(pb), ptr(ps),
             int(pos_offset), ptr(rb), int(row_offset), ptr(lens_out))
-    call = _DeviceCall(k, _lib.load().nq_kv4_append, args, "nq_kv4_append",
-                       (k, v, q, pool, bt, qw, kw, cos_t, sin_t, pos, pb, ps, rb, lens_out), q_out)
-    return call if plan else call.launch()
+    return _launch(plan, k, _lib.load().nq_kv4_append, args, "nq_kv4_append",
+                   (k, v, q, pool, bt, qw, kw, cos_t, sin_t, pos, pb, ps, rb, lens_out), q_out)
 
 
 def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_offset: int = 0,
@@ -202,7 +237,7 @@ def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_off
     _check("kv4_gather", pool, block_table, row_base, k_out, v_out)
     n, H, P, D = _pool4(pool)
     B, dev = block_table.shape[0], pool.device
-    bt = ops._block_table(block_table, B, dev)
+    bt = _table(block_table, B)
     if S < 0 or (row_base is None and not 0 <= row_offset <= bt.shape[1] * P - S):
         raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {bt.shape[1] * P}")
     shape = (B, H, S, D)
@@ -212,18 +247,19 @@ def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_off
             t = torch.empty(shape, dtype=dtype, device=dev)
         elif tuple(t.shape) != shape or t.dtype != dtype:
             raise ValueError(f"{name} must be {shape} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
-        outs.append(ops._rows_out(t, name))
+        else:
+            ops._rows_out(t, name)
+        outs.append(t)
     k, v = outs
     code = ops._code(k)
     if 0 in shape:
         return k, v
     _sizes("kv4_gather", B, S, H)
-    rb = None if row_base is None else _lens(row_base, B, dev, "row_base")
-    st, ptr = _lib.strides3, ops._ptr
-    args = (ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, ptr(k), st(k.stride()[:3]),
-            ptr(v), st(v.stride()[:3]), B, S, H, D, code, ptr(rb), int(row_offset))
-    call = _DeviceCall(pool, _lib.load().nq_kv4_gather, args, "nq_kv4_gather", (pool, bt, rb), (k, v))
-    return call if plan else call.launch()
+    rb = None if row_base is None else _lens(row_base, B, "row_base")
+    st, ptr = _strides3, ops._ptr
+    args = (ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, ptr(k), st(k),
+            ptr(v), st(v), B, S, H, D, code, ptr(rb), int(row_offset))
+    return _launch(plan, pool, _lib.load().nq_kv4_gather, args, "nq_kv4_gather", (pool, bt, rb), (k, v))
 
 
 def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
@@ -246,19 +282,20 @@ def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch
         raise ValueError(f"q must be (B, Hq, {D}) with Hq a multiple of the pool's {H} heads, got {tuple(q.shape)}")
     B, Hq, _ = q.shape
     dt, dev = ops._code(q), q.device
-    bt = ops._block_table(block_table, B, dev)
+    bt = _table(block_table, B)
     if not 0 < max_len <= bt.shape[1] * P:
         raise ValueError(f"max_len must be in [1, {bt.shape[1] * P}] (block table columns x page_size), got {max_len}")
     if out is None:
         out = torch.empty(B, Hq, D, dtype=q.dtype, device=dev)
     elif tuple(out.shape) != (B, Hq, D) or out.dtype != q.dtype:
         raise ValueError(f"out must be {(B, Hq, D)} in {q.dtype}")
-    ops._rows_out(out, "out")
+    else:
+        ops._rows_out(out, "out")
     lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
     if B == 0:
         return (out, lse) if return_lse else out
     _sizes("attention_decode_kv4", B, H, -(-Hq // H // 16) + 1)
-    lens_t = _lens(lens, B, dev)
+    lens_t = _lens(lens, B)
     q = ops._rows_in(q)
     lib = _lib.load()
     need = lib.nq_attn_decode_kv4_workspace_bytes(B, Hq, H, D)
@@ -268,9 +305,8 @@ def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     args = (ptr(q), _strides2(q), ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, ptr(lens_t),
             ptr(out), _strides2(out), ptr(lse), ptr(workspace), workspace.numel() * workspace.element_size(),
             B, Hq, H, D, int(max_len), dt, 0.0 if sm_scale is None else float(sm_scale))
-    call = _DeviceCall(q, lib.nq_attn_decode_kv4, args, "nq_attn_decode_kv4", (q, pool, bt, lens_t, workspace),
-                       (out, lse) if return_lse else out)
-    return call if plan else call.launch()
+    return _launch(plan, q, lib.nq_attn_decode_kv4, args, "nq_attn_decode_kv4", (q, pool, bt, lens_t, workspace),
+                   (out, lse) if return_lse else out)
 
 
 def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
@@ -305,7 +341,7 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
     if lse.dtype != torch.float32 or lse.numel() != B * Hq * S or tuple(lse.shape) not in ((B, Hq, S), (B, Hq)):
         raise ValueError(f"lse must be fp32 {(B, Hq, S)}, got {lse.dtype} {tuple(lse.shape)}")
     dev = q.device
-    bt = ops._block_table(block_table, B, dev)
+    bt = _table(block_table, B)
     if not 0 < max_len <= bt.shape[1] * P:
         raise ValueError(f"max_len must be in [1, {bt.shape[1] * P}] (block table columns x page_size), got {max_len}")
     add = weights is not None
@@ -316,17 +352,16 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
     if B == 0 or S == 0:
         return weights if add else weights.zero_()
     _sizes("attention_key_weights", B, Hq, S)
-    lens_t = _lens(lens, B, dev)
+    lens_t = _lens(lens, B)
     q, lse = ops._rows_in(q), lse.contiguous()
     lib = _lib.load()
     need = lib.nq_key_weights_workspace_bytes(B, Hq, H, S, int(max_len))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     ptr = ops._ptr
-    args = (ptr(q), _lib.strides3(q.stride()[:3]), ptr(k_pool), _lib.strides3(k_pool.stride()[:3]), int(four), n,
+    args = (ptr(q), _strides3(q), ptr(k_pool), _strides3(k_pool), int(four), n,
             ptr(bt), bt.stride(0), bt.shape[1], P, ptr(lens_t), ptr(lse), ptr(weights), _strides2(weights), int(add),
             ptr(ws), need, B, Hq, H, S, D, int(max_len), int(bool(causal)), 0.0 if sm_scale is None else float(sm_scale))
-    call = _DeviceCall(q, lib.nq_key_weights, args, "nq_key_weights", (q, k_pool, bt, lens_t, lse, ws), weights)
-    return call if plan else call.launch()
+    return _launch(plan, q, lib.nq_key_weights, args, "nq_key_weights", (q, k_pool, bt, lens_t, lse, ws), weights)
 
 
 def _check_weights(weights: torch.Tensor, B: int, H: int, least: int) -> None:
@@ -352,7 +387,7 @@ def select_keys(weights: torch.Tensor, lens: torch.Tensor, *, keep: int, recent:
     _check_weights(weights, B, H, 1)
     if keep <= 0 or recent < 0 or first < 0 or recent + first > keep or keep > _MOST:
         raise ValueError(f"keep must be positive and hold first + recent, got {keep}, {first} and {recent}")
-    lens_t = _lens(lens, B, weights.device)
+    lens_t = _lens(lens, B)
     kept = torch.empty(B, H, keep, dtype=torch.int32, device=weights.device)
     if B == 0 or H == 0:
         return kept
@@ -360,8 +395,7 @@ def select_keys(weights: torch.Tensor, lens: torch.Tensor, *, keep: int, recent:
     _sizes("select_keys", W)
     args = (ops._ptr(weights), _strides2(weights), ops._ptr(lens_t), ops._ptr(kept), B, H, W, int(keep), int(recent),
             int(first))
-    call = _DeviceCall(weights, _lib.load().nq_select_keys, args, "nq_select_keys", (weights, lens_t), kept)
-    return call if plan else call.launch()
+    return _launch(plan, weights, _lib.load().nq_select_keys, args, "nq_select_keys", (weights, lens_t), kept)
 
 
 def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], block_table: torch.Tensor,
@@ -392,13 +426,13 @@ def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], bl
         if P <= 0 or P % 32:
             raise ValueError(f"page_size must be a positive multiple of 32, got {P}")
         e = k_pool.element_size()
-        ks, vs = (_lib.strides3([x * e for x in t.stride()[:3]]) for t in (k_pool, v_pool))
+        ks, vs = (_int64s(*(x * e for x in t.stride()[:3])) for t in (k_pool, v_pool))
         row = D * e
     if kept.dtype != torch.int32 or kept.dim() != 3 or kept.shape[1] != H:
         raise ValueError(f"kept must be int32 (B, {H}, keep), got {kept.dtype} {tuple(kept.shape)}")
     B, _, keep = kept.shape
     dev = k_pool.device
-    bt, new = ops._block_table(block_table, B, dev), ops._block_table(new_table, B, dev)
+    bt, new = _table(block_table, B), _table(new_table, B)
     if new.shape[1] * P < keep:
         raise ValueError(f"the new table maps {new.shape[1] * P} rows, {keep} are kept")
     if B and new.data_ptr() == bt.data_ptr():
@@ -416,6 +450,5 @@ def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], bl
     args = (ptr(k_pool), ks, ptr(v_pool), vs, row, D, n, ptr(bt), bt.stride(0), bt.shape[1], ptr(new), new.stride(0),
             new.shape[1], P, ptr(kept), ptr(weights), ptr(out), None if out is None else _strides2(out),
             0 if out is None else out.shape[2], B, H, keep)
-    call = _DeviceCall(k_pool, _lib.load().nq_kv_compact, args, "nq_kv_compact",
-                       (k_pool, v_pool, bt, new, kept, weights), out)
-    return call if plan else call.launch()
+    return _launch(plan, k_pool, _lib.load().nq_kv_compact, args, "nq_kv_compact",
+                   (k_pool, v_pool, bt, new, kept, weights), out)
