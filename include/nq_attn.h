@@ -724,8 +724,8 @@ int nq_select_keys(const float* weights, const int64_t* weight_strides, const in
 
 /*
  * Moves row kept[b, h, i] of each sequence's pages (block_table) to row i of its new pages
- * (new_table, entries of which must not be pages of any block_table row), both in the same
- * pool; -1 moves nothing.  v_pool NULL: k_pool is a 4-bit pool of head_dim, strides {page,
+ * (new_table: each one's own, and none in which any sequence's kept rows lie), both in the
+ * same pool; -1 moves nothing.  v_pool NULL: k_pool is a 4-bit pool of head_dim, strides {page,
  * head} in bytes.  Else K and V pools of rows of row_bytes, strides {page, head, row} in
  * bytes.  weights_out (NULL: none; not weights) receives the kept rows' weights and 0
  * behind them up to width; both fp32 with weight_strides {batch, head}.  Rows of the new

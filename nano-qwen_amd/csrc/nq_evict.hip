@@ -767,6 +767,7 @@ extern "C" int nq_kv_compact(void* k_pool, const int64_t* k_strides, void* v_poo
   int rc = evict_check_table(block_table, bt_stride, bt_cols, page_size, num_pages);
   if (rc == NQ_OK) rc = evict_check_table(new_table, new_stride, new_cols, page_size, num_pages);
   if (rc != NQ_OK) return rc;
+  if (new_table == block_table) return nq_fail(NQ_ERR_INVALID, "new_table must name other pages than block_table");
   if ((int64_t)new_cols * page_size < keep)
     return nq_fail(NQ_ERR_INVALID, "the new table's %d columns hold fewer than the %d kept rows", new_cols, keep);
   const bool four = v_pool == nullptr;

@@ -403,9 +403,9 @@ def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], bl
                plan: bool = False):
     """Move row ``kept[b, h, i]`` of each sequence to row i of its new pages, in the same pool.
 
-    pools: a 4-bit pool, or (k_pool, v_pool) of bf16 or fp32 pages.  ``new_table`` must name
-    pages that no row of ``block_table`` does (what they hold is overwritten while the old
-    pages are read).  ``kept`` as ``select_keys`` gives it; -1 moves nothing, and rows of the
+    pools: a 4-bit pool, or (k_pool, v_pool) of bf16 or fp32 pages.  The new pages must be none
+    of those that any sequence's kept rows lie in (what they hold is overwritten while these
+    are read), and each one's own.  ``kept`` as ``select_keys`` gives it; -1 moves nothing, and rows of the
     new pages behind the last one moved are left as they are.  With ``weights`` (B, Hkv, W >=
     keep) returns a fresh tensor of that shape with the kept rows' weights and 0 behind them,
     else None.

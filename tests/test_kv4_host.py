@@ -1,0 +1,485 @@
+"""The 4-bit cache and eviction without a GPU: refusals, bookkeeping, the work's division."""
+
+import ctypes
+import random
+
+import pytest
+import torch
+
+import nano_qwen_amd as nq
+from nano_qwen_amd import _lib, attention, kv4
+from tests import kv4_reference as ref
+
+A = ctypes.c_void_p(1 << 20)            # aligned addresses, never followed: every call here is refused
+A2 = ctypes.c_void_p(1 << 21)
+ODD = ctypes.c_void_p((1 << 20) + 4)
+
+
+def i64(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+S3 = i64(4096, 1024, 128)
+POOL = i64(64 * 136 * 4, 64 * 136)      # pages of 4 heads, 64 rows of 128 in 136 bytes each
+BF16, F32 = _lib.NQ_DTYPE_BF16, _lib.NQ_DTYPE_F32
+
+APPEND = dict(k=A, ks=S3, v=A, vs=S3, q=None, qs=None, qo=None, qos=None, pool=A, ps=POOL, pages=8, bt=A, bts=4, cols=4,
+              page=64, B=2, S=3, Hq=0, Hkv=4, D=128, dtype=BF16, qw=None, kw=None, eps=1e-6, cos=None, sin=None, max_pos=0,
+              pos=None, pos_base=None, pos_shift=None, pos0=0, row_base=A, row0=0, lens_out=None, stream=None)
+GATHER = dict(pool=A, ps=POOL, pages=8, bt=A, bts=4, cols=4, page=64, k=A, ks=S3, v=A, vs=S3, B=2, S=3, Hkv=4, D=128,
+              dtype=BF16, row_base=None, row0=0, stream=None)
+DECODE = dict(q=A, qs=i64(1024, 128), pool=A, ps=POOL, pages=8, bt=A, bts=4, cols=4, page=64, lens=A, o=A,
+              os=i64(1024, 128), lse=None, ws=A, wsb=1 << 30, B=2, Hq=8, Hkv=4, D=128, max_len=200, dtype=BF16, scale=0.0,
+              stream=None)
+WEIGHTS = dict(q=A, qs=S3, pool=A, ps=i64(32768, 8192, 128), four=0, pages=8, bt=A, bts=4, cols=4, page=64, lens=A, lse=A,
+               w=A, ws=i64(1024, 256), add=0, work=A, workb=1 << 30, B=2, Hq=8, Hkv=4, S=300, D=128, max_len=200, causal=1,
+               scale=0.0, stream=None)
+SELECT = dict(w=A, ws=i64(1024, 256), lens=A, kept=A, B=2, H=4, W=256, keep=100, recent=10, first=4, stream=None)
+COMPACT = dict(k=A, ks=POOL, v=None, vs=None, row=0, D=128, pages=8, bt=A, bts=4, cols=4, new=A2, nbts=2, ncols=2, page=64,
+               kept=A, w=None, wo=None, ws=None, W=0, B=2, H=4, keep=100, stream=None)
+PLAIN = dict(COMPACT, ks=i64(65536, 16384, 256), v=A, vs=i64(65536, 16384, 256), row=256)
+
+REFUSED = [
+    ("nq_kv4_append", APPEND, dict(D=96), b"head_dim"),
+    ("nq_kv4_append", APPEND, dict(D=0), b"head_dim"),
+    ("nq_kv4_append", APPEND, dict(page=48), b"page_size"),
+    ("nq_kv4_append", APPEND, dict(page=0), b"page_size"),
+    ("nq_kv4_append", APPEND, dict(page=1 << 21), b"page_size"),
+    ("nq_kv4_append", APPEND, dict(pool=None), b"required"),
+    ("nq_kv4_append", APPEND, dict(bt=None), b"required"),
+    ("nq_kv4_append", APPEND, dict(pool=ODD), b"16 bytes"),
+    ("nq_kv4_append", APPEND, dict(ps=i64(64 * 136 * 4, 64 * 135)), b"overlap"),
+    ("nq_kv4_append", APPEND, dict(pages=0), b"num_pages"),
+    ("nq_kv4_append", APPEND, dict(bts=3), b"bt_cols"),
+    ("nq_kv4_append", APPEND, dict(B=0), b"positive"),
+    ("nq_kv4_append", APPEND, dict(S=-1), b"positive"),
+    ("nq_kv4_append", APPEND, dict(dtype=7), b"dtype"),
+    ("nq_kv4_append", APPEND, dict(k=ODD), b"aligned"),
+    ("nq_kv4_append", APPEND, dict(ks=i64(4096, 1024, 127)), b"strides"),
+    ("nq_kv4_append", APPEND, dict(cos=A), b"together"),
+    ("nq_kv4_append", APPEND, dict(cos=A, sin=ODD, max_pos=4), b"aligned"),
+    ("nq_kv4_append", APPEND, dict(kw=ODD), b"aligned"),
+    ("nq_kv4_append", APPEND, dict(lens_out=A), b"alias"),
+    ("nq_kv4_append", APPEND, dict(B=1 << 15, S=1 << 12), b"too many rows"),
+    ("nq_kv4_gather", GATHER, dict(v=None), b"required"),
+    ("nq_kv4_gather", GATHER, dict(dtype=2), b"dtype"),
+    ("nq_kv4_gather", GATHER, dict(vs=i64(1, 1, 1)), b"strides"),
+    ("nq_kv4_gather", GATHER, dict(B=1 << 10, S=1 << 20), b"too many rows"),
+    ("nq_kv4_gather", GATHER, dict(S=0), b"positive"),
+    ("nq_attn_decode_kv4", DECODE, dict(Hq=9), b"divisible"),
+    ("nq_attn_decode_kv4", DECODE, dict(Hq=0), b"positive"),
+    ("nq_attn_decode_kv4", DECODE, dict(max_len=257), b"columns"),
+    ("nq_attn_decode_kv4", DECODE, dict(max_len=0), b"positive"),
+    ("nq_attn_decode_kv4", DECODE, dict(lens=None), b"required"),
+    ("nq_attn_decode_kv4", DECODE, dict(q=ODD), b"aligned"),
+    ("nq_attn_decode_kv4", DECODE, dict(os=i64(1024, 4)), b"strides"),
+    ("nq_attn_decode_kv4", DECODE, dict(wsb=1000), b"workspace"),
+    ("nq_attn_decode_kv4", DECODE, dict(ws=None), b"workspace"),
+    ("nq_attn_decode_kv4", DECODE, dict(ws=ODD), b"workspace"),
+    ("nq_attn_decode_kv4", DECODE, dict(dtype=3), b"dtype"),
+    ("nq_key_weights", WEIGHTS, dict(D=48), b"head_dim"),
+    ("nq_key_weights", WEIGHTS, dict(Hq=7), b"divisible"),
+    ("nq_key_weights", WEIGHTS, dict(max_len=300), b"columns"),
+    ("nq_key_weights", WEIGHTS, dict(workb=16), b"workspace"),
+    ("nq_key_weights", WEIGHTS, dict(lse=None), b"required"),
+    ("nq_key_weights", WEIGHTS, dict(qs=i64(4096, 1024, -128)), b"strides"),
+    ("nq_key_weights", WEIGHTS, dict(S=1 << 24), b"rows"),
+    ("nq_key_weights", WEIGHTS, dict(page=100), b"page_size"),
+    ("nq_select_keys", SELECT, dict(keep=0), b"keep"),
+    ("nq_select_keys", SELECT, dict(recent=97), b"keep"),
+    ("nq_select_keys", SELECT, dict(first=-1), b"keep"),
+    ("nq_select_keys", SELECT, dict(w=None), b"required"),
+    ("nq_select_keys", SELECT, dict(B=0), b"positive"),
+    ("nq_kv_compact", COMPACT, dict(new=A), b"new"),
+    ("nq_kv_compact", COMPACT, dict(ncols=1, nbts=1), b"kept"),
+    ("nq_kv_compact", COMPACT, dict(D=256), b"head_dim"),
+    ("nq_kv_compact", COMPACT, dict(w=A), b"together"),
+    ("nq_kv_compact", COMPACT, dict(w=A, wo=A, ws=i64(512, 128), W=128), b"weights_out"),
+    ("nq_kv_compact", COMPACT, dict(w=A, wo=A2, ws=i64(512, 128), W=64), b"together"),
+    ("nq_kv_compact", COMPACT, dict(keep=0), b"positive"),
+    ("nq_kv_compact", PLAIN, dict(row=100), b"16 bytes"),
+    ("nq_kv_compact", PLAIN, dict(ks=i64(65536, 16384, 128)), b"overlap"),
+    ("nq_kv_compact", PLAIN, dict(v=ODD), b"16 bytes"),
+]
+
+
+@pytest.mark.parametrize("fn,base,change,text", REFUSED)
+def test_c_entries_refuse(fn, base, change, text):
+    lib = _lib.load()
+    assert set(change) <= set(base) and len(base) == len(_lib.SIGNATURES[fn][1])
+    rc = getattr(lib, fn)(*dict(base, **change).values())
+    assert rc != _lib.NQ_OK and text in lib.nq_last_error(), lib.nq_last_error()
+
+
+def test_workspaces():
+    lib = _lib.load()
+    rows = 64 * 4
+    assert lib.nq_attn_decode_kv4_workspace_bytes(64, 64, 4, 128) == (512 + rows) * 16 * 130 * 4 + rows * 8
+    assert lib.nq_attn_decode_kv4_workspace_bytes(64, 65, 4, 128) == 0
+    assert lib.nq_key_weights_workspace_bytes(2, 8, 4, 1, 200) == 0      # 2 rows: no partial sums
+    assert lib.nq_key_weights_workspace_bytes(2, 8, 4, 128, 200) == 0    # one chunk
+    assert lib.nq_key_weights_workspace_bytes(2, 8, 4, 129, 200) == 2 * 2 * 4 * 200 * 4
+
+
+@pytest.fixture
+def host_calls(monkeypatch):
+    """The Python checks on host tensors; a call that passes them would raise."""
+    def reached(plan, t, fn, args, name, keep, result):
+        raise AssertionError(f"{name} was not refused")
+    monkeypatch.setattr(kv4, "_check", lambda *a: None)
+    monkeypatch.setattr(kv4, "_launch", reached)
+
+
+def pool4(n=4, H=2, P=32, D=64):
+    return kv4.kv4_empty_pool(n, H, P, D, device="cpu")
+
+
+def rows(B=1, H=2, S=3, D=64, dtype=torch.bfloat16):
+    return torch.zeros(B, H, S, D, dtype=dtype)
+
+
+TABLE = torch.zeros(1, 3, dtype=torch.int32)
+LENS = torch.ones(1, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(k=rows(H=3), v=rows(H=3)), ValueError), (dict(v=rows(S=2)), ValueError), (dict(v=rows(dtype=torch.float32)), TypeError),
+    (dict(k=rows(D=32), v=rows(D=32)), ValueError), (dict(k=rows(dtype=torch.float16), v=rows(dtype=torch.float16)), TypeError),
+    (dict(pool=torch.zeros(4, 2, 32, 64)), ValueError), (dict(pool=torch.zeros(4, 2, 32, 67, dtype=torch.uint8)), ValueError),
+    (dict(pool=torch.zeros(4, 2, 40, 68, dtype=torch.uint8)), ValueError), (dict(pool=pool4()[..., :34]), ValueError),
+    (dict(pool=pool4().transpose(1, 2)), ValueError), (dict(block_table=TABLE.expand(2, 3)), ValueError),
+    (dict(block_table=TABLE[0]), ValueError), (dict(row_offset=94), ValueError), (dict(row_offset=-1), ValueError),
+    (dict(q=rows(S=2)), ValueError), (dict(q=rows(dtype=torch.float32)), TypeError), (dict(q_out=rows()), ValueError),
+    (dict(q=rows(), q_out=rows(H=4)), ValueError), (dict(q=rows(), q_out=rows().transpose(2, 3).contiguous().transpose(2, 3)), ValueError),
+    (dict(q_weight=torch.ones(64)), ValueError), (dict(k_weight=torch.ones(63)), ValueError), (dict(cos=torch.ones(8, 32)), ValueError),
+    (dict(cos=torch.ones(8, 16), sin=torch.ones(8, 16)), ValueError), (dict(cos=torch.ones(8, 32), sin=torch.ones(8, 32), pos_offset=6), IndexError),
+    (dict(lens_out=LENS), ValueError), (dict(lens_out=LENS, row_base=LENS), ValueError),
+    (dict(lens_out=LENS.long(), row_base=LENS), ValueError), (dict(row_base=LENS.expand(2)), ValueError),
+    (dict(pos_shift=LENS.expand(3)), ValueError),
+])
+def test_append_refuses(host_calls, change, error):
+    args = dict(k=rows(), v=rows(), pool=pool4(), block_table=TABLE)
+    args.update(change)
+    with pytest.raises(error):
+        kv4.kv4_append(args.pop("k"), args.pop("v"), args.pop("pool"), args.pop("block_table"), **args)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(S=97), ValueError), (dict(S=-1), ValueError), (dict(S=3, row_offset=94), ValueError), (dict(S=3, dtype=torch.float16), TypeError),
+    (dict(S=3, k_out=rows(S=4)), ValueError), (dict(S=3, v_out=rows(dtype=torch.float32)), ValueError),
+    (dict(S=3, row_base=torch.zeros(2, dtype=torch.int32)), ValueError),
+])
+def test_gather_refuses(host_calls, change, error):
+    with pytest.raises(error):
+        kv4.kv4_gather(pool4(), TABLE, **change)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(q=torch.zeros(1, 3, 64, dtype=torch.bfloat16)), ValueError), (dict(q=rows(S=2)), ValueError), (dict(q=rows(D=32)[:, :, 0]), ValueError),
+    (dict(q=torch.zeros(1, 2, 64, dtype=torch.float16)), TypeError), (dict(max_len=0), ValueError), (dict(max_len=97), ValueError),
+    (dict(lens=LENS.expand(2)), ValueError), (dict(out=torch.zeros(1, 2, 64)), ValueError), (dict(q=torch.zeros(1, 0, 64)), ValueError),
+])
+def test_decode_refuses(host_calls, change, error):
+    args = dict(q=torch.zeros(1, 2, 64, dtype=torch.bfloat16), pool=pool4(), block_table=TABLE, lens=LENS, max_len=90)
+    args.update(change)
+    with pytest.raises(error):
+        kv4.attention_decode_kv4(args.pop("q"), args.pop("pool"), args.pop("block_table"), args.pop("lens"), **args)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(q=rows(dtype=torch.float32)), TypeError), (dict(q=rows(H=3)), ValueError), (dict(k_pool=torch.zeros(4, 2, 32, 64)), TypeError),
+    (dict(k_pool=torch.zeros(4, 2, 40, 64, dtype=torch.bfloat16)), ValueError), (dict(lse=torch.zeros(1, 2, 2)), ValueError),
+    (dict(lse=torch.zeros(1, 2, 3, dtype=torch.float64)), ValueError), (dict(max_len=97), ValueError),
+    (dict(weights=torch.zeros(1, 2, 89)), ValueError), (dict(weights=torch.zeros(1, 2, 90, dtype=torch.float64)), ValueError),
+    (dict(weights=torch.zeros(1, 90, 2).transpose(1, 2)), ValueError), (dict(lens=LENS.expand(2)), ValueError),
+])
+def test_key_weights_refuse(host_calls, change, error):
+    args = dict(q=rows(), k_pool=pool4(), block_table=TABLE, lens=LENS, lse=torch.zeros(1, 2, 3), max_len=90)
+    args.update(change)
+    with pytest.raises(error):
+        first = [args.pop(n) for n in ("q", "k_pool", "block_table", "lens", "lse")]
+        kv4.attention_key_weights(*first, **args)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(keep=0), ValueError), (dict(keep=4, recent=3, first=2), ValueError), (dict(keep=4, recent=-1), ValueError),
+    (dict(keep=2 ** 31), ValueError), (dict(weights=torch.zeros(2, 8)), ValueError), (dict(weights=torch.zeros(1, 2, 8).double()), ValueError),
+    (dict(lens=LENS.expand(2)), ValueError),
+])
+def test_select_refuses(host_calls, change, error):
+    args = dict(dict(weights=torch.zeros(1, 2, 8), lens=LENS, keep=4), **change)
+    with pytest.raises(error):
+        kv4.select_keys(args.pop("weights"), args.pop("lens"), **args)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(kept=torch.zeros(1, 3, 4, dtype=torch.int32)), ValueError), (dict(kept=torch.zeros(1, 2, 4)), ValueError),
+    (dict(kept=torch.zeros(1, 2, 33, dtype=torch.int32)), ValueError), (dict(new_table=TABLE[:, :1]), ValueError),
+    (dict(weights=torch.zeros(1, 2, 3)), ValueError), (dict(pools=(torch.zeros(4, 2, 32, 64), torch.zeros(4, 2, 32, 32))), ValueError),
+    (dict(pools=(torch.zeros(4, 2, 32, 64), torch.zeros(4, 2, 32, 64).bfloat16())), ValueError),
+    (dict(pools=(torch.zeros(4, 2, 32, 64).half(),) * 2), TypeError), (dict(pools=(torch.zeros(4, 2, 40, 64),) * 2), ValueError),
+])
+def test_compact_refuses(host_calls, change, error):
+    args = dict(pools=pool4(), block_table=TABLE, new_table=torch.ones(1, 1, dtype=torch.int32), kept=torch.zeros(1, 2, 4, dtype=torch.int32))
+    args.update(change)
+    with pytest.raises(error):
+        first = [args.pop(n) for n in ("pools", "block_table", "new_table", "kept")]
+        kv4.kv_compact(*first, **args)
+
+
+def test_host_tensors_have_no_path():
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kv4.kv4_append(rows(), rows(), pool4(), TABLE)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kv4.select_keys(torch.zeros(1, 2, 8), LENS, keep=4)
+    for bad in (48, 16, 256, 33):
+        with pytest.raises(ValueError, match="head_dim"):
+            kv4.kv4_empty_pool(1, 1, 32, bad, device="cpu")
+    with pytest.raises(ValueError, match="page_size"):
+        kv4.kv4_empty_pool(1, 1, 48, 64, device="cpu")
+
+
+# ---------------------------------------------------------------- the caches' bookkeeping
+@pytest.fixture
+def plain_eviction(monkeypatch):
+    """select_keys and kv_compact by their definitions, on host tensors."""
+    def select_keys(weights, lens, *, keep, recent, first):
+        out = torch.full((*weights.shape[:2], keep), -1, dtype=torch.int32)
+        for b in range(out.shape[0]):
+            for h in range(out.shape[1]):
+                got = ref.select(weights[b, h], int(lens[b]), keep, recent, first)
+                out[b, h, :len(got)] = torch.tensor(got, dtype=torch.int32)
+        return out
+
+    def kv_compact(pools, table, new, kept, *, weights):
+        out = torch.zeros_like(weights)
+        P = pools[0].shape[2]
+        old = [p.clone() for p in pools]
+        for b in range(kept.shape[0]):
+            rows = int(kept[b].max()) + 1
+            assert not set(new[b].tolist()) & set(table[b, :-(-rows // P)].tolist())
+            for h in range(kept.shape[1]):
+                for i, j in enumerate(kept[b, h].tolist()):
+                    for p, o in zip(pools, old):
+                        p[new[b, i // P], h, i % P] = o[table[b, j // P], h, j % P]
+                    out[b, h, i] = weights[b, h, j]
+        return out
+    monkeypatch.setattr(attention.kv4, "select_keys", select_keys)
+    monkeypatch.setattr(attention.kv4, "kv_compact", kv_compact)
+
+
+def filled(lens, num_pages=20, P=32, H=2, D=8, track=4):
+    c = nq.PagedKVCache(num_pages, page_size=P, track_weights=track)
+    c._setup(len(lens), H, D, torch.bfloat16, "cpu")
+    c._grow(lens)
+    c.host_lens = list(lens)
+    c.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    g = torch.Generator().manual_seed(1)
+    for p in (c.k_pool, c.v_pool):
+        p.copy_(torch.randn(p.shape, generator=g))
+    for b, n in enumerate(lens):
+        c.weights[b, :, :n] = torch.rand(H, n, generator=g)
+    return c
+
+
+def all_pages(c):
+    return sorted(c._free + sum(c._pages, []))
+
+
+@pytest.mark.parametrize("spare", [20, 3])
+def test_evict_in_as_many_goes_as_pages_allow(plain_eviction, spare):
+    lens = [90, 33, 70, 200]
+    used = sum(-(-n // 32) for n in lens)
+    c = filled(lens, num_pages=used + spare)
+    held = [c.gather(b) for b in range(4)]
+    w = c.weights.clone()
+    calls = []
+    real = c._evict_some
+    c._evict_some = lambda rows, *a: (calls.append(list(rows)), real(rows, *a))
+    c.evict(40, recent=8, first=3)
+    assert calls == ([[0, 2, 3]] if spare == 20 else [[0], [2, 3]])
+    assert c.host_lens == [40, 33, 40, 40] == c.lens.tolist() and c.evicted == [50, 0, 30, 160]
+    assert c._shift.tolist() == c.evicted and c._next_positions().tolist() == [90, 33, 70, 200]
+    assert all_pages(c) == list(range(used + spare)) and [len(p) for p in c._pages] == [2] * 4
+    for b, n in enumerate(lens):
+        k, v = c.gather(b)
+        for h in range(2):
+            keep = ref.select(w[b, h], n, 40, 8, 3) if n > 40 else list(range(n))
+            assert torch.equal(k[h], held[b][0][h, keep]) and torch.equal(v[h], held[b][1][h, keep])
+            assert torch.equal(c.weights[b, h, :len(keep)], w[b, h, keep]) and not c.weights[b, h, len(keep):].any()
+    c.evict(40)  # nothing longer: nothing moves
+    assert c.evicted == [50, 0, 30, 160] and len(calls) == (1 if spare == 20 else 2)
+
+
+def test_evict_refuses(plain_eviction):
+    c = filled([90, 33], num_pages=6)
+    for bad in (dict(keep=0), dict(keep=4, recent=3, first=2), dict(keep=4, recent=-1), dict(keep=4, first=-1)):
+        with pytest.raises(ValueError):
+            c.evict(**bad)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        c.evict(64)  # needs two free pages, one is
+    assert c.host_lens == [90, 33] and c.free_pages == 1 and all_pages(c) == list(range(6))
+    with pytest.raises(ValueError, match="track_weights"):
+        nq.PagedKVCache(4, page_size=32).evict(1)
+    with pytest.raises(ValueError):
+        nq.PagedKVCache(4, page_size=32, track_weights=-1)
+    for cls in (nq.PagedKVCache, nq.PagedKVCache4):
+        with pytest.raises(TypeError, match="bfloat16"):
+            cls(4, page_size=32, track_weights=1)._setup(1, 2, 64, torch.float32, "cpu")
+
+
+def test_trimmed_and_freed_sequences_lose_their_weights(plain_eviction):
+    c = filled([90, 70])
+    w = c.weights.clone()
+    c.set_lengths([50, 70])
+    assert not c.weights[0, :, 50:].any() and torch.equal(c.weights[0, :, :50], w[0, :, :50])
+    assert torch.equal(c.weights[1], w[1])
+    c.evict(40)
+    assert c.evicted == [10, 30]
+    c.free(0)
+    assert c.evicted == [0, 30] and not c.weights[0].any() and c._shift.tolist() == [0, 30]
+    c.free(1)
+    assert c._shift is None and c._next_positions() is None
+
+
+def test_expected_lengths():
+    c = filled([0, 0])
+    for bad in ([0, 3], [-1, 2]):
+        with pytest.raises(ValueError):
+            c.expect_lengths(bad)
+    c.expect_lengths(torch.tensor([3, 5]))
+    with pytest.raises(ValueError, match="do not fit"):
+        c._take_expected(2, 4)
+    assert c._take_expected(2, 4) is None  # asked for once
+    c.expect_lengths([3, 5])
+    with pytest.raises(ValueError, match="do not fit"):
+        c._take_expected(3, 8)
+    c.expect_lengths([3, 5])
+    assert c._take_expected(2, 5) == [3, 5]
+
+
+def test_a_4_bit_cache_of_other_rows_refuses():
+    c = nq.PagedKVCache4(4, page_size=32)
+    c._setup(2, 2, 64, torch.bfloat16, "cpu")
+    assert c.pool.shape == (4, 2, 32, 68) and c.pool.dtype == torch.uint8
+    for H, D, dtype in ((4, 64, torch.bfloat16), (2, 128, torch.bfloat16), (2, 64, torch.float32)):
+        with pytest.raises(ValueError, match="pool holds"):
+            c._setup(2, H, D, dtype, "cpu")
+    with pytest.raises(ValueError):
+        nq.PagedKVCache4(4, page_size=32)._setup(2, 2, 96, torch.bfloat16, "cpu")
+
+
+@pytest.mark.parametrize("kw", [dict(kv_bits=8), dict(kv_bits=4), dict(keep=64), dict(page_size=32, keep=0),
+                                dict(page_size=32, keep=8, recent=8), dict(page_size=32, keep=8, recent=-1),
+                                dict(page_size=32, keep=8, first=9, recent=0)])
+def test_generator_refuses(kw):
+    with pytest.raises(ValueError):
+        nq.generate_greedy_batch(None, [[1]], 4, **kw)
+
+
+# ---------------------------------------------------------------- the work's division
+STEP, COST = 32, 24
+
+
+def decode_split(lens, rows_per_batch, groups):
+    """[(workgroup, row, first step, steps)] of the shared 4-bit decode, key steps only."""
+    nb = [-(-n // STEP) + COST if n > 0 else 0 for n in lens]
+    N = sum(nb) * rows_per_batch
+    used, out = min(groups, N), []
+    starts = []  # (global step, row, steps)
+    at = 0
+    for b, n in enumerate(nb):
+        for j in range(rows_per_batch if n else 0):
+            starts.append((at, b * rows_per_batch + j, n))
+            at += n
+    for w in range(used):
+        q0, q1 = w * N // used, (w + 1) * N // used
+        assert q1 > q0
+        for s, r, n in starts:
+            a, z = max(q0, s), min(q1, s + n)
+            if a < z:  # steps [a - s, z - s) of the row, of which the first COST hold no keys
+                out.append((w, r, max(a - s - COST, 0), max(z - s - COST, 0) - max(a - s - COST, 0)))
+    return out, nb
+
+
+def test_shared_decode_covers_every_key_step_once():
+    rng = random.Random(5)
+    for _ in range(60):
+        B, rpb = rng.choice([1, 2, 5, 17]), rng.choice([1, 2, 8])
+        lens = [rng.choice([0, 1, 31, 32, 33, rng.randrange(1, 4000)]) for _ in range(B)]
+        groups = rng.choice([1, 7, 64, 512])
+        parts, nb = decode_split(lens, rpb, groups)
+        slots = set()
+        for r in range(B * rpb):
+            mine = [(w, a, n) for w, row, a, n in parts if row == r]
+            steps = -(-lens[r // rpb] // STEP)
+            assert sorted(s for _, a, n in mine for s in range(a, a + n)) == list(range(steps))
+            ws = [w for w, _, _ in mine]
+            assert ws == list(range(ws[0], ws[-1] + 1)) if ws else steps == 0  # the merge's run has no gap
+            for w in ws:
+                assert w + r < 512 + B * rpb and (w + r not in slots or len(ws) == 1)
+                if len(ws) > 1:
+                    slots.add(w + r)
+
+
+def chunk_ranges(S, G, max_len, causal, chunk, d, rows=256):
+    R = S * G
+    end = (chunk + 1) * rows if R // rows > chunk else R
+    seen = max_len - S + (end - 1) // G + 1 if causal else max_len
+    return (seen + d - 1) // d if seen > 0 else 0
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_key_weight_ranges_reach_every_seen_key(causal):
+    rng = random.Random(6)
+    for _ in range(200):
+        S, G = rng.choice([3, 17, 300, rng.randrange(3, 5000)]), rng.choice([1, 2, 7, 16])
+        max_len, d = rng.randrange(1, 6000), 256 * rng.randrange(1, 9)
+        R = S * G
+        if R <= 16:
+            continue
+        n = -(-R // 256)
+        counts = [chunk_ranges(S, G, max_len, causal, c, d) for c in range(n)]
+        assert counts == sorted(counts) and counts[-1] * d >= max_len
+        for c in range(n):
+            last = min((c + 1) * 256, R) - 1
+            seen = max_len - S + last // G + 1 if causal else max_len  # keys that the chunk's last row sees
+            assert counts[c] * d >= seen
+        # the sum's search: the first chunk that reaches key t, found by halving
+        for t in (0, max_len - 1, rng.randrange(max_len)):
+            lo, hi = 0, n
+            while lo < hi:
+                mid = (lo + hi) // 2
+                if counts[mid] <= t // d:
+                    lo = mid + 1
+                else:
+                    hi = mid
+            assert lo == next(c for c in range(n) if counts[c] > t // d)
+
+
+def test_multiplied_divisions_are_exact():
+    """floor(n / d) by n * floor(2^32 / d) >> 32 and one correction, for n < 2^31."""
+    rng = random.Random(7)
+    for _ in range(20000):
+        d = rng.choice([1, 2, 3, 255, 256, 2 ** 20, rng.randrange(1, 2 ** 31)])
+        n = rng.choice([0, 1, 2 ** 31 - 1, rng.randrange(2 ** 31), min(2 ** 31 - 1, d * rng.randrange(1, 1 + 2 ** 31 // d)),
+                        max(0, min(2 ** 31 - 1, d * rng.randrange(1, 1 + 2 ** 31 // d)) - 1)])
+        m = 0xffffffff if d == 1 else 2 ** 32 // d
+        q = n * m >> 32
+        q += n - q * d >= d
+        assert q == n // d
+
+
+def test_quantiser_definition():
+    """The scale is the smallest of which the block's largest is at most 7 times, and no element is
+    off by more than a fifth of the largest: by (y - 4) / y or (6 - y) / y for y of 4 to 6 scales,
+    1/7 for 7, half a scale of more than 3.5 below."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(500, 64, generator=g) * torch.exp2(torch.randint(-20, 20, (500, 1), generator=g).float())
+    codes, byte = ref.quantise(x)
+    amax = x.reshape(500, 2, 32).abs().amax(-1).double()
+    scale = torch.exp2(byte.double() - 127)
+    assert (amax <= 7 * scale).all() and (amax > 3.5 * scale).all()
+    err = (ref.values(codes, byte) - x.double()).abs().reshape(500, 2, 32)
+    assert (err <= scale[..., None]).all()
+    assert (err <= amax[..., None] / 5).all()
