@@ -77,18 +77,20 @@ def _check(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> N
             raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or give it detached tensors")
 
 
-def _pool4(pool: torch.Tensor) -> Tuple[int, int, int, int]:
-    """(pages, Hkv, page_size, head_dim) of a 4-bit pool."""
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or pool.shape[3] not in _HEAD_DIMS:
+def _pool4(pool: torch.Tensor):
+    """(pages, Hkv, page_size, head_dim), (address, {page, head} strides) of a 4-bit pool."""
+    shape = pool.shape
+    if pool.dtype is not torch.uint8 or len(shape) != 4 or shape[3] not in _HEAD_DIMS:
         raise ValueError("a 4-bit pool is uint8 (pages, Hkv, page_size, 17 D / 16) with D 32, 64 or 128, "
-                         f"got {pool.dtype} {tuple(pool.shape)}")
-    n, H, P, row = pool.shape
+                         f"got {pool.dtype} {tuple(shape)}")
+    n, H, P, row = shape
     if P <= 0 or P % 32:
         raise ValueError(f"page_size must be a positive multiple of 32, got {P}")
     page, head, step, one = pool.stride()
-    if one != 1 or step != row or page % 16 or head % 16 or pool.data_ptr() % 16:
+    at = pool.data_ptr()
+    if one != 1 or step != row or (page | head | at) & 15:
         raise ValueError("a page's head must be contiguous and all of them 16-byte aligned")
-    return n, H, P, _HEAD_DIMS[row]
+    return (n, H, P, _HEAD_DIMS[row]), (at, _int64s(page, head))
 
 
 @lru_cache(maxsize=1024)  # of a program's few layouts: making one takes as long as a launch's other arguments
@@ -100,18 +102,34 @@ def _strides2(t: torch.Tensor):
     return _int64s(*t.stride()[:2])
 
 
-def _strides3(t: torch.Tensor):
-    return _int64s(*t.stride()[:3])
+_OUTER = {torch.bfloat16: 7, torch.float32: 3}  # strides of which are whole 16 bytes
+
+
+def _rows(t: torch.Tensor, out: Optional[str] = None):
+    """(tensor, address, outer strides) of rows as the kernels read them, a copy where t's own
+    are not; of an output, ``out`` its name, an error."""
+    *outer, last = t.stride()
+    at, odd = t.data_ptr(), 0
+    for s in outer:
+        odd |= s
+    if last != 1 or at & 15 or odd & _OUTER[t.dtype]:
+        if out is not None:
+            ops._rows_out(t, out)
+        return _rows(t.contiguous())
+    return t, at, _int64s(*outer)
 
 
 def _i32(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
-def _table(table: torch.Tensor, B: int) -> torch.Tensor:
-    if table.dim() != 2 or table.shape[0] != B:
-        raise ValueError(f"a block table must be (B={B}, pages per sequence), got {tuple(table.shape)}")
-    return _i32(table)
+def _table(table: torch.Tensor, B: int):
+    """(tensor, address, stride, columns)"""
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != B:
+        raise ValueError(f"a block table must be (B={B}, pages per sequence), got {tuple(shape)}")
+    table = _i32(table)
+    return table, table.data_ptr(), table.stride(0), shape[1]
 
 
 def _lens(lens: torch.Tensor, B: int, name: str = "lens") -> torch.Tensor:
@@ -161,29 +179,29 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
     Returns q_out (None without q), or with ``plan=True`` a KernelCall.
     """
     _check("kv4_append", k, v, pool, block_table, q, q_out, pos_base, pos_shift, row_base, lens_out)
-    n, H, P, D = _pool4(pool)
-    if k.dim() != 4 or k.shape != v.shape or k.shape[1] != H or k.shape[3] != D:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be (B, {H}, S, {D}), as the pool")
-    if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+    (n, H, P, D), pages = _pool4(pool)
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[1] != H or shape[3] != D:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must be (B, {H}, S, {D}), as the pool")
+    if k.dtype is not v.dtype or (q is not None and q.dtype is not k.dtype):
         raise TypeError("k, v and q must share one dtype")
     dt = ops._code(k)
-    B, _, S, _ = k.shape
+    B, _, S, _ = shape
+    Hq, q_rows, q_to = 0, (None, None, None), (None, None, None)
     if q is None and (q_out is not None or q_weight is not None):
         raise ValueError("q_out and q_weight go with q")
     if q is not None:
         if q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, S, D):
             raise ValueError(f"q must be (B={B}, Hq, S={S}, D={D}), got {tuple(q.shape)}")
+        Hq = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(B, S, q.shape[1], D, dtype=q.dtype, device=q.device).transpose(1, 2)
+            q_out = torch.empty(B, S, Hq, D, dtype=q.dtype, device=q.device).transpose(1, 2)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype:
             raise ValueError("q_out must match q in shape and dtype")
-        else:
-            ops._rows_out(q_out, "q_out")
-        q = ops._rows_in(q)
-    dev = k.device
-    bt = _table(block_table, B)
-    if row_base is None and not 0 <= row_offset <= bt.shape[1] * P - S:
-        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {bt.shape[1] * P}")
+        q_rows, q_to = _rows(q), _rows(q_out, "q_out")
+    bt, bt_at, bt_stride, cols = _table(block_table, B)
+    if row_base is None and not 0 <= row_offset <= cols * P - S:
+        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {cols * P}")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if lens_out is not None:
@@ -193,37 +211,39 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
             raise ValueError("lens_out must be a contiguous int32 tensor of B elements")
         if lens_out.data_ptr() == row_base.data_ptr() and B:
             raise ValueError("lens_out must not alias row_base")
-    k, v = ops._rows_in(k), ops._rows_in(v)
-    cos_t, sin_t, max_pos = ops._tables(cos, sin, dev)
-    if cos_t is not None and cos_t.shape[1] != D // 2:
-        raise ValueError(f"the tables must be (max_pos, {D // 2}), got {tuple(cos_t.shape)}")
     for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None and w.numel() != D:
             raise ValueError(f"{what} must hold {D} elements, got {tuple(w.shape)}")
-    pos = None
-    if cos_t is not None:
+    cos_t = sin_t = pos = qw = kw = None
+    max_pos = 0
+    if cos is not None:
+        dev = k.device
+        cos_t, sin_t, max_pos = ops._tables(cos, sin, dev)
+        if cos_t.shape[1] != D // 2:
+            raise ValueError(f"the tables must be (max_pos, {D // 2}), got {tuple(cos_t.shape)}")
         if pos_shift is None:
             pos = ops._positions(position_ids, pos_offset, pos_base, B, S, max_pos, dev)
         elif position_ids is not None:
-            pos = _i32(position_ids.expand(B, S))
+            pos = _i32(position_ids.to(dev).expand(B, S))
     if B == 0 or S == 0:
         return q_out
-    Hq = 0 if q is None else q.shape[1]
     _sizes("kv4_append", B, S, Hq + 2 * H)
     pb = None if pos_base is None else _lens(pos_base, B, "pos_base")
     ps = None if pos_shift is None else _lens(pos_shift, B, "pos_shift")
     rb = None if row_base is None else _lens(row_base, B, "row_base")
-    qw, qf = ops._norm_weight(q_weight, dev, dt, _lib.NQ_QWEIGHT_BF16, plan)
-    kw, kf = ops._norm_weight(k_weight, dev, dt, _lib.NQ_KWEIGHT_BF16, plan)
-    st, ptr = _strides3, ops._ptr
-    args = (ptr(k), st(k), ptr(v), st(v),
-            ptr(q), None if q is None else st(q),
-            ptr(q_out), None if q is None else st(q_out),
-            ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, B, S, Hq, H, D, dt | qf | kf,
+    if q_weight is not None:
+        qw, flag = ops._norm_weight(q_weight, k.device, dt, _lib.NQ_QWEIGHT_BF16, plan)
+        dt |= flag
+    if k_weight is not None:
+        kw, flag = ops._norm_weight(k_weight, k.device, dt & ~_lib.NQ_QWEIGHT_BF16, _lib.NQ_KWEIGHT_BF16, plan)
+        dt |= flag
+    ptr = ops._ptr
+    k_rows, v_rows = _rows(k), _rows(v)
+    args = (*k_rows[1:], *v_rows[1:], *q_rows[1:], *q_to[1:], *pages, n, bt_at, bt_stride, cols, P, B, S, Hq, H, D, dt,
             ptr(qw), ptr(kw), float(eps), ptr(cos_t), ptr(sin_t), max_pos, ptr(pos), ptr(pb), ptr(ps),
             int(pos_offset), ptr(rb), int(row_offset), ptr(lens_out))
     return _launch(plan, k, _lib.load().nq_kv4_append, args, "nq_kv4_append",
-                   (k, v, q, pool, bt, qw, kw, cos_t, sin_t, pos, pb, ps, rb, lens_out), q_out)
+                   (k_rows[0], v_rows[0], q_rows[0], pool, bt, qw, kw, cos_t, sin_t, pos, pb, ps, rb, lens_out), q_out)
 
 
 def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_offset: int = 0,
@@ -235,30 +255,26 @@ def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_off
     ``v_out`` may be views of larger buffers.  Rows without a page come back as NaN.
     """
     _check("kv4_gather", pool, block_table, row_base, k_out, v_out)
-    n, H, P, D = _pool4(pool)
-    B, dev = block_table.shape[0], pool.device
-    bt = _table(block_table, B)
-    if S < 0 or (row_base is None and not 0 <= row_offset <= bt.shape[1] * P - S):
-        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {bt.shape[1] * P}")
+    (n, H, P, D), pages = _pool4(pool)
+    B = block_table.shape[0]
+    bt, bt_at, bt_stride, cols = _table(block_table, B)
+    if S < 0 or (row_base is None and not 0 <= row_offset <= cols * P - S):
+        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {cols * P}")
+    if dtype not in _OUTER:
+        raise TypeError(f"unsupported dtype {dtype}; rows are read back as bfloat16 or float32")
     shape = (B, H, S, D)
-    outs = []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is None:
-            t = torch.empty(shape, dtype=dtype, device=dev)
-        elif tuple(t.shape) != shape or t.dtype != dtype:
+        if t is not None and (tuple(t.shape) != shape or t.dtype != dtype):
             raise ValueError(f"{name} must be {shape} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
-        else:
-            ops._rows_out(t, name)
-        outs.append(t)
-    k, v = outs
-    code = ops._code(k)
+    k = torch.empty(shape, dtype=dtype, device=pool.device) if k_out is None else k_out
+    v = torch.empty(shape, dtype=dtype, device=pool.device) if v_out is None else v_out
+    k_rows, v_rows = _rows(k, "k_out"), _rows(v, "v_out")
     if 0 in shape:
         return k, v
     _sizes("kv4_gather", B, S, H)
     rb = None if row_base is None else _lens(row_base, B, "row_base")
-    st, ptr = _strides3, ops._ptr
-    args = (ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, ptr(k), st(k),
-            ptr(v), st(v), B, S, H, D, code, ptr(rb), int(row_offset))
+    args = (*pages, n, bt_at, bt_stride, cols, P, *k_rows[1:], *v_rows[1:], B, S, H, D, ops._code(k), ops._ptr(rb),
+            int(row_offset))
     return _launch(plan, pool, _lib.load().nq_kv4_gather, args, "nq_kv4_gather", (pool, bt, rb), (k, v))
 
 
@@ -275,37 +291,37 @@ def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     stored values; bf16 q rounds the probabilities to bf16, fp32 q keeps 24 bits of both.
     """
     _check("attention_decode_kv4", q, pool, block_table, lens, out, workspace)
-    n, H, P, D = _pool4(pool)
+    (n, H, P, D), pages = _pool4(pool)
     if q.dim() == 4 and q.shape[2] == 1:
         q = q[:, :, 0]
-    if q.dim() != 3 or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % H:
-        raise ValueError(f"q must be (B, Hq, {D}) with Hq a multiple of the pool's {H} heads, got {tuple(q.shape)}")
-    B, Hq, _ = q.shape
-    dt, dev = ops._code(q), q.device
-    bt = _table(block_table, B)
-    if not 0 < max_len <= bt.shape[1] * P:
-        raise ValueError(f"max_len must be in [1, {bt.shape[1] * P}] (block table columns x page_size), got {max_len}")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D or shape[1] == 0 or shape[1] % H:
+        raise ValueError(f"q must be (B, Hq, {D}) with Hq a multiple of the pool's {H} heads, got {tuple(shape)}")
+    B, Hq, _ = shape
+    dt = ops._code(q)
+    bt, bt_at, bt_stride, cols = _table(block_table, B)
+    if not 0 < max_len <= cols * P:
+        raise ValueError(f"max_len must be in [1, {cols * P}] (block table columns x page_size), got {max_len}")
+    dev = q.device
     if out is None:
-        out = torch.empty(B, Hq, D, dtype=q.dtype, device=dev)
-    elif tuple(out.shape) != (B, Hq, D) or out.dtype != q.dtype:
-        raise ValueError(f"out must be {(B, Hq, D)} in {q.dtype}")
-    else:
-        ops._rows_out(out, "out")
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    elif out.shape != shape or out.dtype != q.dtype:
+        raise ValueError(f"out must be {tuple(shape)} in {q.dtype}")
+    out_rows = _rows(out, "out")
     lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
     if B == 0:
         return (out, lse) if return_lse else out
     _sizes("attention_decode_kv4", B, H, -(-Hq // H // 16) + 1)
     lens_t = _lens(lens, B)
-    q = ops._rows_in(q)
+    q_rows = _rows(q)
     lib = _lib.load()
-    need = lib.nq_attn_decode_kv4_workspace_bytes(B, Hq, H, D)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    ptr = ops._ptr
-    args = (ptr(q), _strides2(q), ptr(pool), _strides2(pool), n, ptr(bt), bt.stride(0), bt.shape[1], P, ptr(lens_t),
-            ptr(out), _strides2(out), ptr(lse), ptr(workspace), workspace.numel() * workspace.element_size(),
-            B, Hq, H, D, int(max_len), dt, 0.0 if sm_scale is None else float(sm_scale))
-    return _launch(plan, q, lib.nq_attn_decode_kv4, args, "nq_attn_decode_kv4", (q, pool, bt, lens_t, workspace),
+        workspace = torch.empty(lib.nq_attn_decode_kv4_workspace_bytes(B, Hq, H, D), dtype=torch.uint8, device=dev)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    args = (*q_rows[1:], *pages, n, bt_at, bt_stride, cols, P, lens_t.data_ptr(), *out_rows[1:], ops._ptr(lse),
+            workspace.data_ptr(), workspace.nbytes, B, Hq, H, D, int(max_len), dt, 0.0 if sm_scale is None else float(sm_scale))
+    return _launch(plan, q, lib.nq_attn_decode_kv4, args, "nq_attn_decode_kv4", (q_rows[0], pool, bt, lens_t, workspace),
                    (out, lse) if return_lse else out)
 
 
@@ -323,9 +339,9 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
     first max_len entries a head and it is returned.
     """
     _check("attention_key_weights", q, k_pool, block_table, lens, lse, weights)
-    four = k_pool.dtype == torch.uint8
+    four = k_pool.dtype is torch.uint8
     if four:
-        n, H, P, D = _pool4(k_pool)
+        (n, H, P, D), pages = _pool4(k_pool)
     else:
         ops._pool_check(k_pool, "k_pool")
         n, H, P, D = k_pool.shape
@@ -333,35 +349,35 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
             raise TypeError(f"k_pool must be bfloat16 or a 4-bit pool, got {k_pool.dtype}")
         if P <= 0 or P % 32:
             raise ValueError(f"page_size must be a positive multiple of 32, got {P}")
-    if q.dtype != torch.bfloat16:
+        pages = k_pool.data_ptr(), _int64s(*k_pool.stride()[:3])
+    if q.dtype is not torch.bfloat16:
         raise TypeError(f"q must be bfloat16, got {q.dtype}")
-    if q.dim() != 4 or q.shape[3] != D or q.shape[1] == 0 or q.shape[1] % H:
-        raise ValueError(f"q must be (B, Hq, S, {D}) with Hq a multiple of the pool's {H} heads, got {tuple(q.shape)}")
-    B, Hq, S, _ = q.shape
-    if lse.dtype != torch.float32 or lse.numel() != B * Hq * S or tuple(lse.shape) not in ((B, Hq, S), (B, Hq)):
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != D or shape[1] == 0 or shape[1] % H:
+        raise ValueError(f"q must be (B, Hq, S, {D}) with Hq a multiple of the pool's {H} heads, got {tuple(shape)}")
+    B, Hq, S, _ = shape
+    if lse.dtype is not torch.float32 or tuple(lse.shape) not in ((B, Hq, S), (B, Hq)) or lse.numel() != B * Hq * S:
         raise ValueError(f"lse must be fp32 {(B, Hq, S)}, got {lse.dtype} {tuple(lse.shape)}")
-    dev = q.device
-    bt = _table(block_table, B)
-    if not 0 < max_len <= bt.shape[1] * P:
-        raise ValueError(f"max_len must be in [1, {bt.shape[1] * P}] (block table columns x page_size), got {max_len}")
+    bt, bt_at, bt_stride, cols = _table(block_table, B)
+    if not 0 < max_len <= cols * P:
+        raise ValueError(f"max_len must be in [1, {cols * P}] (block table columns x page_size), got {max_len}")
     add = weights is not None
     if not add:
-        weights = torch.empty(B, H, max_len, dtype=torch.float32, device=dev)
+        weights = torch.empty(B, H, max_len, dtype=torch.float32, device=q.device)
     else:
         _check_weights(weights, B, H, max_len)
     if B == 0 or S == 0:
         return weights if add else weights.zero_()
     _sizes("attention_key_weights", B, Hq, S)
     lens_t = _lens(lens, B)
-    q, lse = ops._rows_in(q), lse.contiguous()
+    q_rows, lse = _rows(q), lse.contiguous()
     lib = _lib.load()
     need = lib.nq_key_weights_workspace_bytes(B, Hq, H, S, int(max_len))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    ptr = ops._ptr
-    args = (ptr(q), _strides3(q), ptr(k_pool), _strides3(k_pool), int(four), n,
-            ptr(bt), bt.stride(0), bt.shape[1], P, ptr(lens_t), ptr(lse), ptr(weights), _strides2(weights), int(add),
-            ptr(ws), need, B, Hq, H, S, D, int(max_len), int(bool(causal)), 0.0 if sm_scale is None else float(sm_scale))
-    return _launch(plan, q, lib.nq_key_weights, args, "nq_key_weights", (q, k_pool, bt, lens_t, lse, ws), weights)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    args = (*q_rows[1:], *pages, int(four), n, bt_at, bt_stride, cols, P, lens_t.data_ptr(), lse.data_ptr(),
+            weights.data_ptr(), _strides2(weights), int(add), ops._ptr(ws), need, B, Hq, H, S, D, int(max_len),
+            int(bool(causal)), 0.0 if sm_scale is None else float(sm_scale))
+    return _launch(plan, q, lib.nq_key_weights, args, "nq_key_weights", (q_rows[0], k_pool, bt, lens_t, lse, ws), weights)
 
 
 def _check_weights(weights: torch.Tensor, B: int, H: int, least: int) -> None:
@@ -405,17 +421,17 @@ def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], bl
 
     pools: a 4-bit pool, or (k_pool, v_pool) of bf16 or fp32 pages.  The new pages must be none
     of those that any sequence's kept rows lie in (what they hold is overwritten while these
-    are read), and each one's own.  ``kept`` as ``select_keys`` gives it; -1 moves nothing, and rows of the
-    new pages behind the last one moved are left as they are.  With ``weights`` (B, Hkv, W >=
-    keep) returns a fresh tensor of that shape with the kept rows' weights and 0 behind them,
-    else None.
+    are read), and each one's own.  ``kept`` as ``select_keys`` gives it; -1 moves nothing, and
+    rows of the new pages behind the last one moved are left as they are.  With ``weights``
+    (B, Hkv, W >= keep) returns a fresh tensor of that shape with the kept rows' weights and 0
+    behind them, else None.
     """
     four = isinstance(pools, torch.Tensor)
     k_pool, v_pool = (pools, None) if four else pools
     _check("kv_compact", k_pool, v_pool, block_table, new_table, kept, weights)
     if four:
-        n, H, P, D = _pool4(k_pool)
-        ks, vs, row = _strides2(k_pool), None, 0
+        (n, H, P, D), (_, ks) = _pool4(k_pool)
+        vs, row = None, 0
     else:
         for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
             ops._pool_check(pool, name)
@@ -431,11 +447,11 @@ def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], bl
     if kept.dtype != torch.int32 or kept.dim() != 3 or kept.shape[1] != H:
         raise ValueError(f"kept must be int32 (B, {H}, keep), got {kept.dtype} {tuple(kept.shape)}")
     B, _, keep = kept.shape
-    dev = k_pool.device
-    bt, new = _table(block_table, B), _table(new_table, B)
-    if new.shape[1] * P < keep:
-        raise ValueError(f"the new table maps {new.shape[1] * P} rows, {keep} are kept")
-    if B and new.data_ptr() == bt.data_ptr():
+    bt, bt_at, bt_stride, cols = _table(block_table, B)
+    new, new_at, new_stride, new_cols = _table(new_table, B)
+    if new_cols * P < keep:
+        raise ValueError(f"the new table maps {new_cols * P} rows, {keep} are kept")
+    if B and new_at == bt_at:
         raise ValueError("new_table must name other pages than block_table")
     out = None
     if weights is not None:
@@ -447,8 +463,8 @@ def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], bl
         return out if out is None or out.numel() == 0 else out.zero_()
     _sizes("kv_compact", B, H, keep)
     ptr, kept = ops._ptr, kept.contiguous()
-    args = (ptr(k_pool), ks, ptr(v_pool), vs, row, D, n, ptr(bt), bt.stride(0), bt.shape[1], ptr(new), new.stride(0),
-            new.shape[1], P, ptr(kept), ptr(weights), ptr(out), None if out is None else _strides2(out),
+    args = (ptr(k_pool), ks, ptr(v_pool), vs, row, D, n, bt_at, bt_stride, cols, new_at, new_stride, new_cols, P, ptr(kept),
+            ptr(weights), ptr(out), None if out is None else _strides2(out),
             0 if out is None else out.shape[2], B, H, keep)
     return _launch(plan, k_pool, _lib.load().nq_kv_compact, args, "nq_kv_compact",
                    (k_pool, v_pool, bt, new, kept, weights), out)

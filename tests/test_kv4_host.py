@@ -178,6 +178,7 @@ def test_gather_refuses(host_calls, change, error):
     (dict(q=torch.zeros(1, 3, 64, dtype=torch.bfloat16)), ValueError), (dict(q=rows(S=2)), ValueError), (dict(q=rows(D=32)[:, :, 0]), ValueError),
     (dict(q=torch.zeros(1, 2, 64, dtype=torch.float16)), TypeError), (dict(max_len=0), ValueError), (dict(max_len=97), ValueError),
     (dict(lens=LENS.expand(2)), ValueError), (dict(out=torch.zeros(1, 2, 64)), ValueError), (dict(q=torch.zeros(1, 0, 64)), ValueError),
+    (dict(workspace=torch.zeros(1, dtype=torch.uint8).expand(1 << 24)), ValueError),
 ])
 def test_decode_refuses(host_calls, change, error):
     args = dict(q=torch.zeros(1, 2, 64, dtype=torch.bfloat16), pool=pool4(), block_table=TABLE, lens=LENS, max_len=90)
