@@ -114,8 +114,9 @@ __device__ __forceinline__ float xor16_add(float v) {
 }
 
 // ---- up to 16 rows (a decode step): every key's score in one MFMA tile.  HBM-bound: K read
-// once.  A wave has all its keys' loads in flight before the first product, 17 KB of 4-bit
-// keys: with 64 keys a wave, 64 sequences of up to 32768 keys (64/4 heads) took 108 us.
+// once, a wave's keys all in flight before its first product: 128 keys of 4 bits or 64 of 16,
+// 9 and 16 KB.  64 sequences of up to 32768 4-bit keys (64/4 heads, 291 MB): 71 us, 4.1 TB/s;
+// with a fill of the result before it 80 us, with 64 keys a wave 82, with 256 102.
 template <int D, bool FOUR>
 __global__ void __launch_bounds__(256) key_weights_step_kernel(KeyWeightParams p) {
   constexpr int NDQ = D / 32;
@@ -143,6 +144,10 @@ __global__ void __launch_bounds__(256) key_weights_step_kernel(KeyWeightParams p
   bf16x8 q[NDQ];
 #pragma unroll
   for (int i = 0; i < NDQ; ++i) q[i] = Vec8<bf16>::load_bf16(qrow + eight_of<D, FOUR>(grp, i) * 8);
+  // a query that saw nothing adds nothing, whatever it holds
+  const bool none = row_offset(p, b, kvh, c16, R) == -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NDQ; ++i) q[i] = none ? bf16x8{} : q[i];
   float off[4];
   int last[4];  // the last key that the row's query sees
 #pragma unroll
@@ -224,7 +229,7 @@ key_weights_kernel(KeyWeightParams p) {
   int chunk = 0, at_range = blockIdx.x;
   if (p.same) {
     chunk = blockIdx.x / p.same;
-    at_range = blockIdx.x % p.same;
+    at_range = (blockIdx.x % p.same + chunk) % p.same;  // each XCD gets first and last ranges alike
   } else {
     for (int n; chunk + 1 < p.chunks && at_range >= (n = chunk_ranges(p, chunk)); ++chunk) at_range -= n;
   }
@@ -289,6 +294,11 @@ key_weights_kernel(KeyWeightParams p) {
     offs[threadIdx.x] = row_offset(p, b, kvh, r0 + threadIdx.x, r0 + rows);
     lasts[threadIdx.x] = hidden + p.G.div(r0 + threadIdx.x);
   }
+  __syncthreads();
+  // a query that saw nothing adds nothing, whatever it holds (NaN behind a padded sequence)
+  if (offs[threadIdx.x] == -INFINITY)
+#pragma unroll
+    for (int i = 0; i < CPR; ++i) *reinterpret_cast<bf16x8*>(qt + threadIdx.x * RB + i * 16) = bf16x8{};
   __syncthreads();
   const int n = (rows + 15) / 16;
   int qoff[NDQ];  // this lane's operands of 16 rows (the swizzle repeats every 16)
@@ -390,9 +400,12 @@ static int64_t key_weight_groups(const KeyWeightParams& p) {
 
 // Keys of a workgroup: the fewest with which all of them are resident at once, two a CU
 // (512 in all), so that none waits for another's end and each waits for its rows once; 1024
-// where more are needed anyway.  2 prompts of 2048, 16/8 heads, causal: 256 keys 48 us, 1024
-// 45, the 768 chosen 39 (480 workgroups); also launched for the ranges that a chunk does not
-// have, of which the XCDs get unequal shares, 56.
+// where more are needed anyway, and 512 where the diagonal cuts most of them.  2 prompts of
+// 2048, 16/8 heads, causal: 256 keys 48 us, 1024 45, the 768 chosen 38 (480 workgroups); also
+// launched for the ranges that a chunk does not have, of which the XCDs get unequal shares,
+// 56.  A prompt of 8192, 32/8 heads: 1024 keys 401 us, 512 336; without turning the ranges by
+// the chunk 537.  2048 queries at the end of 32768 keys, 64/4 heads: 1024 keys 977 us, 512
+// 1040.
 constexpr int KW_FEW_CHUNKS = 64;
 static int key_weight_range(KeyWeightParams p) {
   if (p.chunks <= KW_FEW_CHUNKS)
@@ -400,7 +413,7 @@ static int key_weight_range(KeyWeightParams p) {
       p.range = Divider(range);
       if (key_weight_groups(p) * p.B * p.Hkv <= 512) return range;
     }
-  return 1024;
+  return p.causal && p.S > p.max_len / 2 ? 512 : 1024;
 }
 
 // ---------------------------------------------------------------- selection

@@ -333,10 +333,10 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
     Key t of sequence b and kv head h: the sum of ``exp(scale q . k_t - lse)`` over the query
     heads of h and the queries that see t.  q: (B, Hq, S, D) bf16 as attended (normed and
     rotated), the last S of the sequence's ``lens[b]`` tokens, ``causal`` or all seeing all;
-    lse: the (B, Hq, S) (or, S = 1, (B, Hq)) fp32 log-sum-exp their attention returned
-    (-inf: the query saw nothing).  k_pool: 4-bit pages or bf16 K pages (pages, Hkv,
-    page_size, D).  Keys from lens[b] on get 0.  With ``weights`` the sums are added to its
-    first max_len entries a head and it is returned.
+    lse: the (B, Hq, S) (or, S = 1, (B, Hq)) fp32 log-sum-exp their attention returned (-inf:
+    the query saw nothing and adds nothing, whatever it holds).  k_pool: 4-bit pages or bf16
+    K pages (pages, Hkv, page_size, D).  Keys from lens[b] on get 0.  With ``weights`` the sums
+    are added to its first max_len entries a head and it is returned.
     """
     _check("attention_key_weights", q, k_pool, block_table, lens, lse, weights)
     four = k_pool.dtype is torch.uint8

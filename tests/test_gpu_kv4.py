@@ -380,6 +380,35 @@ def test_key_weights_of_more_queries_than_keys_and_bad_lengths():
     assert torch.isnan(w[2, :, 32:]).all() and torch.isfinite(w[2, :, :32]).all()
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_key_weights_of_many_chunks_of_rows(causal):
+    say(f"key weights: 75 chunks of rows, three ranges of keys, causal={causal}")
+    q, pool, table, kv, lse, scale = weights_case(1, 32, 1, 32, 32, 600, [2500], True, 77)
+    w = nq.attention_key_weights(q, pool, table, torch.tensor([2500], device=DEV), lse, max_len=2500, causal=causal)
+    check_weights(w, q, kv, table, [2500], lse, scale, causal=causal)
+
+
+@pytest.mark.parametrize("four", [True, False])
+@pytest.mark.parametrize("S,Hq", [(1, 4), (3, 4), (40, 4), (300, 6), (65, 4)])
+def test_queries_that_saw_nothing_add_nothing(S, Hq, four):
+    """Whatever they hold: NaN behind a padded sequence's last query, infinities."""
+    say(f"key weights: unused queries S{S} four={four}")
+    q, pool, table, kv, lse, scale = weights_case(2, Hq, 2, 64, 32, S, [400, 350], four, S)
+    lens = torch.tensor([400, 350], dtype=torch.int32, device=DEV)
+    q = q.clone()
+    lse[1, :, -1] = -math.inf
+    lse[0, 1, S // 2] = -math.inf
+    want = nq.attention_key_weights(q, pool, table, lens, lse, max_len=400)
+    q[1, :, -1] = math.nan
+    q[0, 1, S // 2] = math.inf
+    got = nq.attention_key_weights(q, pool, table, lens, lse, max_len=400)
+    assert torch.isfinite(got).all() and torch.equal(got, want)
+    q[0, 2, S - 1] = math.nan  # of one that saw keys: theirs are NaN, the other head's and sequence's are not
+    got = nq.attention_key_weights(q, pool, table, lens, lse, max_len=400)
+    assert torch.isnan(got[0, 2 // (Hq // 2)]).any() and torch.equal(got[0, 1 - 2 // (Hq // 2)], want[0, 1 - 2 // (Hq // 2)])
+    assert torch.equal(got[1], want[1])
+
+
 # ---------------------------------------------------------------- eviction
 
 @pytest.mark.parametrize("lens,keep,recent,first", [
