@@ -778,7 +778,10 @@ class Attention(nn.Module):
         return o
 
     def _paged4_chunk(self, q4, k4, v4, cache, p0, pos, rot, qw, kw):
-        """(o, lse or None) of a chunk over the stored history and its own rows, which it stores."""
+        """(o, lse or None) of a chunk over the stored history and its own rows, which it stores.
+
+        Its K-hat rows are rounded to the model's type, the attention's operand, before their
+        codes: 2^-9 of a value beside the codes' 2^-3."""
         B, H, S, D = q4.shape
         T = p0 + S
         # the attention's operands, as the prefill takes them: (B, T, Hkv, D) storage

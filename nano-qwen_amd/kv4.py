@@ -26,6 +26,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib, ops
+from .losses import _PROXY, _before_dispatch, _dispatch_mode, _is_tracing, _memory
 
 __all__ = ["kv4_empty_pool", "kv4_append", "kv4_gather", "attention_decode_kv4",
            "attention_key_weights", "select_keys", "kv_compact"]
@@ -51,7 +52,12 @@ class _DeviceCall(ops.KernelCall):
 
 
 def _launch(plan: bool, t, fn, args, name, keep, result):
-    """The planned call, or the result of launching it now on t's device and its current stream."""
+    """The planned call, or the result of launching it now on t's device and its current stream.
+
+    A recording of tensor operations would hold the outputs' allocation without the launch
+    that fills them: it is refused."""
+    if _is_tracing() or _dispatch_mode(_PROXY) is not None or _before_dispatch.get(0) is not None:
+        raise RuntimeError(f"{name}: a trace of tensor operations cannot hold this kernel")
     if plan:
         return _DeviceCall(t, fn, args, name, keep, result)
     device = t.get_device()
@@ -66,7 +72,7 @@ def _launch(plan: bool, t, fn, args, name, keep, result):
 def _check(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     """Device tensors of one device that want no gradient."""
     ops._require_device(first)
-    index, grad = first.get_device(), torch.is_grad_enabled()
+    index, grad, dual = first.get_device(), torch.is_grad_enabled(), ops._forward_ad._current_level >= 0
     for t in (first, *others):
         if t is None:
             continue
@@ -75,6 +81,8 @@ def _check(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> N
             raise ValueError(f"{name}: the operands lie on different devices: {first.device} and {t.device}")
         if grad and t.requires_grad:
             raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or give it detached tensors")
+        if dual and ops._forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode gradient: give it the primal tensors")
 
 
 def _pool4(pool: torch.Tensor):
@@ -139,6 +147,11 @@ def _lens(lens: torch.Tensor, B: int, name: str = "lens") -> torch.Tensor:
     return lens
 
 
+def _at(t: Optional[torch.Tensor]):
+    """The address of an operand that may be left out."""
+    return None if t is None else _memory(t)
+
+
 def _sizes(name: str, *sizes: int) -> None:
     n = 1
     for s in sizes:
@@ -171,7 +184,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
     None the rotation.  Positions: ``position_ids``, else ``pos_base[b] + s``, else
     ``pos_offset + s``, plus ``pos_shift[b]`` where given (rows evicted so far).  q: (B, Hq,
     S, D), normed with q_weight and rotated alike into ``q_out`` (by default fresh), the
-    operand of ``attention_decode_kv4``.  ``lens_out`` (int32 (B,), not ``row_base``)
+    operand of ``attention_decode_kv4``.  ``lens_out`` (int32 (B,), none of the inputs)
     receives ``row_base[b] + S``.  Everything up to the codes is fp32: a row is rounded once.
 
     A sequence whose rows lie outside its table's pages stores nothing and keeps its length
@@ -209,8 +222,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
             raise ValueError("lens_out goes with row_base")
         if lens_out.dtype != torch.int32 or not lens_out.is_contiguous() or lens_out.numel() != B:
             raise ValueError("lens_out must be a contiguous int32 tensor of B elements")
-        if lens_out.data_ptr() == row_base.data_ptr() and B:
-            raise ValueError("lens_out must not alias row_base")
+        if B and any(t is not None and t.data_ptr() == lens_out.data_ptr() for t in (row_base, pos_base, pos_shift)):
+            raise ValueError("lens_out must not be row_base, pos_base or pos_shift")
     for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None and w.numel() != D:
             raise ValueError(f"{what} must hold {D} elements, got {tuple(w.shape)}")
@@ -237,11 +250,10 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
     if k_weight is not None:
         kw, flag = ops._norm_weight(k_weight, k.device, dt & ~_lib.NQ_QWEIGHT_BF16, _lib.NQ_KWEIGHT_BF16, plan)
         dt |= flag
-    ptr = ops._ptr
     k_rows, v_rows = _rows(k), _rows(v)
     args = (*k_rows[1:], *v_rows[1:], *q_rows[1:], *q_to[1:], *pages, n, bt_at, bt_stride, cols, P, B, S, Hq, H, D, dt,
-            ptr(qw), ptr(kw), float(eps), ptr(cos_t), ptr(sin_t), max_pos, ptr(pos), ptr(pb), ptr(ps),
-            int(pos_offset), ptr(rb), int(row_offset), ptr(lens_out))
+            _at(qw), _at(kw), float(eps), _at(cos_t), _at(sin_t), max_pos, _at(pos), _at(pb), _at(ps),
+            int(pos_offset), _at(rb), int(row_offset), _at(lens_out))
     return _launch(plan, k, _lib.load().nq_kv4_append, args, "nq_kv4_append",
                    (k_rows[0], v_rows[0], q_rows[0], pool, bt, qw, kw, cos_t, sin_t, pos, pb, ps, rb, lens_out), q_out)
 
@@ -273,7 +285,7 @@ def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_off
         return k, v
     _sizes("kv4_gather", B, S, H)
     rb = None if row_base is None else _lens(row_base, B, "row_base")
-    args = (*pages, n, bt_at, bt_stride, cols, P, *k_rows[1:], *v_rows[1:], B, S, H, D, ops._code(k), ops._ptr(rb),
+    args = (*pages, n, bt_at, bt_stride, cols, P, *k_rows[1:], *v_rows[1:], B, S, H, D, ops._code(k), _at(rb),
             int(row_offset))
     return _launch(plan, pool, _lib.load().nq_kv4_gather, args, "nq_kv4_gather", (pool, bt, rb), (k, v))
 
@@ -366,6 +378,9 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
         weights = torch.empty(B, H, max_len, dtype=torch.float32, device=q.device)
     else:
         _check_weights(weights, B, H, max_len)
+        (s0, n0), (s1, n1) = sorted(((weights.stride(0), B), (weights.stride(1), H)))
+        if (n0 > 1 and s0 < max_len) or (n1 > 1 and s1 < (s0 * (n0 - 1) + max_len if n0 > 1 else max_len)):
+            raise ValueError("weights of one head must not be another's: they are added to at once")
     if B == 0 or S == 0:
         return weights if add else weights.zero_()
     _sizes("attention_key_weights", B, Hq, S)
@@ -462,9 +477,9 @@ def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], bl
     if 0 in kept.shape:
         return out if out is None or out.numel() == 0 else out.zero_()
     _sizes("kv_compact", B, H, keep)
-    ptr, kept = ops._ptr, kept.contiguous()
-    args = (ptr(k_pool), ks, ptr(v_pool), vs, row, D, n, bt_at, bt_stride, cols, new_at, new_stride, new_cols, P, ptr(kept),
-            ptr(weights), ptr(out), None if out is None else _strides2(out),
+    kept = kept.contiguous()
+    args = (_at(k_pool), ks, _at(v_pool), vs, row, D, n, bt_at, bt_stride, cols, new_at, new_stride, new_cols, P, _at(kept),
+            _at(weights), _at(out), None if out is None else _strides2(out),
             0 if out is None else out.shape[2], B, H, keep)
     return _launch(plan, k_pool, _lib.load().nq_kv_compact, args, "nq_kv_compact",
                    (k_pool, v_pool, bt, new, kept, weights), out)

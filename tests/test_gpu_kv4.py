@@ -497,6 +497,61 @@ def test_compact_skips_what_is_no_row_or_page():
     assert torch.equal(v, want)
 
 
+# ---------------------------------------------------------------- large pools
+
+def far(pool, table, pages, n):
+    """The pool's pages as the last ones of a pool of n, and the table for them."""
+    big = torch.empty(n, *pool.shape[1:], dtype=pool.dtype, device=DEV)
+    big[n - pages:] = pool
+    return big, torch.where(table < pages, table + (n - pages), table)
+
+
+@pytest.mark.parametrize("four", [True, False])
+def test_pages_past_4_gib(four):
+    say(f"pages past 4 GiB, four={four}")
+    g = gen(31)
+    lens, P, H, D = [300, 129], 64, 8, 128
+    table, pages = table_for(lens, P, g, spare=4)
+    used = set(table[table < pages].tolist())
+    new = torch.tensor([i for i in range(pages) if i not in used], dtype=torch.int32, device=DEV).view(2, 2)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q = randn(2, 16, D, g=g, dtype=torch.bfloat16)
+    lse = torch.full((2, 16), 3.0, device=DEV)
+    w = torch.rand(2, H, 320, generator=g, device=DEV)
+    kept = nq.select_keys(w, lens_t, keep=100, recent=5)
+    if four:
+        pool = random_pool(pages, H, P, D, g)
+        big, there = far(pool, table, pages, 66000)
+        assert big[-pages:].data_ptr() - big.data_ptr() > 2 ** 32
+        for S in (1, 40):
+            rows = [randn(2, H, S, D, g=g, dtype=torch.bfloat16) for _ in range(2)]
+            base = lens_t - S
+            nq.kv4_append(*rows, pool, table, row_base=base)
+            nq.kv4_append(*rows, big, there, row_base=base)
+            assert torch.equal(big[-pages:], pool)
+        for x, y in zip(nq.kv4_gather(pool, table, S=129), nq.kv4_gather(big, there, S=129)):
+            assert torch.equal(x, y)
+        assert torch.equal(nq.attention_decode_kv4(q, pool, table, lens_t, max_len=300),
+                           nq.attention_decode_kv4(q, big, there, lens_t, max_len=300))
+        keys, far_keys, pools, far_pools = pool, big, pool, big
+    else:
+        pools = tuple(randn(pages, H, P, D, g=g, dtype=torch.bfloat16) for _ in range(2))
+        (keys, values), (far_keys, far_values) = pools, (far(x, table, pages, 33000)[0] for x in pools)
+        there = far(keys[:, :1, :1], table, pages, 33000)[1]
+        far_pools = (far_keys, far_values)
+        assert far_keys[-pages:].data_ptr() - far_keys.data_ptr() > 2 ** 32
+    for S in (1, 20, 200):
+        qs = randn(2, 16, S, D, g=g, dtype=torch.bfloat16)
+        ls = lse[:, :, None].expand(2, 16, S).contiguous()
+        assert torch.equal(nq.attention_key_weights(qs, keys, table, lens_t, ls, max_len=300),
+                           nq.attention_key_weights(qs, far_keys, there, lens_t, ls, max_len=300))
+    n = far_keys.shape[0]
+    nq.kv_compact(pools, table, new, kept)
+    nq.kv_compact(far_pools, there, new + (n - pages), kept)
+    for x, y in ([(pools, far_pools)] if four else zip(pools, far_pools)):
+        assert torch.equal(y[-pages:], x)
+
+
 # ---------------------------------------------------------------- together
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -60,6 +60,8 @@ REFUSED = [
     ("nq_kv4_append", APPEND, dict(cos=A, sin=ODD, max_pos=4), b"aligned"),
     ("nq_kv4_append", APPEND, dict(kw=ODD), b"aligned"),
     ("nq_kv4_append", APPEND, dict(lens_out=A), b"alias"),
+    ("nq_kv4_append", APPEND, dict(lens_out=A2, pos_base=A2), b"alias"),
+    ("nq_kv4_append", APPEND, dict(lens_out=A2, pos_shift=A2), b"alias"),
     ("nq_kv4_append", APPEND, dict(B=1 << 15, S=1 << 12), b"too many rows"),
     ("nq_kv4_gather", GATHER, dict(v=None), b"required"),
     ("nq_kv4_gather", GATHER, dict(dtype=2), b"dtype"),
@@ -154,6 +156,8 @@ LENS = torch.ones(1, dtype=torch.int32)
     (dict(q_weight=torch.ones(64)), ValueError), (dict(k_weight=torch.ones(63)), ValueError), (dict(cos=torch.ones(8, 32)), ValueError),
     (dict(cos=torch.ones(8, 16), sin=torch.ones(8, 16)), ValueError), (dict(cos=torch.ones(8, 32), sin=torch.ones(8, 32), pos_offset=6), IndexError),
     (dict(lens_out=LENS), ValueError), (dict(lens_out=LENS, row_base=LENS), ValueError),
+    (dict(lens_out=LENS, row_base=LENS.clone(), pos_base=LENS), ValueError),
+    (dict(lens_out=LENS, row_base=LENS.clone(), pos_shift=LENS), ValueError),
     (dict(lens_out=LENS.long(), row_base=LENS), ValueError), (dict(row_base=LENS.expand(2)), ValueError),
     (dict(pos_shift=LENS.expand(3)), ValueError),
 ])
@@ -193,6 +197,7 @@ def test_decode_refuses(host_calls, change, error):
     (dict(lse=torch.zeros(1, 2, 3, dtype=torch.float64)), ValueError), (dict(max_len=97), ValueError),
     (dict(weights=torch.zeros(1, 2, 89)), ValueError), (dict(weights=torch.zeros(1, 2, 90, dtype=torch.float64)), ValueError),
     (dict(weights=torch.zeros(1, 90, 2).transpose(1, 2)), ValueError), (dict(lens=LENS.expand(2)), ValueError),
+    (dict(weights=torch.zeros(1, 1, 90).expand(1, 2, 90)), ValueError), (dict(weights=torch.zeros(200).as_strided((1, 2, 90), (0, 89, 1))), ValueError),
 ])
 def test_key_weights_refuse(host_calls, change, error):
     args = dict(q=rows(), k_pool=pool4(), block_table=TABLE, lens=LENS, lse=torch.zeros(1, 2, 3), max_len=90)
@@ -238,6 +243,24 @@ def test_host_tensors_have_no_path():
             kv4.kv4_empty_pool(1, 1, 32, bad, device="cpu")
     with pytest.raises(ValueError, match="page_size"):
         kv4.kv4_empty_pool(1, 1, 48, 64, device="cpu")
+
+
+def test_recordings_and_gradients_are_refused(monkeypatch):
+    """A trace would hold the outputs' allocation without the launch; forward mode has no tangents."""
+    monkeypatch.setattr(kv4.ops, "_require_device", lambda *a: None)
+    lib = type("L", (), {n: staticmethod(lambda *a: 0) for n in _lib.SIGNATURES})
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    weights = torch.rand(1, 2, 8)
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda w: kv4.select_keys(w, LENS, keep=4), (weights,), check_trace=False)
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with pytest.raises(RuntimeError):
+        make_fx(lambda w: kv4.select_keys(w, LENS, keep=4))(weights)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        kv4.select_keys(weights.clone().requires_grad_(), LENS, keep=4)
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        kv4.select_keys(fwd.make_dual(weights, weights), LENS, keep=4)
 
 
 # ---------------------------------------------------------------- the caches' bookkeeping
