@@ -424,7 +424,8 @@ static int key_weight_range(KeyWeightParams p) {
 // bits (11 + 11 + 10, a histogram in LDS for each), then each wave writes its kept rows:
 // its place in the output follows from the counts of the waves before it.  The first 32
 // weights of a lane (32768 in all) stay in registers; of longer rows the rest is read five
-// times, from the cache.
+// times, from the cache.  Bound by its instructions, five passes over 32 weights a lane on one
+// CU: 64 rows of 32768 take 22 us (8 MB; four copies of the histogram changed nothing).
 struct SelectParams {
   const float* w;
   int64_t wsb, wsh;
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_keys_kernel(SelectParams p
     for (int i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = 0;
     __syncthreads();
     each([&](uint32_t key, int) {
-      if (key && (pass == 0 || key >> (shift + bits) == prefix >> (shift + bits)))
+      if (pass == 0 ? key != 0 : key >> (shift + bits) == prefix >> (shift + bits))
         atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1u);
     });
     __syncthreads();
@@ -519,9 +520,14 @@ __global__ void __launch_bounds__(SEL_THREADS) select_keys_kernel(SelectParams p
   // `room` of the keys equal to `prefix` are kept, the lowest indices
   uint32_t more = 0, same = 0;
   each([&](uint32_t key, int) {
-    more += __popcll(__builtin_amdgcn_ballot_w64(key > prefix));
-    same += __popcll(__builtin_amdgcn_ballot_w64(key == prefix));
+    more += key > prefix;
+    same += key == prefix;
   });
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    more += __shfl_xor(more, m, 64);
+    same += __shfl_xor(same, m, 64);
+  }
   if (lane == 0) {
     wave_a[wave] = more;
     wave_b[wave] = same;
@@ -533,15 +539,21 @@ __global__ void __launch_bounds__(SEL_THREADS) select_keys_kernel(SelectParams p
     ties += wave_b[i];
   }
   at += min(ties, room);
-  const uint64_t below = lane == 0 ? 0 : ~0ull >> (64 - lane);
+  // set bits of lanes before this one
+  auto rank_of = [](uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+  };
   each([&](uint32_t key, int i) {
     const uint64_t eq = __builtin_amdgcn_ballot_w64(key == prefix);
-    const bool take = key > prefix || (key == prefix && ties + __popcll(eq & below) < room);
+    bool take = key > prefix;
+    if (eq) {
+      take |= key == prefix && ties + rank_of(eq) < room;
+      ties += __popcll(eq);
+    }
     const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
-    const uint32_t to = at + __popcll(taken & below);
+    const uint32_t to = at + rank_of(taken);
     if (take && to < (uint32_t)(p.keep - p.recent)) kept[to] = i;  // (weights that change meanwhile)
     at += __popcll(taken);
-    ties += __popcll(eq);
   });
 }
 
