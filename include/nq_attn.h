@@ -651,9 +651,9 @@ int nq_policy_loss_bwd(const float* logprobs, int64_t logprobs_stride, const flo
  * smallest power of two, from 2^-126 to 2^125, of which its largest magnitude is at most
  * 7 times; codes round to the nearest, halfway to the even code, beyond 6 to 6.  A block
  * with an infinity or NaN becomes NaN.
- * lens_out (may be NULL, must not alias row_base) receives row_base[b] + S.  A sequence
- * whose rows do not all lie in [0, bt_cols * page_size) appends nothing and keeps its
- * length there.
+ * lens_out (may be NULL, must not alias row_base, pos_base or pos_shift) receives
+ * row_base[b] + S.  A sequence whose rows do not all lie in [0, bt_cols * page_size)
+ * appends nothing and keeps its length there.
  * dtype: of k, v, q and q_out, with NQ_QWEIGHT_BF16 / NQ_KWEIGHT_BF16.
  */
 int nq_kv4_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
@@ -680,9 +680,10 @@ int nq_kv4_gather(const void* pool, const int64_t* pool_strides, int num_pages, 
  * strides {batch, head}, normed and rotated (nq_kv4_append's q_out); o alike; lse: fp32
  * (B, Hq) or NULL.  dtype: of q and o.  Lengths as in nq_attn_decode_fwd: zeros (and LSE
  * -inf) without keys, NaN outside [0, max_len].  workspace: at least
- * nq_attn_decode_kv4_workspace_bytes, 16-byte aligned; calls that overlap need one each.
+ * nq_attn_decode_kv4_workspace_bytes (0: none, NULL allowed; of the current device),
+ * 16-byte aligned; calls that overlap need one each.
  */
-int64_t nq_attn_decode_kv4_workspace_bytes(int B, int Hq, int Hkv, int D);
+int64_t nq_attn_decode_kv4_workspace_bytes(int B, int Hq, int Hkv, int D, int max_len);
 int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const void* pool,
                        const int64_t* pool_strides, int num_pages, const int32_t* block_table,
                        int64_t bt_stride, int bt_cols, int page_size, const int32_t* lens, void* o,
@@ -696,7 +697,7 @@ int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const void* pool
  *   key t of exp(sm_scale q . k_t - lse)
  * for t < lens[b]; rows [lens[b], max_len) are set to 0, or left alone when accumulating.
  * q: bf16 (B, Hq, S, D) as attended (normed and rotated), strides {batch, head, seq}; lse:
- * fp32 (B, Hq, S) contiguous, -inf for a query without keys.  causal: query s sees keys up
+ * fp32 (B, Hq, S) contiguous, -inf for a query without keys (whatever it holds).  causal: query s sees keys up
  * to lens[b] - S + s; else, and for S = 1, all.  k_pool: four_bit: 4-bit pages, strides
  * {page, head} in bytes; else bf16 K pages, strides {page, head, row} in elements.
  * weights: fp32, strides {batch, head}, max_len entries a head.  A length outside
@@ -709,7 +710,8 @@ int nq_key_weights(const void* q, const int64_t* q_strides, const void* k_pool,
                    const int64_t* pool_strides, int four_bit, int num_pages, const int32_t* block_table,
                    int64_t bt_stride, int bt_cols, int page_size, const int32_t* lens, const float* lse,
                    float* weights, const int64_t* weight_strides, int accumulate, void* workspace,
-                   int64_t workspace_bytes, int B, int Hq, int Hkv, int S, int D, int max_len, int causal, float sm_scale, void* stream);
+                   int64_t workspace_bytes, int B, int Hq, int Hkv, int S, int D, int max_len, int causal,
+                   float sm_scale, void* stream);
 
 /*
  * The rows of a cache worth keeping: kept (int32 (B, Hkv, keep), contiguous) receives, in

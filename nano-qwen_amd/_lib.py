@@ -264,7 +264,7 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32, _i32,                # B, S, Hkv, D, dtype
         _p, _i32, _p,                                # row_base, row0, stream
     ]),
-    "nq_attn_decode_kv4_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),  # B, Hq, Hkv, D
+    "nq_attn_decode_kv4_workspace_bytes": (_i64, [_i32] * 5),  # B, Hq, Hkv, D, max_len
     "nq_attn_decode_kv4": (_i32, [
         _p, _i64p,                                   # q, q_strides
         _p, _i64p, _i32, _p, _i64, _i32, _i32,       # pool, strides, num_pages, block_table, bt_stride, bt_cols, page_size

@@ -564,11 +564,6 @@ decode_kv4_kernel(Kv4DecodeParams pp) {
   }
 }
 
-static int64_t kv4_workspace(int B, int Hq, int Hkv, int D) {
-  const int64_t rows = (int64_t)B * Hkv * ((Hq / Hkv + 15) / 16);
-  return (KV4_MAX_GROUPS + rows) * 16 * (D + 2) * (int64_t)sizeof(float) + rows * 2 * (int64_t)sizeof(int32_t);
-}
-
 // Whether each row goes to a workgroup of its own.  Its eight waves take about KV4_STEP_US
 // for a step each; the shared form takes KV4_SHARE_US more, for the schedule, the
 // partials' way to memory and the merge's launch.  Rows of one launch differ in length, and
@@ -581,19 +576,30 @@ static bool kv4_whole_rows(int64_t rows, int max_len, int cus) {
   return own <= shared;
 }
 
+// CUs of the current device (256 where there is none).
+static int kv4_cus() {
+  static int known[64];
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  cus = __atomic_load_n(&known[dev], __ATOMIC_RELAXED);
+  if (cus == 0) {
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+    __atomic_store_n(&known[dev], cus, __ATOMIC_RELAXED);
+  }
+  return cus;
+}
+
+// Partial slots and the rows' covering workgroups; whole rows need none.
+static int64_t kv4_workspace(int B, int Hq, int Hkv, int D, int max_len) {
+  const int64_t rows = (int64_t)B * Hkv * ((Hq / Hkv + 15) / 16);
+  if (kv4_whole_rows(rows, max_len, kv4_cus())) return 0;
+  return (KV4_MAX_GROUPS + rows) * 16 * (D + 2) * (int64_t)sizeof(float) + rows * 2 * (int64_t)sizeof(int32_t);
+}
+
 template <int D, typename T>
 static hipError_t launch_decode_kv4(Kv4DecodeParams pp, hipStream_t st) {
   DecodeParams& p = pp.d;
-  int dev = 0, cus = 0;
-  static int known[64];  // CUs of each device
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return e;
-  cus = (dev >= 0 && dev < 64) ? __atomic_load_n(&known[dev], __ATOMIC_RELAXED) : 0;
-  if (cus == 0) {
-    e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
-    if (e != hipSuccess) return e;
-    if (dev >= 0 && dev < 64) __atomic_store_n(&known[dev], cus, __ATOMIC_RELAXED);
-  }
+  const int cus = kv4_cus();
   const int64_t rows = (int64_t)p.B * p.rows_per_batch;
   if (kv4_whole_rows(rows, p.max_len, cus)) {
     hipLaunchKernelGGL((decode_kv4_kernel<D, T, true>), dim3((unsigned)rows), dim3(KV4_ROW_WAVES * 64), 0, st, pp);
@@ -602,7 +608,7 @@ static hipError_t launch_decode_kv4(Kv4DecodeParams pp, hipStream_t st) {
   const int groups = cus * KV4_PER_CU < KV4_MAX_GROUPS ? cus * KV4_PER_CU : KV4_MAX_GROUPS;
   p.nwaves = groups;
   hipLaunchKernelGGL((decode_kv4_kernel<D, T, false>), dim3((unsigned)groups), dim3(KV4_WAVES * 64), 0, st, pp);
-  e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int threads = rows * DC_MERGE_WIDE_PARTIALS <= groups ? DC_MERGE_MAX_THREADS : DC_THREADS;
   hipLaunchKernelGGL((decode_merge_kernel<D, T>), dim3((unsigned)rows), dim3(threads),
@@ -734,9 +740,9 @@ extern "C" int nq_kv4_gather(const void* pool, const int64_t* pool_strides, int 
   }));
 }
 
-extern "C" int64_t nq_attn_decode_kv4_workspace_bytes(int B, int Hq, int Hkv, int D) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv) return 0;
-  return kv4_workspace(B, Hq, Hkv, D);
+extern "C" int64_t nq_attn_decode_kv4_workspace_bytes(int B, int Hq, int Hkv, int D, int max_len) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_len <= 0 || Hq % Hkv) return 0;
+  return kv4_workspace(B, Hq, Hkv, D, max_len);
 }
 
 extern "C" int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const void* pool,
@@ -763,8 +769,8 @@ extern "C" int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const
     return nq_fail(NQ_ERR_INVALID, "the block table's %d columns hold fewer than max_len %d rows", bt_cols, max_len);
   const int NG = (Hq / Hkv + 15) / 16;
   if ((int64_t)B * Hkv * NG > 0x3fffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more than 2^30 (sequence, kv head) rows");
-  const int64_t need = kv4_workspace(B, Hq, Hkv, D);
-  if (!workspace || workspace_bytes < need || !nq_aligned16(workspace))
+  const int64_t need = kv4_workspace(B, Hq, Hkv, D, max_len);
+  if (need && (!workspace || workspace_bytes < need || !nq_aligned16(workspace)))
     return nq_fail(NQ_ERR_WORKSPACE, "an aligned workspace of %lld bytes is required, %lld given", (long long)need,
                    (long long)workspace_bytes);
   Kv4DecodeParams pp{};

@@ -328,11 +328,13 @@ def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     q_rows = _rows(q)
     lib = _lib.load()
     if workspace is None:
-        workspace = torch.empty(lib.nq_attn_decode_kv4_workspace_bytes(B, Hq, H, D), dtype=torch.uint8, device=dev)
+        need = lib.nq_attn_decode_kv4_workspace_bytes(B, Hq, H, D, int(max_len))
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     elif not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
     args = (*q_rows[1:], *pages, n, bt_at, bt_stride, cols, P, lens_t.data_ptr(), *out_rows[1:], ops._ptr(lse),
-            workspace.data_ptr(), workspace.nbytes, B, Hq, H, D, int(max_len), dt, 0.0 if sm_scale is None else float(sm_scale))
+            _at(workspace), 0 if workspace is None else workspace.nbytes, B, Hq, H, D, int(max_len), dt, 0.0 if sm_scale is None else float(sm_scale))
     return _launch(plan, q, lib.nq_attn_decode_kv4, args, "nq_attn_decode_kv4", (q_rows[0], pool, bt, lens_t, workspace),
                    (out, lse) if return_lse else out)
 

@@ -31,6 +31,7 @@ GATHER = dict(pool=A, ps=POOL, pages=8, bt=A, bts=4, cols=4, page=64, k=A, ks=S3
 DECODE = dict(q=A, qs=i64(1024, 128), pool=A, ps=POOL, pages=8, bt=A, bts=4, cols=4, page=64, lens=A, o=A,
               os=i64(1024, 128), lse=None, ws=A, wsb=1 << 30, B=2, Hq=8, Hkv=4, D=128, max_len=200, dtype=BF16, scale=0.0,
               stream=None)
+SHARED = dict(DECODE, cols=1000, bts=1000, max_len=64000)
 WEIGHTS = dict(q=A, qs=S3, pool=A, ps=i64(32768, 8192, 128), four=0, pages=8, bt=A, bts=4, cols=4, page=64, lens=A, lse=A,
                w=A, ws=i64(1024, 256), add=0, work=A, workb=1 << 30, B=2, Hq=8, Hkv=4, S=300, D=128, max_len=200, causal=1,
                scale=0.0, stream=None)
@@ -75,9 +76,9 @@ REFUSED = [
     ("nq_attn_decode_kv4", DECODE, dict(lens=None), b"required"),
     ("nq_attn_decode_kv4", DECODE, dict(q=ODD), b"aligned"),
     ("nq_attn_decode_kv4", DECODE, dict(os=i64(1024, 4)), b"strides"),
-    ("nq_attn_decode_kv4", DECODE, dict(wsb=1000), b"workspace"),
-    ("nq_attn_decode_kv4", DECODE, dict(ws=None), b"workspace"),
-    ("nq_attn_decode_kv4", DECODE, dict(ws=ODD), b"workspace"),
+    ("nq_attn_decode_kv4", SHARED, dict(wsb=1000), b"workspace"),
+    ("nq_attn_decode_kv4", SHARED, dict(ws=None), b"workspace"),
+    ("nq_attn_decode_kv4", SHARED, dict(ws=ODD), b"workspace"),
     ("nq_attn_decode_kv4", DECODE, dict(dtype=3), b"dtype"),
     ("nq_key_weights", WEIGHTS, dict(D=48), b"head_dim"),
     ("nq_key_weights", WEIGHTS, dict(Hq=7), b"divisible"),
@@ -116,8 +117,9 @@ def test_c_entries_refuse(fn, base, change, text):
 def test_workspaces():
     lib = _lib.load()
     rows = 64 * 4
-    assert lib.nq_attn_decode_kv4_workspace_bytes(64, 64, 4, 128) == (512 + rows) * 16 * 130 * 4 + rows * 8
-    assert lib.nq_attn_decode_kv4_workspace_bytes(64, 65, 4, 128) == 0
+    assert lib.nq_attn_decode_kv4_workspace_bytes(64, 64, 4, 128, 32768) == (512 + rows) * 16 * 130 * 4 + rows * 8
+    assert lib.nq_attn_decode_kv4_workspace_bytes(64, 65, 4, 128, 32768) == 0
+    assert lib.nq_attn_decode_kv4_workspace_bytes(1, 16, 8, 128, 512) == 0   # whole rows a workgroup
     assert lib.nq_key_weights_workspace_bytes(2, 8, 4, 1, 200) == 0      # 2 rows: no partial sums
     assert lib.nq_key_weights_workspace_bytes(2, 8, 4, 128, 200) == 0    # one chunk
     assert lib.nq_key_weights_workspace_bytes(2, 8, 4, 129, 200) == 2 * 2 * 4 * 200 * 4
