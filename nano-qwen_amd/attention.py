@@ -263,12 +263,13 @@ class PagedKVCache:
     prefill, as ``KVCache.set_lengths`` does; ``expect_lengths`` says before it
     how long they are, and it trims them itself.
 
-    With ``track_weights`` (bf16 models) ``weights`` (B, Hkv, rows) sums the
-    attention weight that each cached key gets, over query heads and over the
-    queries of each one-token step and the last ``track_weights`` of each longer
-    forward; ``evict`` then keeps the keys that got most.  A sequence's rows
-    close up, its positions go on: row r of sequence b stands at position
-    r + evicted[b] or before, and the next token at host_lens[b] + evicted[b].
+    With ``track_weights`` (bf16 models) ``weights`` (B, Hkv, rows; 4 bytes for
+    every row that ``max_pages_per_seq`` allows) sums the attention weight that
+    each cached key gets, over query heads and over the queries of each one-token
+    step and the last ``track_weights`` of each longer forward; ``evict`` then
+    keeps the keys that got most.  A sequence's rows close up, its positions go
+    on: row r of sequence b stands at position r + evicted[b] or before, and the
+    next token at host_lens[b] + evicted[b].
     """
 
     def __init__(self, num_pages: int, page_size: int = 64, max_pages_per_seq: Optional[int] = None, *,
@@ -447,13 +448,14 @@ class PagedKVCache:
         new = [[self._free.pop() for _ in range(each)] for _ in rows]
         whole = len(rows) == len(self.host_lens)
         at = None if whole else torch.tensor(rows, device=dev)
-        table, lens, weights = ((t if whole else t.index_select(0, at)) for t in (self.block_table, self.lens, self.weights))
+        held = self.weights[:, :, :max(self.host_lens)]  # what lies behind is 0
+        table, lens, weights = ((t if whole else t.index_select(0, at)) for t in (self.block_table, self.lens, held))
         kept = kv4.select_keys(weights, lens, keep=keep, recent=recent, first=first)
         w = kv4.kv_compact(self._pools(), table, torch.tensor(new, dtype=torch.int32).to(dev), kept, weights=weights)
         if whole:
-            self.weights.copy_(w)
+            held.copy_(w)
         else:
-            self.weights.index_copy_(0, at, w)
+            held.index_copy_(0, at, w)
         for b, pages in zip(rows, new):
             self._free.extend(reversed(self._pages[b]))
             self._pages[b] = pages

@@ -265,6 +265,32 @@ def test_recordings_and_gradients_are_refused(monkeypatch):
         kv4.select_keys(fwd.make_dual(weights, weights), LENS, keep=4)
 
 
+@pytest.mark.parametrize("current", [0, 3])
+def test_launches_go_to_the_tensors_device_and_its_stream(monkeypatch, current):
+    seen = []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            seen.append(("enter", self.index))
+
+        def __exit__(self, *a):
+            seen.append(("exit", self.index))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 1000 + i, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    t = type("T", (), dict(get_device=lambda self: 3, device=torch.device("cuda", 3)))()
+    fn = lambda *a: seen.append(a) or 0  # noqa: E731
+    around = lambda call: [("enter", 3), call, ("exit", 3)] if current != 3 else [call]  # noqa: E731
+    assert kv4._launch(False, t, fn, (1, 2), "f", (), "result") == "result"
+    assert seen == around((1, 2, 1003))
+    seen.clear()
+    plan = kv4._launch(True, t, fn, (1, 2), "f", (), "result")
+    assert seen == [] and plan.launch() == "result" and seen == around((1, 2, 1003))
+
+
 # ---------------------------------------------------------------- the caches' bookkeeping
 @pytest.fixture
 def plain_eviction(monkeypatch):
