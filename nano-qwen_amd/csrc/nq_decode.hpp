@@ -197,12 +197,20 @@ struct Walk {
     const int l = len_of(p, bb);
     return l > 0 ? (l + DC_STEP - 1) / DC_STEP + COST : 0;
   }
-  // false: wave w has no steps.  EVEN: ranges of one size, whichever XCD they run on
+  // false: wave w has no steps.  EVEN: ranges of one size, whichever XCD they run on, and of 8
+  // steps at least, or of sqrt(steps of a row / 2) where that is more: what a wave saves by a
+  // shorter range the merge, a workgroup a row, then takes for more partials.
   template <bool EVEN = false>
   __device__ __forceinline__ bool start(const DecodeParams& p, int lane, int64_t w) {
     const int64_t N = lane_value_i64(total_steps<COST>(p, lane), 0);
     if (N == 0) return false;
-    const int64_t We = waves_used(p, N);
+    int64_t We;
+    if constexpr (EVEN) {
+      const float row = (float)N / ((float)p.B * (float)p.rows_per_batch);
+      We = max(min((int64_t)p.nwaves, N / max(8, (int)__builtin_sqrtf(0.5f * row))), (int64_t)1);
+    } else {
+      We = waves_used(p, N);
+    }
     if (w >= We) return false;
     q = EVEN ? w * N / We : wave_begin(p, N, We, w);
     q1 = EVEN ? (w + 1) * N / We : wave_begin(p, N, We, w + 1);

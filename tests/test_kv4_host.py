@@ -433,11 +433,11 @@ def test_generator_refuses(kw):
 STEP, COST = 32, 24
 
 
-def decode_split(lens, rows_per_batch, groups):
+def decode_split(lens, rows_per_batch, groups, least):
     """[(workgroup, row, first step, steps)] of the shared 4-bit decode, key steps only."""
     nb = [-(-n // STEP) + COST if n > 0 else 0 for n in lens]
     N = sum(nb) * rows_per_batch
-    used, out = min(groups, N), []
+    used, out = max(min(groups, N // least), 1) if N else 0, []
     starts = []  # (global step, row, steps)
     at = 0
     for b, n in enumerate(nb):
@@ -460,7 +460,8 @@ def test_shared_decode_covers_every_key_step_once():
         B, rpb = rng.choice([1, 2, 5, 17]), rng.choice([1, 2, 8])
         lens = [rng.choice([0, 1, 31, 32, 33, rng.randrange(1, 4000)]) for _ in range(B)]
         groups = rng.choice([1, 7, 64, 512])
-        parts, nb = decode_split(lens, rpb, groups)
+        least = rng.choice([8, 9, 40])  # 8, or more for long rows
+        parts, nb = decode_split(lens, rpb, groups, least)
         slots = set()
         for r in range(B * rpb):
             mine = [(w, a, n) for w, row, a, n in parts if row == r]
