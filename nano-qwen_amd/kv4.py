@@ -278,8 +278,8 @@ def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_off
     for name, t in (("k_out", k_out), ("v_out", v_out)):
         if t is not None and (tuple(t.shape) != shape or t.dtype != dtype):
             raise ValueError(f"{name} must be {shape} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
-    k = torch.empty(shape, dtype=dtype, device=pool.device) if k_out is None else k_out
-    v = torch.empty(shape, dtype=dtype, device=pool.device) if v_out is None else v_out
+    k = torch.empty(B, H, S, D, dtype=dtype, device=pool.device) if k_out is None else k_out
+    v = torch.empty_like(k, memory_format=torch.contiguous_format) if v_out is None else v_out
     k_rows, v_rows = _rows(k, "k_out"), _rows(v, "v_out")
     if 0 in shape:
         return k, v
@@ -316,7 +316,7 @@ def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch
         raise ValueError(f"max_len must be in [1, {cols * P}] (block table columns x page_size), got {max_len}")
     dev = q.device
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != q.dtype:
         raise ValueError(f"out must be {tuple(shape)} in {q.dtype}")
     out_rows = _rows(out, "out")
