@@ -93,50 +93,67 @@ struct KeyPages {
     first = min(first, (len - 1) & ~31);
     const int page = p.page.div(first, rel);
     pid = p.bt[b * p.bts + page];
+  }
+  __device__ __forceinline__ void check(const KeyWeightParams& p) {  // waits for the load
     const bool bad = (uint32_t)pid >= (uint32_t)p.npages;
     lost = __builtin_amdgcn_ballot_w64(bad);
     if (bad) pid = 0;
   }
 };
 
-// What a row's -lse adds to its scores, in log2 units: -inf (no weight) for a query that
-// sees no key and for rows past the last.
-__device__ __forceinline__ float row_offset(const KeyWeightParams& p, int b, int kvh, int r, int R) {
+// A row's lse: -inf for rows past the last.
+__device__ __forceinline__ float row_lse_of(const KeyWeightParams& p, int b, int kvh, int r, int R) {
   int g;
   const int s = p.G.div(min(r, R - 1), g);
   const float v = p.lse[((int64_t)b * p.Hq + kvh * p.G.d + g) * p.S + s];
-  return r >= R || v == -INFINITY ? -INFINITY : -v * kLog2e;
+  return r >= R ? -INFINITY : v;
 }
+// What it adds to the row's scores, in log2 units: -inf (no weight) for a query that sees no key.
+__device__ __forceinline__ float row_offset(float lse) { return lse == -INFINITY ? lse : -lse * kLog2e; }
 
-__device__ __forceinline__ float xor16_add(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+// Four values' sums over the wave's four groups of 16 lanes: group g gets that of value g.
+// (The swaps exchange odd groups of the first with even ones of the second, halves likewise.)
+__device__ __forceinline__ float group_sums(const float (&v)[4]) {
+  float y[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), false, false);
+    y[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(y[0]), __float_as_uint(y[1]), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // ---- up to 16 rows (a decode step): every key's score in one MFMA tile.  HBM-bound: K read
-// once, a wave's keys all in flight before its first product: 128 keys of 4 bits or 64 of 16,
-// 9 and 16 KB.  64 sequences of up to 32768 4-bit keys (64/4 heads, 291 MB): 71 us, 4.1 TB/s;
-// with a fill of the result before it 80 us, with 64 keys a wave 82, with 256 102.
-template <int D, bool FOUR>
+// once.  A wave takes 64 keys at a time, of 4-bit pages two to four such runs, the next one
+// on its way; of bf16 pages one.  4-bit codes are read past the caches (cached, 64 sequences
+// of 32768 keys and 4 heads took 121 us for 115); bf16 rows are not, two loads sharing each
+// line (past the caches 260 us for 226 at 1024 to 32768 keys).  64 sequences of as many 4-bit
+// keys (64/4 heads, 291 MB): 61 us, 4.8 TB/s; with a part of 128 keys a wave, all of its
+// loads at once, 73.
+template <int D, bool FOUR, bool ADD>
 __global__ void __launch_bounds__(256) key_weights_step_kernel(KeyWeightParams p) {
   constexpr int NDQ = D / 32;
-  constexpr int RUN = FOUR ? 128 : 64;  // keys of a wave
+  constexpr int RUN = 64;  // keys
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, grp = lane >> 4;
   const int b = blockIdx.z, kvh = blockIdx.y;
-  const int k0 = (blockIdx.x * 4 + wave) * RUN;
+  // Turned by the head: the XCD of a workgroup goes by blockIdx.x where the grid is a multiple
+  // of 8 wide, and only some sequences have last keys (16 wide and not turned: 88 us for 72).
+  const uint32_t x = (blockIdx.x + (uint32_t)(b * p.Hkv + kvh)) % gridDim.x;
+  const int span = p.range.d, k0 = (int)(x * 4 + wave) * span;
   if (k0 >= p.max_len) return;
   const int len = ld_uniform(p.lens, b);
   float* w = p.w + b * p.wsb + kvh * p.wsh;
   const bool bad_len = len < 0 || len > p.max_len;
-  if (bad_len || k0 >= len) {  // no keys here
-    if (!p.add)
-      for (int t = k0 + lane; t < min(k0 + RUN, p.max_len); t += 64) w[t] = bad_len ? __builtin_nanf("") : 0.f;
-    return;
-  }
+  const int runs = bad_len || k0 >= len ? 0 : (min(len - k0, span) + RUN - 1) / RUN;
+  if (!ADD)  // what the runs do not reach
+    for (int t = k0 + runs * RUN + lane; t < min(k0 + span, p.max_len); t += 64) w[t] = bad_len ? __builtin_nanf("") : 0.f;
+  if (runs == 0) return;
+  // what does not hang on the block table is on its way before it is waited for
   KeyPages at;
-  at.load(p, b, k0 + min(lane, RUN / 32 - 1) * 32, len);
+  at.load(p, b, k0 + min(lane, span / 32 - 1) * 32, len);
   const int R = p.S * p.G.d;
   int g;
   const int s = p.G.div(min(c16, R - 1), g);
@@ -144,53 +161,73 @@ __global__ void __launch_bounds__(256) key_weights_step_kernel(KeyWeightParams p
   bf16x8 q[NDQ];
 #pragma unroll
   for (int i = 0; i < NDQ; ++i) q[i] = Vec8<bf16>::load_bf16(qrow + eight_of<D, FOUR>(grp, i) * 8);
-  // a query that saw nothing adds nothing, whatever it holds
-  const bool none = row_offset(p, b, kvh, c16, R) == -INFINITY;
-#pragma unroll
-  for (int i = 0; i < NDQ; ++i) q[i] = none ? bf16x8{} : q[i];
+  const float own = row_lse_of(p, b, kvh, c16, R);
   float off[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) off[e] = row_lse_of(p, b, kvh, grp * 4 + e, R);
+  at.check(p);
+  struct Run {
+    Keys32<D, FOUR, FOUR> k[2];
+    float old;  // the weights so far
+  };
+  auto load = [&](Run& x, int i) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      x.k[u].load(p, __builtin_amdgcn_readlane(at.pid, 2 * i + u), kvh, __builtin_amdgcn_readlane(at.rel, 2 * i + u), c16, grp);
+    if constexpr (ADD) x.old = w[min(k0 + i * RUN + lane, len - 1)];
+  };
+  Run even, odd;
+  load(even, 0);
+  if constexpr (FOUR) load(odd, min(1, runs - 1));
+  // a query that saw nothing adds nothing, whatever it holds
+#pragma unroll
+  for (int i = 0; i < NDQ; ++i) q[i] = own == -INFINITY ? bf16x8{} : q[i];
   int last[4];  // the last key that the row's query sees
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int re = grp * 4 + e;
-    off[e] = row_offset(p, b, kvh, re, R);
-    last[e] = p.causal ? len - p.S + p.G.div(re) : 0x7fffffff;
+    off[e] = row_offset(off[e]);
+    last[e] = p.causal ? len - p.S + p.G.div(grp * 4 + e) : 0x7fffffff;
   }
-  Keys32<D, FOUR, true> keys[RUN / 32];
-#pragma unroll
-  for (int i = 0; i < RUN / 32; ++i)
-    keys[i].load(p, __builtin_amdgcn_readlane(at.pid, i), kvh, __builtin_amdgcn_readlane(at.rel, i), c16, grp);
-  float old[RUN / 64];  // the weights so far
-#pragma unroll
-  for (int i = 0; i < RUN / 64; ++i) {
-    const int t = min(k0 + i * 64 + lane, len - 1);
-    old[i] = p.add ? w[t] : 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < RUN / 64; ++i) {
+  auto weigh = [&](const Run& x, int i) {
     float sum[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       floatx4 sc = floatx4{};
 #pragma unroll
-      for (int d = 0; d < NDQ; ++d) sc = mfma16(q[d], keys[2 * i + t / 2].operand(t & 1, d), sc);
-      const int key = k0 + i * 64 + t * 16 + c16;
-      float x = 0.f;
+      for (int d = 0; d < NDQ; ++d) sc = mfma16(q[d], x.k[t / 2].operand(t & 1, d), sc);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sc[e] = fast_exp2(__builtin_fmaf(sc[e], p.scale_log2, off[e]));
       if (p.causal) {
+        const int key = k0 + i * RUN + t * 16 + c16;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x += key <= last[e] ? sc[e] : 0.f;
-      } else {
-        x = (sc[0] + sc[1]) + (sc[2] + sc[3]);
+        for (int e = 0; e < 4; ++e) sc[e] = key <= last[e] ? sc[e] : 0.f;
       }
-      sum[t] = xor32_sum(xor16_add(x));
-      if (at.lost >> (2 * i + t / 2) & 1) sum[t] = __builtin_nanf("");
+      sum[t] = (sc[0] + sc[1]) + (sc[2] + sc[3]);
     }
-    const float mine = grp == 0 ? sum[0] : grp == 1 ? sum[1] : grp == 2 ? sum[2] : sum[3];
-    const int t = k0 + i * 64 + lane;
-    if (t < len) w[t] = old[i] + mine;
-    else if (!p.add && t < p.max_len) w[t] = 0.f;
+    float mine = group_sums(sum);
+    if (at.lost >> (2 * i + lane / 32) & 1) mine = __builtin_nanf("");
+    const int t = k0 + i * RUN + lane;
+    if (t < len) w[t] = ADD ? x.old + mine : mine;
+    else if (!ADD && t < p.max_len) w[t] = 0.f;
+  };
+  if constexpr (!FOUR) {
+    weigh(even, 0);
+  } else {
+    if (runs == 1) {
+      weigh(even, 0);
+      return;
+    }
+    int i = 0;
+    for (; i + 3 < runs; i += 2) {
+      weigh(even, i);
+      load(even, i + 2);
+      weigh(odd, i + 1);
+      load(odd, i + 3);
+    }
+    weigh(even, i);
+    if (i + 2 < runs) load(even, i + 2);
+    weigh(odd, i + 1);
+    if (i + 2 < runs) weigh(even, i + 2);
   }
 }
 
@@ -254,6 +291,7 @@ key_weights_kernel(KeyWeightParams p) {
   {
     const int l = min(lane, 2 * tiles - 1);
     at.load(p, b, range0 + ((l >> 1) * 4 + wave) * 64 + (l & 1) * 32, len);
+    at.check(p);
   }
   Keys32<D, FOUR, false> keys[2];
   auto load_keys = [&](int i) {
@@ -291,7 +329,7 @@ key_weights_kernel(KeyWeightParams p) {
       for (int i = 0; i < PCS / 2; ++i)
         *reinterpret_cast<bf16x8*>(dst + (half * (PCS / 2) + i) * STEP * RB) = piece[i];
     }
-    offs[threadIdx.x] = row_offset(p, b, kvh, r0 + threadIdx.x, r0 + rows);
+    offs[threadIdx.x] = row_offset(row_lse_of(p, b, kvh, r0 + threadIdx.x, r0 + rows));
     lasts[threadIdx.x] = hidden + p.G.div(r0 + threadIdx.x);
   }
   __syncthreads();
@@ -353,12 +391,8 @@ key_weights_kernel(KeyWeightParams p) {
       pass(seen, min(all, n), std::true_type{});
       pass(max(all, 0), n, std::false_type{});
     }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      acc[t] = xor32_sum(xor16_add(acc[t]));
-      if (at.lost >> (2 * i + t / 2) & 1) acc[t] = __builtin_nanf("");
-    }
-    const float mine = grp == 0 ? acc[0] : grp == 1 ? acc[1] : grp == 2 ? acc[2] : acc[3];
+    float mine = group_sums(acc);
+    if (at.lost >> (2 * i + lane / 32) & 1) mine = __builtin_nanf("");
     const int t = k0 + lane;
     if (t < len) w[t] = add ? w[t] + mine : mine;
     else if (!add && t < p.max_len) w[t] = 0.f;
@@ -386,6 +420,15 @@ __global__ void __launch_bounds__(256) key_weights_sum_kernel(KeyWeightParams p)
   const int len = ld_uniform(p.lens, b);
   if (!p.add) *w = sum;
   else if (len <= p.max_len && t < len) *w += sum;
+}
+
+// Keys of a wave of the 4-bit step kernel, in runs of 64: two runs, and up to four where more
+// than 8192 waves would have two.  64 sequences of 1024 to 32768 keys, 64/4 heads (with a
+// fill of 10 us): four runs 68 us, eight 72, sixteen 77; 256 of up to 1024, 32/8 heads: two
+// 28, four 23.
+static int key_weight_span(const KeyWeightParams& p) {
+  const int64_t runs = ((int64_t)p.max_len + 63) / 64 * p.B * p.Hkv / 8192;
+  return 64 * (int)(runs < 2 ? 2 : (runs > 4 ? 4 : runs));
 }
 
 // Chunks of the rows.
@@ -727,12 +770,15 @@ extern "C" int nq_key_weights(const void* q, const int64_t* q_strides, const voi
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t R = (int64_t)S * p.G.d;
   if (R <= 16) {
-    const int run = four_bit ? 512 : 256;  // keys of a workgroup
-    const dim3 grid((unsigned)((max_len + run - 1) / run), (unsigned)Hkv, (unsigned)B);
+    p.range = Divider(four_bit ? key_weight_span(p) : 64);
+    const int64_t keys = 4 * (int64_t)p.range.d;
+    const dim3 grid((unsigned)((max_len + keys - 1) / keys), (unsigned)Hkv, (unsigned)B);
     return nq_check_launch(with_head_dim(D, [&](auto dc) {
       constexpr int DD = decltype(dc)::value;
-      if (four_bit) hipLaunchKernelGGL((key_weights_step_kernel<DD, true>), grid, dim3(256), 0, st, p);
-      else hipLaunchKernelGGL((key_weights_step_kernel<DD, false>), grid, dim3(256), 0, st, p);
+      if (four_bit && p.add) hipLaunchKernelGGL((key_weights_step_kernel<DD, true, true>), grid, dim3(256), 0, st, p);
+      else if (four_bit) hipLaunchKernelGGL((key_weights_step_kernel<DD, true, false>), grid, dim3(256), 0, st, p);
+      else if (p.add) hipLaunchKernelGGL((key_weights_step_kernel<DD, false, true>), grid, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((key_weights_step_kernel<DD, false, false>), grid, dim3(256), 0, st, p);
       return hipGetLastError();
     }));
   }

@@ -380,6 +380,23 @@ def test_key_weights_of_more_queries_than_keys_and_bad_lengths():
     assert torch.isnan(w[2, :, 32:]).all() and torch.isfinite(w[2, :, :32]).all()
 
 
+@pytest.mark.parametrize("four", [True, False])
+def test_key_weights_of_several_runs_a_wave(four):
+    """Enough keys for waves of two, three and four runs, and last waves of one."""
+    for B, Hkv, top in ((130, 8, 1030), (200, 8, 1030), (300, 8, 1000)):
+        say(f"key weights: {B} sequences of up to {top} keys, four={four}")
+        lens = [(37 * i * i + 61) % (top + 1) for i in range(B - 1)] + [top]
+        q, pool, table, kv, lse, scale = weights_case(B, 2 * Hkv, Hkv, 32, 32, 1, lens, four, B)
+        lens_t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        w = nq.attention_key_weights(q, pool, table, lens_t, lse, max_len=top)
+        base = torch.rand(B, Hkv, top, device=DEV)
+        acc = nq.attention_key_weights(q, pool, table, lens_t, lse, max_len=top, weights=base.clone())
+        some = list(range(0, B, 9)) + [B - 1]
+        pick = lambda x: x[some]  # noqa: E731
+        check_weights(pick(w), pick(q), kv, pick(table), [lens[b] for b in some], pick(lse), scale)
+        check_weights(pick(acc), pick(q), kv, pick(table), [lens[b] for b in some], pick(lse), scale, base=pick(base))
+
+
 @pytest.mark.parametrize("causal", [True, False])
 def test_key_weights_of_many_chunks_of_rows(causal):
     say(f"key weights: 75 chunks of rows, three ranges of keys, causal={causal}")
