@@ -83,6 +83,12 @@ template <int D, bool FOUR, bool ONCE> struct Keys32 {
   }
 };
 
+// i of n, turned by `by`.
+__device__ __forceinline__ uint32_t turned(uint32_t i, uint32_t n, uint32_t by) {
+  i += by % n;
+  return i < n ? i : i - n;
+}
+
 // Where a wave's keys lie: a lane holds the page of the 32 keys from `first` on, which never
 // cross one, and their first row there; past the last key its 32 again.  lost: the pages
 // that are none of the pool's, a bit a lane.
@@ -141,7 +147,7 @@ __global__ void __launch_bounds__(256) key_weights_step_kernel(KeyWeightParams p
   const int b = blockIdx.z, kvh = blockIdx.y;
   // Turned by the head: the XCD of a workgroup goes by blockIdx.x where the grid is a multiple
   // of 8 wide, and only some sequences have last keys (16 wide and not turned: 88 us for 72).
-  const uint32_t x = (blockIdx.x + (uint32_t)(b * p.Hkv + kvh)) % gridDim.x;
+  const uint32_t x = turned(blockIdx.x, gridDim.x, (uint32_t)b * (uint32_t)p.Hkv + (uint32_t)kvh);
   const int span = p.range.d, k0 = (int)(x * 4 + wave) * span;
   if (k0 >= p.max_len) return;
   const int len = ld_uniform(p.lens, b);
@@ -267,9 +273,9 @@ key_weights_kernel(KeyWeightParams p) {
   int chunk = 0, at_range;
   if (p.same) {
     chunk = blockIdx.x / p.same;
-    at_range = (blockIdx.x % p.same + chunk) % p.same;
+    at_range = (int)turned(blockIdx.x % p.same, p.same, chunk);
   } else {
-    at_range = (blockIdx.x + (uint32_t)(b * p.Hkv + kvh)) % gridDim.x;
+    at_range = (int)turned(blockIdx.x, gridDim.x, (uint32_t)b * (uint32_t)p.Hkv + (uint32_t)kvh);
     for (int n; chunk + 1 < p.chunks && at_range >= (n = chunk_ranges(p, chunk)); ++chunk) at_range -= n;
   }
   const int range0 = at_range * (int)p.range.d;
