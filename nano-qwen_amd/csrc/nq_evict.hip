@@ -802,7 +802,7 @@ extern "C" int nq_key_weights(const void* q, const int64_t* q_strides, const voi
   p.range = Divider(key_weight_range(p));
   if (p.chunks > KW_FEW_CHUNKS) p.same = p.range.div(max_len + (int)p.range.d - 1);
   const int64_t groups = p.same ? (int64_t)p.chunks * p.same : key_weight_groups(p);
-  if (groups > 0x7fffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more query rows and keys than one launch takes");
+  if (groups > 0xffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more query rows and keys than one launch takes");
   const dim3 grid((unsigned)groups, (unsigned)Hkv, (unsigned)B);
   hipError_t e = with_head_dim(D, [&](auto dc) {
     constexpr int DD = decltype(dc)::value;
@@ -827,7 +827,8 @@ extern "C" int nq_select_keys(const float* weights, const int64_t* weight_stride
     return nq_fail(NQ_ERR_INVALID, "first %d and recent %d must fit keep %d", first, recent, keep);
   if (!weights || !weight_strides || !lens || !kept)
     return nq_fail(NQ_ERR_INVALID, "weights, their strides, lens and kept are required");
-  if ((int64_t)B * Hkv > 0x7fffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more than 2^31 (sequence, kv head) rows");
+  if ((int64_t)B * Hkv * SEL_THREADS > 0xffffffffll)  // a launch has fewer than 2^32 threads
+    return nq_fail(NQ_ERR_UNSUPPORTED, "more (sequence, kv head) rows than one launch takes");
   SelectParams p{weights, weight_strides[0], weight_strides[1], lens, kept, Hkv, width, keep, recent, first};
   hipLaunchKernelGGL(select_keys_kernel, dim3((unsigned)(B * Hkv)), dim3(SEL_THREADS), 0,
                      reinterpret_cast<hipStream_t>(stream), p);
@@ -883,6 +884,7 @@ extern "C" int nq_kv_compact(void* k_pool, const int64_t* k_strides, void* v_poo
   p.Hkv = Hkv; p.keep = keep; p.W = weights ? width : keep;
   p.row_groups = (keep + CP_ROWS - 1) / CP_ROWS;
   const int64_t groups = p.row_groups + ((int64_t)p.W - keep + 255) / 256;
+  if (groups > 0xffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more kept rows than one launch takes");
   const dim3 grid((unsigned)groups, (unsigned)Hkv, (unsigned)B);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (!four) hipLaunchKernelGGL((compact_rows_kernel<void>), grid, dim3(256), 0, st, p);

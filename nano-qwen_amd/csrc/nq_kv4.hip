@@ -770,7 +770,8 @@ extern "C" int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const
   if ((max_len + page_size - 1) / page_size > bt_cols)
     return nq_fail(NQ_ERR_INVALID, "the block table's %d columns hold fewer than max_len %d rows", bt_cols, max_len);
   const int NG = (Hq / Hkv + 15) / 16;
-  if ((int64_t)B * Hkv * NG > 0x3fffffff) return nq_fail(NQ_ERR_UNSUPPORTED, "more than 2^30 (sequence, kv head) rows");
+  if ((int64_t)B * Hkv * NG * DC_MERGE_MAX_THREADS > 0xffffffffll)  // a launch has fewer than 2^32 threads
+    return nq_fail(NQ_ERR_UNSUPPORTED, "more (sequence, kv head) rows than one launch takes");
   const int64_t need = kv4_workspace(B, Hq, Hkv, D, max_len);
   if (need && (!workspace || workspace_bytes < need || !nq_aligned16(workspace)))
     return nq_fail(NQ_ERR_WORKSPACE, "an aligned workspace of %lld bytes is required, %lld given", (long long)need,

@@ -80,6 +80,7 @@ REFUSED = [
     ("nq_attn_decode_kv4", SHARED, dict(ws=None), b"workspace"),
     ("nq_attn_decode_kv4", SHARED, dict(ws=ODD), b"workspace"),
     ("nq_attn_decode_kv4", DECODE, dict(dtype=3), b"dtype"),
+    ("nq_attn_decode_kv4", DECODE, dict(B=1 << 20), b"one launch"),
     ("nq_key_weights", WEIGHTS, dict(D=48), b"head_dim"),
     ("nq_key_weights", WEIGHTS, dict(Hq=7), b"divisible"),
     ("nq_key_weights", WEIGHTS, dict(max_len=300), b"columns"),
@@ -93,6 +94,7 @@ REFUSED = [
     ("nq_select_keys", SELECT, dict(first=-1), b"keep"),
     ("nq_select_keys", SELECT, dict(w=None), b"required"),
     ("nq_select_keys", SELECT, dict(B=0), b"positive"),
+    ("nq_select_keys", SELECT, dict(B=1 << 20), b"one launch"),
     ("nq_kv_compact", COMPACT, dict(new=A), b"new"),
     ("nq_kv_compact", COMPACT, dict(ncols=1, nbts=1), b"kept"),
     ("nq_kv_compact", COMPACT, dict(D=256), b"head_dim"),
@@ -100,6 +102,7 @@ REFUSED = [
     ("nq_kv_compact", COMPACT, dict(w=A, wo=A, ws=i64(512, 128), W=128), b"weights_out"),
     ("nq_kv_compact", COMPACT, dict(w=A, wo=A2, ws=i64(512, 128), W=64), b"together"),
     ("nq_kv_compact", COMPACT, dict(keep=0), b"positive"),
+    ("nq_kv_compact", COMPACT, dict(keep=1 << 30, ncols=1 << 25, nbts=1 << 25), b"one launch"),
     ("nq_kv_compact", PLAIN, dict(row=100), b"16 bytes"),
     ("nq_kv_compact", PLAIN, dict(ks=i64(65536, 16384, 128)), b"overlap"),
     ("nq_kv_compact", PLAIN, dict(v=ODD), b"16 bytes"),
