@@ -301,6 +301,8 @@ def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     scaled scores.  A sequence without keys gives zeros and -inf, one whose length lies
     outside [0, max_len], or whose pages are not the pool's, NaN.  Products are exact in the
     stored values; bf16 q rounds the probabilities to bf16, fp32 q keeps 24 bits of both.
+    ``workspace``: a contiguous buffer of ``nq_attn_decode_kv4_workspace_bytes``, for one call
+    at a time; by default a fresh one where the call needs it.
     """
     _check("attention_decode_kv4", q, pool, block_table, lens, out, workspace)
     (n, H, P, D), pages = _pool4(pool)
