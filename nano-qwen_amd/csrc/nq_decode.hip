@@ -916,7 +916,7 @@ static int decode_launch_f32(const DecodeParams& d, int D, bool paged, bool appe
   p.B = d.B; p.Hq = d.Hq; p.Hkv = d.Hkv; p.G = d.G; p.S = 1; p.T = d.max_len;
   p.BM = 128 / d.G; p.nqb = 1;
   p.scale_log2 = d.scale_log2;
-  p.kv_lens = d.lens; p.kv_extra = d.append; p.kv_max = d.max_len;
+  p.kv_lens = d.lens; p.kv_extra = d.append; p.kv_max = d.max_len; p.lse_nan = 1;
   if (paged) { p.bt = d.bt; p.bts = d.bts; p.page = d.page; }
   const bool fuse = d.qw != nullptr || d.cos_tab != nullptr;
   return nq_check_launch(launch_prefill_f32(p, D, false, fuse, st));

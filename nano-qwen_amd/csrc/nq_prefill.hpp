@@ -35,6 +35,7 @@ struct PrefillParams {
   // keys - 1.
   const int32_t* kv_lens;
   int kv_extra, kv_max;
+  int lse_nan;  // the LSE of such a length: NaN (decode), else -inf
   // paged K/V (NULL bt = dense): key t of sequence b is row t % page of page
   // bt[b * bts + t / page], strides (ksb, ksh, kss) = (page, head, row)
   const int32_t* bt;

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(64 * PF32_NW) prefill_f32_kernel(PrefillParams
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq)
         *reinterpret_cast<floatx4*>(orow + dd * 32 + gq * 8 + hh * 4) = floatx4{f, f, f, f};
-    if (p.lse && hh == 0) p.lse[((int64_t)b * p.Hq + head) * p.S + qi] = -INFINITY;
+    if (p.lse && hh == 0) p.lse[((int64_t)b * p.Hq + head) * p.S + qi] = p.lse_nan && T < 0 ? f : -INFINITY;
     return;
   }
   const bool none = BIAS && !(l_i > 0.f);  // every key masked by the bias: zeros, as SDPA gives

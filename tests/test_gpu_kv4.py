@@ -672,3 +672,36 @@ def test_plans_launch_again():
     q.mul_(-1)
     second = call.launch().clone()
     assert torch.equal(second, nq.attention_decode_kv4(q, pool, table, lens, max_len=100)) and not torch.equal(first, second)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("append", [False, True])
+@pytest.mark.parametrize("Hq,max_len", [(4, 100), (8, 9000), (2, 33)])
+def test_lse_of_paged_decodes_of_no_and_of_bad_lengths(Hq, max_len, append, dtype):
+    """-inf without keys and NaN outside [0, max_len - append]: a merge and the key weights take
+    -inf for "saw nothing", so a bad length must not look like one."""
+    say(f"paged decode's lse {Hq}/2 max_len {max_len} append={append} {dtype}")
+    g = gen(22)
+    new = int(append)
+    lens = [-1, 0, max_len - new, max_len - new + 1, 2 ** 30, 5]
+    table, pages = table_for([max_len] * len(lens), 32, g)
+    table = table.clamp(max=pages - 1)
+    k, v = (randn(pages, 2, 32, 64, g=g, dtype=dtype) for _ in range(2))
+    q = randn(len(lens), Hq, 64, g=g, dtype=dtype)
+    kw = dict(max_len=max_len)
+    if append:
+        kw.update(k_new=randn(len(lens), 2, 64, g=g, dtype=dtype), v_new=randn(len(lens), 2, 64, g=g, dtype=dtype))
+    o, lse = nq.attention_decode_paged(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device=DEV), return_lse=True, **kw)
+    bad = [0, 3, 4]
+    assert torch.isnan(o[bad]).all() and torch.isnan(lse[bad]).all()
+    good = [i for i in range(len(lens)) if i not in bad]
+    assert torch.isfinite(o[good]).all()
+    for b in good:
+        n = lens[b] + new
+        if n == 0:
+            assert (o[b] == 0).all() and (lse[b] == -math.inf).all()
+            continue
+        _, want, _, spread = ref.attention(q[b], ref.rows_of(k, table[b], n).double(), ref.rows_of(v, table[b], n).double(), 1 / 8)
+        # the bound of the lse test above (an appended row, not normed or rotated, is stored as it is)
+        tol = spread * (2 * 64 + 8) * 2.0 ** -23 + (want.abs() + 1) * 2.0 ** -20 + (n + 64) * 2.0 ** -24
+        assert ((lse[b].double() - want).abs() <= tol).all()
