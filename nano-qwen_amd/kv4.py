@@ -123,7 +123,8 @@ def _rows(t: torch.Tensor, out: Optional[str] = None):
     if last != 1 or at & 15 or odd & _OUTER[t.dtype]:
         if out is not None:
             ops._rows_out(t, out)
-        return _rows(t.contiguous())
+        t = t.clone(memory_format=torch.contiguous_format)  # (contiguous() gives t itself where only its address is off)
+        at, outer = t.data_ptr(), t.stride()[:-1]
     return t, at, _int64s(*outer)
 
 

@@ -705,3 +705,40 @@ def test_lse_of_paged_decodes_of_no_and_of_bad_lengths(Hq, max_len, append, dtyp
         # the bound of the lse test above (an appended row, not normed or rotated, is stored as it is)
         tol = spread * (2 * 64 + 8) * 2.0 ** -23 + (want.abs() + 1) * 2.0 ** -20 + (n + 64) * 2.0 ** -24
         assert ((lse[b].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_operands_off_their_alignment(dtype):
+    """Contiguous rows that start between 16-byte borders, and an axis of one with an odd stride."""
+    say(f"misaligned operands {dtype}")
+    g = gen(61)
+    B, Hq, H, S, D, P, lens = 2, 8, 2, 3, 64, 32, [70, 33]
+
+    def off(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)
+        out = buf[1:].view(t.shape)
+        out.copy_(t)
+        assert out.is_contiguous() and out.data_ptr() % 16
+        return out
+
+    table, pages = table_for([n + S for n in lens], P, g)
+    pool = random_pool(pages, H, P, D, g)
+    other = pool.clone()
+    lens_t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    k, v = (randn(B, H, S, D, g=g, dtype=dtype) for _ in range(2))
+    q = randn(B, Hq, S, D, g=g, dtype=dtype)
+    want = nq.kv4_append(k, v, pool, table, q=q, row_base=lens_t)
+    assert torch.equal(nq.kv4_append(off(k), off(v), other, table, q=off(q), row_base=lens_t), want)
+    assert torch.equal(pool, other)
+    q1 = q[:, :, 0].contiguous()
+    o, lse = nq.attention_decode_kv4(q1, pool, table, lens_t, max_len=70, return_lse=True)
+    for t in (off(q1), q1.as_strided((B, Hq, 1, D), (Hq * D, D, 1, 1))):
+        got, got_lse = nq.attention_decode_kv4(t, pool, table, lens_t, max_len=70, return_lse=True)
+        assert torch.equal(got, o) and torch.equal(got_lse, lse)
+    if dtype == torch.bfloat16:
+        ls = torch.full((B, Hq, S), 4.0, device=DEV)
+        w = nq.attention_key_weights(q, pool, table, lens_t, ls, max_len=70)
+        assert torch.equal(nq.attention_key_weights(off(q), pool, table, lens_t, off(ls), max_len=70), w)
+        one = nq.attention_key_weights(q1[:, :, None], pool, table, lens_t, lse, max_len=70)
+        odd = q1.as_strided((B, Hq, 1, D), (Hq * D, D, 1, 1))
+        assert torch.equal(nq.attention_key_weights(odd, pool, table, lens_t, lse, max_len=70), one)

@@ -539,3 +539,26 @@ def test_quantiser_definition():
     err = (ref.values(codes, byte) - x.double()).abs().reshape(500, 2, 32)
     assert (err <= scale[..., None]).all()
     assert (err <= amax[..., None] / 5).all()
+
+
+# ---------------------------------------------------------------- operands that have to be copied
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_any_layout_are_read_in_place_or_copied_once(dtype):
+    """Among them contiguous tensors that `contiguous()` would return as they are."""
+    base = torch.arange(2 * 4 * 3 * 128 + 8, dtype=torch.float32).to(dtype)
+    n = 2 * 4 * 3 * 128
+    off = base[1:1 + n].view(2, 4, 3, 128)
+    assert off.is_contiguous() and off.data_ptr() % 16
+    odd_axis = base[:2 * 4 * 128].as_strided((2, 1, 4, 128), (512, 131, 128, 1))
+    odd_outer = base[:4 * 3 * 128].as_strided((1, 4, 3, 128), (7, 384, 128, 1))
+    swapped = base[:n].view(2, 4, 128, 3).transpose(2, 3)
+    wide = base[:2 * 4 * 3 * 128].view(2, 4, 3, 128)[..., 1:65]
+    for t in (off, odd_axis, odd_outer, swapped, wide):
+        got, at, strides = kv4._rows(t)
+        assert torch.equal(got, t) and at == got.data_ptr() and at % 16 == 0 and list(strides) == list(got.stride()[:-1])
+        assert got.stride(-1) == 1 and all(s * got.element_size() % 16 == 0 for s in got.stride()[:-1])
+        assert got.data_ptr() != t.data_ptr()
+        with pytest.raises(ValueError, match="16-byte aligned"):
+            kv4._rows(t, "out")
+    for t in (base[:n].view(2, 4, 3, 128), base[:n].view(2, 3, 4, 128).transpose(1, 2), base[:n].view(2, 4, 3, 128)[..., 64:]):
+        assert kv4._rows(t)[0] is t and kv4._rows(t, "out")[0] is t
