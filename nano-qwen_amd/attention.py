@@ -294,7 +294,8 @@ class PagedKVCache:
         self.track_weights = int(track_weights)
         self.weights: Optional[torch.Tensor] = None
         self.evicted: list = []                      # rows evicted of each sequence
-        self._shift: Optional[torch.Tensor] = None   # the same on the device, None while all are 0
+        # the same on the device, kept from the first eviction on: a recorded step holds its address
+        self._shifts: Optional[torch.Tensor] = None
         self._expected: Optional[list] = None
 
     # -- sizes
@@ -391,18 +392,19 @@ class PagedKVCache:
 
     # -- positions and weights
     def _write_shift(self) -> None:
-        if not any(self.evicted):
-            self._shift = None
-            return
-        host = torch.tensor(self.evicted, dtype=torch.int32)
-        if self._shift is None:
-            self._shift = host.to(self.lens.device)
-        else:
-            self._shift.copy_(host)
+        if self._shifts is not None:
+            self._shifts.copy_(torch.tensor(self.evicted, dtype=torch.int32))
+        elif any(self.evicted):
+            self._shifts = torch.tensor(self.evicted, dtype=torch.int32).to(self.lens.device)
+
+    @property
+    def _shift(self) -> Optional[torch.Tensor]:
+        """``evicted`` on the device, None while all are 0."""
+        return self._shifts if any(self.evicted) else None
 
     def _next_positions(self) -> Optional[torch.Tensor]:
         """Each sequence's next position (device), None while it is its length."""
-        return None if self._shift is None else self.lens + self._shift
+        return None if self._shift is None else self.lens + self._shifts
 
     def _take_expected(self, B: int, S: int) -> Optional[list]:
         """What ``expect_lengths`` said of a chunk of S tokens."""
@@ -478,7 +480,7 @@ class PagedKVCache:
         self._pages = []
         self.weights = None
         self.evicted = []
-        self._shift = None
+        self._shifts = None
         self._expected = None
 
     def gather(self, b: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -750,7 +752,9 @@ class Attention(nn.Module):
 
     def _paged_step(self, q4, k4, v4, position_ids, cache, longest, rot, qw, kw):
         lens, lens_next = cache.lens, cache._spare_lens()
-        qp = position_ids if position_ids is not None else cache._next_positions()
+        qp = position_ids
+        if qp is None and cache._shifts is not None:
+            qp = lens + cache._shifts
         o = ops.attention_decode_paged(q4, cache.k_pool, cache.v_pool, cache.block_table, lens,
                                        max_len=longest, k_new=k4, v_new=v4, k_weight=kw,
                                        lens_out=lens_next, q_weight=qw, q_pos=qp, q_pos0=-1,
@@ -767,7 +771,7 @@ class Attention(nn.Module):
     def _paged4_step(self, q4, k4, v4, position_ids, cache, longest, rot, qw, kw):
         """One launch normalises, rotates and stores, the next ones attend the stored row too."""
         lens, lens_next = cache.lens, cache._spare_lens()
-        pos = {"position_ids": position_ids} if position_ids is not None else {"pos_base": lens, "pos_shift": cache._shift}
+        pos = {"position_ids": position_ids} if position_ids is not None else {"pos_base": lens, "pos_shift": cache._shifts}
         q_hat = kv4.kv4_append(k4, v4, cache.pool, cache.block_table, q=q4, q_weight=qw, k_weight=kw, row_base=lens,
                                lens_out=lens_next, **rot, **pos)
         track = bool(cache.track_weights)

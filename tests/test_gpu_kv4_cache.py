@@ -276,3 +276,53 @@ def test_a_captured_step_of_the_module_replays():
             assert torch.equal(out, want)
         else:
             assert torch.isnan(out).all()
+
+
+@pytest.mark.parametrize("kind", [nq.PagedKVCache, nq.PagedKVCache4])
+@torch.no_grad()
+def test_a_step_recorded_after_an_eviction_follows_the_counts(kind):
+    """Back to none, when the sequences that evicted begin anew, and to others."""
+    say(f"step recorded after an eviction {kind.__name__}")
+    attn = module(seed=13)
+    h = (0.5 * randn(2, 130, 256, seed=14)).to(DEV, torch.bfloat16)
+
+    def fresh():
+        c = kind(num_pages=12, page_size=32, max_pages_per_seq=4, track_weights=8)
+        attn(h[:, :60], kv_cache=c)
+        c.evict(40, recent=8)
+        return c
+
+    def anew(c, keep):
+        c.free(0)
+        c.free(1)
+        c.weights.zero_()  # a replay's row, which the cache was not told of, has one
+        attn(h[:, :60], kv_cache=c)
+        if keep:
+            c.evict(40, recent=8)
+        else:
+            c.set_lengths([40, 40])
+    eager, recorded = fresh(), fresh()
+    x = h[:, 60:61].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attn(x, kv_cache=recorded)  # warm up, taken back
+        recorded.set_lengths([40, 40])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attn(x, kv_cache=recorded)
+    reads = recorded._lens_spare  # the lengths that the recorded step reads
+    for keep in (None, False, True, False):
+        if keep is not None:
+            for c in (eager, recorded):
+                anew(c, keep)
+        junk = [torch.full((2,), 1 << 20, dtype=torch.int32, device=DEV) for _ in range(64)]  # where freed counts would lie
+        at = [n + e for n, e in zip(eager.host_lens, eager.evicted)]
+        assert at == ([60, 60] if keep in (None, True) else [40, 40])
+        reads.fill_(40)
+        graph.replay()
+        want = attn(x, kv_cache=eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), keep
+        del junk

@@ -562,3 +562,23 @@ def test_rows_of_any_layout_are_read_in_place_or_copied_once(dtype):
             kv4._rows(t, "out")
     for t in (base[:n].view(2, 4, 3, 128), base[:n].view(2, 3, 4, 128).transpose(1, 2), base[:n].view(2, 4, 3, 128)[..., 64:]):
         assert kv4._rows(t)[0] is t and kv4._rows(t, "out")[0] is t
+
+
+# ---------------------------------------------------------------- what recorded steps hold
+def test_the_evicted_counts_stay_where_a_recorded_step_reads_them(plain_eviction):
+    c = filled([90, 70])
+    c.evict(40)
+    held = c._shifts
+    assert held.tolist() == [50, 30]
+    c.free(0)
+    c.free(1)
+    assert c._shifts is held and held.tolist() == [0, 0] and c.evicted == [0, 0]
+    c._grow([60, 50])
+    c.host_lens = [60, 50]
+    c.lens.copy_(torch.tensor([60, 50], dtype=torch.int32))
+    c.evict(45)
+    assert c._shifts is held and held.tolist() == [15, 5]
+    c.set_lengths([0, 45])
+    assert c._shifts is held and held.tolist() == [0, 5] and c._next_positions().tolist() == [0, 50]
+    c.reset()
+    assert c._shifts is None
