@@ -251,7 +251,9 @@ class PagedKVCache:
     ``v_pool`` of shape (num_pages, Hkv, page_size, D).  Pages are taken from
     a free list as sequences grow and returned by ``free`` / ``reset``, so
     sequences of very different lengths share one pool without padding to
-    the longest.  ``page_size`` is a multiple of 32.
+    the longest.  ``page_size`` is a multiple of 32.  A forward captured in a
+    graph stays at the lengths of its capture: replayed at longer ones it
+    gives NaN.
 
     Semantics are the causal ones with true positions: a multi-token forward
     appends its rows after each sequence's current length (causal attention

@@ -742,3 +742,54 @@ def test_operands_off_their_alignment(dtype):
         one = nq.attention_key_weights(q1[:, :, None], pool, table, lens_t, lse, max_len=70)
         odd = q1.as_strided((B, Hq, 1, D), (Hq * D, D, 1, 1))
         assert torch.equal(nq.attention_key_weights(odd, pool, table, lens_t, lse, max_len=70), one)
+
+
+def test_a_captured_loop_advances_its_lengths():
+    """The step of the documentation: bounded by the rows that the table maps, its lengths advanced
+    in the graph, over a page border; each replay as the eager step, and against the definition."""
+    say("captured decode loop")
+    g = gen(71)
+    B, Hq, H, D, P, cols = 2, 8, 2, 64, 32, 4
+    cos, sin = (t.to(DEV) for t in rope_tables(D, 512, 10000.0))
+    table = torch.randperm(B * cols, generator=g, device=DEV).int().view(B, cols)
+    pool = random_pool(B * cols, H, P, D, g)
+    eager_pool = pool.clone()
+    k, v, q = (randn(B, h, 1, D, g=g, dtype=torch.bfloat16) for h in (H, H, Hq))
+    kw, qw = (1 + 0.1 * randn(D, g=g) for _ in range(2))
+    start = [60, 91]
+
+    def step(pool, lens, grown, w):
+        qh = nq.kv4_append(k, v, pool, table, q=q, q_weight=qw, k_weight=kw, cos=cos, sin=sin, pos_base=lens,
+                           row_base=lens, lens_out=grown)
+        o, lse = nq.attention_decode_kv4(qh, pool, table, grown, max_len=cols * P, return_lse=True)
+        nq.attention_key_weights(qh, pool, table, grown, lse, max_len=cols * P, weights=w)
+        lens.add_(1)
+        return qh, o, lse
+
+    def state():
+        lens = torch.tensor(start, dtype=torch.int32, device=DEV)
+        return lens, torch.empty_like(lens), torch.zeros(B, H, cols * P, device=DEV)
+    mine, theirs = state(), state()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(pool, *mine)
+    torch.cuda.current_stream().wait_stream(side)
+    pool.copy_(eager_pool)
+    mine[0].copy_(torch.tensor(start))
+    mine[2].zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(pool, *mine)
+    for i in range(8):
+        for t in (k, v, q):
+            t.copy_(randn(*t.shape, g=g))
+        graph.replay()
+        got = [t.clone() for t in held]
+        want = step(eager_pool, *theirs)
+        torch.cuda.synchronize()
+        for a, b in zip((*got, pool, *mine), (*want, eager_pool, *theirs)):
+            assert torch.equal(a, b), i
+        lens = [n + i + 1 for n in start]
+        check_decode(got[1], got[2], got[0][:, :, 0], pool, table, lens, P, f"replay {i}")
+    assert mine[0].tolist() == [n + 8 for n in start]
