@@ -679,7 +679,7 @@ int nq_kv4_gather(const void* pool, const int64_t* pool_strides, int num_pages, 
  * Single-token GQA attention over keys [0, lens[b]) of 4-bit pages.  q: (B, Hq, D),
  * strides {batch, head}, normed and rotated (nq_kv4_append's q_out); o alike; lse: fp32
  * (B, Hq) or NULL.  dtype: of q and o.  Lengths as in nq_attn_decode_fwd: zeros (and LSE
- * -inf) without keys, NaN outside [0, max_len].  workspace: at least
+ * -inf) without keys, NaN outside [0, max_len], which is at most 2^30.  workspace: at least
  * nq_attn_decode_kv4_workspace_bytes (0: none, NULL allowed; of the current device),
  * 16-byte aligned; calls that overlap need one each.
  */
@@ -718,8 +718,8 @@ int nq_key_weights(const void* q, const int64_t* q_strides, const void* k_pool,
  * ascending order, the first `first` rows, the last `recent` of lens[b], and of those in
  * between the heaviest, equal weights by the lower index (NaN above every number); -1
  * behind them where a sequence holds fewer than keep.  weights: fp32, strides {batch,
- * head}, width entries a head.  first + recent <= keep.  A length outside [0, width]
- * keeps nothing.
+ * head}, width entries a head.  first + recent <= keep; width and keep are at most 2^30.
+ * A length outside [0, width] keeps nothing.
  */
 int nq_select_keys(const float* weights, const int64_t* weight_strides, const int32_t* lens, int32_t* kept,
                    int B, int Hkv, int width, int keep, int recent, int first, void* stream);

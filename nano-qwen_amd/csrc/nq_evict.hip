@@ -827,6 +827,8 @@ extern "C" int nq_select_keys(const float* weights, const int64_t* weight_stride
     return nq_fail(NQ_ERR_INVALID, "first %d and recent %d must fit keep %d", first, recent, keep);
   if (!weights || !weight_strides || !lens || !kept)
     return nq_fail(NQ_ERR_INVALID, "weights, their strides, lens and kept are required");
+  if (width > (1 << 30) || keep > (1 << 30))  // indices, rounded up to a workgroup's rounds, are ints
+    return nq_fail(NQ_ERR_UNSUPPORTED, "at most 2^30 weights and kept rows a head");
   if ((int64_t)B * Hkv * SEL_THREADS > 0xffffffffll)  // a launch has fewer than 2^32 threads
     return nq_fail(NQ_ERR_UNSUPPORTED, "more (sequence, kv head) rows than one launch takes");
   SelectParams p{weights, weight_strides[0], weight_strides[1], lens, kept, Hkv, width, keep, recent, first};

@@ -572,7 +572,7 @@ decode_kv4_kernel(Kv4DecodeParams pp) {
 // the host knows no more than the longest: the shared work is taken as half of it.
 constexpr float KV4_STEP_US = 0.9f, KV4_SHARE_US = 7.f;
 static bool kv4_whole_rows(int64_t rows, int max_len, int cus) {
-  const int64_t turns = (max_len + DC_STEP * KV4_ROW_WAVES - 1) / (DC_STEP * KV4_ROW_WAVES);
+  const int64_t turns = ((int64_t)max_len + DC_STEP * KV4_ROW_WAVES - 1) / (DC_STEP * KV4_ROW_WAVES);
   const float own = (float)((rows + cus - 1) / cus) * turns * KV4_STEP_US;
   const float shared = 0.5f * (float)rows * turns / cus * KV4_STEP_US + KV4_SHARE_US;
   return own <= shared;
@@ -769,6 +769,8 @@ extern "C" int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const
       return nq_fail(NQ_ERR_INVALID, "q and o strides must be multiples of 16 bytes");
   if ((max_len + page_size - 1) / page_size > bt_cols)
     return nq_fail(NQ_ERR_INVALID, "the block table's %d columns hold fewer than max_len %d rows", bt_cols, max_len);
+  if (max_len > (1 << 30))  // keys, rounded up to whole steps, are ints
+    return nq_fail(NQ_ERR_UNSUPPORTED, "at most 2^30 keys, got max_len %d", max_len);
   const int NG = (Hq / Hkv + 15) / 16;
   if ((int64_t)B * Hkv * NG * DC_MERGE_MAX_THREADS > 0xffffffffll)  // a launch has fewer than 2^32 threads
     return nq_fail(NQ_ERR_UNSUPPORTED, "more (sequence, kv head) rows than one launch takes");

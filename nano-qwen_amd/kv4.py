@@ -33,6 +33,7 @@ __all__ = ["kv4_empty_pool", "kv4_append", "kv4_gather", "attention_decode_kv4",
 
 _HEAD_DIMS = {17 * d // 16: d for d in (32, 64, 128)}  # bytes of a row -> head_dim
 _MOST = 2 ** 31 - 1  # the C entries' int, to which ctypes cuts a larger number without a word
+_MOST_KEYS = 2 ** 30  # of a sequence: the kernels count them, rounded up to their steps, in ints
 
 
 class _DeviceCall(ops.KernelCall):
@@ -137,6 +138,8 @@ def _table(table: torch.Tensor, B: int):
     shape = table.shape
     if len(shape) != 2 or shape[0] != B:
         raise ValueError(f"a block table must be (B={B}, pages per sequence), got {tuple(shape)}")
+    if shape[1] > _MOST:
+        raise ValueError(f"a block table has fewer than 2^31 columns, got {shape[1]}")
     table = _i32(table)
     return table, table.data_ptr(), table.stride(0), shape[1]
 
@@ -146,6 +149,11 @@ def _lens(lens: torch.Tensor, B: int, name: str = "lens") -> torch.Tensor:
     if lens.numel() != B:
         raise ValueError(f"{name} must hold one number per sequence ({B}), got shape {tuple(lens.shape)}")
     return lens
+
+
+def _rows_fit(first: int, S: int, mapped: int, row_base: Optional[torch.Tensor]) -> None:
+    if S < 0 or (row_base is None and not 0 <= first <= min(mapped, _MOST) - S):
+        raise ValueError(f"rows {first} .. {first + S - 1} lie outside the {min(mapped, _MOST)} of the block table")
 
 
 def _at(t: Optional[torch.Tensor]):
@@ -214,8 +222,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
             raise ValueError("q_out must match q in shape and dtype")
         q_rows, q_to = _rows(q), _rows(q_out, "q_out")
     bt, bt_at, bt_stride, cols = _table(block_table, B)
-    if row_base is None and not 0 <= row_offset <= cols * P - S:
-        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {cols * P}")
+    _rows_fit(row_offset, S, cols * P, row_base)
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if lens_out is not None:
@@ -271,8 +278,7 @@ def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_off
     (n, H, P, D), pages = _pool4(pool)
     B = block_table.shape[0]
     bt, bt_at, bt_stride, cols = _table(block_table, B)
-    if S < 0 or (row_base is None and not 0 <= row_offset <= cols * P - S):
-        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {cols * P}")
+    _rows_fit(row_offset, S, cols * P, row_base)
     if dtype not in _OUTER:
         raise TypeError(f"unsupported dtype {dtype}; rows are read back as bfloat16 or float32")
     shape = (B, H, S, D)
@@ -315,8 +321,9 @@ def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     B, Hq, _ = shape
     dt = ops._code(q)
     bt, bt_at, bt_stride, cols = _table(block_table, B)
-    if not 0 < max_len <= cols * P:
-        raise ValueError(f"max_len must be in [1, {cols * P}] (block table columns x page_size), got {max_len}")
+    if not 0 < max_len <= min(cols * P, _MOST_KEYS):
+        raise ValueError(f"max_len must be in [1, {min(cols * P, _MOST_KEYS)}] (block table columns x page_size, 2^30), "
+                         f"got {max_len}")
     dev = q.device
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -376,8 +383,9 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
     if lse.dtype is not torch.float32 or tuple(lse.shape) not in ((B, Hq, S), (B, Hq)) or lse.numel() != B * Hq * S:
         raise ValueError(f"lse must be fp32 {(B, Hq, S)}, got {lse.dtype} {tuple(lse.shape)}")
     bt, bt_at, bt_stride, cols = _table(block_table, B)
-    if not 0 < max_len <= cols * P:
-        raise ValueError(f"max_len must be in [1, {cols * P}] (block table columns x page_size), got {max_len}")
+    if not 0 < max_len <= min(cols * P, _MOST_KEYS):
+        raise ValueError(f"max_len must be in [1, {min(cols * P, _MOST_KEYS)}] (block table columns x page_size, 2^30), "
+                         f"got {max_len}")
     add = weights is not None
     if not add:
         weights = torch.empty(B, H, max_len, dtype=torch.float32, device=q.device)
@@ -421,14 +429,14 @@ def select_keys(weights: torch.Tensor, lens: torch.Tensor, *, keep: int, recent:
         raise ValueError(f"weights must be (B, Hkv, W), got {tuple(weights.shape)}")
     B, H, W = weights.shape
     _check_weights(weights, B, H, 1)
-    if keep <= 0 or recent < 0 or first < 0 or recent + first > keep or keep > _MOST:
-        raise ValueError(f"keep must be positive and hold first + recent, got {keep}, {first} and {recent}")
+    if keep <= 0 or recent < 0 or first < 0 or recent + first > keep or max(keep, W) > _MOST_KEYS:
+        raise ValueError(f"keep must be positive and hold first + recent, got {keep}, {first} and {recent}, "
+                         f"and neither it nor the weights' {W} pass 2^30")
     lens_t = _lens(lens, B)
     kept = torch.empty(B, H, keep, dtype=torch.int32, device=weights.device)
     if B == 0 or H == 0:
         return kept
     _sizes("select_keys", B, H)
-    _sizes("select_keys", W)
     args = (ops._ptr(weights), _strides2(weights), ops._ptr(lens_t), ops._ptr(kept), B, H, W, int(keep), int(recent),
             int(first))
     return _launch(plan, weights, _lib.load().nq_select_keys, args, "nq_select_keys", (weights, lens_t), kept)
@@ -476,6 +484,7 @@ def kv_compact(pools: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], bl
     out = None
     if weights is not None:
         _check_weights(weights, B, H, keep)
+        _sizes("kv_compact", weights.shape[2])
         out = torch.empty_like(weights, memory_format=torch.contiguous_format)
         if weights.stride() != out.stride():
             weights = weights.contiguous()

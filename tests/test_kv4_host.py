@@ -582,3 +582,51 @@ def test_the_evicted_counts_stay_where_a_recorded_step_reads_them(plain_eviction
     assert c._shifts is held and held.tolist() == [0, 5] and c._next_positions().tolist() == [0, 50]
     c.reset()
     assert c._shifts is None
+
+
+# ---------------------------------------------------------------- numbers past the kernels' ints
+MOST = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("fn,base,change,text", [
+    # the loops over kept rows and weights step by 1024 from below these: their ints would wrap
+    ("nq_select_keys", SELECT, dict(keep=MOST), b"2^30"),
+    ("nq_select_keys", SELECT, dict(keep=2 ** 30 + 1), b"2^30"),
+    ("nq_select_keys", SELECT, dict(W=MOST), b"2^30"),
+    # (len + 31) / 32 steps
+    ("nq_attn_decode_kv4", DECODE, dict(max_len=MOST, page=1 << 20, cols=2048, bts=2048, ps=i64(136 << 22, 136 << 20)), b"2^30"),
+    ("nq_key_weights", WEIGHTS, dict(max_len=MOST, page=1 << 20, cols=2048, bts=2048), b"2^30"),
+])
+def test_c_entries_refuse_what_their_ints_cannot_count(fn, base, change, text):
+    test_c_entries_refuse(fn, base, change, text)
+
+
+def big_pool(P=1 << 20):
+    """One page of 2^20 rows (torch.empty touches no memory), and a table that names it 8192 times."""
+    return kv4.kv4_empty_pool(1, 1, P, 32, device="cpu"), torch.zeros(1, 8192, dtype=torch.int32)
+
+
+def test_numbers_past_an_int_are_refused(host_calls):
+    """ctypes would cut them: row 2^32 + 3 would be stored as row 3."""
+    pool, table = big_pool()
+    r = rows(H=1, S=1, D=32)
+    q = torch.zeros(1, 1, 32, dtype=torch.bfloat16)
+    for far in (2 ** 32 + 3, 2 ** 31 - 1):
+        with pytest.raises(ValueError, match="outside"):
+            kv4.kv4_append(r, r, pool, table, row_offset=far)
+        with pytest.raises(ValueError, match="outside"):
+            kv4.kv4_gather(pool, table, S=1, row_offset=far)
+    with pytest.raises(AssertionError, match="was not refused"):
+        kv4.kv4_append(r, r, pool, table, row_offset=2 ** 31 - 2)
+    for far in (2 ** 32 + 5, 2 ** 30 + 1):
+        with pytest.raises(ValueError, match="max_len"):
+            kv4.attention_decode_kv4(q, pool, table, LENS, max_len=far)
+        with pytest.raises(ValueError, match="max_len"):
+            kv4.attention_key_weights(r, pool, table, LENS, torch.zeros(1, 1, 1), max_len=far)
+    with pytest.raises(ValueError, match="2\\^30"):
+        kv4.select_keys(torch.zeros(1, 1, 8), LENS, keep=2 ** 30 + 1)
+    wide = torch.empty(1, 1, 2 ** 32 + 8, device="meta")
+    with pytest.raises(ValueError, match="2\\^30"):
+        kv4.select_keys(wide, LENS, keep=8)
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv4.kv_compact(pool, TABLE, torch.zeros(1, 1, dtype=torch.int32) + 1, torch.zeros(1, 1, 8, dtype=torch.int32), weights=wide)
