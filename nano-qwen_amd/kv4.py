@@ -73,13 +73,21 @@ def _launch(plan: bool, t, fn, args, name, keep, result):
 def _check(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     """Device tensors of one device that want no gradient."""
     ops._require_device(first)
-    index, grad, dual = first.get_device(), torch.is_grad_enabled(), ops._forward_ad._current_level >= 0
-    for t in (first, *others):
-        if t is None:
-            continue
-        if t.get_device() != index:
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
             ops._require_device(t)
             raise ValueError(f"{name}: the operands lie on different devices: {first.device} and {t.device}")
+    _check_gradients(name, first, *others)
+
+
+def _check_gradients(name: str, *operands: Optional[torch.Tensor]) -> None:
+    grad, dual = torch.is_grad_enabled(), ops._forward_ad._current_level >= 0
+    if not (grad or dual):
+        return
+    for t in operands:
+        if t is None:
+            continue
         if grad and t.requires_grad:
             raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or give it detached tensors")
         if dual and ops._forward_ad.unpack_dual(t).tangent is not None:
@@ -201,6 +209,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
     Returns q_out (None without q), or with ``plan=True`` a KernelCall.
     """
     _check("kv4_append", k, v, pool, block_table, q, q_out, pos_base, pos_shift, row_base, lens_out)
+    _check_gradients("kv4_append", q_weight, k_weight, cos, sin)  # which may lie on other devices
     (n, H, P, D), pages = _pool4(pool)
     shape = k.shape
     if len(shape) != 4 or shape != v.shape or shape[1] != H or shape[3] != D:

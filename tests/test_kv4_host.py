@@ -630,3 +630,26 @@ def test_numbers_past_an_int_are_refused(host_calls):
         kv4.select_keys(wide, LENS, keep=8)
     with pytest.raises(ValueError, match="2\\^31"):
         kv4.kv_compact(pool, TABLE, torch.zeros(1, 1, dtype=torch.int32) + 1, torch.zeros(1, 1, 8, dtype=torch.int32), weights=wide)
+
+
+@pytest.mark.parametrize("name", ["k", "v", "q", "q_weight", "k_weight", "cos", "sin"])
+def test_append_refuses_any_operand_that_wants_a_gradient(monkeypatch, name):
+    monkeypatch.setattr(kv4.ops, "_require_device", lambda *a: None)
+    monkeypatch.setattr(kv4, "_launch", lambda plan, t, fn, args, name, keep, result: result)
+    args = dict(k=rows(), v=rows(), q=rows(H=4), q_weight=torch.ones(64), k_weight=torch.ones(64), cos=torch.ones(8, 32),
+                sin=torch.ones(8, 32))
+
+    def call(**change):
+        a = dict(args, **change)
+        return kv4.kv4_append(a.pop("k"), a.pop("v"), pool4(), TABLE, **a)
+    leaf = args[name].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        call(**{name: leaf})
+    with pytest.raises(RuntimeError, match="no gradient"):
+        call(**{name: torch.nn.Parameter(args[name])})
+    with torch.no_grad():
+        call(**{name: leaf})
+    call(**{name: leaf.detach()})
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        call(**{name: fwd.make_dual(args[name], args[name])})
