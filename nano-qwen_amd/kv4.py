@@ -251,10 +251,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
         cos_t, sin_t, max_pos = ops._tables(cos, sin, dev)
         if cos_t.shape[1] != D // 2:
             raise ValueError(f"the tables must be (max_pos, {D // 2}), got {tuple(cos_t.shape)}")
-        if pos_shift is None:
-            pos = ops._positions(position_ids, pos_offset, pos_base, B, S, max_pos, dev)
-        elif position_ids is not None:
-            pos = _i32(position_ids.to(dev).expand(B, S))
+        pos = ops._positions(position_ids, pos_offset, pos_base, B, S, max_pos, dev)  # a shift only adds to them
     if B == 0 or S == 0:
         return q_out
     _sizes("kv4_append", B, S, Hq + 2 * H)

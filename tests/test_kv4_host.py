@@ -653,3 +653,16 @@ def test_append_refuses_any_operand_that_wants_a_gradient(monkeypatch, name):
     import torch.autograd.forward_ad as fwd
     with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         call(**{name: fwd.make_dual(args[name], args[name])})
+
+
+@pytest.mark.parametrize("shift", [None, LENS])
+@pytest.mark.parametrize("change", [dict(position_ids=torch.tensor([[0, 7, 8]])), dict(position_ids=torch.tensor([-1, 0, 1])),
+                                    dict(pos_offset=6), dict(pos_offset=-1), dict(pos_offset=2 ** 32)])
+def test_positions_outside_the_tables_are_refused_shifted_or_not(host_calls, change, shift):
+    tables = dict(cos=torch.ones(8, 32), sin=torch.ones(8, 32))
+    with pytest.raises(IndexError):
+        kv4.kv4_append(rows(), rows(), pool4(), TABLE, pos_shift=shift, **tables, **change)
+    with pytest.raises(AssertionError, match="was not refused"):
+        kv4.kv4_append(rows(), rows(), pool4(), TABLE, pos_shift=shift, pos_offset=5, **tables)
+    with pytest.raises(AssertionError, match="was not refused"):
+        kv4.kv4_append(rows(), rows(), pool4(), TABLE, pos_shift=shift, position_ids=torch.tensor([[7, 0, 3]]), **tables)
