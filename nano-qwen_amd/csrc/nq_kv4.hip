@@ -675,8 +675,10 @@ extern "C" int nq_kv4_append(const void* k, const int64_t* k_strides, const void
     return nq_fail(NQ_ERR_INVALID, "cos and sin tables go together, with max_pos > 0");
   if (!nq_aligned16(q_weight) || !nq_aligned16(k_weight) || !nq_aligned16(cos_tab) || !nq_aligned16(sin_tab))
     return nq_fail(NQ_ERR_INVALID, "norm weights and tables must be 16-byte aligned");
-  if (lens_out && (lens_out == row_base || lens_out == pos_base || lens_out == pos_shift))
-    return nq_fail(NQ_ERR_INVALID, "lens_out must not alias row_base, pos_base or pos_shift");
+  const uintptr_t out = reinterpret_cast<uintptr_t>(lens_out), lens_bytes = (uintptr_t)B * sizeof(int32_t);
+  for (const int32_t* in : {row_base, pos_base, pos_shift})  // each read by all of a sequence's rows
+    if (lens_out && in && reinterpret_cast<uintptr_t>(in) < out + lens_bytes && out < reinterpret_cast<uintptr_t>(in) + lens_bytes)
+      return nq_fail(NQ_ERR_INVALID, "lens_out must not alias row_base, pos_base or pos_shift");
   const int64_t rows = (int64_t)B * S * ((int64_t)Hq + 2 * (int64_t)Hkv);
   if (rows * (D / 16) > KV4_MOST_LANES) return nq_fail(NQ_ERR_UNSUPPORTED, "too many rows for one call");
   p.k = k; p.ksb = k_strides[0]; p.ksh = k_strides[1]; p.kss = k_strides[2];

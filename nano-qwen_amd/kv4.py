@@ -164,6 +164,15 @@ def _rows_fit(first: int, S: int, mapped: int, row_base: Optional[torch.Tensor])
         raise ValueError(f"rows {first} .. {first + S - 1} lie outside the {min(mapped, _MOST)} of the block table")
 
 
+def _overlap(t: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether t lies in the memory from out's first to its last element."""
+    if t.numel() == 0:
+        return False
+    first, start = t.data_ptr(), out.data_ptr()
+    last = first + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) * t.element_size()
+    return first < start + out.numel() * out.element_size() and start < last + t.element_size()
+
+
 def _at(t: Optional[torch.Tensor]):
     """The address of an operand that may be left out."""
     return None if t is None else _memory(t)
@@ -239,8 +248,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
             raise ValueError("lens_out goes with row_base")
         if lens_out.dtype != torch.int32 or not lens_out.is_contiguous() or lens_out.numel() != B:
             raise ValueError("lens_out must be a contiguous int32 tensor of B elements")
-        if B and any(t is not None and t.data_ptr() == lens_out.data_ptr() for t in (row_base, pos_base, pos_shift)):
-            raise ValueError("lens_out must not be row_base, pos_base or pos_shift")
+        if B and any(t is not None and _overlap(t, lens_out) for t in (row_base, pos_base, pos_shift)):
+            raise ValueError("lens_out must not share memory with row_base, pos_base or pos_shift")
     for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None and w.numel() != D:
             raise ValueError(f"{what} must hold {D} elements, got {tuple(w.shape)}")

@@ -666,3 +666,24 @@ def test_positions_outside_the_tables_are_refused_shifted_or_not(host_calls, cha
         kv4.kv4_append(rows(), rows(), pool4(), TABLE, pos_shift=shift, pos_offset=5, **tables)
     with pytest.raises(AssertionError, match="was not refused"):
         kv4.kv4_append(rows(), rows(), pool4(), TABLE, pos_shift=shift, position_ids=torch.tensor([[7, 0, 3]]), **tables)
+
+
+@pytest.mark.parametrize("name", ["row_base", "pos_base", "pos_shift"])
+def test_lengths_written_over_lengths_read_are_refused(host_calls, name):
+    """lens_out as a view that starts among the other's elements: the C entry and the Python call."""
+    buf = torch.ones(12, dtype=torch.int32)
+    r = rows(B=4)
+    table = TABLE.expand(4, 3).contiguous()
+
+    def call(t, out):
+        args = {"row_base": buf.new_ones(4), name: t}
+        kv4.kv4_append(r, r, pool4(), table, lens_out=out, **args)
+    for t, out in ((buf[1:5], buf[4:8]), (buf[4:8], buf[1:5]), (buf[:4], buf[:4]), (buf[0:8:2], buf[3:7])):
+        with pytest.raises(ValueError, match="share memory"):
+            call(t, out)
+    for t, out in ((buf[:4], buf[4:8]), (buf[8:], buf[4:8])):
+        with pytest.raises(AssertionError, match="was not refused"):
+            call(t, out)
+    at = lambda n: ctypes.c_void_p((1 << 22) + 4 * n)  # noqa: E731
+    for t, out in ((at(0), at(1)), (at(1), at(0)), (at(1), at(1))):  # of B = 2
+        test_c_entries_refuse("nq_kv4_append", APPEND, {name: t, "lens_out": out}, b"alias")
