@@ -336,17 +336,18 @@ class PagedKVCache:
 
     def _grow(self, new_lens) -> None:
         """Map pages so that sequence b can hold new_lens[b] rows."""
-        changed = False
+        missing = []
         for b, n in enumerate(new_lens):
             need = -(-n // self.page_size)
             if need > self.max_pages_per_seq:
                 raise ValueError(f"sequence {b} needs {need} pages, max_pages_per_seq is {self.max_pages_per_seq}")
-            while len(self._pages[b]) < need:
-                if not self._free:
-                    raise RuntimeError("PagedKVCache is out of pages")
-                self._pages[b].append(self._free.pop())
-                changed = True
-        if changed:
+            missing.append(max(need - len(self._pages[b]), 0))
+        # all of them or none: a page that is taken is in the table
+        if sum(missing) > len(self._free):
+            raise RuntimeError("PagedKVCache is out of pages")
+        if any(missing):
+            for pages, m in zip(self._pages, missing):
+                pages.extend(self._free.pop() for _ in range(m))
             self._write_table()
 
     def _write_table(self) -> None:

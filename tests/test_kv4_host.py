@@ -687,3 +687,21 @@ def test_lengths_written_over_lengths_read_are_refused(host_calls, name):
     at = lambda n: ctypes.c_void_p((1 << 22) + 4 * n)  # noqa: E731
     for t, out in ((at(0), at(1)), (at(1), at(0)), (at(1), at(1))):  # of B = 2
         test_c_entries_refuse("nq_kv4_append", APPEND, {name: t, "lens_out": out}, b"alias")
+
+
+# ---------------------------------------------------------------- what a failed call leaves behind
+def test_growing_takes_all_pages_or_none():
+    """A sequence that got its pages before another found none had them in no table: the next
+    growth saw nothing to write, and its rows went to page 0."""
+    c = nq.PagedKVCache(3, page_size=32, max_pages_per_seq=4)
+    c._setup(2, 1, 32, torch.bfloat16, "cpu")
+    c._grow([20, 20])
+    c.host_lens = [20, 20]
+    with pytest.raises(RuntimeError, match="out of pages"):
+        c._grow([50, 50])
+    assert [len(p) for p in c._pages] == [1, 1] and c.free_pages == 1
+    with pytest.raises(ValueError, match="max_pages_per_seq"):
+        c._grow([50, 1000])
+    assert [len(p) for p in c._pages] == [1, 1] and c.free_pages == 1
+    c._grow([50, 20])
+    assert c.block_table[0, :2].tolist() == c._pages[0] and len(set(sum(c._pages, []))) == 3
