@@ -450,7 +450,9 @@ class PagedKVCache:
 
     def _evict_some(self, rows: list, keep: int, recent: int, first: int, each: int) -> None:
         dev = self.lens.device
-        new = [[self._free.pop() for _ in range(each)] for _ in rows]
+        # the pages stay free until the rows have moved: a call that fails on the way loses none
+        taken = self._free[:-len(rows) * each - 1:-1]
+        new = [taken[i:i + each] for i in range(0, len(taken), each)]
         whole = len(rows) == len(self.host_lens)
         at = None if whole else torch.tensor(rows, device=dev)
         held = self.weights[:, :, :max(self.host_lens)]  # what lies behind is 0
@@ -461,6 +463,7 @@ class PagedKVCache:
             held.copy_(w)
         else:
             held.index_copy_(0, at, w)
+        del self._free[-len(taken):]
         for b, pages in zip(rows, new):
             self._free.extend(reversed(self._pages[b]))
             self._pages[b] = pages

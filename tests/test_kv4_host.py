@@ -705,3 +705,27 @@ def test_growing_takes_all_pages_or_none():
     assert [len(p) for p in c._pages] == [1, 1] and c.free_pages == 1
     c._grow([50, 20])
     assert c.block_table[0, :2].tolist() == c._pages[0] and len(set(sum(c._pages, []))) == 3
+
+
+@pytest.mark.parametrize("fails", ["select_keys", "kv_compact"])
+@pytest.mark.parametrize("spare", [20, 3])
+def test_an_eviction_that_fails_loses_no_pages(plain_eviction, monkeypatch, fails, spare):
+    lens = [90, 33, 70, 200]
+    used = sum(-(-n // 32) for n in lens)
+    c, other = filled(lens, num_pages=used + spare), filled(lens, num_pages=used + spare)
+    state = lambda x: (x._free, x._pages, x.host_lens, x.evicted, x.lens.tolist(), x.block_table.tolist())  # noqa: E731
+    before = repr(state(c))
+    weights = c.weights.clone()
+
+    def out_of_memory(*a, **k):
+        raise torch.OutOfMemoryError("no memory")
+    with monkeypatch.context() as m:
+        m.setattr(attention.kv4, fails, out_of_memory)
+        for _ in range(3):
+            with pytest.raises(torch.OutOfMemoryError):
+                c.evict(40, recent=8)
+    assert repr(state(c)) == before and torch.equal(c.weights, weights) and all_pages(c) == list(range(used + spare))
+    c.evict(40, recent=8)
+    other.evict(40, recent=8)
+    assert repr(state(c)) == repr(state(other)) and torch.equal(c.weights, other.weights)
+    assert all_pages(c) == list(range(used + spare))
