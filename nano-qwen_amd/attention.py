@@ -712,7 +712,6 @@ class Attention(nn.Module):
             ops.check_position_span(0, max(n + e for n, e in zip(new, cache.evicted)),
                                     self.rotary_emb.max_position_embeddings)
         rot = {"eps": eps, "cos": cos, "sin": sin}
-        expected = cache._take_expected(B, S)
         if S == 1:
             cache._grow(new)
             step = self._paged4_step if isinstance(cache, PagedKVCache4) else self._paged_step
@@ -722,6 +721,7 @@ class Attention(nn.Module):
             raise NotImplementedError("a multi-token forward into a PagedKVCache needs every sequence "
                                       "at the same length")
         cache._grow(new)
+        expected = cache._take_expected(B, S)
         p0 = past[0]
         at = cache._next_positions()
         if position_ids is not None:

@@ -729,3 +729,44 @@ def test_an_eviction_that_fails_loses_no_pages(plain_eviction, monkeypatch, fail
     other.evict(40, recent=8)
     assert repr(state(c)) == repr(state(other)) and torch.equal(c.weights, other.weights)
     assert all_pages(c) == list(range(used + spare))
+
+
+def stub_forward(monkeypatch, max_pos=1024):
+    """An Attention whose kernels do nothing: a call of _paged_forward on host tensors."""
+    attn = nq.Attention(nq.AttentionConfig(hidden_size=64, num_attention_heads=2, num_key_value_heads=1, head_dim=32,
+                                           max_position_embeddings=max_pos))
+    monkeypatch.setattr(attention.ops, "kv_append_paged", lambda *a, **k: None)
+    monkeypatch.setattr(attention.ops, "attention_prefill_paged", lambda q, *a, **k: q)
+    monkeypatch.setattr(attention.ops, "attention_decode_paged",
+                        lambda q, kp, vp, table, lens, *, lens_out, **k: (lens_out.copy_(lens + 1), q)[1])
+    attn.o_proj = torch.nn.Identity()
+
+    def forward(cache, S):
+        q, k, v = (torch.zeros(2, h, S, 32, dtype=torch.bfloat16) for h in (2, 1, 1))
+        with torch.no_grad():
+            attn._paged_forward(q, k, v, None, cache, None, None, None, None, 1e-6)
+    return forward
+
+
+def test_expected_lengths_wait_for_the_next_longer_forward(monkeypatch):
+    """Neither a one-token forward nor one that cannot run uses them up."""
+    forward = stub_forward(monkeypatch)
+    c = nq.PagedKVCache(6, page_size=32, max_pages_per_seq=8)
+    forward(c, 3)
+    c.expect_lengths([5, 20])
+    forward(c, 1)
+    assert c.host_lens == [4, 4]
+    with pytest.raises(RuntimeError, match="out of pages"):
+        forward(c, 100)
+    with pytest.raises(IndexError):
+        forward(c, 2000)
+    assert c.host_lens == [4, 4] == c.lens.tolist()
+    forward(c, 20)
+    assert c.host_lens == [9, 24] == c.lens.tolist()
+    c.set_lengths([9, 9])
+    forward(c, 2)
+    assert c.host_lens == [11, 11]  # asked for once
+    c.expect_lengths([1, 3])
+    with pytest.raises(ValueError, match="do not fit"):
+        forward(c, 2)
+    assert c.host_lens == [11, 11] == c.lens.tolist()
