@@ -33,6 +33,7 @@ __all__ = ["kv4_empty_pool", "kv4_append", "kv4_gather", "attention_decode_kv4",
 
 _HEAD_DIMS = {17 * d // 16: d for d in (32, 64, 128)}  # bytes of a row -> head_dim
 _MOST = 2 ** 31 - 1  # the C entries' int, to which ctypes cuts a larger number without a word
+_MOST_REACH = 2 ** 30  # elements that 256 query rows of the key weights span, by their strides
 _MOST_KEYS = 2 ** 30  # of a sequence: the kernels count them, rounded up to their steps, in ints
 
 
@@ -413,6 +414,8 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
         return weights if add else weights.zero_()
     _sizes("attention_key_weights", B, Hq, S)
     lens_t = _lens(lens, B)
+    if q.stride(1) * (Hq // H) > _MOST_REACH or q.stride(2) * 257 > _MOST_REACH:  # tokens first: rows as near as they go
+        q = q.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
     q_rows, lse = _rows(q), lse.contiguous()
     lib = _lib.load()
     need = lib.nq_key_weights_workspace_bytes(B, Hq, H, S, int(max_len))

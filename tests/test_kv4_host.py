@@ -770,3 +770,29 @@ def test_expected_lengths_wait_for_the_next_longer_forward(monkeypatch):
     with pytest.raises(ValueError, match="do not fit"):
         forward(c, 2)
     assert c.host_lens == [11, 11] == c.lens.tolist()
+
+
+def test_queries_far_apart_are_copied(monkeypatch):
+    """The last queries of a long prompt lie as far apart as the prompt's heads do; the kernel
+    addresses 256 rows with 32-bit offsets."""
+    seen = []
+    monkeypatch.setattr(kv4, "_check", lambda *a: None)
+    monkeypatch.setattr(kv4, "_launch", lambda plan, t, fn, args, name, keep, result: seen.append((args, keep[0])) or result)
+    base = torch.empty(2 ** 30 + 2 ** 27, dtype=torch.bfloat16)  # touched at a few rows only
+
+    def call(q):
+        kv4.attention_key_weights(q, pool4(D=32, H=1), TABLE, LENS, torch.zeros(q.shape[:3]), max_len=90)
+        args, kept = seen.pop()
+        assert args[0] == kept.data_ptr() and list(args[1]) == list(kept.stride()[:3])
+        return kept
+    head = 2 ** 29 + 8
+    far = base.as_strided((1, 2, 3, 32), (0, head, 64, 1))
+    for h in range(2):
+        for s in range(3):
+            far[0, h, s] = torch.arange(32) + 100 * h + 10 * s
+    got = call(far)
+    assert torch.equal(got, far) and got.stride()[1:] == (32, 64, 1)
+    got = call(base.as_strided((1, 2, 3, 32), (0, 32, 2 ** 29, 1)))
+    assert got.stride()[1:] == (32, 64, 1)
+    near = base.as_strided((1, 2, 3, 32), (0, 2 ** 29, 64, 1))
+    assert call(near) is near
