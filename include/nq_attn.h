@@ -703,7 +703,8 @@ int nq_attn_decode_kv4(const void* q, const int64_t* q_strides, const void* pool
  * weights: fp32, strides {batch, head}, max_len entries a head.  A length outside
  * [0, max_len] gives NaN (accumulating: nothing), a page outside the pool NaN at its keys.
  * Sums are taken in a fixed order.  workspace: nq_key_weights_workspace_bytes (0: none,
- * NULL allowed), 16-byte aligned.
+ * NULL allowed; for more than 256 rows, S times the query heads of a kv head, a float for
+ * each 256 of them, kv head and key), 16-byte aligned.
  */
 int64_t nq_key_weights_workspace_bytes(int B, int Hq, int Hkv, int S, int max_len);
 int nq_key_weights(const void* q, const int64_t* q_strides, const void* k_pool,

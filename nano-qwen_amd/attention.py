@@ -266,7 +266,9 @@ class PagedKVCache:
     how long they are, and it trims them itself.
 
     With ``track_weights`` (bf16 models) ``weights`` (B, Hkv, rows; 4 bytes for
-    every row that ``max_pages_per_seq`` allows) sums the attention weight that
+    every row that ``max_pages_per_seq`` allows each sequence: with its default,
+    the whole pool, B / D of a bf16 pool's bytes and 64 B / 17 D of a 4-bit
+    one's, so give it the longest sequence's pages) sums the attention weight that
     each cached key gets, over query heads and over the queries of each one-token
     step and the last ``track_weights`` of each longer forward; ``evict`` then
     keeps the keys that got most.  A sequence's rows close up, its positions go

@@ -115,6 +115,7 @@ __device__ __forceinline__ float row_lse_of(const KeyWeightParams& p, int b, int
   return r >= R ? -INFINITY : v;
 }
 // What it adds to the row's scores, in log2 units: -inf (no weight) for a query that sees no key.
+// The product is rounded to fp32: 2^-24 |lse| of a weight, as much as by the rounding of lse itself.
 __device__ __forceinline__ float row_offset(float lse) { return lse == -INFINITY ? lse : -lse * kLog2e; }
 
 // Four values' sums over the wave's four groups of 16 lanes: group g gets that of value g.

@@ -376,7 +376,9 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
     lse: the (B, Hq, S) (or, S = 1, (B, Hq)) fp32 log-sum-exp their attention returned (-inf:
     the query saw nothing and adds nothing, whatever it holds).  k_pool: 4-bit pages or bf16
     K pages (pages, Hkv, page_size, D).  Keys from lens[b] on get 0.  With ``weights`` the sums
-    are added to its first max_len entries a head and it is returned.
+    are added to its first max_len entries a head and it is returned.  More than 256 rows (queries
+    times query heads of a kv head) take a workspace of 4 bytes a key, kv head and 256 of them:
+    32768 queries over as many keys, 64/4 heads, 1.07 GB.
     """
     _check("attention_key_weights", q, k_pool, block_table, lens, lse, weights)
     four = k_pool.dtype is torch.uint8
