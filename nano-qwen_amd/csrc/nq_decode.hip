@@ -977,18 +977,18 @@ extern "C" int nq_attn_decode_fwd(const void* q, const int64_t* q_strides, const
   return decode_launch<false, false>(p, D, dtype, stream);
 }
 
-static int decode_paged(const void* q, const int64_t* q_strides, const void* k_new,
-                                        const int64_t* k_new_strides, const void* v_new,
-                                        const int64_t* v_new_strides, const float* k_weight,
-                                        void* k_pool, const int64_t* k_pool_strides, void* v_pool,
-                                        const int64_t* v_pool_strides, const int32_t* block_table,
-                                        int64_t bt_stride, int page_size, const int32_t* lens,
-                                        int32_t* lens_out, void* o, const int64_t* o_strides,
-                                        void* workspace, int64_t workspace_bytes, int B, int Hq,
-                                        int Hkv, int D, int max_len, int chunk, int dtype,
-                                        const float* q_weight, float eps, const float* cos_tab,
-                                        const float* sin_tab, int max_pos, const int32_t* q_pos,
-                                        int q_pos0, float sm_scale, float* lse, void* stream) {
+extern "C" int nq_attn_decode_paged_lse_fwd(const void* q, const int64_t* q_strides, const void* k_new,
+                                            const int64_t* k_new_strides, const void* v_new,
+                                            const int64_t* v_new_strides, const float* k_weight,
+                                            void* k_pool, const int64_t* k_pool_strides, void* v_pool,
+                                            const int64_t* v_pool_strides, const int32_t* block_table,
+                                            int64_t bt_stride, int page_size, const int32_t* lens,
+                                            int32_t* lens_out, void* o, const int64_t* o_strides,
+                                            void* workspace, int64_t workspace_bytes, int B, int Hq,
+                                            int Hkv, int D, int max_len, int chunk, int dtype,
+                                            const float* q_weight, float eps, const float* cos_tab,
+                                            const float* sin_tab, int max_pos, const int32_t* q_pos,
+                                            int q_pos0, float sm_scale, float* lse, void* stream) {
   nq_clear_error();
   DecodeParams p{};
   int rc = decode_setup(p, q, q_strides, k_pool_strides, v_pool_strides, o, o_strides, workspace,
@@ -1045,29 +1045,11 @@ extern "C" int nq_attn_decode_paged_fwd(const void* q, const int64_t* q_strides,
                                         const float* q_weight, float eps, const float* cos_tab,
                                         const float* sin_tab, int max_pos, const int32_t* q_pos,
                                         int q_pos0, float sm_scale, void* stream) {
-  return decode_paged(q, q_strides, k_new, k_new_strides, v_new, v_new_strides, k_weight, k_pool, k_pool_strides, v_pool, v_pool_strides,
-                      block_table, bt_stride, page_size, lens, lens_out, o, o_strides, workspace, workspace_bytes, B, Hq,
-                      Hkv, D, max_len, chunk, dtype, q_weight, eps, cos_tab, sin_tab, max_pos, q_pos, q_pos0, sm_scale,
-                      nullptr, stream);
-}
-
-extern "C" int nq_attn_decode_paged_lse_fwd(const void* q, const int64_t* q_strides, const void* k_new,
-                                        const int64_t* k_new_strides, const void* v_new,
-                                        const int64_t* v_new_strides, const float* k_weight,
-                                        void* k_pool, const int64_t* k_pool_strides, void* v_pool,
-                                        const int64_t* v_pool_strides, const int32_t* block_table,
-                                        int64_t bt_stride, int page_size, const int32_t* lens,
-                                        int32_t* lens_out, void* o, const int64_t* o_strides,
-                                        void* workspace, int64_t workspace_bytes, int B, int Hq,
-                                        int Hkv, int D, int max_len, int chunk, int dtype,
-                                        const float* q_weight, float eps, const float* cos_tab,
-                                        const float* sin_tab, int max_pos, const int32_t* q_pos,
-                                        int q_pos0, float sm_scale, float* lse,
-                                        void* stream) {
-  return decode_paged(q, q_strides, k_new, k_new_strides, v_new, v_new_strides, k_weight, k_pool, k_pool_strides, v_pool, v_pool_strides,
-                      block_table, bt_stride, page_size, lens, lens_out, o, o_strides, workspace, workspace_bytes, B, Hq,
-                      Hkv, D, max_len, chunk, dtype, q_weight, eps, cos_tab, sin_tab, max_pos, q_pos, q_pos0, sm_scale,
-                      lse, stream);
+  return nq_attn_decode_paged_lse_fwd(q, q_strides, k_new, k_new_strides, v_new, v_new_strides, k_weight, k_pool,
+                                      k_pool_strides, v_pool, v_pool_strides, block_table, bt_stride, page_size, lens,
+                                      lens_out, o, o_strides, workspace, workspace_bytes, B, Hq, Hkv, D, max_len, chunk,
+                                      dtype, q_weight, eps, cos_tab, sin_tab, max_pos, q_pos, q_pos0, sm_scale, nullptr,
+                                      stream);
 }
 
 // ---------------------------------------------------------------- no allocation
