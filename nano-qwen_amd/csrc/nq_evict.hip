@@ -134,8 +134,8 @@ __device__ __forceinline__ float group_sums(const float (&v)[4]) {
 // ---- up to 16 rows (a decode step): every key's score in one MFMA tile.  HBM-bound: K read
 // once.  A wave takes 64 keys at a time, of 4-bit pages two to four such runs, the next one
 // on its way; of bf16 pages one.  4-bit codes are read past the caches (cached, 64 sequences
-// of 32768 keys and 4 heads took 121 us for 115); bf16 rows are not, two loads sharing each
-// line (past the caches 260 us for 226 at 1024 to 32768 keys).  64 sequences of as many 4-bit
+// of 32768 keys and 4 heads took 119 us for 110); bf16 rows are not, two loads sharing each
+// line (past the caches 241 us for 212 at 1024 to 32768 keys).  64 sequences of as many 4-bit
 // keys (64/4 heads, 291 MB): 61 us, 4.8 TB/s; with a part of 128 keys a wave, all of its
 // loads at once, 73.
 template <int D, bool FOUR, bool ADD>
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) key_weights_step_kernel(KeyWeightParams p
   const int c16 = lane & 15, grp = lane >> 4;
   const int b = blockIdx.z, kvh = blockIdx.y;
   // Turned by the head: the XCD of a workgroup goes by blockIdx.x where the grid is a multiple
-  // of 8 wide, and only some sequences have last keys (16 wide and not turned: 88 us for 72).
+  // of 8 wide, and only some sequences have last keys (not turned: 88 us for 69).
   const uint32_t x = turned(blockIdx.x, gridDim.x, (uint32_t)b * (uint32_t)p.Hkv + (uint32_t)kvh);
   const int span = p.range.d, k0 = (int)(x * 4 + wave) * span;
   if (k0 >= p.max_len) return;
@@ -270,7 +270,7 @@ key_weights_kernel(KeyWeightParams p) {
   const int b = blockIdx.z, kvh = blockIdx.y;
   // the workgroups of chunk 0, then those of chunk 1, ...: as many as each has ranges, or
   // (many chunks) as many as the last has.  Turned by the head or the chunk, as in the step
-  // kernel: 16 sequences of up to 16384 4-bit keys, 64 queries, 32/8 heads took 131 us, now 93.
+  // kernel: 16 sequences of up to 16384 4-bit keys, 64 queries, 32/8 heads take 97 us, not turned 135.
   int chunk = 0, at_range;
   if (p.same) {
     chunk = blockIdx.x / p.same;
@@ -455,9 +455,9 @@ static int64_t key_weight_groups(const KeyWeightParams& p) {
 // where more are needed anyway, and 512 where the diagonal cuts most of them.  2 prompts of
 // 2048, 16/8 heads, causal: 256 keys 48 us, 1024 45, the 768 chosen 38 (480 workgroups); also
 // launched for the ranges that a chunk does not have, of which the XCDs get unequal shares,
-// 56.  A prompt of 8192, 32/8 heads: 1024 keys 401 us, 512 336; without turning the ranges by
-// the chunk 537.  2048 queries at the end of 32768 keys, 64/4 heads: 1024 keys 977 us, 512
-// 1040.
+// 56.  A prompt of 8192, 32/8 heads: 1024 keys 401 us, 512 349; without turning the ranges by
+// the chunk 548.  2048 queries at the end of 32768 keys, 64/4 heads: 1024 keys 966 us, 512
+// 1024.
 constexpr int KW_FEW_CHUNKS = 64;
 static int key_weight_range(KeyWeightParams p) {
   if (p.chunks <= KW_FEW_CHUNKS)
@@ -614,8 +614,9 @@ __global__ void __launch_bounds__(SEL_THREADS) select_keys_kernel(SelectParams p
 // row (K and V rows; of 4-bit pages codes and scales), and its weight.  A workgroup moves
 // 64 rows: their places are worked out once, in LDS, then each thread has all its pieces
 // of a part in flight.  HBM-bound, each kept row read and written once, past the caches: 8
-// x 8 heads, 8192 of 32768 bf16 rows (D = 128, K and V, 537 MB) take 100 us, as a contiguous
-// copy of as much; through the caches 184.
+// x 8 heads, 8192 of 32768 bf16 rows (D = 128, K and V, 537 MB) take 104 us, as a contiguous
+// copy of as much; through the caches 117.  As many 4-bit rows (143 MB): 42 us, 3.4 TB/s;
+// through the caches 71.
 struct RowPart {
   int64_t off;    // of the part within a page's head (bytes)
   int stride;     // between rows (bytes)

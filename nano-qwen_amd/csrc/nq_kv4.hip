@@ -72,8 +72,8 @@ __device__ __forceinline__ uint32_t kv4_codes8(const floatx8& x, float scale) {
 // normed and rotated in fp32 and rounded once, to their codes; q rows likewise, to
 // q_out.  The tokens of a head are consecutive lanes, so a page's codes and scales are
 // written in runs.  HBM-bound: each row read once, 17 D / 32 bytes written.  4 sequences,
-// 2048 tokens, 8 heads of 128, K and V (42 MB): 9.8 us, 4.3 TB/s; with the heads of a
-// token consecutive 10.7.  A single token of 64 sequences: 3.8 us, the launch and its
+// 2048 tokens, 8 heads of 128, K and V (42 MB): 10.4 us, 4.1 TB/s; with the heads of a
+// token consecutive 9% more.  A single token of 64 sequences: 4.0 us, the launch and its
 // dependent loads.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendParams p) {
@@ -161,7 +161,7 @@ struct Kv4GatherParams {
 // A row's 16 elements a lane, 8 of either half, so that each store of a wave fills whole
 // lines; the rows of a head consecutive; the codes read past the caches, where the rows
 // written lie for their reader.  HBM-bound by its writes: 8192 rows of 4 sequences and
-// 8 heads of 128, K and V (170 MB), take 30 us, 5.7 TB/s.  With the append above, over
+// 8 heads of 128, K and V (170 MB), take 31 us, 5.5 TB/s.  With the append above, over
 // changing pools, 46.4 us; 53.7 with 16 adjacent elements a lane, 47.9 with the codes
 // cached.  A row without a page reads as NaN.
 template <int D, typename T>
@@ -202,10 +202,11 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4GatherParams p) {
 // ---------------------------------------------------------------- decode
 // o = softmax(scale q K^T) V over the keys [0, lens[b]) of each sequence.  Rows (sequence,
 // kv head, up to 16 query heads) are cut into steps of 32 keys as in the bf16 decode
-// (nq_decode.hip); a workgroup of eight waves takes a contiguous range of a row's steps,
-// its waves every eighth step each, and joins them in LDS.  Either a workgroup takes a
-// whole row and writes its output (few or short rows: one launch), or a persistent grid
-// shares the steps of all rows evenly, and partials meet in the bf16 decode's merge.
+// (nq_decode.hip); a workgroup takes a contiguous range of a row's steps, each of its W waves
+// every W-th step, and joins them in LDS.  Either a workgroup of eight waves takes a whole
+// row and writes its output (few or short rows: one launch), or a persistent grid of
+// workgroups of four shares the steps of all rows evenly, and partials meet in the bf16
+// decode's merge.
 //
 // How a step's 32 keys reach the matrix cores:
 //   K: a 16-key tile is one load per lane of D/4 consecutive elements of a row, in the
@@ -216,16 +217,19 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4GatherParams p) {
 //     to a wave-private LDS tile and come back transposed, as in the bf16 decode.
 // Codes times a power of two are exact in bf16, so the products are those of a bf16
 // cache that held the same values.  fp32 queries: q and the probabilities are split into
-// three bf16 terms each (8 + 8 + 8 significant bits), three MFMAs in place of one.
+// three bf16 terms each (8 + 8 + 8 significant bits), three MFMAs in place of one.  bf16
+// queries: the probabilities are rounded to bf16 for the second product, as in the bf16
+// decode; outputs lie 1.9-2.0e-3 from 64 bits (2-norm), 1.6e-3 of it their own rounding.
 //
 // The running maximum is raised only for a score more than 2^8 above it: most steps then
 // exchange nothing between lanes and rescale no output, and the sums, held in fp32, have
 // room for the larger terms.
 //
 // HBM-bound: 17/16 D bytes a cached row and kv head.  64 sequences of 1024 to 32768 keys, 64/4
-// heads, D = 128 (539 MB): 98.5 us with the merge, the workgroups on average at work for 77
-// us of it (7.0 TB/s).  Waves that each took a range of their own (2048 of them, and
-// partials) took 107; a whole row to a workgroup there 132, its rows differing in length.
+// heads, D = 128 (539 MB): 93 us, 5.8 TB/s, and 4.6 for the merge.  What remains is uneven
+// ends: workgroups of equal ranges end between 64 and 94 us (a tenth by 70, nine by 89).
+// Waves that each took a range of their own (2048 of them, and partials) took 107 with the
+// merge; a whole row to a workgroup there 132, its rows differing in length.
 // Loads of two steps in flight a wave; three or four gained nothing.
 constexpr int KV4_ROW_WAVES = 8;          // of a workgroup that takes a row of its own
 constexpr int KV4_WAVES = 4;              // of one of the persistent grid's
@@ -233,7 +237,7 @@ constexpr int KV4_PER_CU = 2;             // of which a CU holds this many
 constexpr int KV4_MAX_GROUPS = 256 * KV4_PER_CU;
 // What a row's start counts for in the split, in steps: its workgroup waits for block table,
 // first codes and the join, about 4.5 us, in which the CU's other one goes on.  At 0, 64
-// sequences of 1024 to 32768 keys (64/4 heads) took 105 us, at 24 101.
+// sequences of 1024 to 32768 keys (64/4 heads) took 105 us, at 24 99.
 constexpr int KV4_ROW_COST = 24;
 constexpr int KV4_DEPTH = 2;              // steps of a wave whose loads are in flight
 constexpr float KV4_SLACK = 8.f;          // log2 of how far a score may exceed the running maximum
@@ -326,7 +330,7 @@ decode_kv4_kernel(Kv4DecodeParams pp) {
     }
   } else {
     // Even ranges: weighted as the bf16 decode's are, 64 sequences of up to 32768 keys took
-    // 101 us, even 98.5.  (The wave of the walk is a workgroup here.)  Their least size: one
+    // 101 us, even 99.  (The wave of the walk is a workgroup here.)  Their least size: one
     // sequence of 10000 keys, 8/1 heads, took 26 us over 338 workgroups of a step, 13 over 42
     // of 8; of 32768, 64/4 heads, 29 over 512 and 20 over 190.
     if (!at.template start<true>(p, lane, blockIdx.x)) return;
@@ -373,7 +377,7 @@ decode_kv4_kernel(Kv4DecodeParams pp) {
     const int kvh = j / p.NG, hg = j % p.NG;
     const bool whole = ls == 0 && nseg == nb;
     const int kend = min(len, (ls + nseg) * DC_STEP);
-    const int mine = nseg > wave ? (nseg - wave + W - 1) / W : 0;  // steps ls + wave + 8 i
+    const int mine = nseg > wave ? (nseg - wave + W - 1) / W : 0;  // steps ls + wave + W i
 
     // the pages of this wave's steps [wbase, wbase + 64), one per lane
     int wbase = 0, win = 0;
