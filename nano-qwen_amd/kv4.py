@@ -74,25 +74,24 @@ def _launch(plan: bool, t, fn, args, name, keep, result):
 def _check(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     """Device tensors of one device that want no gradient."""
     ops._require_device(first)
-    index = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != index:
-            ops._require_device(t)
-            raise ValueError(f"{name}: the operands lie on different devices: {first.device} and {t.device}")
-    _check_gradients(name, first, *others)
-
-
-def _check_gradients(name: str, *operands: Optional[torch.Tensor]) -> None:
-    grad, dual = torch.is_grad_enabled(), ops._forward_ad._current_level >= 0
-    if not (grad or dual):
-        return
-    for t in operands:
+    index, grad, dual = first.get_device(), torch.is_grad_enabled(), ops._forward_ad._current_level >= 0
+    for t in (first, *others):
         if t is None:
             continue
-        if grad and t.requires_grad:
-            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or give it detached tensors")
-        if dual and ops._forward_ad.unpack_dual(t).tangent is not None:
-            raise RuntimeError(f"{name} has no forward-mode gradient: give it the primal tensors")
+        if t.get_device() != index:
+            ops._require_device(t)
+            raise ValueError(f"{name}: the operands lie on different devices: {first.device} and {t.device}")
+        if dual or (grad and t.requires_grad):
+            _check_gradient(name, t)
+
+
+def _check_gradient(name: str, t: Optional[torch.Tensor]) -> None:
+    if t is None:
+        return
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or give it detached tensors")
+    if ops._forward_ad._current_level >= 0 and ops._forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name} has no forward-mode gradient: give it the primal tensors")
 
 
 def _pool4(pool: torch.Tensor):
@@ -160,11 +159,6 @@ def _lens(lens: torch.Tensor, B: int, name: str = "lens") -> torch.Tensor:
     return lens
 
 
-def _rows_fit(first: int, S: int, mapped: int, row_base: Optional[torch.Tensor]) -> None:
-    if S < 0 or (row_base is None and not 0 <= first <= min(mapped, _MOST) - S):
-        raise ValueError(f"rows {first} .. {first + S - 1} lie outside the {min(mapped, _MOST)} of the block table")
-
-
 def _overlap(t: torch.Tensor, out: torch.Tensor) -> bool:
     """Whether t lies in the memory from out's first to its last element."""
     if t.numel() == 0:
@@ -219,7 +213,9 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
     Returns q_out (None without q), or with ``plan=True`` a KernelCall.
     """
     _check("kv4_append", k, v, pool, block_table, q, q_out, pos_base, pos_shift, row_base, lens_out)
-    _check_gradients("kv4_append", q_weight, k_weight, cos, sin)  # which may lie on other devices
+    if torch.is_grad_enabled() or ops._forward_ad._current_level >= 0:
+        for t in (q_weight, k_weight, cos, sin):  # which may lie on other devices
+            _check_gradient("kv4_append", t)
     (n, H, P, D), pages = _pool4(pool)
     shape = k.shape
     if len(shape) != 4 or shape != v.shape or shape[1] != H or shape[3] != D:
@@ -241,7 +237,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, block_table
             raise ValueError("q_out must match q in shape and dtype")
         q_rows, q_to = _rows(q), _rows(q_out, "q_out")
     bt, bt_at, bt_stride, cols = _table(block_table, B)
-    _rows_fit(row_offset, S, cols * P, row_base)
+    if row_base is None and not 0 <= row_offset <= min(cols * P, _MOST) - S:
+        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {min(cols * P, _MOST)}")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if lens_out is not None:
@@ -294,7 +291,8 @@ def kv4_gather(pool: torch.Tensor, block_table: torch.Tensor, *, S: int, row_off
     (n, H, P, D), pages = _pool4(pool)
     B = block_table.shape[0]
     bt, bt_at, bt_stride, cols = _table(block_table, B)
-    _rows_fit(row_offset, S, cols * P, row_base)
+    if S < 0 or (row_base is None and not 0 <= row_offset <= min(cols * P, _MOST) - S):
+        raise ValueError(f"rows {row_offset} .. {row_offset + S - 1} lie outside the block table's {min(cols * P, _MOST)}")
     if dtype not in _OUTER:
         raise TypeError(f"unsupported dtype {dtype}; rows are read back as bfloat16 or float32")
     shape = (B, H, S, D)
@@ -337,7 +335,7 @@ def attention_decode_kv4(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     B, Hq, _ = shape
     dt = ops._code(q)
     bt, bt_at, bt_stride, cols = _table(block_table, B)
-    if not 0 < max_len <= min(cols * P, _MOST_KEYS):
+    if not 0 < max_len <= cols * P or max_len > _MOST_KEYS:
         raise ValueError(f"max_len must be in [1, {min(cols * P, _MOST_KEYS)}] (block table columns x page_size, 2^30), "
                          f"got {max_len}")
     dev = q.device
@@ -401,7 +399,7 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
     if lse.dtype is not torch.float32 or tuple(lse.shape) not in ((B, Hq, S), (B, Hq)) or lse.numel() != B * Hq * S:
         raise ValueError(f"lse must be fp32 {(B, Hq, S)}, got {lse.dtype} {tuple(lse.shape)}")
     bt, bt_at, bt_stride, cols = _table(block_table, B)
-    if not 0 < max_len <= min(cols * P, _MOST_KEYS):
+    if not 0 < max_len <= cols * P or max_len > _MOST_KEYS:
         raise ValueError(f"max_len must be in [1, {min(cols * P, _MOST_KEYS)}] (block table columns x page_size, 2^30), "
                          f"got {max_len}")
     add = weights is not None
@@ -416,7 +414,8 @@ def attention_key_weights(q: torch.Tensor, k_pool: torch.Tensor, block_table: to
         return weights if add else weights.zero_()
     _sizes("attention_key_weights", B, Hq, S)
     lens_t = _lens(lens, B)
-    if q.stride(1) * (Hq // H) > _MOST_REACH or q.stride(2) * 257 > _MOST_REACH:  # tokens first: rows as near as they go
+    _, head, token, _ = q.stride()
+    if head * (Hq // H) > _MOST_REACH or token * 257 > _MOST_REACH:  # tokens first: rows as near as they go
         q = q.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
     q_rows, lse = _rows(q), lse.contiguous()
     lib = _lib.load()
