@@ -160,12 +160,11 @@ def _lens(lens: torch.Tensor, B: int, name: str = "lens") -> torch.Tensor:
 
 
 def _overlap(t: torch.Tensor, out: torch.Tensor) -> bool:
-    """Whether t lies in the memory from out's first to its last element."""
-    if t.numel() == 0:
+    """Whether numbers t, read where they lie (not by a copy of them), share memory with out."""
+    if t.dtype is not torch.int32 or not t.is_contiguous():
         return False
-    first, start = t.data_ptr(), out.data_ptr()
-    last = first + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) * t.element_size()
-    return first < start + out.numel() * out.element_size() and start < last + t.element_size()
+    a, b = t.data_ptr(), out.data_ptr()
+    return a < b + out.nbytes and b < a + t.nbytes
 
 
 def _at(t: Optional[torch.Tensor]):
